@@ -234,6 +234,10 @@ PyMethodDef g_methods[] = {
     ENTRY(frwq_slws_noalloc_opts),
     ENTRY(frwq_slws_offsets),
     ENTRY(frwq_slws_offsets_opts),
+    ENTRY(mx4_quantize),
+    ENTRY(mx4_dequantize),
+    ENTRY(mx4_fc),
+    ENTRY(group_norm),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods,

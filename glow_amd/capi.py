@@ -12,6 +12,8 @@ LIB_PATH = os.path.join(_PKG, "libglow_mi355x.so")
 
 FUSED_U8_F32, FUSED_U8_F16, FUSED_U4_F16, FUSED_U4_F32 = 0, 1, 2, 3
 ACT_NONE, ACT_RELU, ACT_CLIP, ACT_TANH, ACT_SIGMOID, ACT_LEAKY_RELU = range(6)
+ACT_SILU = 6                                 # of mx4_fc and group_norm only
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_MX4 = range(4)
 SCHEMA_ASYMMETRIC, SCHEMA_SYMMETRIC, SCHEMA_SYMMETRIC_WITH_UNSIGNED, \
     SCHEMA_SYMMETRIC_POWER2 = range(4)
 QTY_INT8, QTY_INT16, QTY_INT32, QTY_UINT8 = 8, 16, 32, 108
@@ -53,6 +55,8 @@ EXPORTS = [
     "mi355x_specialize_bias_qparams", "mi355x_channelwise_quantize_conv_host",
     "mi355x_gemm_requant_hint", "mi355x_gemm_requant_hint_host",
     "mi355x_copy_segments", "mi355x_set_device", "mi355x_stream_query", "mi355x_host_is_pinned",
+    "mi355x_mx4_row_bytes", "mi355x_mx4_quantize_host", "mi355x_mx4_quantize", "mi355x_mx4_dequantize",
+    "mi355x_mx4_fc_workspace_bytes", "mi355x_mx4_fc", "mi355x_group_norm_workspace_bytes", "mi355x_group_norm",
 ]
 
 
@@ -107,6 +111,8 @@ def lib():
         l.mi355x_last_error.restype = C.c_char_p
         l.mi355x_fused_row_bytes.restype = C.c_size_t
         l.mi355x_fused_row_bytes.argtypes = [C.c_size_t, C.c_int]
+        l.mi355x_mx4_row_bytes.restype = C.c_size_t
+        l.mi355x_mx4_row_bytes.argtypes = [C.c_size_t]
         l.mi355x_arena_bytes.restype = C.c_uint64
         l.mi355x_arena_bytes.argtypes = [C.c_void_p]
         l.mi355x_quantize_scale_offset_32to8.restype = None
@@ -1496,4 +1502,108 @@ def rwq_slws(data, scales, offsets, weights, indices, lengths):
                                 _vp(d_w), _vp(d_i), C.c_int(indices.dtype == np.int64),
                                 _sz(indices.size), _vp(d_l), _sz(lengths.size),
                                 _sz(data.shape[1]), _vp(None)))
+    return out.numpy()
+
+
+# ---- microscaled 4-bit rows, their product, group norm ---------------------------
+# Rows of TYPE_MX4 are uint8 arrays [rows, mx4_row_bytes(cols)]. numpy has no bfloat16: the
+# conveniences take and give such tensors as uint16 arrays of their bits.
+
+def mx4_row_bytes(cols):
+    return lib().mi355x_mx4_row_bytes(cols)
+
+
+def mx4_quantize_host(x):
+    x = np.ascontiguousarray(x, np.float32)
+    rows, cols = x.shape
+    out = np.zeros((rows, mx4_row_bytes(cols)), np.uint8)
+    check(lib().mi355x_mx4_quantize_host(_vp(x), _sz(rows), _sz(cols), _vp(out)))
+    return out
+
+
+def launch_mx4_quantize(dst, dst_row_bytes, src, src_type, src_row_bytes, rows, cols, stream=None):
+    (_native or native()).mx4_quantize(dst, dst_row_bytes, src, src_type, src_row_bytes, rows, cols, stream)
+
+
+def launch_mx4_dequantize(dst, dst_type, dst_row_bytes, src, src_row_bytes, rows, cols, stream=None):
+    (_native or native()).mx4_dequantize(dst, dst_type, dst_row_bytes, src, src_row_bytes, rows, cols, stream)
+
+
+def mx4_fc_workspace_bytes(M, K, N, in_type):
+    n = C.c_size_t(0)
+    check(lib().mi355x_mx4_fc_workspace_bytes(_sz(M), _sz(K), _sz(N), C.c_int(in_type), C.byref(n)))
+    return n.value
+
+
+def launch_mx4_fc(out, out_type, out_row_bytes, in_, in_type, in_row_bytes, weights, weights_row_bytes, bias,
+                  M, K, N, activation=ACT_NONE, workspace=None, workspace_bytes=0, stream=None):
+    (_native or native()).mx4_fc(out, out_type, out_row_bytes, in_, in_type, in_row_bytes, weights,
+                                 weights_row_bytes, bias, M, K, N, activation, workspace, workspace_bytes, stream)
+
+
+def group_norm_workspace_bytes(N, pixels, C_, groups):
+    n = C.c_size_t(0)
+    check(lib().mi355x_group_norm_workspace_bytes(_sz(N), _sz(pixels), _sz(C_), _sz(groups), C.byref(n)))
+    return n.value
+
+
+def launch_group_norm(out, out_type, out_row_bytes, in_, in_type, in_row_bytes, gamma, beta, N, pixels, C_, groups,
+                      epsilon=1e-5, activation=ACT_NONE, workspace=None, workspace_bytes=0, stream=None):
+    (_native or native()).group_norm(out, out_type, out_row_bytes, in_, in_type, in_row_bytes, gamma, beta, N,
+                                     pixels, C_, groups, epsilon, activation, workspace, workspace_bytes, stream)
+
+
+_FLOAT_DTYPES = {TYPE_F32: np.float32, TYPE_F16: np.float16, TYPE_BF16: np.uint16}
+
+
+def _float_rows(x, type_):
+    x = np.ascontiguousarray(x)
+    assert x.dtype == _FLOAT_DTYPES[type_], (x.dtype, type_)
+    return x
+
+
+def mx4_quantize(x, type_=TYPE_F32):
+    x = _float_rows(x, type_)
+    rows, cols = x.shape
+    dx, out = to_device(x), DeviceBuffer.empty((rows, mx4_row_bytes(cols)), np.uint8)
+    launch_mx4_quantize(out, out.shape[1], dx, type_, x.strides[0], rows, cols)
+    return out.numpy()
+
+
+def mx4_dequantize(q, cols, type_=TYPE_F32):
+    q = np.ascontiguousarray(q, np.uint8)
+    dq, out = to_device(q), DeviceBuffer.empty((q.shape[0], cols), _FLOAT_DTYPES[type_])
+    launch_mx4_dequantize(out, type_, cols * out.dtype.itemsize, dq, q.shape[1], q.shape[0], cols)
+    return out.numpy()
+
+
+def mx4_fc(x, in_type, weights, bias, K, out_type=TYPE_F32, activation=ACT_NONE):
+    """x [M, K] of a float type, or rows of TYPE_MX4; weights: rows of TYPE_MX4."""
+    x = np.ascontiguousarray(x, np.uint8) if in_type == TYPE_MX4 else _float_rows(x, in_type)
+    weights = np.ascontiguousarray(weights, np.uint8)
+    M, N = x.shape[0], weights.shape[0]
+    shape = (M, mx4_row_bytes(N) if out_type == TYPE_MX4 else N)
+    out = DeviceBuffer.empty(shape, np.uint8 if out_type == TYPE_MX4 else _FLOAT_DTYPES[out_type])
+    dx, dw = to_device(x), to_device(weights)
+    db = to_device(np.ascontiguousarray(bias, np.float32)) if bias is not None else None
+    n = mx4_fc_workspace_bytes(M, K, N, in_type)
+    ws = DeviceBuffer(n) if n else None
+    launch_mx4_fc(out, out_type, shape[1] * out.dtype.itemsize, dx, in_type, x.shape[1] * x.dtype.itemsize, dw,
+                  weights.shape[1], db, M, K, N, activation, ws, n)
+    return out.numpy()
+
+
+def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-5, activation=ACT_NONE, type_=TYPE_F32, out_type=None):
+    """x [N, pixels, C] of a float type; out_type TYPE_MX4 gives rows [N, pixels, row bytes]."""
+    x = _float_rows(x, type_)
+    out_type = type_ if out_type is None else out_type
+    N, pixels, C_ = x.shape
+    shape = (N, pixels, mx4_row_bytes(C_) if out_type == TYPE_MX4 else C_)
+    out = DeviceBuffer.empty(shape, np.uint8 if out_type == TYPE_MX4 else x.dtype)
+    dx = to_device(x)
+    dg, db = (to_device(np.ascontiguousarray(v, np.float32)) if v is not None else None for v in (gamma, beta))
+    n = group_norm_workspace_bytes(N, pixels, C_, groups)
+    ws = DeviceBuffer(n) if n else None
+    launch_group_norm(out, out_type, shape[2] * out.dtype.itemsize, dx, type_, C_ * x.itemsize, dg, db, N, pixels,
+                      C_, groups, epsilon, activation, ws, n)
     return out.numpy()

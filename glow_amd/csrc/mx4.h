@@ -1,0 +1,173 @@
+// Microscaled 4-bit rows (laid out as mx4_layout.h says): the conversions and the checks of
+// arguments that the kernels over them share.
+#ifndef GLOW_MI355X_MX4_H
+#define GLOW_MI355X_MX4_H
+
+#include "common.h"
+#include "mx4_layout.h"
+
+namespace mi355x {
+
+// ---- element types ---------------------------------------------------------------
+
+struct F32 {
+  typedef float T;
+  static constexpr int kSize = 4;
+  static __device__ __forceinline__ float to(float v) { return v; }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+struct F16 {
+  typedef _Float16 T;
+  static constexpr int kSize = 2;
+  static __device__ __forceinline__ float to(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 from(float v) { return (_Float16)v; }
+};
+struct BF16 {
+  typedef __bf16 T;
+  static constexpr int kSize = 2;
+  static __device__ __forceinline__ float to(__bf16 v) { return (float)v; }
+  static __device__ __forceinline__ __bf16 from(float v) { return (__bf16)v; }
+};
+struct MX4 {
+  typedef uint8_t T;
+  static constexpr int kSize = 0;
+};
+
+// Eight neighbouring values from any address that is one of an element: loads of sixteen
+// bytes need no more alignment than that.
+template <class E> struct __attribute__((packed, aligned(E::kSize))) Eight { typename E::T v[8]; };
+
+template <class E>
+__device__ __forceinline__ void load8(float (&x)[8], const typename E::T *p) {
+  const Eight<E> e = *reinterpret_cast<const Eight<E> *>(p);
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = E::to(e.v[j]);
+}
+// The same at the end of a row: `left` values, zeros behind them.
+template <class E>
+__device__ __forceinline__ void load8_end(float (&x)[8], const typename E::T *p, int left) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = j < left ? E::to(p[j]) : 0.0f;
+}
+template <class E>
+__device__ __forceinline__ void store8(typename E::T *p, const float (&x)[8]) {
+  Eight<E> e;
+#pragma unroll
+  for (int j = 0; j < 8; j++) e.v[j] = E::from(x[j]);
+  *reinterpret_cast<Eight<E> *>(p) = e;
+}
+template <class E>
+__device__ __forceinline__ void store8_end(typename E::T *p, const float (&x)[8], int left) {
+#pragma unroll
+  for (int j = 0; j < 8; j++)
+    if (j < left) p[j] = E::from(x[j]);
+}
+
+// ---- blocks ------------------------------------------------------------------------
+
+// The largest magnitude as its bits: of IEEE numbers without their signs these are ordered
+// as whole numbers are, infinity above every number and NaN above infinity.
+__device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t largest8(const float (&x)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) m = max(m, magnitude_bits(x[j]));
+  return m;
+}
+// The scale byte of a block whose largest magnitude has these bits: its exponent less the 2
+// of E2M1's largest value, 0 at least; 255, NaN, for infinities and NaN.
+__device__ __forceinline__ uint32_t mx4_scale_byte(uint32_t bits) {
+  const uint32_t e = bits >> 23;
+  return e == 255 ? 255 : e > 2 ? e - 2 : 0;
+}
+// 2^(byte - 127); 2^-127 is no normal number. NaN blocks have codes of zero, whatever the
+// values: their scale here is any that makes codes of zeros.
+__device__ __forceinline__ float mx4_scale(uint32_t byte) {
+  return __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
+// Eight values as codes, rounded to nearest with ties to even and saturated at 6 by the
+// conversion instruction.
+__device__ __forceinline__ uint32_t mx4_codes8(const float (&x)[8], uint32_t byte) {
+  const float s = mx4_scale(byte);
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+  return byte == 255 ? 0 : w;
+}
+typedef float mx4_v2f __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void mx4_values8(float (&x)[8], uint32_t codes, uint32_t byte) {
+  const float s = mx4_scale(byte);
+  const mx4_v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 0);
+  const mx4_v2f b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 1);
+  const mx4_v2f c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 2);
+  const mx4_v2f d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 3);
+  const float nan = __builtin_nanf("");
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    x[j] = byte == 255 ? nan : a[j];
+    x[2 + j] = byte == 255 ? nan : b[j];
+    x[4 + j] = byte == 255 ? nan : c[j];
+    x[6 + j] = byte == 255 ? nan : d[j];
+  }
+}
+// The largest of four neighbouring lanes, in all four.
+__device__ __forceinline__ uint32_t quad_max(uint32_t m) {
+  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true)); // lanes 1 0 3 2
+  return max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true)); // 2 3 0 1
+}
+
+// A group's sixteen lanes, eight columns each, write it: codes, the word of scales, and
+// behind the last group the zeros that fill the row up. `l` is the lane of the group.
+__device__ __forceinline__ void mx4_store_group(uint8_t *row, int groups, int g, int l,
+                                                const float (&x)[8]) {
+  const uint32_t byte = mx4_scale_byte(quad_max(largest8(x)));
+  reinterpret_cast<uint32_t *>(row + (size_t)g * kMxGroupBytes)[l] = mx4_codes8(x, byte);
+  // lanes 0, 4, 8, 12 hold the four scales: each lane's byte in its place, joined by or
+  uint32_t word = (l & 3) == 0 ? byte << (8 * (l >> 2)) : 0;
+  word |= (uint32_t)__builtin_amdgcn_mov_dpp((int)word, 0x124, 0xf, 0xf, true); // row_ror:4
+  word |= (uint32_t)__builtin_amdgcn_mov_dpp((int)word, 0x128, 0xf, 0xf, true); // row_ror:8
+  uint32_t *scales = reinterpret_cast<uint32_t *>(row + (size_t)groups * kMxGroupBytes);
+  if (l == 0) scales[g] = word;
+  else if (g == groups - 1 && l < 4 && l <= ((-groups) & 3)) scales[g + l] = 0;
+}
+
+// ---- checks of arguments -----------------------------------------------------------
+
+inline bool float_type(int type) { return type == MI355X_F32 || type == MI355X_F16 || type == MI355X_BF16; }
+inline size_t float_size(int type) { return type == MI355X_F32 ? 4 : 2; }
+
+// Whether a tensor of rows can be addressed: pointer, distance between rows. Says why not.
+inline int check_rows(const char *what, const void *p, int type, size_t row_bytes, size_t rows, size_t cols) {
+  MI355X_REQUIRE(type == MI355X_MX4 || float_type(type), "%s: unknown element type %d", what, type);
+  MI355X_REQUIRE(cols <= 0x7fffffff && rows <= 0x7fffffff,
+                 "%s: %zu x %zu, up to 2^31 - 1 each are supported", what, rows, cols);
+  const size_t align = type == MI355X_MX4 ? 16 : float_size(type);
+  const size_t least = type == MI355X_MX4 ? mx4_row_bytes_of(cols) : cols * align;
+  MI355X_REQUIRE(row_bytes >= least, "%s: rows %zu bytes apart, %zu columns take %zu", what, row_bytes, cols, least);
+  MI355X_REQUIRE(row_bytes % align == 0 && (uintptr_t)p % align == 0,
+                 "%s: the address and the distance between rows have to be multiples of %zu", what, align);
+  size_t span;
+  MI355X_REQUIRE(!__builtin_mul_overflow(rows, row_bytes, &span) && span <= PTRDIFF_MAX,
+                 "%s: %zu rows %zu bytes apart", what, rows, row_bytes);
+  MI355X_REQUIRE(p || rows == 0 || least == 0, "%s: NULL", what);
+  return MI355X_OK;
+}
+// Bytes from the first to the last one that a tensor of rows uses.
+inline size_t rows_span(int type, size_t row_bytes, size_t rows, size_t cols) {
+  if (!rows) return 0;
+  return (rows - 1) * row_bytes + (type == MI355X_MX4 ? mx4_row_bytes_of(cols) : cols * float_size(type));
+}
+inline bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a_bytes && b_bytes && a && b && x < y + b_bytes && y < x + a_bytes;
+}
+
+// Launches the quantisation of checked rows (mx4.hip).
+int mx4_quantize_launch(uint8_t *dst, size_t dst_row_bytes, const void *src, int src_type,
+                        size_t src_row_bytes, size_t rows, size_t cols, hipStream_t st);
+
+} // namespace mi355x
+
+#endif

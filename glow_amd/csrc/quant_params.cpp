@@ -6,6 +6,7 @@
 // same integers (reference lib/Quantization/Base/Base.cpp:234-565,
 // include/glow/Quantization/Base/Base.h:323-678).
 #include "common.h"
+#include "mx4_layout.h"
 
 #include <algorithm>
 #include <cmath>
@@ -370,6 +371,47 @@ int mi355x_fc_chain_pack_host(int8_t *packed, int32_t *columns, const int8_t *we
     columns[padded + n] = out_pre[n];
     columns[2 * padded + n] = out_scale[n];
     columns[3 * padded + n] = out_post[n];
+  }
+  return MI355X_OK;
+}
+
+// E2M1 code of v, |v| < 8: nearest, ties to the even code, over 6 to 6. The values below 2
+// are half apart, to 4 one, to 6 two; nearbyint takes ties to even.
+static uint8_t e2m1_code(float v) {
+  const float a = std::fabs(v);
+  int code;
+  if (a < 2) code = (int)std::nearbyint(a * 2);
+  else if (a < 4) code = (int)std::nearbyint(a) + 2;
+  else code = std::min((int)std::nearbyint(a / 2) + 4, 7);
+  return (uint8_t)(code | (std::signbit(v) ? 8 : 0));
+}
+
+int mi355x_mx4_quantize_host(const float *in, size_t rows, size_t cols, uint8_t *out) {
+  if (!rows || !cols) return MI355X_OK;
+  MI355X_REQUIRE(in && out, "NULL tensor");
+  const size_t groups = mi355x::mx4_groups(cols), row_bytes = mi355x::mx4_row_bytes_of(cols);
+  for (size_t r = 0; r < rows; r++) {
+    const float *x = in + r * cols;
+    uint8_t *row = out + r * row_bytes, *scales = row + groups * mi355x::kMxGroupBytes;
+    std::memset(row, 0, row_bytes);
+    for (size_t b = 0; b * 32 < cols; b++) {
+      const size_t n = std::min<size_t>(32, cols - b * 32);
+      float most = 0;
+      bool finite = true;
+      for (size_t j = 0; j < n; j++) {
+        const float a = std::fabs(x[b * 32 + j]);
+        finite = finite && std::isfinite(a);
+        most = std::max(most, a);
+      }
+      if (!finite) {
+        scales[b] = 255;
+        continue;
+      }
+      const int e = most > 0 ? std::max(std::ilogb(most) - 2, -127) : -127;
+      scales[b] = (uint8_t)(e + 127);
+      for (size_t j = 0; j < n; j++)
+        row[b * 16 + j / 2] |= (uint8_t)(e2m1_code(std::ldexp(x[b * 32 + j], -e)) << (4 * (j & 1)));
+    }
   }
   return MI355X_OK;
 }

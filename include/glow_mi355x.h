@@ -772,7 +772,9 @@ typedef struct {
  * act_args are the quantized arguments emitConstQuantActivationArgs builds
  * (LLVMIRGen.cpp:618-662): CLIP {min, max}; LEAKY_RELU {pre, post, scale}. */
 enum { MI355X_ACT_NONE = 0, MI355X_ACT_RELU = 1, MI355X_ACT_CLIP = 2,
-       MI355X_ACT_TANH = 3, MI355X_ACT_SIGMOID = 4, MI355X_ACT_LEAKY_RELU = 5 };
+       MI355X_ACT_TANH = 3, MI355X_ACT_SIGMOID = 4, MI355X_ACT_LEAKY_RELU = 5,
+       /* v / (1 + exp(-v)): of mi355x_mx4_fc and mi355x_group_norm only */
+       MI355X_ACT_SILU = 6 };
 
 /* libjit_channelwise_quantized_conv2d_i8_i32 / _i8_i8 (reference
  * lib/LLVMIRCodeGen/libjit/libjit_conv.cpp:151-239, 530-562). Eight int32[OC]
@@ -886,6 +888,82 @@ int mi355x_conv2d_i8_opts(int8_t *out, const int8_t *in, const int8_t *filter,
                      const int32_t *act_args, const int32_t *filter_row_sums,
                      void *stream,
                      const mi355x_launch_opts *opts);
+
+/* ---- microscaled 4-bit rows, their product, and group norm ---------------------- */
+/* No counterpart in the reference, whose narrowest products are of int8: the 4-bit floats
+ * that the matrix cores multiply at twice the rate of 8 bits. The steps between two layers
+ * of a network (group norm or the product in front, its bias and activation) hand
+ * microscaled rows on themselves. Inference only: nothing here has a gradient. */
+
+/* Element types of these entry points. */
+enum { MI355X_F32 = 0, MI355X_F16 = 1, MI355X_BF16 = 2, MI355X_MX4 = 3 };
+
+/* MI355X_MX4: rows of 4-bit floats (E2M1: 0 0.5 1 1.5 2 3 4 6 and their negatives; code =
+ * 8 * sign + index) in blocks of 32 columns, each with a power of two (E8M0: 2^(byte - 127),
+ * byte 255: the whole block is NaN). A row of `cols` columns is P = ceil(cols / 128) groups:
+ *   64 * P bytes  codes, two to a byte, the even column in the low half
+ *    4 * P bytes  the scale byte of each block of 32
+ *   zeros up to a multiple of 16 bytes
+ * mi355x_mx4_row_bytes says how many bytes that is. Codes and scales past `cols` are zero;
+ * whoever makes rows in another way has to see to that. Rows lie on multiples of 16 bytes,
+ * any distance of at least mi355x_mx4_row_bytes apart; what is between two rows is neither
+ * read nor written.
+ *
+ * In all of these, `row_bytes` is the distance between rows in bytes: for float types a
+ * multiple of the element's size, rows at any address that is one too. Tensors of no rows
+ * or columns are a no-op. Results may not overlap what they are made from, except where it
+ * says so. Sizes up to 2^31 - 1 each. */
+size_t mi355x_mx4_row_bytes(size_t cols);
+/* Each block of 32: m = the largest magnitude, scale 2^max(floor(log2 m) - 2, -127) (byte
+ * 0 for a block of zeros), codes = value / scale rounded to nearest, ties to even, and
+ * saturated at 6. A block that holds an infinity or a NaN becomes NaN. On HOST buffers,
+ * rows mi355x_mx4_row_bytes apart (weights, once, when a network is loaded). */
+int mi355x_mx4_quantize_host(const float *in, size_t rows, size_t cols, uint8_t *out);
+/* The same on the device, from any of the float types. */
+int mi355x_mx4_quantize(uint8_t *dst, size_t dst_row_bytes, const void *src, int src_type,
+                        size_t src_row_bytes, size_t rows, size_t cols, void *stream);
+/* The values that rows stand for, rounded to nearest where the type is narrower (fp16: what
+ * is past its range becomes an infinity). */
+int mi355x_mx4_dequantize(void *dst, int dst_type, size_t dst_row_bytes, const uint8_t *src,
+                          size_t src_row_bytes, size_t rows, size_t cols, void *stream);
+
+/* FullyConnected over microscaled weights, and the pointwise convolution of a channels-last
+ * image (its pixels are the rows):
+ *   out[m][n] = activation(bias[n] + sum over k of in[m][k] * weights[n][k])
+ * in       [M x K] float of any type, quantized first by the rule above (in the workspace,
+ *          where one is asked for), or MI355X_MX4
+ * weights  MI355X_MX4 [N x K]
+ * bias     float [N], or NULL
+ * out      [M x N] of any type; MI355X_MX4: quantized by the rule above from the 32-bit
+ *          results, ready to be the next layer's input
+ * Products are exact, sums are held in 32 bits in no particular order (equal calls give
+ * equal bits); sums whose magnitude is below 2^-126 may be zero. A NaN block makes NaN of
+ * what it takes part in. K = 0: the activation of the bias. activation: MI355X_ACT_NONE,
+ * _RELU or _SILU.
+ * workspace: device memory of mi355x_mx4_fc_workspace_bytes, on a multiple of 16 and
+ * overlapping no tensor; NULL where that is 0. A call leaves nothing in it for the next, and
+ * calls that may run at the same time need one each. */
+int mi355x_mx4_fc_workspace_bytes(size_t M, size_t K, size_t N, int in_type, size_t *bytes);
+int mi355x_mx4_fc(void *out, int out_type, size_t out_row_bytes, const void *in, int in_type,
+                  size_t in_row_bytes, const uint8_t *weights, size_t weights_row_bytes,
+                  const float *bias, size_t M, size_t K, size_t N, int activation, void *workspace,
+                  size_t workspace_bytes, void *stream);
+
+/* Group norm over channels-last tensors in [N x pixels x C] of a float type, C / groups
+ * neighbouring channels of all pixels of a sample to a group:
+ *   out = activation((in - mean) / sqrt(variance + epsilon) * gamma[c] + beta[c])
+ * with the mean and the variance (over all values, not one less) of the group, both held in
+ * 32 bits. out: of the input's type, also in place (same address and distance between rows),
+ * or MI355X_MX4, quantized from the 32-bit results: the input of mi355x_mx4_fc. gamma, beta:
+ * float [C], or NULL (1 and 0). activation as above. row_bytes: the distance between pixels;
+ * samples follow each other. A NaN or an infinity makes NaN of its group. workspace as
+ * above, of mi355x_group_norm_workspace_bytes. */
+int mi355x_group_norm_workspace_bytes(size_t N, size_t pixels, size_t C, size_t groups,
+                                      size_t *bytes);
+int mi355x_group_norm(void *out, int out_type, size_t out_row_bytes, const void *in, int in_type,
+                      size_t in_row_bytes, const float *gamma, const float *beta, size_t N,
+                      size_t pixels, size_t C, size_t groups, float epsilon, int activation,
+                      void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- fused-rowwise SparseLengths(Weighted)Sum ----------------------------------- */
 
