@@ -1,30 +1,310 @@
 // Group norm with an activation over channels-last tensors.
 //
 // Values x[n][p][c]; a group is C / groups neighbouring channels over all pixels of a
-// sample: y = act((x - mean) / sqrt(variance + epsilon) * gamma[c] + beta[c]). Two launches:
-// a workgroup for each group finds its mean and the mean square of what is left of it, in
-// two passes; then sixteen lanes take 128 channels of a pixel, eight each, as the writers of
-// microscaled rows do.
+// sample: y = act((x - mean) / sqrt(variance + epsilon) * gamma[c] + beta[c]).
+//
+// A slice is some neighbouring groups of a sample, 128 bytes of a pixel if they give as
+// much: whole lines. A thread holds eight channels of every stride-th pixel, a power of two
+// of neighbouring lanes the slice's channels, so that a thread's channels never change.
+// Two ways:
+//   resident  a workgroup reads a slice into its registers (up to 64 a thread: 256 KB a
+//             workgroup, half of a CU's), finds mean and variance, and writes it: one launch,
+//             every value read once
+//   in parts  slices that do not fit, or too few of them to fill the chip: one launch
+//             leaves mean and sum of squares of every part of a slice's pixels in the
+//             workspace, a second joins them and writes
+// Sums are exact in kind: a thread's own mean first and the squares of what is left of it,
+// then the threads' (or parts') means and what they are off the whole's; no difference of
+// large sums is ever formed, whatever the mean is.
 #include "mx4.h"
+
+#include <algorithm>
 
 namespace mi355x {
 
 struct GroupStats {
-  float mean, scale;      // scale: 1 / sqrt(variance + epsilon)
+  float mean, square;     // of a part: sum of the squares of what is left of the mean
 };
 struct GroupNorm {
   uint8_t *out;
   const uint8_t *in;
   size_t out_row_bytes, in_row_bytes;
   const float *gamma, *beta;
-  GroupStats *stats;      // [N][groups]
-  long long rows;         // N * pixels
+  GroupStats *stats;      // [N][groups][chunks]
   int pixels, C, groups, per;
   float epsilon;
   int act;
+  int samples;            // of this launch
+  // a slice is `in_slice` groups, `width` channels; 2^lg_vec lanes hold one pixel of it
+  int in_slice, width, slices, lg_vec;
+  int chunks, chunk_pixels;
+  int by_die;             // neighbouring slices of a sample on one die
+  int channel_groups;     // of a microscaled result's row
+  size_t mx4_bytes;       // of its row
 };
 
-constexpr int kGnThreads = 256;
+enum { kGnResident, kGnStats, kGnApply };
+constexpr int kGnMost = 1024;         // threads of a workgroup
+constexpr int kGnMostChunks = 128;    // parts of a slice
+
+// Sums over a slice's pixels and a group's channels, to s_group[0 .. in_slice). x[j] is a
+// thread's sum for channel j of its eight, or x[0] that of all eight where they lie in one
+// group. Lanes of a wave that hold the same channels are summed first, then a wave takes a
+// group.
+template <int NV>
+__device__ __forceinline__ void gn_reduce(float (&x)[NV], float *s_part, float *s_group, const GroupNorm &p) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
+  const int V = 1 << p.lg_vec;
+  for (int d = V; d < 64; d <<= 1)
+#pragma unroll
+    for (int j = 0; j < NV; j++) x[j] += __shfl_xor(x[j], d);
+  const int rows = V < 64 ? waves : (int)blockDim.x >> p.lg_vec;
+  __syncthreads();
+  if (V >= 64 || lane < V) {
+    const int row = V < 64 ? wave : tid >> p.lg_vec;
+#pragma unroll
+    for (int j = 0; j < NV; j++) s_part[((row << p.lg_vec) + (tid & (V - 1))) * NV + j] = x[j];
+  }
+  __syncthreads();
+  const int len = NV == 1 ? p.per >> 3 : p.per;
+  for (int g = wave; g < p.in_slice; g += waves) {
+    float t = 0;
+    if (len < 64) {
+      for (int e = lane; e < len * rows; e += 64) {
+        const int row = e / len;
+        t += s_part[(row << p.lg_vec) * NV + g * len + (e - row * len)];
+      }
+    } else {
+      for (int row = 0; row < rows; row++)
+        for (int e = lane; e < len; e += 64) t += s_part[(row << p.lg_vec) * NV + g * len + e];
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) t += __shfl_xor(t, d);
+    if (lane == 0) s_group[g] = t;
+  }
+  __syncthreads();
+}
+
+// Writes one pixel's eight channels.
+template <class E, class OUT, int ACT, int NV>
+__device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, bool block_inside,
+                                         const typename E::Eight &raw, const float (&mean)[NV],
+                                         const float (&scale)[8], const float (&shift)[8], const GroupNorm &p) {
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float v = activate<ACT>(fmaf(E::get(raw, j) - mean[NV == 1 ? 0 : j], scale[j], shift[j]));
+    y[j] = OUT::kSize || j < left ? v : 0.0f;
+  }
+  if constexpr (OUT::kSize == 0) {
+    const uint32_t byte = mx4_scale_byte(quad_max(largest8(y)));
+    if (block_inside) {
+      *reinterpret_cast<uint32_t *>(row + (c >> 1)) = mx4_codes8(y, byte);
+      if ((c & 31) == 0) row[(size_t)p.channel_groups * kMxGroupBytes + (c >> 5)] = (uint8_t)byte;
+    }
+  } else {
+    typename OUT::T *o = reinterpret_cast<typename OUT::T *>(row) + c;
+    if (left >= 8) store8<OUT>(o, y);
+    else store8_end<OUT>(o, y, left);
+  }
+}
+
+template <class E, class OUT, int R, int MODE, int NV>
+__global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
+  extern __shared__ __attribute__((aligned(16))) float s_mem[];
+  float *s_group = s_mem, *s_second = s_mem + p.in_slice, *s_part = s_mem + 2 * p.in_slice;
+  const int tid = threadIdx.x, V = 1 << p.lg_vec;
+  const int v = tid & (V - 1), first = tid >> p.lg_vec, stride = (int)blockDim.x >> p.lg_vec;
+
+  unsigned id = blockIdx.x;
+  const int chunk = (int)(id % (unsigned)p.chunks);
+  id /= (unsigned)p.chunks;
+  int sample, slice;
+  if (p.by_die) {            // consecutive workgroups are dealt over the eight dies
+    const unsigned die = id & 7, at = id >> 3;
+    sample = (int)(die + 8 * (at / (unsigned)p.slices));
+    slice = (int)(at % (unsigned)p.slices);
+    if (sample >= p.samples) return;
+  } else {
+    sample = (int)(id / (unsigned)p.slices);
+    slice = (int)(id % (unsigned)p.slices);
+  }
+  const int c0 = slice * p.width, c = c0 + v * 8;
+  const int c_end = min(p.C, c0 + p.width), left = c_end - c;
+  const int px0 = chunk * p.chunk_pixels, px_end = min(p.pixels, px0 + p.chunk_pixels);
+  const uint8_t *in = p.in + (size_t)sample * p.pixels * p.in_row_bytes + (ptrdiff_t)c * E::kSize;
+
+  typename E::Eight raw[R];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int px = from + first + i * stride;
+      if (first + i * stride < px_end - from) {
+        const typename E::T *at = reinterpret_cast<const typename E::T *>(in + (size_t)px * p.in_row_bytes);
+        if (left >= 8) raw[i] = load_eight<E>(at);
+        else raw[i] = load_eight_end<E>(at, left);
+      }
+    }
+  };
+  // pixels of this thread among those of a block that begins at `from`
+  auto mine = [&](int from) {
+    const int rest = px_end - from - first;
+    return left > 0 && rest > 0 ? min(R, (rest - 1) / stride + 1) : 0;
+  };
+  const int block = R * stride;
+  const float of_group = (float)p.per;
+
+  load(px0);
+  if constexpr (MODE != kGnApply) {
+    // a thread's own count (exact: a part has 2^24 pixels at most), mean and squares
+    float count = 0, mean[NV], square[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) mean[j] = square[j] = 0;
+    for (int from = px0;;) {
+      const int n = mine(from);
+      if (n > 0) {
+        float m[NV], q[NV];
+#pragma unroll
+        for (int j = 0; j < NV; j++) m[j] = q[j] = 0;
+#pragma unroll
+        for (int i = 0; i < R; i++)
+          if (i < n)
+#pragma unroll
+            for (int j = 0; j < 8; j++) m[NV == 1 ? 0 : j] += E::get(raw[i], j);
+        const float here = (float)n * (8 / NV), over = 1.0f / here;
+#pragma unroll
+        for (int j = 0; j < NV; j++) m[j] *= over;
+#pragma unroll
+        for (int i = 0; i < R; i++)
+          if (i < n)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const float d = E::get(raw[i], j) - m[NV == 1 ? 0 : j];
+              q[NV == 1 ? 0 : j] = fmaf(d, d, q[NV == 1 ? 0 : j]);
+            }
+        if (MODE == kGnResident || count == 0) {
+          count = here;
+#pragma unroll
+          for (int j = 0; j < NV; j++) mean[j] = m[j], square[j] = q[j];
+        } else {             // joins two sets: the squares of each, and of what their means are apart
+          const float all = count + here, part = here / all;
+#pragma unroll
+          for (int j = 0; j < NV; j++) {
+            const float d = m[j] - mean[j];
+            mean[j] = fmaf(d, part, mean[j]);
+            square[j] += fmaf(d * d, count * part, q[j]);
+          }
+          count = all;
+        }
+      }
+      if (MODE == kGnResident || px_end - from <= block) break;
+      from += block;
+      load(from);
+    }
+    const float total = (float)(px_end - px0) * of_group;
+    float x[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) x[j] = mean[j] * count;
+    gn_reduce<NV>(x, s_part, s_group, p);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int g = left > 0 ? min((v * 8 + j) / p.per, p.in_slice - 1) : 0;
+      const float d = mean[j] - s_group[g] / total;
+      x[j] = left > 0 ? fmaf(d * d, count, square[j]) : 0.0f;
+    }
+    gn_reduce<NV>(x, s_part, s_second, p);
+    const int groups = (c_end - c0) / p.per;
+    for (int g = tid; g < groups; g += (int)blockDim.x) {
+      const float m = s_group[g] / total;
+      if constexpr (MODE == kGnStats)
+        p.stats[((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks + chunk] = GroupStats{m, s_second[g]};
+      else {
+        s_group[g] = m;
+        s_second[g] = 1.0f / sqrtf(s_second[g] / total + p.epsilon);
+      }
+    }
+    if (MODE == kGnStats) return;
+  } else {
+    // joins the parts: their means, then their squares and what their means are off the whole's
+    const int lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
+    const int groups = (c_end - c0) / p.per;
+    const float total = (float)p.pixels * of_group;
+    for (int g = wave; g < groups; g += waves) {
+      const GroupStats *s = p.stats + ((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks;
+      GroupStats own[kGnMostChunks / 64];
+      float m = 0, q = 0;
+#pragma unroll
+      for (int i = 0; i < kGnMostChunks / 64; i++) {
+        const int k = lane + 64 * i;
+        own[i] = k < p.chunks ? s[k] : GroupStats{0, 0};
+        const float n = (float)min(p.chunk_pixels, p.pixels - k * p.chunk_pixels) * of_group;
+        if (k < p.chunks) m = fmaf(own[i].mean, n, m);
+      }
+#pragma unroll
+      for (int d = 32; d; d >>= 1) m += __shfl_xor(m, d);
+      m /= total;
+#pragma unroll
+      for (int i = 0; i < kGnMostChunks / 64; i++) {
+        const int k = lane + 64 * i;
+        const float n = (float)min(p.chunk_pixels, p.pixels - k * p.chunk_pixels) * of_group, d = own[i].mean - m;
+        if (k < p.chunks) q += fmaf(d * d, n, own[i].square);
+      }
+#pragma unroll
+      for (int d = 32; d; d >>= 1) q += __shfl_xor(q, d);
+      if (lane == 0) {
+        s_group[g] = m;
+        s_second[g] = 1.0f / sqrtf(q / total + p.epsilon);
+      }
+    }
+  }
+  __syncthreads();
+
+  float mean[NV], scale[8], shift[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const bool inside = j < left;
+    const int g = inside ? (v * 8 + j) / p.per : 0;
+    if (NV == 8 || j == 0) mean[NV == 1 ? 0 : j] = s_group[g];
+    scale[j] = s_second[g] * (p.gamma && inside ? p.gamma[c + j] : 1.0f);
+    shift[j] = p.beta && inside ? p.beta[c + j] : 0.0f;
+  }
+  uint8_t *out = p.out + (size_t)sample * p.pixels * p.out_row_bytes;
+  // microscaled: lanes up to the end of the slice's last block
+  const bool inside = OUT::kSize ? left > 0 : c < ((c_end + 31) & ~31);
+  auto write = [&](int from, auto act) {
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int px = from + first + i * stride;
+      if (first + i * stride < px_end - from && (OUT::kSize == 0 || inside))
+        gn_write<E, OUT, decltype(act)::value, NV>(out + (size_t)px * p.out_row_bytes, c, left, inside, raw[i], mean,
+                                                   scale, shift, p);
+    }
+  };
+  for (int from = px0;;) {
+    if (p.act == MI355X_ACT_RELU) write(from, std::integral_constant<int, MI355X_ACT_RELU>());
+    else if (p.act == MI355X_ACT_SILU) write(from, std::integral_constant<int, MI355X_ACT_SILU>());
+    else write(from, std::integral_constant<int, MI355X_ACT_NONE>());
+    if (MODE == kGnResident || px_end - from <= block) break;
+    from += block;
+    load(from);
+  }
+  if constexpr (OUT::kSize == 0) {
+    // what lies behind the last block of a row: codes and scales of blocks past C, and the end
+    if (c_end == p.C) {
+      const int blocks = (p.C + 31) / 32, codes = p.channel_groups * kMxGroupBytes;
+      const int tail = codes + blocks, tail_end = (int)p.mx4_bytes;
+      for (int at = first; at < px_end - px0; at += stride) {
+        uint8_t *row = out + (size_t)(px0 + at) * p.out_row_bytes;
+        for (int b = blocks * 16 + v * 4; b < codes; b += V * 4) *reinterpret_cast<uint32_t *>(row + b) = 0;
+        for (int b = tail + v; b < tail_end; b += V) row[b] = 0;
+      }
+    }
+  }
+}
+
+// Groups too wide for a workgroup's lanes: a workgroup finds a group's mean and squares in
+// two passes over it, then sixteen lanes take 128 channels of a pixel.
+constexpr int kGnWideThreads = 256;
 
 __device__ __forceinline__ float block_sum(float v, float *s_part) {
 #pragma unroll
@@ -34,45 +314,38 @@ __device__ __forceinline__ float block_sum(float v, float *s_part) {
   __syncthreads();
   float t = 0;
 #pragma unroll
-  for (int w = 0; w < kGnThreads / 64; w++) t += s_part[w];
+  for (int w = 0; w < kGnWideThreads / 64; w++) t += s_part[w];
   return t;
 }
 
 template <class E>
-__global__ __launch_bounds__(kGnThreads) void group_norm_stats_kernel(GroupNorm p) {
-  __shared__ float s_part[kGnThreads / 64];
+__global__ __launch_bounds__(kGnWideThreads) void group_norm_wide_stats_kernel(GroupNorm p) {
+  __shared__ float s_part[kGnWideThreads / 64];
   const int group = (int)(blockIdx.x % (unsigned)p.groups);
   const size_t sample = blockIdx.x / (unsigned)p.groups;
   const uint8_t *base = p.in + sample * p.pixels * p.in_row_bytes + (size_t)group * p.per * E::kSize;
-  const long long n = (long long)p.pixels * p.per;
-  auto value = [&](long long i) {
-    return E::to(reinterpret_cast<const typename E::T *>(base + (size_t)(i / p.per) * p.in_row_bytes)[i % p.per]);
+  const float n = (float)p.pixels * (float)p.per;
+  auto each = [&](auto &&f) {
+    for (int px = 0; px < p.pixels; px++) {
+      const typename E::T *row = reinterpret_cast<const typename E::T *>(base + (size_t)px * p.in_row_bytes);
+      for (int i = threadIdx.x; i < p.per; i += kGnWideThreads) f(E::to(row[i]));
+    }
   };
   float sum = 0;
-  for (long long i = threadIdx.x; i < n; i += kGnThreads) sum += value(i);
-  const float mean = block_sum(sum, s_part) / (float)n;
+  each([&](float x) { sum += x; });
+  const float mean = block_sum(sum, s_part) / n;
   float square = 0;
-  for (long long i = threadIdx.x; i < n; i += kGnThreads) {
-    const float d = value(i) - mean;
-    square = fmaf(d, d, square);
-  }
-  const float var = block_sum(square, s_part) / (float)n;
-  if (threadIdx.x == 0) p.stats[blockIdx.x] = GroupStats{mean, 1.0f / sqrtf(var + p.epsilon)};
-}
-
-__device__ __forceinline__ float gn_act(float v, int act) {
-  if (act == MI355X_ACT_RELU) return v < 0 ? 0.0f : v;     // (NaN stays)
-  if (act == MI355X_ACT_SILU) return v / (1.0f + expf(-v));
-  return v;
+  each([&](float x) { square = fmaf(x - mean, x - mean, square); });
+  square = block_sum(square, s_part);
+  if (threadIdx.x == 0) p.stats[blockIdx.x] = GroupStats{mean, 1.0f / sqrtf(square / n + p.epsilon)};
 }
 
 template <class E, class OUT>
-__global__ __launch_bounds__(kGnThreads) void group_norm_apply_kernel(GroupNorm p, int channel_groups,
-                                                                      unsigned long long units) {
+__global__ __launch_bounds__(kGnWideThreads) void group_norm_wide_apply_kernel(GroupNorm p, unsigned long long units) {
   const int l = threadIdx.x & 15;
   for (unsigned long long u = blockIdx.x * 16ull + (threadIdx.x >> 4); u < units; u += gridDim.x * 16ull) {
-    const size_t row = u / (unsigned)channel_groups;
-    const int g = (int)(u % (unsigned)channel_groups), c = g * kMxGroup + l * 8;
+    const size_t row = u / (unsigned)p.channel_groups;
+    const int g = (int)(u % (unsigned)p.channel_groups), c = g * kMxGroup + l * 8;
     const typename E::T *in = reinterpret_cast<const typename E::T *>(p.in + row * p.in_row_bytes) + c;
     const int left = p.C - c;
     float x[8];
@@ -83,14 +356,13 @@ __global__ __launch_bounds__(kGnThreads) void group_norm_apply_kernel(GroupNorm 
     for (int j = 0; j < 8; j++) {
       if (j < left) {
         const GroupStats s = stats[(c + j) / p.per];
-        float y = (x[j] - s.mean) * s.scale;
-        y = fmaf(y, p.gamma ? p.gamma[c + j] : 1.0f, p.beta ? p.beta[c + j] : 0.0f);
-        x[j] = gn_act(y, p.act);
+        x[j] = activate(fmaf(x[j] - s.mean, s.square * (p.gamma ? p.gamma[c + j] : 1.0f), p.beta ? p.beta[c + j] : 0.0f),
+                        p.act);
       }
     }
     uint8_t *out = p.out + row * p.out_row_bytes;
     if constexpr (OUT::kSize == 0) {
-      mx4_store_group(out, channel_groups, g, l, x);
+      mx4_store_group(out, p.channel_groups, g, l, x);
     } else if (left > 0) {
       typename OUT::T *o = reinterpret_cast<typename OUT::T *>(out) + c;
       if (left >= 8) store8<OUT>(o, x);
@@ -99,16 +371,133 @@ __global__ __launch_bounds__(kGnThreads) void group_norm_apply_kernel(GroupNorm 
   }
 }
 
-template <class E>
-static int group_norm_launch(const GroupNorm &p, size_t N, bool mx4, hipStream_t st) {
-  group_norm_stats_kernel<E><<<(unsigned)(N * p.groups), kGnThreads, 0, st>>>(p);
-  if (int rc = check_launch("group_norm")) return rc;
-  const int channel_groups = (int)mx4_groups((size_t)p.C);
-  const unsigned long long units = (unsigned long long)p.rows * channel_groups;
-  const unsigned blocks = (unsigned)(units / 16 + 1 < 65536 ? units / 16 + 1 : 65536);
-  if (mx4) group_norm_apply_kernel<E, MX4><<<blocks, kGnThreads, 0, st>>>(p, channel_groups, units);
-  else group_norm_apply_kernel<E, E><<<blocks, kGnThreads, 0, st>>>(p, channel_groups, units);
+// ---- how a call is cut -------------------------------------------------------------
+
+// Parts of a slice: enough for four workgroups a CU over the whole call.
+static int gn_most_chunks(size_t N, size_t pixels) {
+  const size_t n = N < 1024 ? 1024 / N : 1;
+  return (int)std::min<size_t>({n, pixels, (size_t)kGnMostChunks});
+}
+
+struct GnPlan {
+  bool wide, resident;
+  int threads, regs;      // pixels a thread holds at a time
+};
+static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
+  GnPlan plan{};
+  // a slice that is written as blocks begins with one
+  int unit = 1;
+  if (mx4)
+    while (unit < 32 && (long long)unit * p.per % 32) unit *= 2;
+  unit = std::min(unit, p.groups);
+  int k = unit;
+  while (k < p.groups && (long long)k * p.per * size < 128) k = std::min(k + unit, p.groups);
+  auto set = [&](int groups) {
+    p.in_slice = groups;
+    p.width = (int)std::min<long long>((long long)groups * p.per, 0x7fffffff);
+    p.slices = (p.groups + groups - 1) / groups;
+    p.lg_vec = mx4 ? 2 : 0;
+    while (p.lg_vec < 11 && (8 << p.lg_vec) < p.width) p.lg_vec++;
+  };
+  set(k);
+  if (p.lg_vec > 10) {
+    plan.wide = true;
+    return plan;
+  }
+  // (sixteen of 16 bits with eight channels' sums each spill registers)
+  const int most_regs = size == 4 || p.per % 8 ? 8 : 16;
+  auto fits = [&] { return p.pixels <= (long long)(kGnMost >> p.lg_vec) * most_regs; };
+  // narrower slices where they are too few for the chip, or too large for a workgroup
+  const int whole = k;
+  while (k > unit && ((long long)N * p.slices < 256 || !fits())) {
+    k = std::max(unit, k / 2 / unit * unit);
+    set(k);
+  }
+  plan.resident = fits() && ((long long)N * p.slices >= 128 || (long long)p.pixels * p.width * size <= 65536);
+  if (plan.resident) {
+    // few pixels a thread as long as the workgroup is small, so that several share a CU
+    plan.threads = std::max(64, 1 << p.lg_vec);
+    plan.regs = 1;
+    auto holds = [&] { return (long long)(plan.threads >> p.lg_vec) * plan.regs; };
+    while (holds() < p.pixels) {
+      if (plan.regs < 4 || plan.threads >= kGnMost) plan.regs *= 2;
+      else plan.threads *= 2;
+    }
+    p.chunks = 1;
+    p.chunk_pixels = p.pixels;
+    return plan;
+  }
+  set(whole);
+  plan.threads = std::max(256, 1 << p.lg_vec);
+  plan.regs = 4;
+  const int stride = plan.threads >> p.lg_vec;
+  const int chunks = std::max(1, std::min<int>(gn_most_chunks(N, (size_t)p.pixels),
+                                               (int)(1024 / std::min<long long>(1024, (long long)N * p.slices))));
+  p.chunk_pixels = (int)std::min<long long>(p.pixels, ((long long)p.pixels + (long long)chunks * stride - 1) /
+                                                          ((long long)chunks * stride) * stride);
+  p.chunks = (p.pixels + p.chunk_pixels - 1) / p.chunk_pixels;
+  return plan;
+}
+
+template <class E, class OUT, int R, int MODE, int NV>
+static int gn_launch_one(const GroupNorm &p, const GnPlan &plan, hipStream_t st) {
+  const int V = 1 << p.lg_vec;
+  const int rows = V < 64 ? plan.threads / 64 : plan.threads >> p.lg_vec;
+  const size_t lds = (2 * (size_t)p.in_slice + (MODE == kGnApply ? 0 : (size_t)rows * V * NV)) * 4;
+  const size_t sets = (size_t)(p.by_die ? (p.samples + 7) / 8 * 8 : p.samples) * p.slices * p.chunks;
+  group_norm_kernel<E, OUT, R, MODE, NV><<<(unsigned)sets, plan.threads, lds, st>>>(p);
   return check_launch("group_norm");
+}
+template <class E, class OUT, int MODE, int NV>
+static int gn_launch_regs(const GroupNorm &p, const GnPlan &plan, hipStream_t st) {
+  if constexpr (MODE != kGnResident) return gn_launch_one<E, OUT, 4, MODE, NV>(p, plan, st);
+  else {
+    if (plan.regs == 1) return gn_launch_one<E, OUT, 1, MODE, NV>(p, plan, st);
+    if (plan.regs == 2) return gn_launch_one<E, OUT, 2, MODE, NV>(p, plan, st);
+    if (plan.regs == 4) return gn_launch_one<E, OUT, 4, MODE, NV>(p, plan, st);
+    if constexpr (E::kSize == 2 && NV == 1)
+      if (plan.regs == 16) return gn_launch_one<E, OUT, 16, MODE, NV>(p, plan, st);
+    return gn_launch_one<E, OUT, 8, MODE, NV>(p, plan, st);
+  }
+}
+template <class E, class OUT, int NV>
+static int gn_launch_as(const GroupNorm &p, const GnPlan &plan, hipStream_t st) {
+  if (plan.resident) return gn_launch_regs<E, OUT, kGnResident, NV>(p, plan, st);
+  // (the first launch does not depend on the result's type)
+  if (int rc = gn_launch_regs<E, E, kGnStats, NV>(p, plan, st)) return rc;
+  return gn_launch_regs<E, OUT, kGnApply, NV>(p, plan, st);
+}
+template <class E, class OUT>
+static int gn_launch(GroupNorm p, size_t N, hipStream_t st) {
+  const GnPlan plan = gn_plan(p, N, E::kSize, OUT::kSize == 0);
+  // 2^32 threads are a launch's limit: more samples than that go in turns
+  const size_t per_sample = plan.wide ? (size_t)p.groups * kGnWideThreads
+                                      : (size_t)p.slices * p.chunks * plan.threads;
+  const size_t most = std::max<size_t>(1, 0xf0000000ull / per_sample / 8 * 8);
+  const uint8_t *in = p.in;
+  uint8_t *out = p.out;
+  for (size_t done = 0; done < N; done += most) {
+    p.samples = (int)std::min(most, N - done);
+    p.in = in + done * p.pixels * p.in_row_bytes;
+    p.out = out + done * p.pixels * p.out_row_bytes;
+    int rc;
+    if (plan.wide) {
+      group_norm_wide_stats_kernel<E><<<(unsigned)((size_t)p.samples * p.groups), kGnWideThreads, 0, st>>>(p);
+      if ((rc = check_launch("group_norm"))) return rc;
+      const unsigned long long units = (unsigned long long)p.samples * p.pixels * p.channel_groups;
+      const unsigned blocks = (unsigned)std::min<unsigned long long>(units / 16 + 1, 65536);
+      group_norm_wide_apply_kernel<E, OUT><<<blocks, kGnWideThreads, 0, st>>>(p, units);
+      rc = check_launch("group_norm");
+    } else {
+      // slices of a sample share lines where they are narrower than 128 bytes, or rows do not
+      // start on one: they go to one die, whose L2 then has the line whole
+      p.by_die = plan.resident && p.slices > 1 && p.samples >= 64;
+      // eight channels of a vector lie in one group where groups are made of such vectors
+      rc = p.per % 8 == 0 ? gn_launch_as<E, OUT, 1>(p, plan, st) : gn_launch_as<E, OUT, 8>(p, plan, st);
+    }
+    if (rc) return rc;
+  }
+  return MI355X_OK;
 }
 
 } // namespace mi355x
@@ -126,10 +515,7 @@ int mi355x_group_norm_workspace_bytes(size_t N, size_t pixels, size_t C, size_t 
     *bytes = 0;
     return MI355X_OK;
   }
-  if (N * groups > (1u << 23))
-    return fail(MI355X_ERR_NOT_SUPPORTED, "group_norm: %zu samples of %zu groups, up to 2^23 in all are supported", N,
-                groups);
-  *bytes = N * groups * sizeof(GroupStats);
+  *bytes = N * groups * gn_most_chunks(N, pixels) * sizeof(GroupStats);
   return MI355X_OK;
 }
 
@@ -163,7 +549,7 @@ int mi355x_group_norm(void *out, int out_type, size_t out_row_bytes, const void 
   MI355X_REQUIRE(!overlaps(workspace, need, out, out_span) && !overlaps(workspace, need, in, in_span) &&
                      !overlaps(workspace, need, gamma, 4 * C) && !overlaps(workspace, need, beta, 4 * C),
                  "group_norm: the workspace overlaps a tensor");
-  GroupNorm p;
+  GroupNorm p{};
   p.out = static_cast<uint8_t *>(out);
   p.in = static_cast<const uint8_t *>(in);
   p.out_row_bytes = out_row_bytes;
@@ -171,18 +557,19 @@ int mi355x_group_norm(void *out, int out_type, size_t out_row_bytes, const void 
   p.gamma = gamma;
   p.beta = beta;
   p.stats = static_cast<GroupStats *>(workspace);
-  p.rows = (long long)(N * pixels);
   p.pixels = (int)pixels;
   p.C = (int)C;
   p.groups = (int)groups;
   p.per = (int)(C / groups);
   p.epsilon = epsilon;
   p.act = activation;
+  p.channel_groups = (int)mx4_groups(C);
+  p.mx4_bytes = mx4_row_bytes_of(C);
   hipStream_t st = as_stream(stream);
   const bool mx4 = out_type == MI355X_MX4;
-  if (in_type == MI355X_F32) return group_norm_launch<F32>(p, N, mx4, st);
-  if (in_type == MI355X_F16) return group_norm_launch<F16>(p, N, mx4, st);
-  return group_norm_launch<BF16>(p, N, mx4, st);
+  if (in_type == MI355X_F32) return mx4 ? gn_launch<F32, MX4>(p, N, st) : gn_launch<F32, F32>(p, N, st);
+  if (in_type == MI355X_F16) return mx4 ? gn_launch<F16, MX4>(p, N, st) : gn_launch<F16, F16>(p, N, st);
+  return mx4 ? gn_launch<BF16, MX4>(p, N, st) : gn_launch<BF16, BF16>(p, N, st);
 }
 
 } // extern "C"

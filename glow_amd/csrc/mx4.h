@@ -10,57 +10,104 @@ namespace mi355x {
 
 // ---- element types ---------------------------------------------------------------
 
+// E::Eight: eight neighbouring values in the registers they fill, from any address that is
+// one of an element (loads of sixteen bytes need no more alignment than that).
+typedef float mx_v8f __attribute__((ext_vector_type(8)));
+typedef _Float16 mx_v8h __attribute__((ext_vector_type(8)));
+typedef uint32_t mx_v4u __attribute__((ext_vector_type(4)));
+
 struct F32 {
   typedef float T;
+  typedef mx_v8f Eight;
+  typedef Eight Eight1 __attribute__((aligned(4)));
   static constexpr int kSize = 4;
   static __device__ __forceinline__ float to(float v) { return v; }
   static __device__ __forceinline__ float from(float v) { return v; }
+  static __device__ __forceinline__ float get(const Eight &e, int j) { return e[j]; }
+  static __device__ __forceinline__ Eight put(const float (&x)[8]) {
+    return Eight{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+  }
 };
 struct F16 {
   typedef _Float16 T;
+  typedef mx_v8h Eight;
+  typedef Eight Eight1 __attribute__((aligned(2)));
   static constexpr int kSize = 2;
   static __device__ __forceinline__ float to(_Float16 v) { return (float)v; }
   static __device__ __forceinline__ _Float16 from(float v) { return (_Float16)v; }
+  static __device__ __forceinline__ float get(const Eight &e, int j) { return (float)e[j]; }
+  static __device__ __forceinline__ Eight put(const float (&x)[8]) {
+    Eight e;
+#pragma unroll
+    for (int j = 0; j < 8; j++) e[j] = (_Float16)x[j];
+    return e;
+  }
 };
 struct BF16 {
   typedef __bf16 T;
+  typedef mx_v4u Eight;                     // a value is the upper half of its float's bits
+  typedef Eight Eight1 __attribute__((aligned(2)));
   static constexpr int kSize = 2;
   static __device__ __forceinline__ float to(__bf16 v) { return (float)v; }
   static __device__ __forceinline__ __bf16 from(float v) { return (__bf16)v; }
+  static __device__ __forceinline__ float get(const Eight &e, int j) {
+    return __uint_as_float(j & 1 ? e[j >> 1] & 0xffff0000u : e[j >> 1] << 16);
+  }
+  static __device__ __forceinline__ Eight put(const float (&x)[8]) {
+    typedef __bf16 Two __attribute__((ext_vector_type(2)));
+    Eight e;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      e[j] = __builtin_bit_cast(uint32_t, Two{(__bf16)x[2 * j], (__bf16)x[2 * j + 1]});
+    return e;
+  }
 };
 struct MX4 {
   typedef uint8_t T;
   static constexpr int kSize = 0;
 };
 
-// Eight neighbouring values from any address that is one of an element: loads of sixteen
-// bytes need no more alignment than that.
-template <class E> struct __attribute__((packed, aligned(E::kSize))) Eight { typename E::T v[8]; };
-
-template <class E>
-__device__ __forceinline__ void load8(float (&x)[8], const typename E::T *p) {
-  const Eight<E> e = *reinterpret_cast<const Eight<E> *>(p);
-#pragma unroll
-  for (int j = 0; j < 8; j++) x[j] = E::to(e.v[j]);
+template <class E> __device__ __forceinline__ typename E::Eight load_eight(const typename E::T *p) {
+  return *reinterpret_cast<const typename E::Eight1 *>(p);
 }
-// The same at the end of a row: `left` values, zeros behind them.
-template <class E>
-__device__ __forceinline__ void load8_end(float (&x)[8], const typename E::T *p, int left) {
+// The same at the end of a row: `left` values (none where it is not positive), zeros behind.
+template <class E> __device__ __forceinline__ typename E::Eight load_eight_end(const typename E::T *p, int left) {
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = j < left ? E::to(p[j]) : 0.0f;
+  return E::put(x);                          // (exact: the values are of the type)
+}
+template <class E> __device__ __forceinline__ void load8(float (&x)[8], const typename E::T *p) {
+  const typename E::Eight e = load_eight<E>(p);
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = E::get(e, j);
+}
+template <class E> __device__ __forceinline__ void load8_end(float (&x)[8], const typename E::T *p, int left) {
 #pragma unroll
   for (int j = 0; j < 8; j++) x[j] = j < left ? E::to(p[j]) : 0.0f;
 }
-template <class E>
-__device__ __forceinline__ void store8(typename E::T *p, const float (&x)[8]) {
-  Eight<E> e;
-#pragma unroll
-  for (int j = 0; j < 8; j++) e.v[j] = E::from(x[j]);
-  *reinterpret_cast<Eight<E> *>(p) = e;
+template <class E> __device__ __forceinline__ void store8(typename E::T *p, const float (&x)[8]) {
+  *reinterpret_cast<typename E::Eight1 *>(p) = E::put(x);
 }
 template <class E>
 __device__ __forceinline__ void store8_end(typename E::T *p, const float (&x)[8], int left) {
 #pragma unroll
   for (int j = 0; j < 8; j++)
     if (j < left) p[j] = E::from(x[j]);
+}
+
+// v / (1 + exp(-v)) with the hardware's exp2 and reciprocal: off by |v| + 4 steps of 2^-24 at
+// most, next to nothing beside a 16- or 4-bit result's own rounding, and two instructions
+// for the twenty of a correctly rounded quotient. exp2's infinity for v below -88 gives -0.
+__device__ __forceinline__ float silu(float v) {
+  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
+__device__ __forceinline__ float relu(float v) { return v < 0 ? 0.0f : v; } // NaN stays
+template <int ACT> __device__ __forceinline__ float activate(float v) {
+  return ACT == MI355X_ACT_RELU ? relu(v) : ACT == MI355X_ACT_SILU ? silu(v) : v;
+}
+__device__ __forceinline__ float activate(float v, int act) {
+  return act == MI355X_ACT_RELU ? relu(v) : act == MI355X_ACT_SILU ? silu(v) : v;
 }
 
 // ---- blocks ------------------------------------------------------------------------

@@ -28,12 +28,6 @@ struct MxFc {
   int act;
 };
 
-__device__ __forceinline__ float fc_act(float v, int act) {
-  if (act == MI355X_ACT_RELU) return v < 0 ? 0.0f : v;     // (NaN stays)
-  if (act == MI355X_ACT_SILU) return v / (1.0f + expf(-v));
-  return v;
-}
-
 // One wave, one 32x32 tile, fragments straight from memory.
 template <class OUT>
 __global__ __launch_bounds__(64) void mx4_fc_kernel(MxFc p, int tiles_n) {
@@ -61,7 +55,7 @@ __global__ __launch_bounds__(64) void mx4_fc_kernel(MxFc p, int tiles_n) {
 #pragma unroll
   for (int i = 0; i < 16; i++) {
     const int n = n0 + 8 * (i >> 2) + 4 * half + (i & 3);
-    acc[i] = n < p.N ? fc_act(acc[i] + (p.bias ? p.bias[n] : 0.0f), p.act) : 0.0f;
+    acc[i] = n < p.N ? activate(acc[i] + (p.bias ? p.bias[n] : 0.0f), p.act) : 0.0f;
   }
   uint8_t *out = p.out + (size_t)m * p.out_row_bytes;
   if constexpr (OUT::kSize == 0) {
