@@ -281,9 +281,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
     }
   };
   for (int from = px0;;) {
-    if (p.act == MI355X_ACT_RELU) write(from, std::integral_constant<int, MI355X_ACT_RELU>());
-    else if (p.act == MI355X_ACT_SILU) write(from, std::integral_constant<int, MI355X_ACT_SILU>());
-    else write(from, std::integral_constant<int, MI355X_ACT_NONE>());
+    with_activation(p.act, [&](auto act) { write(from, act); });
     if (MODE == kGnResident || px_end - from <= block) break;
     from += block;
     load(from);
@@ -352,17 +350,19 @@ __global__ __launch_bounds__(kGnWideThreads) void group_norm_wide_apply_kernel(G
     if (left >= 8) load8<E>(x, in);
     else load8_end<E>(x, in, left);
     const GroupStats *stats = p.stats + row / (unsigned)p.pixels * p.groups;
+    with_activation(p.act, [&](auto act) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      if (j < left) {
-        const GroupStats s = stats[(c + j) / p.per];
-        x[j] = activate(fmaf(x[j] - s.mean, s.square * (p.gamma ? p.gamma[c + j] : 1.0f), p.beta ? p.beta[c + j] : 0.0f),
-                        p.act);
+      for (int j = 0; j < 8; j++) {
+        if (j < left) {
+          const GroupStats s = stats[(c + j) / p.per];
+          x[j] = activate<decltype(act)::value>(fmaf(x[j] - s.mean, s.square * (p.gamma ? p.gamma[c + j] : 1.0f),
+                                                     p.beta ? p.beta[c + j] : 0.0f));
+        }
       }
-    }
+    });
     uint8_t *out = p.out + row * p.out_row_bytes;
     if constexpr (OUT::kSize == 0) {
-      mx4_store_group(out, p.channel_groups, g, l, x);
+      mx4_store_group<F32>(out, p.channel_groups, g, l, F32::put(x));
     } else if (left > 0) {
       typename OUT::T *o = reinterpret_cast<typename OUT::T *>(out) + c;
       if (left >= 8) store8<OUT>(o, x);

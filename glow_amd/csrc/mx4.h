@@ -6,6 +6,8 @@
 #include "common.h"
 #include "mx4_layout.h"
 
+#include <type_traits>
+
 namespace mi355x {
 
 // ---- element types ---------------------------------------------------------------
@@ -36,6 +38,17 @@ struct F16 {
   static __device__ __forceinline__ float to(_Float16 v) { return (float)v; }
   static __device__ __forceinline__ _Float16 from(float v) { return (_Float16)v; }
   static __device__ __forceinline__ float get(const Eight &e, int j) { return (float)e[j]; }
+  // magnitudes of a pair as a word of whole numbers, and the float's bits of one of them
+  static __device__ __forceinline__ uint32_t pair(const Eight &e, int i) {
+    return __builtin_bit_cast(mx_v4u, e)[i];
+  }
+  static __device__ __forceinline__ uint32_t float_bits(uint32_t half) {
+    return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)half));
+  }
+  template <int SEL> static __device__ __forceinline__ uint32_t codes2(uint32_t old, uint32_t two, float scale) {
+    typedef _Float16 Two __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(Two, two), scale, SEL);
+  }
   static __device__ __forceinline__ Eight put(const float (&x)[8]) {
     Eight e;
 #pragma unroll
@@ -52,6 +65,12 @@ struct BF16 {
   static __device__ __forceinline__ __bf16 from(float v) { return (__bf16)v; }
   static __device__ __forceinline__ float get(const Eight &e, int j) {
     return __uint_as_float(j & 1 ? e[j >> 1] & 0xffff0000u : e[j >> 1] << 16);
+  }
+  static __device__ __forceinline__ uint32_t pair(const Eight &e, int i) { return e[i]; }
+  static __device__ __forceinline__ uint32_t float_bits(uint32_t half) { return half << 16; }
+  template <int SEL> static __device__ __forceinline__ uint32_t codes2(uint32_t old, uint32_t two, float scale) {
+    typedef __bf16 Two __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(Two, two), scale, SEL);
   }
   static __device__ __forceinline__ Eight put(const float (&x)[8]) {
     typedef __bf16 Two __attribute__((ext_vector_type(2)));
@@ -106,8 +125,13 @@ __device__ __forceinline__ float relu(float v) { return v < 0 ? 0.0f : v; } // N
 template <int ACT> __device__ __forceinline__ float activate(float v) {
   return ACT == MI355X_ACT_RELU ? relu(v) : ACT == MI355X_ACT_SILU ? silu(v) : v;
 }
-__device__ __forceinline__ float activate(float v, int act) {
-  return act == MI355X_ACT_RELU ? relu(v) : act == MI355X_ACT_SILU ? silu(v) : v;
+// f(std::integral_constant<int, ACT>) of the activation: the choice is made once, outside of
+// loops (inside one the compiler computes all of them for every value: 8 of 17 us of a
+// 256x256 tile without a K loop).
+template <class F> __device__ __forceinline__ void with_activation(int act, F &&f) {
+  if (act == MI355X_ACT_RELU) f(std::integral_constant<int, MI355X_ACT_RELU>());
+  else if (act == MI355X_ACT_SILU) f(std::integral_constant<int, MI355X_ACT_SILU>());
+  else f(std::integral_constant<int, MI355X_ACT_NONE>());
 }
 
 // ---- blocks ------------------------------------------------------------------------
@@ -143,6 +167,45 @@ __device__ __forceinline__ uint32_t mx4_codes8(const float (&x)[8], uint32_t byt
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
   return byte == 255 ? 0 : w;
 }
+// The same of eight values in their own type's registers. 16-bit types are never widened: the
+// largest magnitude is found two values at a time and the conversion takes pairs (half the
+// instructions of the way through floats).
+template <class E> __device__ __forceinline__ uint32_t largest8(const typename E::Eight &e) {
+  if constexpr (E::kSize == 4) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) m = max(m, magnitude_bits(e[j]));
+    return m;
+  } else {
+    typedef uint16_t Two __attribute__((ext_vector_type(2)));
+    Two m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(Two, E::pair(e, i) & 0x7fff7fffu));
+    return max((uint32_t)m[0], (uint32_t)m[1]);
+  }
+}
+// What largest8 gives as a float's bits (16-bit types: after the maximum over the block).
+template <class E> __device__ __forceinline__ uint32_t largest_bits(uint32_t m) {
+  if constexpr (E::kSize == 4) return m;
+  else return E::float_bits(m);
+}
+template <class E> __device__ __forceinline__ uint32_t mx4_codes8_of(const typename E::Eight &e, uint32_t byte) {
+  uint32_t w = 0;
+  const float s = mx4_scale(byte);
+  if constexpr (E::kSize == 4) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, e[0], e[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, e[2], e[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, e[4], e[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, e[6], e[7], s, 3);
+  } else {
+    w = E::template codes2<0>(w, E::pair(e, 0), s);
+    w = E::template codes2<1>(w, E::pair(e, 1), s);
+    w = E::template codes2<2>(w, E::pair(e, 2), s);
+    w = E::template codes2<3>(w, E::pair(e, 3), s);
+  }
+  return byte == 255 ? 0 : w;
+}
 typedef float mx4_v2f __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void mx4_values8(float (&x)[8], uint32_t codes, uint32_t byte) {
   const float s = mx4_scale(byte);
@@ -167,10 +230,11 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t m) {
 
 // A group's sixteen lanes, eight columns each, write it: codes, the word of scales, and
 // behind the last group the zeros that fill the row up. `l` is the lane of the group.
+template <class E>
 __device__ __forceinline__ void mx4_store_group(uint8_t *row, int groups, int g, int l,
-                                                const float (&x)[8]) {
-  const uint32_t byte = mx4_scale_byte(quad_max(largest8(x)));
-  reinterpret_cast<uint32_t *>(row + (size_t)g * kMxGroupBytes)[l] = mx4_codes8(x, byte);
+                                                const typename E::Eight &x) {
+  const uint32_t byte = mx4_scale_byte(largest_bits<E>(quad_max(largest8<E>(x))));
+  reinterpret_cast<uint32_t *>(row + (size_t)g * kMxGroupBytes)[l] = mx4_codes8_of<E>(x, byte);
   // lanes 0, 4, 8, 12 hold the four scales: each lane's byte in its place, joined by or
   uint32_t word = (l & 3) == 0 ? byte << (8 * (l >> 2)) : 0;
   word |= (uint32_t)__builtin_amdgcn_mov_dpp((int)word, 0x124, 0xf, 0xf, true); // row_ror:4

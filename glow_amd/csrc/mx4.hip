@@ -56,10 +56,10 @@ __global__ __launch_bounds__(kMxThreads) void mx4_quantize_kernel(uint8_t *dst, 
     if (!p.inside) continue;                       // whole groups: their sixteen lanes stay together
     const typename E::T *row = reinterpret_cast<const typename E::T *>(src + (size_t)p.row * src_row_bytes);
     const int c = p.group * kMxGroup + p.l * 8;
-    float x[8];
-    if (c <= r.cols - 8) load8<E>(x, row + c);
-    else load8_end<E>(x, row + c, r.cols - c);
-    mx4_store_group(dst + (size_t)p.row * dst_row_bytes, r.groups, p.group, p.l, x);
+    typename E::Eight x;
+    if (c <= r.cols - 8) x = load_eight<E>(row + c);
+    else x = load_eight_end<E>(row + c, r.cols - c);
+    mx4_store_group<E>(dst + (size_t)p.row * dst_row_bytes, r.groups, p.group, p.l, x);
   }
 }
 

@@ -5,18 +5,59 @@
 // and products are summed in 32 bits. The weights are the first operand, so that a lane's
 // results belong to one row of the output and lie in fours of neighbouring columns: what a
 // microscaled result's blocks and wide stores want.
+#include "mx4_small.h"
 #include "mx4_tiles.h"
 
 namespace mi355x {
 
-template <class OUT>
-static int fc_launch(const MxFc &p, hipStream_t st) {
-  const long long n = p.N, m = p.M;
-  if (((n + 255) / 256) * ((m + 255) / 256) >= 192)
-    return mx4_fc_tile_launch<OUT, 256, 256, 128, 64, 4, 1>(p, st);
-  if (((n + 127) / 128) * ((m + 127) / 128) >= 192)
-    return mx4_fc_tile_launch<OUT, 128, 128, 64, 64, 4, 2>(p, st);
-  return mx4_fc_tile_launch<OUT, 64, 64, 32, 32, 4, 4>(p, st);
+// Which kernel a product runs: small tiles of 16 or 32 rows and columns with K over the waves
+// (mx4_small.h) while they give each CU one workgroup or less, the smallest that do; else tiles
+// of 64 to 256 through LDS. us, 16x16 / 32x16 / 32x32 / 64x64 tiles, fp16 results: 1 x 4096 x
+// 4096 4.4 / - / - / 11.4, 500 x 512 x 512 3.8 / 3.3 / 3.4 / 4.2, 256 x 2048 x 1024 7.9 / 6.6 /
+// 5.6 / 7.4, 64 x 4096 x 8192 34 / 24 / 18 / 11.5 (rows x K x columns). Up to four rows 16x16
+// holds its own over any number of columns (1 x 4096 x 16384 10.9 / 11.9): the input is next
+// to nothing then.
+enum FcTile { kFc16, kFc32x16, kFc32, kFc64, kFc128, kFc256 };
+static FcTile fc_tile(long long M, long long N, bool mx4_out) {
+  const long long most = 288;
+  const long long m16 = (M + 15) / 16, m32 = (M + 31) / 32, n16 = (N + 15) / 16, n32 = (N + 31) / 32;
+  if (mx4_out) {                   // a microscaled result's columns go by blocks of 32
+    if (m16 * n32 <= most || M <= 4) return kFc16;
+  } else {
+    if (m16 * n16 <= most || M <= 4) return kFc16;
+    if (m32 * n16 <= most) return kFc32x16;
+  }
+  if (m32 * n32 <= most) return kFc32;
+  if (((N + 255) / 256) * ((M + 255) / 256) >= 192) return kFc256;
+  if (((N + 127) / 128) * ((M + 127) / 128) >= 192) return kFc128;
+  return kFc64;
+}
+// Whether a float input is quantised by the kernel itself: every workgroup does so for its rows,
+// which a launch in front saves where they are many bytes. us, in the kernel / in front: 128 x
+// 1024 x 1024 of fp16 4.9 / 5.6 (64 KB of rows), 16 x 4096 x 4096 8.6 / 8.3 (128 KB), 64 x 4096 x
+// 4096 15.3 / 12.3 (256 KB), 61 x 415 x 509 of fp32 3.5 / 5.0.
+static bool fc_quantizes(FcTile tile, long long M, long long K, size_t size) {
+  return tile <= kFc32 && std::min(M, tile == kFc16 ? 16LL : 32LL) * K * (long long)size <= 96 * 1024;
+}
+
+template <class IN, class OUT> static int fc_small(const MxFc &p, int K, FcTile tile, hipStream_t st) {
+  if constexpr (OUT::kSize == 0) {
+    return tile == kFc16 ? mx4_fc_small_launch<IN, OUT, 1, 2>(p, K, st) : mx4_fc_small_launch<IN, OUT, 2, 2>(p, K, st);
+  } else {
+    return tile == kFc16      ? mx4_fc_small_launch<IN, OUT, 1, 1>(p, K, st)
+           : tile == kFc32x16 ? mx4_fc_small_launch<IN, OUT, 2, 1>(p, K, st)
+                              : mx4_fc_small_launch<IN, OUT, 2, 2>(p, K, st);
+  }
+}
+template <class OUT> static int fc_launch(const MxFc &p, int K, int in_type, FcTile tile, hipStream_t st) {
+  if (tile <= kFc32)
+    return in_type == MI355X_F32   ? fc_small<F32, OUT>(p, K, tile, st)
+           : in_type == MI355X_F16 ? fc_small<F16, OUT>(p, K, tile, st)
+           : in_type == MI355X_BF16 ? fc_small<BF16, OUT>(p, K, tile, st)
+                                    : fc_small<MX4, OUT>(p, K, tile, st);
+  return tile == kFc256   ? mx4_fc_tile_launch<OUT, 256, 256, 128, 64, 4, 1>(p, st)
+         : tile == kFc128 ? mx4_fc_tile_launch<OUT, 128, 128, 64, 64, 4, 2>(p, st)
+                          : mx4_fc_tile_launch<OUT, 64, 64, 32, 32, 4, 4>(p, st);
 }
 
 } // namespace mi355x
@@ -31,7 +72,12 @@ int mi355x_mx4_fc_workspace_bytes(size_t M, size_t K, size_t N, int in_type, siz
                  in_type);
   MI355X_REQUIRE(M <= 0x7fffffff && K <= 0x7fffffff && N <= 0x7fffffff,
                  "mx4_fc_workspace_bytes: %zu x %zu x %zu, up to 2^31 - 1 each are supported", M, K, N);
-  *bytes = in_type == MI355X_MX4 ? 0 : M * mx4_row_bytes_of(K);
+  *bytes = 0;
+  if (in_type == MI355X_MX4 || !M || !N) return MI355X_OK;
+  // (whatever the result's type)
+  for (bool mx4_out : {false, true})
+    if (!fc_quantizes(fc_tile((long long)M, (long long)N, mx4_out), (long long)M, (long long)K, float_size(in_type)))
+      *bytes = M * mx4_row_bytes_of(K);
   return MI355X_OK;
 }
 
@@ -64,11 +110,16 @@ int mi355x_mx4_fc(void *out, int out_type, size_t out_row_bytes, const void *in,
     MI355X_REQUIRE(!overlaps(workspace, need, out, out_span) && !overlaps(workspace, need, in, in_span) &&
                        !overlaps(workspace, need, weights, w_span) && !overlaps(workspace, need, bias, 4 * N),
                    "mx4_fc: the workspace overlaps a tensor");
+  }
+  const FcTile tile = fc_tile((long long)M, (long long)N, out_type == MI355X_MX4);
+  if (in_type != MI355X_MX4 && !fc_quantizes(tile, (long long)M, (long long)K, float_size(in_type))) {
     p.in = static_cast<const uint8_t *>(workspace);
     p.in_row_bytes = mx4_row_bytes_of(K);
-    if (int rc = mx4_quantize_launch(static_cast<uint8_t *>(workspace), p.in_row_bytes, in, in_type, in_row_bytes, M,
-                                     K, st))
-      return rc;
+    if (K)
+      if (int rc = mx4_quantize_launch(static_cast<uint8_t *>(workspace), p.in_row_bytes, in, in_type, in_row_bytes, M,
+                                       K, st))
+        return rc;
+    in_type = MI355X_MX4;
   }
   p.out = static_cast<uint8_t *>(out);
   p.out_row_bytes = out_row_bytes;
@@ -80,10 +131,11 @@ int mi355x_mx4_fc(void *out, int out_type, size_t out_row_bytes, const void *in,
   p.groups = (int)mx4_groups(K);
   p.out_groups = (int)mx4_groups(N);
   p.act = activation;
-  if (out_type == MI355X_F32) return fc_launch<F32>(p, st);
-  if (out_type == MI355X_F16) return fc_launch<F16>(p, st);
-  if (out_type == MI355X_BF16) return fc_launch<BF16>(p, st);
-  return fc_launch<MX4>(p, st);
+  const int k = (int)K;
+  if (out_type == MI355X_F32) return fc_launch<F32>(p, k, in_type, tile, st);
+  if (out_type == MI355X_F16) return fc_launch<F16>(p, k, in_type, tile, st);
+  if (out_type == MI355X_BF16) return fc_launch<BF16>(p, k, in_type, tile, st);
+  return fc_launch<MX4>(p, k, in_type, tile, st);
 }
 
 } // extern "C"

@@ -211,8 +211,9 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
   __syncthreads();
 
   const int nw = n0 + wn * WN;                     // first column of this wave
+  with_activation(p.act, [&](auto act) {
   auto value = [&](int i, int j, int r) {          // column i * 32 + 16 * half + r of row j * 32 + l32
-    return activate(acc[i][j][r] + s_bias[wn * WN + i * 32 + 16 * half + r], p.act);
+    return activate<decltype(act)::value>(acc[i][j][r] + s_bias[wn * WN + i * 32 + 16 * half + r]);
   };
   if constexpr (OUT::kSize == 0) {
     const int blocks = 4 * p.out_groups;
@@ -284,6 +285,7 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
       wave_fence();
     }
   }
+  });
 }
 
 template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS>

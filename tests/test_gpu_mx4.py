@@ -140,6 +140,30 @@ def test_fc_results_of_every_type(M, K, N, out_type):
         check(capi.mx4_fc(x, ref.MX4, w, None, K, out_type, act), want, err, out_type, N)
 
 
+@pytest.mark.parametrize("out_type", [ref.F32, ref.F16, ref.BF16, ref.MX4])
+@pytest.mark.parametrize("M, K, N", [(1801, 150, 2003), (1793, 1040, 1798), (3201, 160, 4098), (3090, 1300, 3851)])
+def test_fc_of_large_results(M, K, N, out_type):
+    # the tiles of 128 and 256: one step of K and two, an odd count past a group of scales
+    rng = np.random.default_rng(M + out_type)
+    x, a, w = product(rng, M, K, N, ref.MX4)
+    bias = rng.normal(0, 1, N).astype(np.float32)
+    act = (0, 1, 6)[(K + out_type) % 3]
+    want, err = ref.fc(a, ref.values(w, K), bias.astype(np.float64), act)
+    check(capi.mx4_fc(x, ref.MX4, w, bias, K, out_type, act), want, err, out_type, N)
+
+
+@pytest.mark.parametrize("in_type", [ref.F32, ref.F16, ref.BF16])
+@pytest.mark.parametrize("M, K, N", [(1, 4096, 70), (4, 515, 3000), (31, 96, 700), (90, 1050, 290)])
+def test_float_inputs_give_what_their_rows_give(M, K, N, in_type):
+    """Quantised by the product or in front of it: the same bits."""
+    rng = np.random.default_rng(K)
+    x, _, w = product(rng, M, K, N, in_type)
+    rows = capi.mx4_quantize(x, in_type)
+    for out_type in (ref.F32, ref.MX4):
+        np.testing.assert_array_equal(capi.mx4_fc(x, in_type, w, None, K, out_type),
+                                      capi.mx4_fc(rows, ref.MX4, w, None, K, out_type))
+
+
 @pytest.mark.parametrize("M, N", [(1, 40), (20, 200), (300, 300)])
 def test_fc_of_no_columns_is_the_bias(M, N):
     bias = np.linspace(-2, 2, N).astype(np.float32)
