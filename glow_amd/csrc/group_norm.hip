@@ -47,17 +47,23 @@ enum { kGnResident, kGnStats, kGnApply };
 constexpr int kGnMost = 1024;         // threads of a workgroup
 constexpr int kGnMostChunks = 128;    // parts of a slice
 
-// Sums over a slice's pixels and a group's channels, to s_group[0 .. in_slice). x[j] is a
-// thread's sum for channel j of its eight, or x[0] that of all eight where they lie in one
+// Sums over a slice's pixels and a group's channels, to s_group[0 .. in_slice). x[i] is a
+// thread's sum over part i of its eight channels: NV parts, the fewest that each lie in one
 // group. Lanes of a wave that hold the same channels are summed first, then a wave takes a
 // group.
 template <int NV>
 __device__ __forceinline__ void gn_reduce(float (&x)[NV], float *s_part, float *s_group, const GroupNorm &p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
   const int V = 1 << p.lg_vec;
-  for (int d = V; d < 64; d <<= 1)
 #pragma unroll
-    for (int j = 0; j < NV; j++) x[j] += __shfl_xor(x[j], d);
+  for (int j = 0; j < NV; j++) {
+    if (V <= 8) x[j] = add_rotated<8>(x[j]);
+    if (V <= 4) x[j] = add_rotated<4>(x[j]);
+    if (V <= 2) x[j] = add_rotated<2>(x[j]);
+    if (V <= 1) x[j] = add_rotated<1>(x[j]);
+    if (V <= 16) x[j] = add_across16(x[j]);
+    if (V <= 32) x[j] = add_across32(x[j]);
+  }
   const int rows = V < 64 ? waves : (int)blockDim.x >> p.lg_vec;
   __syncthreads();
   if (V >= 64 || lane < V) {
@@ -66,7 +72,7 @@ __device__ __forceinline__ void gn_reduce(float (&x)[NV], float *s_part, float *
     for (int j = 0; j < NV; j++) s_part[((row << p.lg_vec) + (tid & (V - 1))) * NV + j] = x[j];
   }
   __syncthreads();
-  const int len = NV == 1 ? p.per >> 3 : p.per;
+  const int len = p.per / (8 / NV);
   for (int g = wave; g < p.in_slice; g += waves) {
     float t = 0;
     if (len < 64) {
@@ -78,14 +84,39 @@ __device__ __forceinline__ void gn_reduce(float (&x)[NV], float *s_part, float *
       for (int row = 0; row < rows; row++)
         for (int e = lane; e < len; e += 64) t += s_part[(row << p.lg_vec) * NV + g * len + e];
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) t += __shfl_xor(t, d);
+    t = wave_sum(t);
     if (lane == 0) s_group[g] = t;
   }
   __syncthreads();
 }
 
-// Writes one pixel's eight channels.
+// The sum of eight values: of 16-bit types two to an instruction.
+template <class E> __device__ __forceinline__ float gn_sum8(const typename E::Eight &e, float sum) {
+  if constexpr (std::is_same_v<E, F16>) {
+    typedef _Float16 Two __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2(Two{e[2 * i], e[2 * i + 1]}, Two{1, 1}, sum, false);
+  } else if constexpr (std::is_same_v<E, BF16>) {
+    typedef __bf16 Two __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(Two, (uint32_t)e[i]), Two{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) sum += E::get(e, j);
+  }
+  return sum;
+}
+// x - mean of a value; of fp16 one instruction with the widening (`one` hides a factor of 1 that
+// would be taken out of it).
+template <class E> __device__ __forceinline__ float gn_less(const typename E::Eight &e, int j, float mean, float one) {
+  if constexpr (std::is_same_v<E, F16>) return fmaf((float)e[j], one, -mean);
+  else return E::get(e, j) - mean;
+}
+
+// Writes one pixel's eight channels. 32-bit values lose the mean first; of 16-bit ones it is
+// in the shift, which is off by half a step of mean * scale then, less than the values'
+// own rounding.
 template <class E, class OUT, int ACT, int NV>
 __device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, bool block_inside,
                                          const typename E::Eight &raw, const float (&mean)[NV],
@@ -93,7 +124,8 @@ __device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, bool blo
   float y[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    const float v = activate<ACT>(fmaf(E::get(raw, j) - mean[NV == 1 ? 0 : j], scale[j], shift[j]));
+    const float x = E::kSize == 2 ? E::get(raw, j) : E::get(raw, j) - mean[j * NV / 8];
+    const float v = activate<ACT>(fmaf(x, scale[j], shift[j]));
     y[j] = OUT::kSize || j < left ? v : 0.0f;
   }
   if constexpr (OUT::kSize == 0) {
@@ -155,9 +187,19 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
   const float of_group = (float)p.per;
 
   load(px0);
+  // (asked for with the values: the statistics are in between)
+  float scale[8], shift[8];
+  if constexpr (MODE != kGnStats) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      scale[j] = p.gamma && j < left ? p.gamma[c + j] : 1.0f;
+      shift[j] = p.beta && j < left ? p.beta[c + j] : 0.0f;
+    }
+  }
   if constexpr (MODE != kGnApply) {
     // a thread's own count (exact: a part has 2^24 pixels at most), mean and squares
-    float count = 0, mean[NV], square[NV];
+    float count = 0, mean[NV], square[NV], one = 1.0f;
+    asm("" : "+s"(one));
 #pragma unroll
     for (int j = 0; j < NV; j++) mean[j] = square[j] = 0;
     for (int from = px0;;) {
@@ -168,9 +210,13 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
         for (int j = 0; j < NV; j++) m[j] = q[j] = 0;
 #pragma unroll
         for (int i = 0; i < R; i++)
-          if (i < n)
+          if (i < n) {
+            if constexpr (NV == 1) m[0] = gn_sum8<E>(raw[i], m[0]);
+            else {
 #pragma unroll
-            for (int j = 0; j < 8; j++) m[NV == 1 ? 0 : j] += E::get(raw[i], j);
+              for (int j = 0; j < 8; j++) m[j * NV / 8] += E::get(raw[i], j);
+            }
+          }
         const float here = (float)n * (8 / NV), over = 1.0f / here;
 #pragma unroll
         for (int j = 0; j < NV; j++) m[j] *= over;
@@ -179,8 +225,8 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
           if (i < n)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-              const float d = E::get(raw[i], j) - m[NV == 1 ? 0 : j];
-              q[NV == 1 ? 0 : j] = fmaf(d, d, q[NV == 1 ? 0 : j]);
+              const float d = gn_less<E>(raw[i], j, m[j * NV / 8], one);
+              q[j * NV / 8] = fmaf(d, d, q[j * NV / 8]);
             }
         if (MODE == kGnResident || count == 0) {
           count = here;
@@ -208,7 +254,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
     gn_reduce<NV>(x, s_part, s_group, p);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int g = left > 0 ? min((v * 8 + j) / p.per, p.in_slice - 1) : 0;
+      const int g = left > 0 ? min((v * 8 + j * (8 / NV)) / p.per, p.in_slice - 1) : 0;
       const float d = mean[j] - s_group[g] / total;
       x[j] = left > 0 ? fmaf(d * d, count, square[j]) : 0.0f;
     }
@@ -240,17 +286,14 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
         const float n = (float)min(p.chunk_pixels, p.pixels - k * p.chunk_pixels) * of_group;
         if (k < p.chunks) m = fmaf(own[i].mean, n, m);
       }
-#pragma unroll
-      for (int d = 32; d; d >>= 1) m += __shfl_xor(m, d);
-      m /= total;
+      m = wave_sum(m) / total;
 #pragma unroll
       for (int i = 0; i < kGnMostChunks / 64; i++) {
         const int k = lane + 64 * i;
         const float n = (float)min(p.chunk_pixels, p.pixels - k * p.chunk_pixels) * of_group, d = own[i].mean - m;
         if (k < p.chunks) q += fmaf(d * d, n, own[i].square);
       }
-#pragma unroll
-      for (int d = 32; d; d >>= 1) q += __shfl_xor(q, d);
+      q = wave_sum(q);
       if (lane == 0) {
         s_group[g] = m;
         s_second[g] = 1.0f / sqrtf(q / total + p.epsilon);
@@ -259,14 +302,13 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
   }
   __syncthreads();
 
-  float mean[NV], scale[8], shift[8];
+  float mean[NV];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    const bool inside = j < left;
-    const int g = inside ? (v * 8 + j) / p.per : 0;
-    if (NV == 8 || j == 0) mean[NV == 1 ? 0 : j] = s_group[g];
-    scale[j] = s_second[g] * (p.gamma && inside ? p.gamma[c + j] : 1.0f);
-    shift[j] = p.beta && inside ? p.beta[c + j] : 0.0f;
+    const int i = j * NV / 8, g = j < left ? (v * 8 + j) / p.per : 0;
+    if (j % (8 / NV) == 0) mean[i] = s_group[g];
+    scale[j] *= s_second[g];
+    if (E::kSize == 2) shift[j] = fmaf(-mean[i], scale[j], shift[j]);
   }
   uint8_t *out = p.out + (size_t)sample * p.pixels * p.out_row_bytes;
   // microscaled: lanes up to the end of the slice's last block
@@ -305,8 +347,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
 constexpr int kGnWideThreads = 256;
 
 __device__ __forceinline__ float block_sum(float v, float *s_part) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -390,8 +431,10 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
   if (mx4)
     while (unit < 32 && (long long)unit * p.per % 32) unit *= 2;
   unit = std::min(unit, p.groups);
+  // slices that share lines run on one die, whose L2 then has the line whole
+  const bool by_die = N >= 8;
   int k = unit;
-  while (k < p.groups && (long long)k * p.per * size < 128) k = std::min(k + unit, p.groups);
+  while (k < p.groups && (long long)k * p.per * size < (by_die ? 64 : 128)) k = std::min(k + unit, p.groups);
   auto set = [&](int groups) {
     p.in_slice = groups;
     p.width = (int)std::min<long long>((long long)groups * p.per, 0x7fffffff);
@@ -405,34 +448,45 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
     return plan;
   }
   // (sixteen of 16 bits with eight channels' sums each spill registers)
-  const int most_regs = size == 4 || p.per % 8 ? 8 : 16;
+  const int most_regs = size == 4 || p.per % 4 ? 8 : 16;
   auto fits = [&] { return p.pixels <= (long long)(kGnMost >> p.lg_vec) * most_regs; };
-  // narrower slices where they are too few for the chip, or too large for a workgroup
-  const int whole = k;
-  while (k > unit && ((long long)N * p.slices < 256 || !fits())) {
+  // Narrower slices where they are too few for the chip, or too large for a workgroup, down to
+  // 32 bytes: below, as many lines are asked for and less is used of each (64 x 3136 x 256 of
+  // fp16, slices of 64 / 32 / 16 bytes: 53 / 64 / 82 us).
+  const int wide = k;
+  while (k > unit && (long long)(k / 2 / unit * unit) * p.per * size >= 32 && ((long long)N * p.slices < 256 || !fits())) {
     k = std::max(unit, k / 2 / unit * unit);
     set(k);
   }
+  // Few large slices leave most of the chip idle: 1 x 3136 x 256 of fp16 resident in 16 slices 9.8
+  // us, in parts 9.4; 1 x 784 x 512 in 32 slices of 25 KB 6.7, in parts 9.6.
   plan.resident = fits() && ((long long)N * p.slices >= 128 || (long long)p.pixels * p.width * size <= 65536);
   if (plan.resident) {
-    // few pixels a thread as long as the workgroup is small, so that several share a CU
+    // few pixels a thread as long as the workgroup is small, so that several share a CU (32 x 784 x
+    // 512, microscaled, 64 bytes: 512 threads of eight pixels 16.3 us, 1024 of four 19.7)
     plan.threads = std::max(64, 1 << p.lg_vec);
     plan.regs = 1;
     auto holds = [&] { return (long long)(plan.threads >> p.lg_vec) * plan.regs; };
     while (holds() < p.pixels) {
-      if (plan.regs < 4 || plan.threads >= kGnMost) plan.regs *= 2;
+      if (plan.regs < 4 || plan.threads >= kGnMost || (plan.threads >= 512 && plan.regs < 8)) plan.regs *= 2;
       else plan.threads *= 2;
     }
     p.chunks = 1;
     p.chunk_pixels = p.pixels;
     return plan;
   }
-  set(whole);
-  plan.threads = std::max(256, 1 << p.lg_vec);
+  // In parts: slices of 64 bytes, a workgroup for each CU (4 x 16384 x 128 of fp16: 16 parts of 64
+  // bytes 17.7 us, 64 parts of 128 bytes 20.5, 128 parts 26; the second launch reads all parts of
+  // its slice), smaller ones where that leaves a workgroup less than four pixels a thread.
+  k = unit;
+  while (k < wide && (long long)k * p.per * size < 64) k = std::min(k + unit, p.groups);
+  set(k);
   plan.regs = 4;
-  const int stride = plan.threads >> p.lg_vec;
   const int chunks = std::max(1, std::min<int>(gn_most_chunks(N, (size_t)p.pixels),
-                                               (int)(1024 / std::min<long long>(1024, (long long)N * p.slices))));
+                                               (int)(256 / std::min<long long>(256, (long long)N * p.slices))));
+  plan.threads = std::max(512, 1 << p.lg_vec);
+  if ((long long)(plan.threads >> p.lg_vec) * plan.regs * chunks > p.pixels) plan.threads = std::max(256, 1 << p.lg_vec);
+  const int stride = plan.threads >> p.lg_vec;
   p.chunk_pixels = (int)std::min<long long>(p.pixels, ((long long)p.pixels + (long long)chunks * stride - 1) /
                                                           ((long long)chunks * stride) * stride);
   p.chunks = (p.pixels + p.chunk_pixels - 1) / p.chunk_pixels;
@@ -455,7 +509,7 @@ static int gn_launch_regs(const GroupNorm &p, const GnPlan &plan, hipStream_t st
     if (plan.regs == 1) return gn_launch_one<E, OUT, 1, MODE, NV>(p, plan, st);
     if (plan.regs == 2) return gn_launch_one<E, OUT, 2, MODE, NV>(p, plan, st);
     if (plan.regs == 4) return gn_launch_one<E, OUT, 4, MODE, NV>(p, plan, st);
-    if constexpr (E::kSize == 2 && NV == 1)
+    if constexpr (E::kSize == 2 && NV <= 2)
       if (plan.regs == 16) return gn_launch_one<E, OUT, 16, MODE, NV>(p, plan, st);
     return gn_launch_one<E, OUT, 8, MODE, NV>(p, plan, st);
   }
@@ -489,11 +543,10 @@ static int gn_launch(GroupNorm p, size_t N, hipStream_t st) {
       group_norm_wide_apply_kernel<E, OUT><<<blocks, kGnWideThreads, 0, st>>>(p, units);
       rc = check_launch("group_norm");
     } else {
-      // slices of a sample share lines where they are narrower than 128 bytes, or rows do not
-      // start on one: they go to one die, whose L2 then has the line whole
-      p.by_die = plan.resident && p.slices > 1 && p.samples >= 64;
-      // eight channels of a vector lie in one group where groups are made of such vectors
-      rc = p.per % 8 == 0 ? gn_launch_as<E, OUT, 1>(p, plan, st) : gn_launch_as<E, OUT, 8>(p, plan, st);
+      p.by_die = plan.resident && p.slices > 1 && p.samples >= 8;
+      rc = p.per % 8 == 0   ? gn_launch_as<E, OUT, 1>(p, plan, st)
+           : p.per % 4 == 0 ? gn_launch_as<E, OUT, 2>(p, plan, st)
+                            : gn_launch_as<E, OUT, 8>(p, plan, st);
     }
     if (rc) return rc;
   }

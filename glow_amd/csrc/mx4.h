@@ -222,6 +222,32 @@ __device__ __forceinline__ void mx4_values8(float (&x)[8], uint32_t codes, uint3
     x[6 + j] = byte == 255 ? nan : d[j];
   }
 }
+// A value with its counterpart 16 or 32 lanes away, in both: x and the one swapped in.
+__device__ __forceinline__ uint32_t max_across16(uint32_t m) {
+  const auto s = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return max((uint32_t)s[0], (uint32_t)s[1]);
+}
+__device__ __forceinline__ uint32_t max_across32(uint32_t m) {
+  const auto s = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  return max((uint32_t)s[0], (uint32_t)s[1]);
+}
+__device__ __forceinline__ float add_across16(float x) {
+  const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ float add_across32(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+// x + x of the lane N further on in the row of sixteen: the lanes of a row N apart hold their
+// sum once this is done for 8, 4, .. down to N.
+template <int N> __device__ __forceinline__ float add_rotated(float x) {
+  return x + __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), 0x120 + N, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = add_rotated<1>(add_rotated<2>(add_rotated<4>(add_rotated<8>(x))));
+  return add_across32(add_across16(x));
+}
 // The largest of four neighbouring lanes, in all four.
 __device__ __forceinline__ uint32_t quad_max(uint32_t m) {
   m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true)); // lanes 1 0 3 2

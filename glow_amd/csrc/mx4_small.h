@@ -142,8 +142,7 @@ __global__ __launch_bounds__(kSmallWaves * 64, 2) void mx4_fc_small_kernel(MxFc 
       for (int c = 0; c < NT; c++)
 #pragma unroll
         for (int i = 0; i < 4; i++) most = max(most, magnitude_bits(y[c][i]));
-      most = max(most, (uint32_t)__shfl_xor((int)most, 16));
-      most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+      most = max_across32(max_across16(most));
       const uint32_t byte = mx4_scale_byte(most);
       const float x8[8] = {y[0][0], y[0][1], y[0][2], y[0][3], y[1][0], y[1][1], y[1][2], y[1][3]};
       const uint32_t codes = mx4_codes8(x8, byte);

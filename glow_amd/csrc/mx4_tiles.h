@@ -232,7 +232,7 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
           x[r >> 3][r & 7] = nw + i * 32 + 16 * half + r < p.N ? y : 0.0f;
           most = max(most, magnitude_bits(x[r >> 3][r & 7]));
         }
-        most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+        most = max_across32(most);
         const uint32_t byte = mx4_scale_byte(most);
         bytes |= byte << (8 * i);
         const uint32_t lo = mx4_codes8(x[0], byte), hi = mx4_codes8(x[1], byte);
