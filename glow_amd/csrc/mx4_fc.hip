@@ -5,6 +5,7 @@
 // and products are summed in 32 bits. The weights are the first operand, so that a lane's
 // results belong to one row of the output and lie in fours of neighbouring columns: what a
 // microscaled result's blocks and wide stores want.
+#include "mx4_short.h"
 #include "mx4_small.h"
 #include "mx4_tiles.h"
 
@@ -17,8 +18,11 @@ namespace mi355x {
 // 5.6 / 7.4, 64 x 4096 x 8192 34 / 24 / 18 / 11.5 (rows x K x columns). Up to four rows 16x16
 // holds its own over any number of columns (1 x 4096 x 16384 10.9 / 11.9): the input is next
 // to nothing then.
-enum FcTile { kFc16, kFc32x16, kFc32, kFc64, kFc128, kFc256 };
-static FcTile fc_tile(long long M, long long N, bool mx4_out) {
+// Up to 512 columns the larger tiles need no ring (mx4_short.h): 4096 x 512 x 256 4.7 / 3.8, 25088 x
+// 512 x 128 7.6 / 5.4, 8192 x 512 x 4096 29.5 (256x256 tiles) / 24.7 (128x128 without a ring; 64x64
+// 27.0).
+enum FcTile { kFc16, kFc32x16, kFc32, kFcShort64, kFcShort128, kFc64, kFc128, kFc256 };
+static FcTile fc_tile(long long M, long long K, long long N, bool mx4_out) {
   const long long most = 288;
   const long long m16 = (M + 15) / 16, m32 = (M + 31) / 32, n16 = (N + 15) / 16, n32 = (N + 31) / 32;
   if (mx4_out) {                   // a microscaled result's columns go by blocks of 32
@@ -28,15 +32,21 @@ static FcTile fc_tile(long long M, long long N, bool mx4_out) {
     if (m32 * n16 <= most) return kFc32x16;
   }
   if (m32 * n32 <= most) return kFc32;
+  if (K <= kShortGroups * kMxGroup)
+    return N > 64 && ((N + 127) / 128) * ((M + 127) / 128) >= 512 ? kFcShort128 : kFcShort64;
   if (((N + 255) / 256) * ((M + 255) / 256) >= 192) return kFc256;
   if (((N + 127) / 128) * ((M + 127) / 128) >= 192) return kFc128;
   return kFc64;
 }
 // Whether a float input is quantised by the kernel itself: every workgroup does so for its rows,
-// which a launch in front saves where they are many bytes. us, in the kernel / in front: 128 x
-// 1024 x 1024 of fp16 4.9 / 5.6 (64 KB of rows), 16 x 4096 x 4096 8.6 / 8.3 (128 KB), 64 x 4096 x
-// 4096 15.3 / 12.3 (256 KB), 61 x 415 x 509 of fp32 3.5 / 5.0.
-static bool fc_quantizes(FcTile tile, long long M, long long K, size_t size) {
+// which a launch in front saves where they are many bytes, or shared by many workgroups. us, in the
+// kernel / in front: 128 x 1024 x 1024 of fp16 4.9 / 5.6 (64 KB of rows), 16 x 4096 x 4096 8.6 / 8.3
+// (128 KB), 64 x 4096 x 4096 15.3 / 12.3 (256 KB), 61 x 415 x 509 of fp32 3.5 / 5.0; 64x64 tiles
+// without a ring: 4096 x 13 x 512 of fp32 4.7 / 5.8 (3 KB, 8 tiles to a row), 25088 x 512 x 128 of
+// fp16 11.1 / 13.8 (64 KB, 2), 2000 x 400 x 500 of fp32 8.2 / 6.9 (100 KB, 8), 8192 x 256 x 1024 of
+// fp16 10.8 / 10.0 (32 KB, 16).
+static bool fc_quantizes(FcTile tile, long long M, long long K, long long N, size_t size) {
+  if (tile == kFcShort64) return 64 * K * (long long)size <= 64 * 1024 && N <= 8 * 64;
   return tile <= kFc32 && std::min(M, tile == kFc16 ? 16LL : 32LL) * K * (long long)size <= 96 * 1024;
 }
 
@@ -55,6 +65,12 @@ template <class OUT> static int fc_launch(const MxFc &p, int K, int in_type, FcT
            : in_type == MI355X_F16 ? fc_small<F16, OUT>(p, K, tile, st)
            : in_type == MI355X_BF16 ? fc_small<BF16, OUT>(p, K, tile, st)
                                     : fc_small<MX4, OUT>(p, K, tile, st);
+  if (tile == kFcShort64)
+    return in_type == MI355X_F32    ? mx4_fc_short_launch<F32, OUT, 64, 64, 32, 32, 4>(p, K, st)
+           : in_type == MI355X_F16  ? mx4_fc_short_launch<F16, OUT, 64, 64, 32, 32, 4>(p, K, st)
+           : in_type == MI355X_BF16 ? mx4_fc_short_launch<BF16, OUT, 64, 64, 32, 32, 4>(p, K, st)
+                                    : mx4_fc_short_launch<MX4, OUT, 64, 64, 32, 32, 4>(p, K, st);
+  if (tile == kFcShort128) return mx4_fc_short_launch<MX4, OUT, 128, 128, 64, 64, 2>(p, K, st);
   return tile == kFc256   ? mx4_fc_tile_launch<OUT, 256, 256, 128, 64, 4, 1>(p, st)
          : tile == kFc128 ? mx4_fc_tile_launch<OUT, 128, 128, 64, 64, 4, 2>(p, st)
                           : mx4_fc_tile_launch<OUT, 64, 64, 32, 32, 4, 4>(p, st);
@@ -76,7 +92,8 @@ int mi355x_mx4_fc_workspace_bytes(size_t M, size_t K, size_t N, int in_type, siz
   if (in_type == MI355X_MX4 || !M || !N) return MI355X_OK;
   // (whatever the result's type)
   for (bool mx4_out : {false, true})
-    if (!fc_quantizes(fc_tile((long long)M, (long long)N, mx4_out), (long long)M, (long long)K, float_size(in_type)))
+    if (!fc_quantizes(fc_tile((long long)M, (long long)K, (long long)N, mx4_out), (long long)M, (long long)K, (long long)N,
+                      float_size(in_type)))
       *bytes = M * mx4_row_bytes_of(K);
   return MI355X_OK;
 }
@@ -111,8 +128,8 @@ int mi355x_mx4_fc(void *out, int out_type, size_t out_row_bytes, const void *in,
                        !overlaps(workspace, need, weights, w_span) && !overlaps(workspace, need, bias, 4 * N),
                    "mx4_fc: the workspace overlaps a tensor");
   }
-  const FcTile tile = fc_tile((long long)M, (long long)N, out_type == MI355X_MX4);
-  if (in_type != MI355X_MX4 && !fc_quantizes(tile, (long long)M, (long long)K, float_size(in_type))) {
+  const FcTile tile = fc_tile((long long)M, (long long)K, (long long)N, out_type == MI355X_MX4);
+  if (in_type != MI355X_MX4 && !fc_quantizes(tile, (long long)M, (long long)K, (long long)N, float_size(in_type))) {
     p.in = static_cast<const uint8_t *>(workspace);
     p.in_row_bytes = mx4_row_bytes_of(K);
     if (K)

@@ -45,6 +45,97 @@ struct MxTile {
   static constexpr size_t kLds = (size_t)kBias + BN * 4;
 };
 
+// The end of a tile: biases, activation, and the results on their way out. `bias` is column
+// tid's; a wave stages its results in LDS where nothing that is still needed lies.
+template <class OUT, int BN, int BM, int WN, int WM>
+__device__ __forceinline__ void mx4_tile_results(mx_v16f (&acc)[WN / 32][WM / 32], const MxFc &p, int8_t *lds,
+                                                 float *s_bias, float bias, int m0, int n0) {
+  constexpr int TN = WN / 32, TM = WM / 32, kWavesN = BN / WN, kOutRow = WN * OUT::kSize + 16;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave % kWavesN, wm = wave / kWavesN;
+  const int l32 = lane & 31, half = lane >> 5;
+  if (tid < BN) s_bias[tid] = bias;
+  __syncthreads();
+
+  const int nw = n0 + wn * WN;                     // first column of this wave
+  with_activation(p.act, [&](auto act) {
+  auto value = [&](int i, int j, int r) {          // column i * 32 + 16 * half + r of row j * 32 + l32
+    return activate<decltype(act)::value>(acc[i][j][r] + s_bias[wn * WN + i * 32 + 16 * half + r]);
+  };
+  if constexpr (OUT::kSize == 0) {
+    const int blocks = 4 * p.out_groups;
+#pragma unroll
+    for (int j = 0; j < TM; j++) {
+      const int m = m0 + wm * WM + j * 32 + l32;
+      uint8_t *row = p.out + (size_t)m * p.out_row_bytes;
+      uint32_t bytes = 0;
+#pragma unroll
+      for (int i = 0; i < TN; i++) {
+        float x[2][8];
+        uint32_t most = 0;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const float y = value(i, j, r);
+          x[r >> 3][r & 7] = nw + i * 32 + 16 * half + r < p.N ? y : 0.0f;
+          most = max(most, magnitude_bits(x[r >> 3][r & 7]));
+        }
+        most = max_across32(most);
+        const uint32_t byte = mx4_scale_byte(most);
+        bytes |= byte << (8 * i);
+        const uint32_t lo = mx4_codes8(x[0], byte), hi = mx4_codes8(x[1], byte);
+        if (m < p.M && nw / 32 + i < blocks)
+          *reinterpret_cast<uint2 *>(row + nw / 2 + i * 16 + 8 * half) = make_uint2(lo, hi);
+      }
+      // (a wave's columns are whole groups, or a part of one: all of its blocks exist or none)
+      uint8_t *scales = row + (size_t)p.out_groups * kMxGroupBytes;
+      if (m < p.M && half == 0 && nw / 32 < blocks) {
+        if constexpr (TN == 4) *reinterpret_cast<uint32_t *>(scales + nw / 32) = bytes;
+        else if constexpr (TN == 2) *reinterpret_cast<uint16_t *>(scales + nw / 32) = (uint16_t)bytes;
+        else scales[nw / 32] = (uint8_t)bytes;
+      }
+      // the zeros behind the last group's scales
+      if (m < p.M && half == 1 && nw / 32 <= blocks - 1 && blocks - 1 < nw / 32 + TN)
+        for (int w = 0; w < ((-p.out_groups) & 3); w++) reinterpret_cast<uint32_t *>(scales)[p.out_groups + w] = 0;
+    }
+  } else {
+    // through LDS: a lane's sixteen columns are a piece of a line, a row's columns of a wave whole ones
+    typedef typename OUT::T E;
+    constexpr int PER = 16 / OUT::kSize, LPR = WN / PER;   // columns of a store, lanes of a row
+    typedef E Chunk __attribute__((ext_vector_type(PER)));
+    typedef Chunk Chunk1 __attribute__((aligned(OUT::kSize)));
+    int8_t *stage = lds + wave * 32 * kOutRow;
+#pragma unroll
+    for (int j = 0; j < TM; j++) {
+#pragma unroll
+      for (int i = 0; i < TN; i++)
+#pragma unroll
+        for (int q = 0; q < 16 / PER; q++) {
+          Chunk c;
+#pragma unroll
+          for (int r = 0; r < PER; r++) c[r] = OUT::from(value(i, j, q * PER + r));
+          *reinterpret_cast<Chunk *>(stage + l32 * kOutRow + (i * 32 + 16 * half + q * PER) * OUT::kSize) = c;
+        }
+      wave_fence();
+      const int n = nw + (lane % LPR) * PER;
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += 64 / LPR) {
+        const int r = r0 + lane / LPR, m = m0 + wm * WM + j * 32 + r;
+        const Chunk c = *reinterpret_cast<const Chunk *>(stage + r * kOutRow + (lane % LPR) * 16);
+        if (m < p.M && n < p.N) {
+          E *at = reinterpret_cast<E *>(p.out + (size_t)m * p.out_row_bytes) + n;
+          if (n + PER <= p.N) *reinterpret_cast<Chunk1 *>(at) = c;
+          else
+            for (int e = 0; e < PER; e++)
+              if (n + e < p.N) at[e] = c[e];
+        }
+      }
+      wave_fence();
+    }
+  }
+  });
+}
+
 template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS>
 __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM / WM) / 4) void mx4_fc_tile_kernel(
     MxFc p, int tiles_n, int tiles_m) {
@@ -206,86 +297,7 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
   }
   dma_wait<0>();                                   // the re-reads, before LDS is used again
   __syncthreads();
-  float *s_bias = reinterpret_cast<float *>(lds + T::kBias);
-  if (tid < BN) s_bias[tid] = bias;
-  __syncthreads();
-
-  const int nw = n0 + wn * WN;                     // first column of this wave
-  with_activation(p.act, [&](auto act) {
-  auto value = [&](int i, int j, int r) {          // column i * 32 + 16 * half + r of row j * 32 + l32
-    return activate<decltype(act)::value>(acc[i][j][r] + s_bias[wn * WN + i * 32 + 16 * half + r]);
-  };
-  if constexpr (OUT::kSize == 0) {
-    const int blocks = 4 * p.out_groups;
-#pragma unroll
-    for (int j = 0; j < TM; j++) {
-      const int m = m0 + wm * WM + j * 32 + l32;
-      uint8_t *row = p.out + (size_t)m * p.out_row_bytes;
-      uint32_t bytes = 0;
-#pragma unroll
-      for (int i = 0; i < TN; i++) {
-        float x[2][8];
-        uint32_t most = 0;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const float y = value(i, j, r);
-          x[r >> 3][r & 7] = nw + i * 32 + 16 * half + r < p.N ? y : 0.0f;
-          most = max(most, magnitude_bits(x[r >> 3][r & 7]));
-        }
-        most = max_across32(most);
-        const uint32_t byte = mx4_scale_byte(most);
-        bytes |= byte << (8 * i);
-        const uint32_t lo = mx4_codes8(x[0], byte), hi = mx4_codes8(x[1], byte);
-        if (m < p.M && nw / 32 + i < blocks)
-          *reinterpret_cast<uint2 *>(row + nw / 2 + i * 16 + 8 * half) = make_uint2(lo, hi);
-      }
-      // (a wave's columns are whole groups, or a part of one: all of its blocks exist or none)
-      uint8_t *scales = row + (size_t)p.out_groups * kMxGroupBytes;
-      if (m < p.M && half == 0 && nw / 32 < blocks) {
-        if constexpr (TN == 4) *reinterpret_cast<uint32_t *>(scales + nw / 32) = bytes;
-        else if constexpr (TN == 2) *reinterpret_cast<uint16_t *>(scales + nw / 32) = (uint16_t)bytes;
-        else scales[nw / 32] = (uint8_t)bytes;
-      }
-      // the zeros behind the last group's scales
-      if (m < p.M && half == 1 && nw / 32 <= blocks - 1 && blocks - 1 < nw / 32 + TN)
-        for (int w = 0; w < ((-p.out_groups) & 3); w++) reinterpret_cast<uint32_t *>(scales)[p.out_groups + w] = 0;
-    }
-  } else {
-    // through LDS: a lane's sixteen columns are a piece of a line, a row's columns of a wave whole ones
-    typedef typename OUT::T E;
-    constexpr int PER = 16 / OUT::kSize, LPR = WN / PER;   // columns of a store, lanes of a row
-    typedef E Chunk __attribute__((ext_vector_type(PER)));
-    typedef Chunk Chunk1 __attribute__((aligned(OUT::kSize)));
-    int8_t *stage = lds + wave * 32 * T::kOutRow;
-#pragma unroll
-    for (int j = 0; j < TM; j++) {
-#pragma unroll
-      for (int i = 0; i < TN; i++)
-#pragma unroll
-        for (int q = 0; q < 16 / PER; q++) {
-          Chunk c;
-#pragma unroll
-          for (int r = 0; r < PER; r++) c[r] = OUT::from(value(i, j, q * PER + r));
-          *reinterpret_cast<Chunk *>(stage + l32 * T::kOutRow + (i * 32 + 16 * half + q * PER) * OUT::kSize) = c;
-        }
-      wave_fence();
-      const int n = nw + (lane % LPR) * PER;
-#pragma unroll
-      for (int r0 = 0; r0 < 32; r0 += 64 / LPR) {
-        const int r = r0 + lane / LPR, m = m0 + wm * WM + j * 32 + r;
-        const Chunk c = *reinterpret_cast<const Chunk *>(stage + r * T::kOutRow + (lane % LPR) * 16);
-        if (m < p.M && n < p.N) {
-          E *at = reinterpret_cast<E *>(p.out + (size_t)m * p.out_row_bytes) + n;
-          if (n + PER <= p.N) *reinterpret_cast<Chunk1 *>(at) = c;
-          else
-            for (int e = 0; e < PER; e++)
-              if (n + e < p.N) at[e] = c[e];
-        }
-      }
-      wave_fence();
-    }
-  }
-  });
+  mx4_tile_results<OUT, BN, BM, WN, WM>(acc, p, lds, reinterpret_cast<float *>(lds + T::kBias), bias, m0, n0);
 }
 
 template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS>

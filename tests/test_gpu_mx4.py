@@ -141,7 +141,8 @@ def test_fc_results_of_every_type(M, K, N, out_type):
 
 
 @pytest.mark.parametrize("out_type", [ref.F32, ref.F16, ref.BF16, ref.MX4])
-@pytest.mark.parametrize("M, K, N", [(1801, 150, 2003), (1793, 1040, 1798), (3201, 160, 4098), (3090, 1300, 3851)])
+@pytest.mark.parametrize("M, K, N", [(1801, 150, 2003), (1793, 1040, 1798), (3201, 160, 4098), (3090, 1300, 3851), (3000, 512, 3001),
+                                     (1990, 650, 150), (10000, 385, 65)])
 def test_fc_of_large_results(M, K, N, out_type):
     # the tiles of 128 and 256: one step of K and two, an odd count past a group of scales
     rng = np.random.default_rng(M + out_type)
@@ -153,7 +154,8 @@ def test_fc_of_large_results(M, K, N, out_type):
 
 
 @pytest.mark.parametrize("in_type", [ref.F32, ref.F16, ref.BF16])
-@pytest.mark.parametrize("M, K, N", [(1, 4096, 70), (4, 515, 3000), (31, 96, 700), (90, 1050, 290)])
+@pytest.mark.parametrize("M, K, N", [(1, 4096, 70), (4, 515, 3000), (31, 96, 700), (90, 1050, 290), (1990, 13, 300),
+                                     (2000, 511, 190), (700, 300, 2000)])
 def test_float_inputs_give_what_their_rows_give(M, K, N, in_type):
     """Quantised by the product or in front of it: the same bits."""
     rng = np.random.default_rng(K)

@@ -124,12 +124,12 @@ def test_fc_refuses(change, word):
 
 
 def test_fc_refuses_a_workspace_that_does_not_fit():
-    M, K, N = 3000, 100, 100
+    M, K, N = 3000, 1000, 1000
     need = capi.mx4_fc_workspace_bytes(M, K, N, capi.TYPE_F32)
     assert capi.mx4_fc_workspace_bytes(M, K, N, capi.TYPE_MX4) == 0
     assert capi.mx4_fc_workspace_bytes(1, K, N, capi.TYPE_F32) == 0       # a single row needs none
-    assert need >= M * 80
-    a = dict(in_type=0, in_row=400, M=M, K=K, N=N)
+    assert need >= M * capi.mx4_row_bytes(K)
+    a = dict(in_type=0, in_row=4000, M=M, K=K, N=N, w_row=capi.mx4_row_bytes(K), out_row=4000)
     for change in (dict(), dict(ws=S, ws_bytes=need - 1), dict(ws=S + 4, ws_bytes=need)):
         refused("mi355x_mx4_fc", fc_args(**a, **change), "workspace")
     refused("mi355x_mx4_fc", fc_args(**a, ws=R + 160, ws_bytes=need), "overlaps")
