@@ -47,16 +47,30 @@ enum { kGnResident, kGnStats, kGnApply };
 constexpr int kGnMost = 1024;         // threads of a workgroup
 constexpr int kGnMostChunks = 128;    // parts of a slice
 
-// Sums over a slice's pixels and a group's channels, to s_group[0 .. in_slice). x[i] is a
-// thread's sum over part i of its eight channels: NV parts, the fewest that each lie in one
-// group. Lanes of a wave that hold the same channels are summed first, then a wave takes a
-// group.
-template <int NV>
-__device__ __forceinline__ void gn_reduce(float (&x)[NV], float *s_part, float *s_group, const GroupNorm &p) {
+// The group of a channel, and of those behind it (a division for each of eight costs more than
+// the statistics do).
+struct GnGroup {
+  int group, in;
+  __device__ __forceinline__ GnGroup(int channel, int per)
+      : group((int)((unsigned)channel / (unsigned)per)), in(channel - group * per) {}
+  __device__ __forceinline__ void next(int per) {
+    if (++in == per) in = 0, group++;
+  }
+};
+
+// Sums over a slice's pixels and a group's channels, to s_group[0 .. in_slice). A thread's eight
+// channels are NP parts that each lie in one group: one where groups are whole vectors, two (the
+// first channels and the rest) where a vector meets two groups at most, else one for each
+// channel. x[i] is the sum over part i, its place in a row of s_part `at` + i; parts before `from`
+// are another thread's. Lanes of a wave that hold the same channels are summed first, then a
+// wave takes a group.
+template <int NP>
+__device__ __forceinline__ void gn_reduce(float (&x)[NP], float *s_part, float *s_group, int at, int from,
+                                          const GroupNorm &p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
   const int V = 1 << p.lg_vec;
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
+  for (int j = 0; j < NP; j++) {
     if (V <= 8) x[j] = add_rotated<8>(x[j]);
     if (V <= 4) x[j] = add_rotated<4>(x[j]);
     if (V <= 2) x[j] = add_rotated<2>(x[j]);
@@ -69,20 +83,27 @@ __device__ __forceinline__ void gn_reduce(float (&x)[NV], float *s_part, float *
   if (V >= 64 || lane < V) {
     const int row = V < 64 ? wave : tid >> p.lg_vec;
 #pragma unroll
-    for (int j = 0; j < NV; j++) s_part[((row << p.lg_vec) + (tid & (V - 1))) * NV + j] = x[j];
+    for (int j = 0; j < NP; j++)
+      if (NP < 8 || j >= from) s_part[(row << p.lg_vec) * NP + at + j] = x[j];
   }
   __syncthreads();
-  const int len = p.per / (8 / NV);
   for (int g = wave; g < p.in_slice; g += waves) {
+    // a group's parts in a row: `len` of them from `begin` on, `apart` places from each other; where
+    // it begins within a vector, the first is that vector's second part
+    const int channel = g * p.per;
+    const int begin = NP == 8 ? channel : (channel >> 3) * NP, apart = NP == 2 ? 2 : 1;
+    const int inner = NP == 2 && (channel & 7) ? 1 : 0;
+    const int len = NP == 8 ? p.per : ((channel + p.per - 1) >> 3) - (channel >> 3) + 1;
     float t = 0;
     if (len < 64) {
       for (int e = lane; e < len * rows; e += 64) {
-        const int row = e / len;
-        t += s_part[(row << p.lg_vec) * NV + g * len + (e - row * len)];
+        const int row = (int)((unsigned)e / (unsigned)len), k = e - row * len;
+        t += s_part[(row << p.lg_vec) * NP + begin + k * apart + (k == 0 ? inner : 0)];
       }
     } else {
       for (int row = 0; row < rows; row++)
-        for (int e = lane; e < len; e += 64) t += s_part[(row << p.lg_vec) * NV + g * len + e];
+        for (int k = lane; k < len; k += 64)
+          t += s_part[(row << p.lg_vec) * NP + begin + k * apart + (k == 0 ? inner : 0)];
     }
     t = wave_sum(t);
     if (lane == 0) s_group[g] = t;
@@ -117,14 +138,14 @@ template <class E> __device__ __forceinline__ float gn_less(const typename E::Ei
 // Writes one pixel's eight channels. 32-bit values lose the mean first; of 16-bit ones it is
 // in the shift, which is off by half a step of mean * scale then, less than the values'
 // own rounding.
-template <class E, class OUT, int ACT, int NV>
-__device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, bool block_inside,
-                                         const typename E::Eight &raw, const float (&mean)[NV],
+template <class E, class OUT, int ACT, int NM>
+__device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, int twice, bool block_inside,
+                                         const typename E::Eight &raw, const float (&mean)[NM],
                                          const float (&scale)[8], const float (&shift)[8], const GroupNorm &p) {
   float y[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    const float x = E::kSize == 2 ? E::get(raw, j) : E::get(raw, j) - mean[j * NV / 8];
+    const float x = E::kSize == 2 ? E::get(raw, j) : E::get(raw, j) - mean[NM == 1 ? 0 : j];
     const float v = activate<ACT>(fmaf(x, scale[j], shift[j]));
     y[j] = OUT::kSize || j < left ? v : 0.0f;
   }
@@ -135,13 +156,18 @@ __device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, bool blo
       if ((c & 31) == 0) row[(size_t)p.channel_groups * kMxGroupBytes + (c >> 5)] = (uint8_t)byte;
     }
   } else {
+    // (two lanes of a wave that store the same channels store the same bits; lanes of two waves may
+    // not, in place: one may not have read yet what the other overwrites)
     typename OUT::T *o = reinterpret_cast<typename OUT::T *>(row) + c;
-    if (left >= 8) store8<OUT>(o, y);
-    else store8_end<OUT>(o, y, left);
+    if (left >= 8 && (twice == 0 || p.lg_vec <= 6)) store8<OUT>(o, y);
+    else
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (j >= twice && j < left) o[j] = OUT::from(y[j]);
   }
 }
 
-template <class E, class OUT, int R, int MODE, int NV>
+template <class E, class OUT, int R, int MODE, int NP>
 __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
   extern __shared__ __attribute__((aligned(16))) float s_mem[];
   float *s_group = s_mem, *s_second = s_mem + p.in_slice, *s_part = s_mem + 2 * p.in_slice;
@@ -161,8 +187,14 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
     sample = (int)(id / (unsigned)p.slices);
     slice = (int)(id % (unsigned)p.slices);
   }
-  const int c0 = slice * p.width, c = c0 + v * 8;
-  const int c_end = min(p.C, c0 + p.width), left = c_end - c;
+  const int c0 = slice * p.width, c_end = min(p.C, c0 + p.width);
+  // The last vector of a slice that is no whole number of them begins earlier and overlaps the one in
+  // front (a load of eight instead of eight of one, for the whole wave); `twice` channels are that
+  // one's in the statistics. Blocks of microscaled rows begin where they begin.
+  int c = c0 + v * 8;
+  const int twice = NP > 1 && OUT::kSize && c < c_end && c_end - c0 >= 8 ? max(0, c + 8 - c_end) : 0;
+  c -= twice;
+  const int left = c_end - c;
   const int px0 = chunk * p.chunk_pixels, px_end = min(p.pixels, px0 + p.chunk_pixels);
   const uint8_t *in = p.in + (size_t)sample * p.pixels * p.in_row_bytes + (ptrdiff_t)c * E::kSize;
 
@@ -187,81 +219,122 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
   const float of_group = (float)p.per;
 
   load(px0);
-  // (asked for with the values: the statistics are in between)
   float scale[8], shift[8];
-  if constexpr (MODE != kGnStats) {
+  auto load_affine = [&]() {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       scale[j] = p.gamma && j < left ? p.gamma[c + j] : 1.0f;
       shift[j] = p.beta && j < left ? p.beta[c + j] : 0.0f;
     }
-  }
+  };
+  // asked for with the values, ahead of the statistics, where registers are left for it
+  if constexpr (MODE != kGnStats && R < 16) load_affine();
   if constexpr (MODE != kGnApply) {
-    // a thread's own count (exact: a part has 2^24 pixels at most), mean and squares
-    float count = 0, mean[NV], square[NV], one = 1.0f;
+    // a thread's own counts (exact: a part of a slice has 2^24 pixels at most), means and squares.
+    // Channel j belongs to part `j >= border` of two, to its own of eight.
+    int border = 8;
+    if (NP == 2 && left > 0) {
+      const GnGroup own(v * 8, p.per);
+      border = min(8, twice + p.per - own.in);
+    }
+    const int channels_lo = border - twice, channels_hi = 8 - border;
+    float count[NP], mean[NP], square[NP], one = 1.0f;
     asm("" : "+s"(one));
 #pragma unroll
-    for (int j = 0; j < NV; j++) mean[j] = square[j] = 0;
+    for (int j = 0; j < NP; j++) count[j] = mean[j] = square[j] = 0;
     for (int from = px0;;) {
       const int n = mine(from);
       if (n > 0) {
-        float m[NV], q[NV];
+        constexpr int NA = NP == 1 ? 1 : 8;       // sums in the loop over pixels
+        float m[NA], q[NA], here[NP], own[NP], rest[NP];
 #pragma unroll
-        for (int j = 0; j < NV; j++) m[j] = q[j] = 0;
+        for (int j = 0; j < NA; j++) m[j] = q[j] = 0;
 #pragma unroll
         for (int i = 0; i < R; i++)
           if (i < n) {
-            if constexpr (NV == 1) m[0] = gn_sum8<E>(raw[i], m[0]);
+            if constexpr (NP == 1) m[0] = gn_sum8<E>(raw[i], m[0]);
             else {
 #pragma unroll
-              for (int j = 0; j < 8; j++) m[j * NV / 8] += E::get(raw[i], j);
+              for (int j = 0; j < 8; j++) m[j] += E::get(raw[i], j);
             }
           }
-        const float here = (float)n * (8 / NV), over = 1.0f / here;
+        if constexpr (NP == 1) {
+          here[0] = (float)n * 8;
+          m[0] *= 1.0f / here[0];
+          own[0] = m[0];
+        } else if constexpr (NP == 2) {
+          here[0] = (float)(n * channels_lo);
+          here[1] = (float)(n * channels_hi);
+          float lo = 0, hi = 0;
 #pragma unroll
-        for (int j = 0; j < NV; j++) m[j] *= over;
+          for (int j = 0; j < 8; j++) {
+            lo += j >= twice && j < border ? m[j] : 0.0f;
+            hi += j >= border ? m[j] : 0.0f;
+          }
+          own[0] = lo * (1.0f / here[0]);
+          own[1] = channels_hi ? hi * (1.0f / here[1]) : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; j++) m[j] = j < border ? own[0] : own[1];
+        } else {
+          const float over = 1.0f / (float)n;
+#pragma unroll
+          for (int j = 0; j < 8; j++) here[j] = (float)n, m[j] *= over, own[j] = m[j];
+        }
 #pragma unroll
         for (int i = 0; i < R; i++)
           if (i < n)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-              const float d = gn_less<E>(raw[i], j, m[j * NV / 8], one);
-              q[j * NV / 8] = fmaf(d, d, q[j * NV / 8]);
+              const float d = gn_less<E>(raw[i], j, m[NP == 1 ? 0 : j], one);
+              q[NP == 1 ? 0 : j] = fmaf(d, d, q[NP == 1 ? 0 : j]);
             }
-        if (MODE == kGnResident || count == 0) {
-          count = here;
+        if constexpr (NP == 2) {
+          rest[0] = rest[1] = 0;
 #pragma unroll
-          for (int j = 0; j < NV; j++) mean[j] = m[j], square[j] = q[j];
-        } else {             // joins two sets: the squares of each, and of what their means are apart
-          const float all = count + here, part = here / all;
-#pragma unroll
-          for (int j = 0; j < NV; j++) {
-            const float d = m[j] - mean[j];
-            mean[j] = fmaf(d, part, mean[j]);
-            square[j] += fmaf(d * d, count * part, q[j]);
+          for (int j = 0; j < 8; j++) {
+            rest[0] += j >= twice && j < border ? q[j] : 0.0f;
+            rest[1] += j >= border ? q[j] : 0.0f;
           }
-          count = all;
+        } else {
+#pragma unroll
+          for (int j = 0; j < NP; j++) rest[j] = q[j];
+        }
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+          if (MODE == kGnResident || count[j] == 0) {
+            count[j] = here[j], mean[j] = own[j], square[j] = rest[j];
+          } else {           // joins two sets: the squares of each, and of what their means are apart
+            const float all = count[j] + here[j], part = here[j] / all, d = own[j] - mean[j];
+            mean[j] = fmaf(d, part, mean[j]);
+            square[j] += fmaf(d * d, count[j] * part, rest[j]);
+            count[j] = all;
+          }
         }
       }
       if (MODE == kGnResident || px_end - from <= block) break;
       from += block;
       load(from);
     }
-    const float total = (float)(px_end - px0) * of_group;
-    float x[NV];
+    const float total = (float)(px_end - px0) * of_group, over = 1.0f / total;
+    const int at = NP == 8 ? c - c0 : v * NP;
+    float x[NP];
 #pragma unroll
-    for (int j = 0; j < NV; j++) x[j] = mean[j] * count;
-    gn_reduce<NV>(x, s_part, s_group, p);
+    for (int j = 0; j < NP; j++) x[j] = mean[j] * count[j];
+    gn_reduce<NP>(x, s_part, s_group, at, twice, p);
+    {
+      GnGroup of(NP == 8 ? c - c0 : v * 8, p.per);
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-      const int g = left > 0 ? min((v * 8 + j * (8 / NV)) / p.per, p.in_slice - 1) : 0;
-      const float d = mean[j] - s_group[g] / total;
-      x[j] = left > 0 ? fmaf(d * d, count, square[j]) : 0.0f;
+      for (int j = 0; j < NP; j++) {
+        const float d = mean[j] - s_group[left > 0 ? min(of.group, p.in_slice - 1) : 0] * over;
+        x[j] = left > 0 ? fmaf(d * d, count[j], square[j]) : 0.0f;
+        if (NP == 8) of.next(p.per);
+        else of.group++;
+      }
     }
-    gn_reduce<NV>(x, s_part, s_second, p);
+    gn_reduce<NP>(x, s_part, s_second, at, twice, p);
     const int groups = (c_end - c0) / p.per;
     for (int g = tid; g < groups; g += (int)blockDim.x) {
-      const float m = s_group[g] / total;
+      const float m = s_group[g] * over;
       if constexpr (MODE == kGnStats)
         p.stats[((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks + chunk] = GroupStats{m, s_second[g]};
       else {
@@ -302,13 +375,17 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
   }
   __syncthreads();
 
-  float mean[NV];
+  if constexpr (R >= 16) load_affine();
+  constexpr int NM = NP == 1 ? 1 : 8;
+  float mean[NM];
+  GnGroup of(c - c0, p.per);
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    const int i = j * NV / 8, g = j < left ? (v * 8 + j) / p.per : 0;
-    if (j % (8 / NV) == 0) mean[i] = s_group[g];
+    const int g = j < left ? of.group : 0;
+    if (NM == 8 || j == 0) mean[NM == 1 ? 0 : j] = s_group[g];
     scale[j] *= s_second[g];
-    if (E::kSize == 2) shift[j] = fmaf(-mean[i], scale[j], shift[j]);
+    if (E::kSize == 2) shift[j] = fmaf(-mean[NM == 1 ? 0 : j], scale[j], shift[j]);
+    if (NM == 8) of.next(p.per);
   }
   uint8_t *out = p.out + (size_t)sample * p.pixels * p.out_row_bytes;
   // microscaled: lanes up to the end of the slice's last block
@@ -318,7 +395,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
     for (int i = 0; i < R; i++) {
       const int px = from + first + i * stride;
       if (first + i * stride < px_end - from && (OUT::kSize == 0 || inside))
-        gn_write<E, OUT, decltype(act)::value, NV>(out + (size_t)px * p.out_row_bytes, c, left, inside, raw[i], mean,
+        gn_write<E, OUT, decltype(act)::value, NM>(out + (size_t)px * p.out_row_bytes, c, left, twice, inside, raw[i], mean,
                                                    scale, shift, p);
     }
   };
@@ -420,6 +497,8 @@ static int gn_most_chunks(size_t N, size_t pixels) {
   return (int)std::min<size_t>({n, pixels, (size_t)kGnMostChunks});
 }
 
+// Parts of a thread's eight channels that lie in one group each (gn_reduce).
+static int gn_parts(int per) { return per % 8 == 0 ? 1 : per >= 7 || per == 4 ? 2 : 8; }
 struct GnPlan {
   bool wide, resident;
   int threads, regs;      // pixels a thread holds at a time
@@ -447,8 +526,9 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
     plan.wide = true;
     return plan;
   }
-  // (sixteen of 16 bits with eight channels' sums each spill registers)
-  const int most_regs = size == 4 || p.per % 4 ? 8 : 16;
+  // (as many as leave room for the sums: one for a thread, two parts, or eight)
+  const int parts = gn_parts(p.per);
+  const int most_regs = size == 2 ? (parts == 1 ? 16 : 8) : (parts == 8 ? 4 : 8);
   auto fits = [&] { return p.pixels <= (long long)(kGnMost >> p.lg_vec) * most_regs; };
   // Narrower slices where they are too few for the chip, or too large for a workgroup, down to
   // 32 bytes: below, as many lines are asked for and less is used of each (64 x 3136 x 256 of
@@ -493,33 +573,34 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
   return plan;
 }
 
-template <class E, class OUT, int R, int MODE, int NV>
+template <class E, class OUT, int R, int MODE, int NP>
 static int gn_launch_one(const GroupNorm &p, const GnPlan &plan, hipStream_t st) {
   const int V = 1 << p.lg_vec;
   const int rows = V < 64 ? plan.threads / 64 : plan.threads >> p.lg_vec;
-  const size_t lds = (2 * (size_t)p.in_slice + (MODE == kGnApply ? 0 : (size_t)rows * V * NV)) * 4;
+  const size_t lds = (2 * (size_t)p.in_slice + (MODE == kGnApply ? 0 : (size_t)rows * V * NP)) * 4;
   const size_t sets = (size_t)(p.by_die ? (p.samples + 7) / 8 * 8 : p.samples) * p.slices * p.chunks;
-  group_norm_kernel<E, OUT, R, MODE, NV><<<(unsigned)sets, plan.threads, lds, st>>>(p);
+  group_norm_kernel<E, OUT, R, MODE, NP><<<(unsigned)sets, plan.threads, lds, st>>>(p);
   return check_launch("group_norm");
 }
-template <class E, class OUT, int MODE, int NV>
+template <class E, class OUT, int MODE, int NP>
 static int gn_launch_regs(const GroupNorm &p, const GnPlan &plan, hipStream_t st) {
-  if constexpr (MODE != kGnResident) return gn_launch_one<E, OUT, 4, MODE, NV>(p, plan, st);
+  if constexpr (MODE != kGnResident) return gn_launch_one<E, OUT, 4, MODE, NP>(p, plan, st);
   else {
-    if (plan.regs == 1) return gn_launch_one<E, OUT, 1, MODE, NV>(p, plan, st);
-    if (plan.regs == 2) return gn_launch_one<E, OUT, 2, MODE, NV>(p, plan, st);
-    if (plan.regs == 4) return gn_launch_one<E, OUT, 4, MODE, NV>(p, plan, st);
-    if constexpr (E::kSize == 2 && NV <= 2)
-      if (plan.regs == 16) return gn_launch_one<E, OUT, 16, MODE, NV>(p, plan, st);
-    return gn_launch_one<E, OUT, 8, MODE, NV>(p, plan, st);
+    if (plan.regs == 1) return gn_launch_one<E, OUT, 1, MODE, NP>(p, plan, st);
+    if (plan.regs == 2) return gn_launch_one<E, OUT, 2, MODE, NP>(p, plan, st);
+    if (plan.regs == 4) return gn_launch_one<E, OUT, 4, MODE, NP>(p, plan, st);
+    if constexpr (E::kSize == 2 && NP == 1)
+      if (plan.regs == 16) return gn_launch_one<E, OUT, 16, MODE, NP>(p, plan, st);
+    if constexpr (E::kSize == 2 || NP < 8) return gn_launch_one<E, OUT, 8, MODE, NP>(p, plan, st);
+    return fail(MI355X_ERR_RUNTIME, "group_norm: %d pixels a thread", plan.regs);
   }
 }
-template <class E, class OUT, int NV>
+template <class E, class OUT, int NP>
 static int gn_launch_as(const GroupNorm &p, const GnPlan &plan, hipStream_t st) {
-  if (plan.resident) return gn_launch_regs<E, OUT, kGnResident, NV>(p, plan, st);
+  if (plan.resident) return gn_launch_regs<E, OUT, kGnResident, NP>(p, plan, st);
   // (the first launch does not depend on the result's type)
-  if (int rc = gn_launch_regs<E, E, kGnStats, NV>(p, plan, st)) return rc;
-  return gn_launch_regs<E, OUT, kGnApply, NV>(p, plan, st);
+  if (int rc = gn_launch_regs<E, E, kGnStats, NP>(p, plan, st)) return rc;
+  return gn_launch_regs<E, OUT, kGnApply, NP>(p, plan, st);
 }
 template <class E, class OUT>
 static int gn_launch(GroupNorm p, size_t N, hipStream_t st) {
@@ -544,9 +625,10 @@ static int gn_launch(GroupNorm p, size_t N, hipStream_t st) {
       rc = check_launch("group_norm");
     } else {
       p.by_die = plan.resident && p.slices > 1 && p.samples >= 8;
-      rc = p.per % 8 == 0   ? gn_launch_as<E, OUT, 1>(p, plan, st)
-           : p.per % 4 == 0 ? gn_launch_as<E, OUT, 2>(p, plan, st)
-                            : gn_launch_as<E, OUT, 8>(p, plan, st);
+      const int parts = gn_parts(p.per);
+      rc = parts == 1   ? gn_launch_as<E, OUT, 1>(p, plan, st)
+           : parts == 2 ? gn_launch_as<E, OUT, 2>(p, plan, st)
+                        : gn_launch_as<E, OUT, 8>(p, plan, st);
     }
     if (rc) return rc;
   }
