@@ -3,9 +3,8 @@
 //
 // A step is 64 bytes of codes of every row of both operands, moved from global memory
 // straight into LDS, and two slices of 64 columns for the matrix cores, whose lanes read one
-// block (16 bytes) each. Scale bytes travel apart from the codes: 16 bytes of a row are four
-// steps' words, so that a row's line is asked for a quarter as often, a quarter of the rows
-// with every step. Weights are the first operand and their rows are permuted on the way
+// block (16 bytes) each. Scale bytes travel apart from the codes, with every fourth step: 16
+// bytes of a row are four steps' words. Weights are the first operand and their rows are permuted on the way
 // into LDS: a lane ends with sixteen neighbouring columns of one output row.
 #ifndef GLOW_MI355X_MX4_TILES_H
 #define GLOW_MI355X_MX4_TILES_H
@@ -142,9 +141,10 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
   typedef MxTile<OUT, BN, BM, WN, WM, STAGES> T;
   constexpr int WAVES = T::kWaves, TN = WN / 32, TM = WM / 32;
   constexpr int A_LOADS = BN / 16 / WAVES, B_LOADS = BM / 16 / WAVES;  // 16 rows an instruction
-  constexpr int CODES = A_LOADS + B_LOADS, LOADS = CODES + 1;          // and one of scales
-  constexpr int SL = (BN + BM) / (4 * WAVES);                          // lanes of that one
-  static_assert(BN / 16 % WAVES == 0 && BM / 16 % WAVES == 0 && SL * 4 * WAVES == BN + BM && SL <= 64, "tile");
+  constexpr int LOADS = A_LOADS + B_LOADS;
+  constexpr int ROWS = (BN + BM) / WAVES;                              // whose scales a wave moves
+  constexpr int SLOADS = (ROWS + 63) / 64, SLANES = ROWS < 64 ? ROWS : 64;
+  static_assert(BN / 16 % WAVES == 0 && BM / 16 % WAVES == 0 && SLOADS * SLANES == ROWS, "tile");
   // (with more slots a group's scales would be asked for while others read the ones they replace)
   static_assert((STAGES == 3 || STAGES == 4) && (STAGES - 1) * LOADS < 64, "ring depth");
 
@@ -171,33 +171,38 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
   // stored there is swizzled, so that fragment reads meet no bank twice
   const int kc = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
   const uint32_t lds0 = lds_address(lds);
-  const uint8_t *src[CODES];
-  uint32_t dst[CODES];
+  const uint8_t *src[LOADS], *scale_src[SLOADS];
+  uint32_t dst[LOADS];
 #pragma unroll
-  for (int i = 0; i < CODES; i++) {
+  for (int i = 0; i < LOADS; i++) {
     const int g = (i < A_LOADS ? i : i - A_LOADS) * WAVES + wave, s = g * 16 + (lane >> 2);
     src[i] = (i < A_LOADS ? weight_row(s) : input_row(s)) + kc;
     dst[i] = lds0 + (i < A_LOADS ? 0 : BN * 64) + g * 1024;
   }
-  // the scales of steps 4 * group ..: part `q` of the rows
+#pragma unroll
+  for (int i = 0; i < SLOADS; i++) {
+    const int s = wave * ROWS + i * 64 + (lane & (SLANES - 1));
+    scale_src[i] = (s < BN ? weight_row(s) : input_row(s - BN)) + (size_t)KT * kMxGroupBytes;
+  }
+  const uint32_t scale_dst = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + T::kRing + wave * ROWS * 16));
+  // the scales of steps 4 * group and on
   const int last_group = (KT - 1) >> 2;
-  auto issue_scales = [&](int group, int q) {
-    const int s0 = (q * WAVES + wave) * SL, s = s0 + lane;
-    if (lane < SL) {
-      const uint8_t *row = s < BN ? weight_row(s) : input_row(s - BN);
-      dma16(row + (size_t)KT * 64 + (size_t)min(group, last_group) * 16,
-            lds0 + T::kRing + (uint32_t)(group & 1) * T::kScales + (uint32_t)s0 * 16);
-    }
+  auto issue_scales = [&](int group) {
+    const uint32_t slot = (uint32_t)(group & 1) * T::kScales;
+    const int at = min(group, last_group) * 16;
+#pragma unroll
+    for (int i = 0; i < SLOADS; i++)
+      if (SLANES == 64 || lane < SLANES) dma16(scale_src[i] + at, slot, scale_dst + i * 1024);
   };
-  // load x of the step that goes to ring offset `ring`
+  // load x of a step, to ring offset `ring`; behind the last one of every fourth step the scales of
+  // the four steps that come after its own
   auto issue = [&](int step, uint32_t ring, int x) {
-    if (x < CODES) dma16(src[x] + (size_t)min(step, KT - 1) * 64, ring, dst[x]);
-    else issue_scales((step >> 2) + 1, step & 3);
+    dma16(src[x] + (size_t)min(step, KT - 1) * 64, ring, dst[x]);
+    if (x == LOADS - 1 && (step & 3) == 0) issue_scales((step >> 2) + 1);
   };
   constexpr int H0 = LOADS / 2;
   if (KT > 0) {
-#pragma unroll
-    for (int q = 0; q < 4; q++) issue_scales(0, q);
+    issue_scales(0);
 #pragma unroll
     for (int s = 0; s < STAGES - 1; s++)
 #pragma unroll
@@ -268,7 +273,9 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
   };
 
   if (KT > 0) {
-    dma_wait<(STAGES - 2) * LOADS + H0>();        // step 0 and the first scales have landed
+    // Step 0 and the first scales have landed. (The counts leave out that scales may be among the
+    // loads in flight: one of a step that need not have landed is waited for then.)
+    dma_wait<(STAGES - 2) * LOADS + H0>();
     __syncthreads();
     read_quads(0);
 #pragma unroll
