@@ -608,7 +608,9 @@ static int gn_launch(GroupNorm p, size_t N, hipStream_t st) {
   // 2^32 threads are a launch's limit: more samples than that go in turns
   const size_t per_sample = plan.wide ? (size_t)p.groups * kGnWideThreads
                                       : (size_t)p.slices * p.chunks * plan.threads;
-  const size_t most = std::max<size_t>(1, 0xf0000000ull / per_sample / 8 * 8);
+  if (per_sample > 0xf0000000ull / 8)
+    return fail(MI355X_ERR_NOT_SUPPORTED, "group_norm: %d channels in %d groups", p.C, p.groups);
+  const size_t most = 0xf0000000ull / per_sample / 8 * 8;
   const uint8_t *in = p.in;
   uint8_t *out = p.out;
   for (size_t done = 0; done < N; done += most) {

@@ -34,9 +34,17 @@ static FcTile fc_tile(long long M, long long K, long long N, bool mx4_out) {
   if (m32 * n32 <= most) return kFc32;
   if (K <= kShortGroups * kMxGroup)
     return N > 64 && ((N + 127) / 128) * ((M + 127) / 128) >= 512 ? kFcShort128 : kFcShort64;
-  if (((N + 255) / 256) * ((M + 255) / 256) >= 192) return kFc256;
-  if (((N + 127) / 128) * ((M + 127) / 128) >= 192) return kFc128;
-  return kFc64;
+  // Tiles through the ring: what a CU takes for its share of them, us behind a launch's own three, a
+  // tile's ends and its steps of K. Estimated / measured: 2048 x 2048 x 2048 in tiles of 64 / 128 / 256
+  // 15.5 / 8.9 / 23.2, 14 / 9 / 19; 1024 x 4096 x 4096 27 / 15.3 / 38, 24 / 14.7 / 27; 4096 x 8192 x
+  // 4096 - / 112 / 69, 169 / 98 / 65.
+  const double steps = (double)((K + kMxGroup - 1) / kMxGroup);
+  auto share = [&](long long tile) {
+    return (double)((((N + tile - 1) / tile) * ((M + tile - 1) / tile) + 255) / 256);
+  };
+  const double us64 = share(64) * (1.0 + 0.18 * steps), us128 = share(128) * (2.5 + 0.40 * steps),
+               us256 = share(256) * (8.0 + 0.95 * steps);
+  return us256 <= us128 && us256 <= us64 ? kFc256 : us128 <= us64 ? kFc128 : kFc64;
 }
 // Whether a float input is quantised by the kernel itself: every workgroup does so for its rows,
 // which a launch in front saves where they are many bytes, or shared by many workgroups. us, in the

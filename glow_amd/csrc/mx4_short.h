@@ -14,23 +14,22 @@ constexpr int kShortGroups = 4;
 
 template <class OUT, int BN, int BM, int WN, int WM>
 constexpr int mx4_short_bias(int groups) {
-  constexpr int kStaging = OUT::kSize ? (BN / WN) * (BM / WM) * 32 * (WN * OUT::kSize + 16) : 0;
-  const int main = groups * (BN + BM) * 64 + (BN + BM) * 16;
-  return main > kStaging ? main : kStaging;
+  typedef MxTile<OUT, BN, BM, WN, WM> T;
+  return groups * T::kStep + T::kScales > T::kStaging ? groups * T::kStep + T::kScales : T::kStaging;
 }
 
 template <class IN, class OUT, int BN, int BM, int WN, int WM, int BLOCKS>
 __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM / WM) / 4) void mx4_fc_short_kernel(
     MxFc p, int K, int tiles_n, int tiles_m) {
-  constexpr int WAVES = (BN / WN) * (BM / WM), TN = WN / 32, TM = WM / 32, THREADS = WAVES * 64;
+  typedef MxTile<OUT, BN, BM, WN, WM> T;
+  constexpr int WAVES = T::kWaves, TN = T::TN, TM = T::TM, THREADS = T::kThreads, kStep = T::kStep;
   constexpr int A_LOADS = BN / 16 / WAVES, B_LOADS = IN::kSize ? 0 : BM / 16 / WAVES;
-  constexpr int kStep = (BN + BM) * 64;
-  static_assert(BN / 16 % WAVES == 0 && BM / 16 % WAVES == 0 && THREADS >= BN && BN % 64 == 0 && BM % 64 == 0, "tile");
+  static_assert(BN / 16 % WAVES == 0 && BM / 16 % WAVES == 0 && BN % 64 == 0 && BM % 64 == 0, "tile");
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = wave % (BN / WN), wm = wave / (BN / WN);
-  const int l32 = lane & 31, half = lane >> 5;
+  const int wn = wave % T::kWavesN, wm = wave / T::kWavesN;
+  const int l16 = lane & 15, q = lane >> 4;
   int tm, tn;
   tile_of_block(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN, KT = p.groups;
@@ -38,7 +37,7 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
 
   // rows past the end re-read the last one; their results are not used
   auto weight_row = [&](int s) {
-    return p.weights + (size_t)min(n0 + (s & ~31) + perm_row16(s & 31), p.N - 1) * p.weights_row_bytes;
+    return p.weights + (size_t)min(n0 + mx4_weight_column<T::S>(s), p.N - 1) * p.weights_row_bytes;
   };
   auto input_row = [&](int s) { return p.in + (size_t)min(m0 + s, p.M - 1) * p.in_row_bytes; };
   float bias = 0.0f;
@@ -53,7 +52,7 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
       dma16((s < BN ? weight_row(s) : input_row(s - BN)) + (size_t)KT * kMxGroupBytes,
             lds0 + (uint32_t)(KT * kStep) + (uint32_t)s0 * 16);
     }
-    const int kc = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+    const int kc = ((lane & 3) ^ mx4_swizzle(lane >> 2)) * 16;
 #pragma unroll
     for (int i = 0; i < A_LOADS + B_LOADS; i++) {
       const int g = (i < A_LOADS ? i : i - A_LOADS) * WAVES + wave, s = g * 16 + (lane >> 2);
@@ -83,7 +82,7 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
               v4i codes;
               int byte;
               x[d][i].codes(codes, byte);
-              *reinterpret_cast<v4i *>(lds + (t + d) * kStep + (BN + s) * 64 + ((b ^ ((s >> 2) & 3)) << 4)) = codes;
+              *reinterpret_cast<v4i *>(lds + (t + d) * kStep + (BN + s) * 64 + ((b ^ mx4_swizzle(s)) << 4)) = codes;
               scales[(BN + s) * 16 + (t + d) * 4 + b] = (int8_t)byte;
             }
       }
@@ -92,34 +91,29 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
     __syncthreads();
   }
 
-  mx_v16f acc[TN][TM];
+  mx_v4f acc[TN][TM];
 #pragma unroll
   for (int i = 0; i < TN; i++)
 #pragma unroll
     for (int j = 0; j < TM; j++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
-  const int swz = (lane >> 2) & 3;
+      for (int r = 0; r < 4; r++) acc[i][j][r] = 0.0f;
+  const int frag_off = l16 * 64 + ((q ^ mx4_swizzle(l16)) << 4), byte_off = l16 * 16 + q;
   for (int t = 0; t < KT; t++) {
-    v4i frag[2][TN + TM];
+    v4i frag[TN + TM];
     int scale[TN + TM];
 #pragma unroll
     for (int f = 0; f < TN + TM; f++) {
-      const int row = (f < TN ? wn * WN + f * 32 : BN + wm * WM + (f - TN) * 32) + l32;
-#pragma unroll
-      for (int ks = 0; ks < 2; ks++)
-        frag[ks][f] = *reinterpret_cast<const v4i *>(lds + t * kStep + row * 64 + (((ks * 2 + half) ^ swz) << 4));
-      scale[f] = (int)(*reinterpret_cast<const uint32_t *>(scales + row * 16 + t * 4) >> (8 * half));
+      const int row = f < TN ? wn * WN + f * 16 : BN + wm * WM + (f - TN) * 16;
+      frag[f] = *reinterpret_cast<const v4i *>(lds + t * kStep + row * 64 + frag_off);
+      scale[f] = reinterpret_cast<const uint8_t *>(scales)[row * 16 + t * 4 + byte_off];
     }
 #pragma unroll
     for (int i = 0; i < TN; i++)
 #pragma unroll
-      for (int j = 0; j < TM; j++) {
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(frag[0][i]), fp4_operand(frag[0][TN + j]),
-                                                                    acc[i][j], 4, 4, 0, scale[i], 0, scale[TN + j]);
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(frag[1][i]), fp4_operand(frag[1][TN + j]),
-                                                                    acc[i][j], 4, 4, 2, scale[i], 2, scale[TN + j]);
-      }
+      for (int j = 0; j < TM; j++)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(frag[i]), fp4_operand(frag[TN + j]),
+                                                                     acc[i][j], 4, 4, 0, scale[i], 0, scale[TN + j]);
   }
   __syncthreads();
   mx4_tile_results<OUT, BN, BM, WN, WM>(acc, p, lds,
@@ -135,7 +129,7 @@ static int mx4_fc_short_launch(const MxFc &p, int K, hipStream_t st) {
   if (int rc = set_lds_attr(kern, lds(kShortGroups), attr_set)) return rc;
   const long long columns = OUT::kSize ? p.N : (long long)p.out_groups * kMxGroup;
   const long long tiles_n = (columns + BN - 1) / BN, tiles_m = ((long long)p.M + BM - 1) / BM;
-  constexpr int THREADS = (BN / WN) * (BM / WM) * 64;
+  constexpr int THREADS = MxTile<OUT, BN, BM, WN, WM>::kThreads;
   if (tiles_n * tiles_m > (1 << 22))
     return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_fc: %d x %d results", p.M, p.N);
   kern<<<(unsigned)(tiles_n * tiles_m), THREADS, lds(p.groups), st>>>(p, K, (int)tiles_n, (int)tiles_m);

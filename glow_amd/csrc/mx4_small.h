@@ -13,8 +13,6 @@
 
 namespace mi355x {
 
-typedef float mx_v4f __attribute__((ext_vector_type(4)));
-
 // What a lane holds of a block of an input row before it is multiplied.
 template <class IN> struct SmallBlock {
   typename IN::Eight v[4];

@@ -2,10 +2,15 @@
 // steps of 128 columns through a ring in LDS.
 //
 // A step is 64 bytes of codes of every row of both operands, moved from global memory
-// straight into LDS, and two slices of 64 columns for the matrix cores, whose lanes read one
-// block (16 bytes) each. Scale bytes travel apart from the codes, with every fourth step: 16
-// bytes of a row are four steps' words. Weights are the first operand and their rows are permuted on the way
-// into LDS: a lane ends with sixteen neighbouring columns of one output row.
+// straight into LDS, and one scaled matrix instruction of 16x16 results for each pair of
+// sixteen rows, whose lanes read one block (16 bytes) each. Scale bytes travel apart from the
+// codes, with every fourth step: 16 bytes of a row are four steps' words. Weights are the
+// first operand and their rows are permuted on the way into LDS: a lane ends with sixteen
+// neighbouring columns of one output row (eight, where a wave has 32).
+//
+// Random codes draw so much power that the instructions alone, from registers, reach 6.5
+// PFLOP/s in their 32x32 form and 7.5 in this one (zeros: 9.5); that is what bounds the large
+// tiles besides the ends of a tile, where all CUs write or wait together.
 #ifndef GLOW_MI355X_MX4_TILES_H
 #define GLOW_MI355X_MX4_TILES_H
 
@@ -15,7 +20,7 @@
 namespace mi355x {
 
 typedef int mx_v8i __attribute__((ext_vector_type(8)));
-typedef float mx_v16f __attribute__((ext_vector_type(16)));
+typedef float mx_v4f __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ mx_v8i fp4_operand(v4i v) { return mx_v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
 
@@ -30,146 +35,170 @@ struct MxFc {
   int act;
 };
 
-template <class OUT, int BN, int BM, int WN, int WM, int STAGES>
+// The place of weight rows in a tile's LDS: subtile t of the S that a group of 16 S columns has holds
+// in its row 4 q + i the group's column 4 S q + 4 t + i. A matrix instruction gives a lane rows 4 q .. 4
+// q + 3 (q = lane / 16) of each subtile: with these, 4 S neighbouring columns.
+template <int S> __device__ __forceinline__ int mx4_weight_column(int slot) {
+  const int in = slot & (16 * S - 1);
+  return (slot - in) + 4 * S * ((in >> 2) & 3) + 4 * (in >> 4) + (in & 3);
+}
+
+// Chunk k of a row lies at k ^ this in LDS. Reads of sixteen bytes are served sixteen lanes at a time,
+// 0-3, 12-15, 20-23 and 24-27 first: rows 0-3 and 12-15 of chunk 0, 4-11 of chunk 1. With these
+// they meet no bank twice.
+__device__ __forceinline__ int mx4_swizzle(int row) { return -(row >> 2) & 3; }
+
+template <class OUT, int BN, int BM, int WN, int WM>
 struct MxTile {
-  static constexpr int kWavesN = BN / WN, kWaves = (BN / WN) * (BM / WM);
-  static constexpr int kStage = (BN + BM) * 64;                       // a step's codes
-  static constexpr int kRing = STAGES * kStage;
-  static constexpr int kScales = (BN + BM) * 16;                      // four steps' scales
-  // a wave's results on their way out: 32 rows, 16 bytes apart from a whole number of banks
+  static constexpr int kWavesN = BN / WN, kWaves = (BN / WN) * (BM / WM), kThreads = kWaves * 64;
+  static constexpr int TN = WN / 16, TM = WM / 16;
+  static constexpr int S = TN < 4 ? TN : 4;                 // subtiles of a group of columns
+  static constexpr int kStep = (BN + BM) * 64;              // a step's codes
+  static constexpr int kScales = (BN + BM) * 16;            // four steps' scales
+  // a wave's results on their way out: 16 rows, 16 bytes apart from a whole number of banks
   static constexpr int kOutRow = WN * OUT::kSize + 16;
-  static constexpr int kStaging = OUT::kSize ? kWaves * 32 * kOutRow : 0;
-  static constexpr int kMain = kRing + 2 * kScales;
-  static constexpr int kBias = kMain > kStaging ? kMain : kStaging;   // where the biases lie
-  static constexpr size_t kLds = (size_t)kBias + BN * 4;
+  static constexpr int kStaging = OUT::kSize ? kWaves * 16 * kOutRow : 0;
+  static_assert(TN % S == 0 && S % 2 == 0 && kThreads >= BN, "tile");
 };
 
 // The end of a tile: biases, activation, and the results on their way out. `bias` is column
 // tid's; a wave stages its results in LDS where nothing that is still needed lies.
 template <class OUT, int BN, int BM, int WN, int WM>
-__device__ __forceinline__ void mx4_tile_results(mx_v16f (&acc)[WN / 32][WM / 32], const MxFc &p, int8_t *lds,
+__device__ __forceinline__ void mx4_tile_results(mx_v4f (&acc)[WN / 16][WM / 16], const MxFc &p, int8_t *lds,
                                                  float *s_bias, float bias, int m0, int n0) {
-  constexpr int TN = WN / 32, TM = WM / 32, kWavesN = BN / WN, kOutRow = WN * OUT::kSize + 16;
+  typedef MxTile<OUT, BN, BM, WN, WM> T;
+  constexpr int S = T::S, GROUPS = T::TN / S, COLS = 4 * S;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = wave % kWavesN, wm = wave / kWavesN;
-  const int l32 = lane & 31, half = lane >> 5;
+  const int wn = wave % T::kWavesN, wm = wave / T::kWavesN;
+  const int l16 = lane & 15, q = lane >> 4;
   if (tid < BN) s_bias[tid] = bias;
   __syncthreads();
 
   const int nw = n0 + wn * WN;                     // first column of this wave
   with_activation(p.act, [&](auto act) {
-  auto value = [&](int i, int j, int r) {          // column i * 32 + 16 * half + r of row j * 32 + l32
-    return activate<decltype(act)::value>(acc[i][j][r] + s_bias[wn * WN + i * 32 + 16 * half + r]);
-  };
-  if constexpr (OUT::kSize == 0) {
-    const int blocks = 4 * p.out_groups;
+    // column g * 16 S + 4 S q + r of row j * 16 + l16
+    auto value = [&](int g, int j, int r) {
+      return activate<decltype(act)::value>(acc[g * S + r / 4][j][r % 4] + s_bias[wn * WN + g * 16 * S + COLS * q + r]);
+    };
+    if constexpr (OUT::kSize == 0) {
+      const int blocks = 4 * p.out_groups;
 #pragma unroll
-    for (int j = 0; j < TM; j++) {
-      const int m = m0 + wm * WM + j * 32 + l32;
-      uint8_t *row = p.out + (size_t)m * p.out_row_bytes;
-      uint32_t bytes = 0;
+      for (int j = 0; j < T::TM; j++) {
+        const int m = m0 + wm * WM + j * 16 + l16;
+        uint8_t *row = p.out + (size_t)m * p.out_row_bytes;
+        uint8_t *scales = row + (size_t)p.out_groups * kMxGroupBytes;
 #pragma unroll
-      for (int i = 0; i < TN; i++) {
-        float x[2][8];
-        uint32_t most = 0;
+        for (int g = 0; g < GROUPS; g++) {
+          float x[COLS / 8][8];
+          uint32_t most = 0;
+          const int n = nw + g * 16 * S + COLS * q;
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const float y = value(i, j, r);
-          x[r >> 3][r & 7] = nw + i * 32 + 16 * half + r < p.N ? y : 0.0f;
-          most = max(most, magnitude_bits(x[r >> 3][r & 7]));
+          for (int r = 0; r < COLS; r++) {
+            const float y = value(g, j, r);
+            x[r / 8][r % 8] = n + r < p.N ? y : 0.0f;
+            most = max(most, magnitude_bits(x[r / 8][r % 8]));
+          }
+          // a block of 32 columns is two lanes' or four lanes'
+          most = max_across16(most);
+          if constexpr (S == 2) most = max_across32(most);
+          const uint32_t byte = mx4_scale_byte(most);
+          if (m < p.M && n / 32 < blocks) {
+            if constexpr (S == 4) {
+              *reinterpret_cast<uint2 *>(row + n / 2) = make_uint2(mx4_codes8(x[0], byte), mx4_codes8(x[1], byte));
+            } else {
+              *reinterpret_cast<uint32_t *>(row + n / 2) = mx4_codes8(x[0], byte);
+            }
+            if (n % 32 == 0) scales[n / 32] = (uint8_t)byte;
+          }
         }
-        most = max_across32(most);
-        const uint32_t byte = mx4_scale_byte(most);
-        bytes |= byte << (8 * i);
-        const uint32_t lo = mx4_codes8(x[0], byte), hi = mx4_codes8(x[1], byte);
-        if (m < p.M && nw / 32 + i < blocks)
-          *reinterpret_cast<uint2 *>(row + nw / 2 + i * 16 + 8 * half) = make_uint2(lo, hi);
+        // the zeros behind the last group's scales
+        if (m < p.M && nw / 32 <= blocks - 1 && blocks - 1 < (nw + WN) / 32 && q < ((-p.out_groups) & 3))
+          reinterpret_cast<uint32_t *>(scales)[p.out_groups + q] = 0;
       }
-      // (a wave's columns are whole groups, or a part of one: all of its blocks exist or none)
-      uint8_t *scales = row + (size_t)p.out_groups * kMxGroupBytes;
-      if (m < p.M && half == 0 && nw / 32 < blocks) {
-        if constexpr (TN == 4) *reinterpret_cast<uint32_t *>(scales + nw / 32) = bytes;
-        else if constexpr (TN == 2) *reinterpret_cast<uint16_t *>(scales + nw / 32) = (uint16_t)bytes;
-        else scales[nw / 32] = (uint8_t)bytes;
+    } else {
+      // through LDS: a lane's columns are a piece of a line, a row's columns of a wave whole ones
+      typedef typename OUT::T E;
+      constexpr int PER = 16 / OUT::kSize, LPR = WN / PER;   // columns of a store, lanes of a row
+      typedef E Chunk __attribute__((ext_vector_type(PER)));
+      typedef Chunk Chunk1 __attribute__((aligned(OUT::kSize)));
+      int8_t *stage = lds + wave * 16 * T::kOutRow;
+#pragma unroll
+      for (int j = 0; j < T::TM; j++) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++)
+#pragma unroll
+          for (int k = 0; k < COLS / PER; k++) {
+            Chunk c;
+#pragma unroll
+            for (int r = 0; r < PER; r++) c[r] = OUT::from(value(g, j, k * PER + r));
+            *reinterpret_cast<Chunk *>(stage + l16 * T::kOutRow + (g * 16 * S + COLS * q + k * PER) * OUT::kSize) = c;
+          }
+        wave_fence();
+        const int n = nw + (lane % LPR) * PER;
+        constexpr int kPass = 64 / LPR < 16 ? 64 / LPR : 16;
+#pragma unroll
+        for (int r0 = 0; r0 < 16; r0 += kPass) {
+          const int r = r0 + lane / LPR, m = m0 + wm * WM + j * 16 + r;
+          if (r < 16 && m < p.M && n < p.N) {
+            const Chunk c = *reinterpret_cast<const Chunk *>(stage + r * T::kOutRow + (lane % LPR) * 16);
+            E *at = reinterpret_cast<E *>(p.out + (size_t)m * p.out_row_bytes) + n;
+            if (n + PER <= p.N) *reinterpret_cast<Chunk1 *>(at) = c;
+            else
+#pragma unroll
+              for (int e = 0; e < PER; e++)
+                if (n + e < p.N) at[e] = c[e];
+          }
+        }
+        wave_fence();
       }
-      // the zeros behind the last group's scales
-      if (m < p.M && half == 1 && nw / 32 <= blocks - 1 && blocks - 1 < nw / 32 + TN)
-        for (int w = 0; w < ((-p.out_groups) & 3); w++) reinterpret_cast<uint32_t *>(scales)[p.out_groups + w] = 0;
     }
-  } else {
-    // through LDS: a lane's sixteen columns are a piece of a line, a row's columns of a wave whole ones
-    typedef typename OUT::T E;
-    constexpr int PER = 16 / OUT::kSize, LPR = WN / PER;   // columns of a store, lanes of a row
-    typedef E Chunk __attribute__((ext_vector_type(PER)));
-    typedef Chunk Chunk1 __attribute__((aligned(OUT::kSize)));
-    int8_t *stage = lds + wave * 32 * kOutRow;
-#pragma unroll
-    for (int j = 0; j < TM; j++) {
-#pragma unroll
-      for (int i = 0; i < TN; i++)
-#pragma unroll
-        for (int q = 0; q < 16 / PER; q++) {
-          Chunk c;
-#pragma unroll
-          for (int r = 0; r < PER; r++) c[r] = OUT::from(value(i, j, q * PER + r));
-          *reinterpret_cast<Chunk *>(stage + l32 * kOutRow + (i * 32 + 16 * half + q * PER) * OUT::kSize) = c;
-        }
-      wave_fence();
-      const int n = nw + (lane % LPR) * PER;
-#pragma unroll
-      for (int r0 = 0; r0 < 32; r0 += 64 / LPR) {
-        const int r = r0 + lane / LPR, m = m0 + wm * WM + j * 32 + r;
-        const Chunk c = *reinterpret_cast<const Chunk *>(stage + r * kOutRow + (lane % LPR) * 16);
-        if (m < p.M && n < p.N) {
-          E *at = reinterpret_cast<E *>(p.out + (size_t)m * p.out_row_bytes) + n;
-          if (n + PER <= p.N) *reinterpret_cast<Chunk1 *>(at) = c;
-          else
-            for (int e = 0; e < PER; e++)
-              if (n + e < p.N) at[e] = c[e];
-        }
-      }
-      wave_fence();
-    }
-  }
   });
 }
+
+template <class OUT, int BN, int BM, int WN, int WM, int STAGES>
+struct MxRing : MxTile<OUT, BN, BM, WN, WM> {
+  typedef MxTile<OUT, BN, BM, WN, WM> T;
+  static constexpr int kRing = STAGES * T::kStep, kMain = kRing + 2 * T::kScales;
+  static constexpr int kBias = kMain > T::kStaging ? kMain : T::kStaging;   // where the biases lie
+  static constexpr size_t kLds = (size_t)kBias + BN * 4;
+};
 
 template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS>
 __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM / WM) / 4) void mx4_fc_tile_kernel(
     MxFc p, int tiles_n, int tiles_m) {
-  typedef MxTile<OUT, BN, BM, WN, WM, STAGES> T;
-  constexpr int WAVES = T::kWaves, TN = WN / 32, TM = WM / 32;
+  typedef MxRing<OUT, BN, BM, WN, WM, STAGES> T;
+  constexpr int WAVES = T::kWaves, TN = T::TN, TM = T::TM;
   constexpr int A_LOADS = BN / 16 / WAVES, B_LOADS = BM / 16 / WAVES;  // 16 rows an instruction
   constexpr int LOADS = A_LOADS + B_LOADS;
   constexpr int ROWS = (BN + BM) / WAVES;                              // whose scales a wave moves
   constexpr int SLOADS = (ROWS + 63) / 64, SLANES = ROWS < 64 ? ROWS : 64;
   static_assert(BN / 16 % WAVES == 0 && BM / 16 % WAVES == 0 && SLOADS * SLANES == ROWS, "tile");
-  // (with more slots a group's scales would be asked for while others read the ones they replace)
-  static_assert((STAGES == 3 || STAGES == 4) && (STAGES - 1) * LOADS < 64, "ring depth");
+  // (with another number of slots scales would be asked for while others read the ones they replace)
+  static_assert(STAGES == 4 && (STAGES - 1) * LOADS + SLOADS < 64, "ring depth");
 
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave % T::kWavesN, wm = wave / T::kWavesN;
-  const int l32 = lane & 31, half = lane >> 5;
+  const int l16 = lane & 15, q = lane >> 4;
 
   int tm, tn;
   tile_of_block(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
   const int KT = p.groups;
 
-  // slot s of the weights' part of a ring slot holds this row; rows past the end re-read the
-  // last one, and their results are not used
-  auto weight_row = [&](int s) { return p.weights + (size_t)min(n0 + (s & ~31) + perm_row16(s & 31), p.N - 1) * p.weights_row_bytes; };
+  // rows past the end re-read the last one, and their results are not used
+  auto weight_row = [&](int s) {
+    return p.weights + (size_t)min(n0 + mx4_weight_column<T::S>(s), p.N - 1) * p.weights_row_bytes;
+  };
   auto input_row = [&](int s) { return p.in + (size_t)min(m0 + s, p.M - 1) * p.in_row_bytes; };
 
   float bias = 0.0f;
   if (tid < BN && p.bias && n0 + tid < p.N) bias = p.bias[n0 + tid];
 
-  // lane i of a load owns row i / 4 of its sixteen and the LDS chunk i % 4 of it; the chunk
-  // stored there is swizzled, so that fragment reads meet no bank twice
-  const int kc = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+  // lane i of a load owns row i / 4 of its sixteen and the LDS chunk i % 4 of it
+  const int kc = ((lane & 3) ^ mx4_swizzle(lane >> 2)) * 16;
   const uint32_t lds0 = lds_address(lds);
   const uint8_t *src[LOADS], *scale_src[SLOADS];
   uint32_t dst[LOADS];
@@ -194,11 +223,12 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
     for (int i = 0; i < SLOADS; i++)
       if (SLANES == 64 || lane < SLANES) dma16(scale_src[i] + at, slot, scale_dst + i * 1024);
   };
-  // load x of a step, to ring offset `ring`; behind the last one of every fourth step the scales of
-  // the four steps that come after its own
+  // Load x of a step, to ring offset `ring`; behind the last one of every fourth step the scales of
+  // the four steps that follow: step 4 g + 3 is asked for while step 4 g is multiplied, when every wave
+  // has read the last of the scales that these replace, those of steps up to 4 g - 1.
   auto issue = [&](int step, uint32_t ring, int x) {
     dma16(src[x] + (size_t)min(step, KT - 1) * 64, ring, dst[x]);
-    if (x == LOADS - 1 && (step & 3) == 0) issue_scales((step >> 2) + 1);
+    if (x == LOADS - 1 && (step & 3) == 3) issue_scales((step >> 2) + 1);
   };
   constexpr int H0 = LOADS / 2;
   if (KT > 0) {
@@ -206,70 +236,57 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
 #pragma unroll
     for (int s = 0; s < STAGES - 1; s++)
 #pragma unroll
-      for (int x = 0; x < LOADS; x++) issue(s, s * T::kStage, x);
+      for (int x = 0; x < LOADS; x++) issue(s, s * T::kStep, x);
 #pragma unroll
-    for (int x = 0; x < H0; x++) issue(STAGES - 1, (STAGES - 1) * T::kStage, x);
+    for (int x = 0; x < H0; x++) issue(STAGES - 1, (STAGES - 1) * T::kStep, x);
   }
 
-  mx_v16f acc[TN][TM];
+  mx_v4f acc[TN][TM];
 #pragma unroll
   for (int i = 0; i < TN; i++)
 #pragma unroll
     for (int j = 0; j < TM; j++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+      for (int r = 0; r < 4; r++) acc[i][j][r] = 0.0f;
 
-  const int swz = (lane >> 2) & 3;
-  int frag_off[2];
-#pragma unroll
-  for (int ks = 0; ks < 2; ks++) frag_off[ks] = l32 * 64 + (((ks * 2 + half) ^ swz) << 4);
-  const int a_base = wn * WN * 64, b_base = BN * 64 + wm * WM * 64;
-  v4i frag[2][TN + TM];
-  auto read_frag = [&](const int8_t *stage, int ks, int f) {
-    const int8_t *at = f < TN ? stage + a_base + f * 2048 : stage + b_base + (f - TN) * 2048;
-    frag[ks][f] = *reinterpret_cast<const v4i *>(at + frag_off[ks]);
+  // A lane reads block q of row l16 of a subtile and its scale byte. The weights' fragments are used
+  // row by row: those of the first half are replaced during the second, the others during the
+  // next step's first half; the input's next ones wait in registers of their own. (Two bodies that
+  // swap the two sets would save the moves, but the loop's two exits make copies of all results.)
+  const int frag_off = l16 * 64 + ((q ^ mx4_swizzle(l16)) << 4), byte_off = l16 * 16 + q;
+  v4i wf[TN], xf[TM], xn[TM];
+  int ws[TN], xs[TM], xsn[TM];
+  auto read_weights = [&](const int8_t *stage, const int8_t *scales, int i) {
+    wf[i] = *reinterpret_cast<const v4i *>(stage + (wn * WN + i * 16) * 64 + frag_off);
+    ws[i] = reinterpret_cast<const uint8_t *>(scales)[(wn * WN + i * 16) * 16 + byte_off];
   };
-  // four steps' scale words of the rows a lane feeds, the current step's first
-  v4i quad[TN + TM];
-  int scale[TN + TM];
-  auto read_quads = [&](int group) {
-    const int8_t *at = lds + T::kRing + (group & 1) * T::kScales + l32 * 16;
-#pragma unroll
-    for (int f = 0; f < TN + TM; f++)
-      quad[f] = *reinterpret_cast<const v4i *>(at + (f < TN ? wn * WN + f * 32 : BN + wm * WM + (f - TN) * 32) * 16);
+  auto read_input = [&](const int8_t *stage, const int8_t *scales, int j) {
+    xn[j] = *reinterpret_cast<const v4i *>(stage + (BN + wm * WM + j * 16) * 64 + frag_off);
+    xsn[j] = reinterpret_cast<const uint8_t *>(scales)[(BN + wm * WM + j * 16) * 16 + byte_off];
   };
-  auto take_scales = [&]() {
-    // a lane of the upper half feeds blocks 1 and 3 of a step: bytes 0 and 2 from here
-#pragma unroll
-    for (int f = 0; f < TN + TM; f++) {
-      scale[f] = (int)((uint32_t)quad[f][0] >> (8 * half));
-      quad[f] = v4i{quad[f][1], quad[f][2], quad[f][3], 0};
-    }
+  auto scales_of = [&](int step) {
+    return lds + T::kRing + ((step >> 2) & 1) * T::kScales + (step & 3) * 4;
   };
-  constexpr int MFMAS = TN * TM, FRAGS = TN + TM;
-  // the matrix instructions of a slice, memory operations of the next one spread between them
-  auto multiply = [&](auto ks, auto &&between) {
-    constexpr int KS = decltype(ks)::value;
+  constexpr int HALF = TN / 2, MFMAS = HALF * TM;
+  // half a step's matrix instructions, memory operations spread between them: a wave issues in
+  // order, so that a burst of them would hold back the instructions behind it
+  auto multiply = [&](auto half, int reads, auto &&read, int loads, auto &&load) {
+    constexpr int I0 = decltype(half)::value * HALF;
 #pragma unroll
-    for (int i = 0; i < TN; i++)
+    for (int i = 0; i < HALF; i++)
 #pragma unroll
       for (int j = 0; j < TM; j++) {
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-            fp4_operand(frag[KS][i]), fp4_operand(frag[KS][TN + j]), acc[i][j], 4, 4, 2 * KS, scale[i], 2 * KS,
-            scale[TN + j]);
+        const int t = i * TM + j;
+        acc[I0 + i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            fp4_operand(wf[I0 + i]), fp4_operand(xf[j]), acc[I0 + i][j], 4, 4, 0, ws[I0 + i], 0, xs[j]);
         __builtin_amdgcn_sched_barrier(0);
-        between(i * TM + j);
+#pragma unroll
+        for (int f = t * reads / MFMAS; f < (t + 1) * reads / MFMAS; f++) read(f);
+#pragma unroll
+        for (int x = 0; x < loads; x++)
+          if (min(MFMAS - 1, (2 * x + 1) * MFMAS / (2 * loads)) == t) load(x);
         __builtin_amdgcn_sched_barrier(0);
       }
-  };
-  auto frags_in_slot = [&](int t, const int8_t *stage, int ks) {
-#pragma unroll
-    for (int f = t * FRAGS / MFMAS; f < (t + 1) * FRAGS / MFMAS; f++) read_frag(stage, ks, f);
-  };
-  auto loads_in_slot = [&](int t, int step, uint32_t ring, int from, int n) {
-#pragma unroll
-    for (int x = 0; x < n; x++)
-      if (min(MFMAS - 1, (2 * x + 1) * MFMAS / (2 * n)) == t) issue(step, ring, from + x);
   };
 
   if (KT > 0) {
@@ -277,27 +294,32 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
     // loads in flight: one of a step that need not have landed is waited for then.)
     dma_wait<(STAGES - 2) * LOADS + H0>();
     __syncthreads();
-    read_quads(0);
 #pragma unroll
-    for (int f = 0; f < FRAGS; f++) read_frag(lds, 0, f);
-    uint32_t ring_cur = 0, ring_prev = (STAGES - 1) * T::kStage;
+    for (int j = 0; j < TM; j++) read_input(lds, scales_of(0), j);
+#pragma unroll
+    for (int i = 0; i < HALF; i++) read_weights(lds, scales_of(0), i);
+    uint32_t ring_cur = 0, ring_prev = (STAGES - 1) * T::kStep;
     for (int kt = 0; kt < KT; kt++) {
-      const uint32_t ring_next = ring_cur + T::kStage == T::kRing ? 0u : ring_cur + T::kStage;
+      const uint32_t ring_next = ring_cur + T::kStep == T::kRing ? 0u : ring_cur + T::kStep;
       const int8_t *cur = lds + ring_cur, *nxt = lds + ring_next;
-      take_scales();
-      multiply(std::integral_constant<int, 0>(), [&](int t) {
-        frags_in_slot(t, cur, 1);
-        loads_in_slot(t, kt + STAGES - 1, ring_prev, H0, LOADS - H0);
-      });
-      // step kt + 1 has landed once only the steps behind it are pending; past the barrier every
-      // wave holds step kt in registers, so that its slot is free
+      const int8_t *cur_scales = scales_of(kt), *nxt_scales = scales_of(kt + 1);
+#pragma unroll
+      for (int j = 0; j < TM; j++) xf[j] = xn[j], xs[j] = xsn[j];
+      multiply(
+          std::integral_constant<int, 0>(), HALF, [&](int f) { read_weights(cur, cur_scales, HALF + f); },
+          LOADS - H0, [&](int x) { issue(kt + STAGES - 1, ring_prev, H0 + x); });
+      // Step kt + 1 has landed once only the steps behind it are pending; past the barrier every
+      // wave holds step kt in registers, so that its slot is free.
       dma_wait<(STAGES - 2) * LOADS>();
       __syncthreads();
-      if ((kt & 3) == 3) read_quads((kt >> 2) + 1);
-      multiply(std::integral_constant<int, 1>(), [&](int t) {
-        frags_in_slot(t, nxt, 0);
-        loads_in_slot(t, kt + STAGES, ring_cur, 0, H0);
-      });
+      // (what is read past the last step is not used)
+      multiply(
+          std::integral_constant<int, 1>(), TM + HALF,
+          [&](int f) {
+            if (f < TM) read_input(nxt, nxt_scales, f);
+            else read_weights(nxt, nxt_scales, f - TM);
+          },
+          H0, [&](int x) { issue(kt + STAGES, ring_cur, x); });
       ring_prev = ring_cur;
       ring_cur = ring_next;
     }
@@ -309,7 +331,7 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
 
 template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS>
 static int mx4_fc_tile_launch(const MxFc &p, hipStream_t st) {
-  typedef MxTile<OUT, BN, BM, WN, WM, STAGES> T;
+  typedef MxRing<OUT, BN, BM, WN, WM, STAGES> T;
   auto kern = mx4_fc_tile_kernel<OUT, BN, BM, WN, WM, STAGES, BLOCKS>;
   static std::atomic<uint64_t> attr_set{0};
   if (int rc = set_lds_attr(kern, T::kLds, attr_set)) return rc;
@@ -318,7 +340,7 @@ static int mx4_fc_tile_launch(const MxFc &p, hipStream_t st) {
   const long long tiles_n = (columns + BN - 1) / BN, tiles_m = ((long long)p.M + BM - 1) / BM;
   if (tiles_n * tiles_m > (1 << 22))
     return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_fc: %d x %d results", p.M, p.N);
-  kern<<<(unsigned)(tiles_n * tiles_m), T::kWaves * 64, T::kLds, st>>>(p, (int)tiles_n, (int)tiles_m);
+  kern<<<(unsigned)(tiles_n * tiles_m), T::kThreads, T::kLds, st>>>(p, (int)tiles_n, (int)tiles_m);
   return check_launch("mx4_fc");
 }
 
