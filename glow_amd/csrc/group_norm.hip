@@ -87,13 +87,23 @@ __device__ __forceinline__ void gn_reduce(float (&x)[NP], float *s_part, float *
       if (NP < 8 || j >= from) s_part[(row << p.lg_vec) * NP + at + j] = x[j];
   }
   __syncthreads();
-  for (int g = wave; g < p.in_slice; g += waves) {
+  // many small groups: a thread each, instead of wave after wave
+  const int most = NP == 8 ? p.per : (p.per + 6) / 8 + 1;
+  const bool thread_each = p.in_slice > waves && most * rows <= 32;
+  for (int g = thread_each ? tid : wave; g < p.in_slice; g += thread_each ? (int)blockDim.x : waves) {
     // a group's parts in a row: `len` of them from `begin` on, `apart` places from each other; where
     // it begins within a vector, the first is that vector's second part
     const int channel = g * p.per;
     const int begin = NP == 8 ? channel : (channel >> 3) * NP, apart = NP == 2 ? 2 : 1;
     const int inner = NP == 2 && (channel & 7) ? 1 : 0;
     const int len = NP == 8 ? p.per : ((channel + p.per - 1) >> 3) - (channel >> 3) + 1;
+    if (thread_each) {
+      float t = 0;
+      for (int row = 0; row < rows; row++)
+        for (int k = 0; k < len; k++) t += s_part[(row << p.lg_vec) * NP + begin + k * apart + (k == 0 ? inner : 0)];
+      s_group[g] = t;
+      continue;
+    }
     float t = 0;
     if (len < 64) {
       for (int e = lane; e < len * rows; e += 64) {
@@ -530,11 +540,14 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
   const int parts = gn_parts(p.per);
   const int most_regs = size == 2 ? (parts == 1 ? 16 : 8) : (parts == 8 ? 4 : 8);
   auto fits = [&] { return p.pixels <= (long long)(kGnMost >> p.lg_vec) * most_regs; };
-  // Narrower slices where they are too few for the chip, or too large for a workgroup, down to
-  // 32 bytes: below, as many lines are asked for and less is used of each (64 x 3136 x 256 of
-  // fp16, slices of 64 / 32 / 16 bytes: 53 / 64 / 82 us).
-  const int wide = k;
-  while (k > unit && (long long)(k / 2 / unit * unit) * p.per * size >= 32 && ((long long)N * p.slices < 256 || !fits())) {
+  // Narrower slices where they are too few for the chip, or too large for a workgroup: as many lines
+  // are asked for then, and less is used of each (64 x 3136 x 256 of fp16, slices of 64 / 32 / 16
+  // bytes: 53 / 64 / 82 us), but the launch in front that parts need is saved (26 x 2733 x 32 of bf16:
+  // 16 bytes on one die 10.7, in parts 18.1; 7 x 870 x 96 of fp16: 24 bytes 10.2, 66 bytes 15.8; 1 x
+  // 3136 x 256 of fp16 over all dies: 16 bytes 12.7, in parts 9.1).
+  const int wide = k, least = by_die ? 16 : 24;
+  while (k > unit && (long long)(k / 2 / unit * unit) * p.per * size >= least &&
+         ((long long)N * p.slices < 256 || !fits())) {
     k = std::max(unit, k / 2 / unit * unit);
     set(k);
   }
