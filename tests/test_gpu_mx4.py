@@ -22,7 +22,7 @@ def spread(rng, rows, cols):
 
 @pytest.mark.parametrize("type_", TYPES)
 @pytest.mark.parametrize("rows, cols", [(1, 1), (1, 32), (3, 33), (5, 127), (2, 128), (7, 129), (61, 415), (33, 1000),
-                                        (1, 5000), (4, 2049), (300, 13), (1, 65537)])
+                                        (1, 5000), (4, 2049), (300, 13), (1, 65537), (8197, 2049), (270000, 65)])
 def test_quantize_is_the_definition(type_, rows, cols):
     x = ref.to_type(spread(np.random.default_rng(rows * cols), rows, cols), type_)
     np.testing.assert_array_equal(capi.mx4_quantize(x, type_), ref.rows_of(ref.to_f64(x, type_)))
