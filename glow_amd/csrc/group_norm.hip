@@ -16,6 +16,11 @@
 // Sums are exact in kind: a thread's own mean first and the squares of what is left of it,
 // then the threads' (or parts') means and what they are off the whole's; no difference of
 // large sums is ever formed, whatever the mean is.
+//
+// us: 64 x 3136 x 256 of fp16 53 (206 MB, 3.9 TB/s: 40 at the rate of a large copy; a workgroup fills a
+// CU and reads, computes and writes in turn), 32 x 784 x 512 of bf16 with SiLU to microscaled rows 16.5
+// (32 MB; 14.1 without SiLU: all CUs read, then compute, then write), 1 x 49 x 512 4.5 (the launch and
+// two rounds of sums), 4 x 16384 x 128 in parts 18, 3 x 1225 x 100 of fp32 in parts 8.9 (two launches).
 #include "mx4.h"
 
 #include <algorithm>
@@ -205,7 +210,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
   const int twice = NP > 1 && OUT::kSize && c < c_end && c_end - c0 >= 8 ? max(0, c + 8 - c_end) : 0;
   c -= twice;
   const int left = c_end - c;
-  const int px0 = chunk * p.chunk_pixels, px_end = min(p.pixels, px0 + p.chunk_pixels);
+  const int px0 = chunk * p.chunk_pixels, px_end = px0 + min(p.chunk_pixels, p.pixels - px0);
   const uint8_t *in = p.in + (size_t)sample * p.pixels * p.in_row_bytes + (ptrdiff_t)c * E::kSize;
 
   typename E::Eight raw[R];
@@ -362,19 +367,21 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
       const GroupStats *s = p.stats + ((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks;
       GroupStats own[kGnMostChunks / 64];
       float m = 0, q = 0;
+      auto values = [&](int k) {     // of part k
+        return (float)min(p.chunk_pixels, p.pixels - min(k, p.chunks - 1) * p.chunk_pixels) * of_group;
+      };
 #pragma unroll
       for (int i = 0; i < kGnMostChunks / 64; i++) {
         const int k = lane + 64 * i;
         own[i] = k < p.chunks ? s[k] : GroupStats{0, 0};
-        const float n = (float)min(p.chunk_pixels, p.pixels - k * p.chunk_pixels) * of_group;
-        if (k < p.chunks) m = fmaf(own[i].mean, n, m);
+        if (k < p.chunks) m = fmaf(own[i].mean, values(k), m);
       }
       m = wave_sum(m) / total;
 #pragma unroll
       for (int i = 0; i < kGnMostChunks / 64; i++) {
         const int k = lane + 64 * i;
-        const float n = (float)min(p.chunk_pixels, p.pixels - k * p.chunk_pixels) * of_group, d = own[i].mean - m;
-        if (k < p.chunks) q += fmaf(d * d, n, own[i].square);
+        const float d = own[i].mean - m;
+        if (k < p.chunks) q += fmaf(d * d, values(k), own[i].square);
       }
       q = wave_sum(q);
       if (lane == 0) {
@@ -429,8 +436,9 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
   }
 }
 
-// Groups too wide for a workgroup's lanes: a workgroup finds a group's mean and squares in
-// two passes over it, then sixteen lanes take 128 channels of a pixel.
+// Slices too wide for a workgroup's lanes, over 8192 channels (a group of that many, or 32 of an odd
+// number each to microscaled rows): a workgroup finds a group's mean and squares in two passes
+// over it, then sixteen lanes take 128 channels of a pixel.
 constexpr int kGnWideThreads = 256;
 
 __device__ __forceinline__ float block_sum(float v, float *s_part) {
@@ -501,7 +509,8 @@ __global__ __launch_bounds__(kGnWideThreads) void group_norm_wide_apply_kernel(G
 
 // ---- how a call is cut -------------------------------------------------------------
 
-// Parts of a slice: enough for four workgroups a CU over the whole call.
+// The most parts that a slice of this call may be cut into, whatever its types: what the workspace has
+// room for.
 static int gn_most_chunks(size_t N, size_t pixels) {
   const size_t n = N < 1024 ? 1024 / N : 1;
   return (int)std::min<size_t>({n, pixels, (size_t)kGnMostChunks});

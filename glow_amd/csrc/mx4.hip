@@ -4,8 +4,13 @@
 namespace mi355x {
 
 // A lane holds eight neighbouring columns, sixteen lanes a group, and a workgroup of 256
-// threads sixteen groups: up to sixteen of one row, or one each of sixteen rows. Both
-// kernels are bound by what they move; the conversion is one instruction for two values.
+// threads sixteen groups: up to sixteen of one row, or one each of sixteen rows. A block is
+// four lanes: its largest magnitude takes two exchanges of neighbouring lanes, and 16-bit values
+// are neither widened for that nor for the conversion, one instruction for two values.
+//
+// Bound by what they move: 8192 x 4096 of bf16 21 us to microscaled rows and 14 us back (85 MB
+// each: 4.0 and 6.0 TB/s, where copying 1 GiB reaches 5.2 and 100 MiB in the last-level cache
+// 8.3). Four shares a thread with their loads ahead of the first conversion take longer (25 and 15).
 constexpr int kMxThreads = 256;
 
 struct MxRows {

@@ -38,6 +38,57 @@ def test_group_norm(n, pixels, C, groups, type_):
         ref.check_mx4(rows.reshape(n * pixels, -1), C, want.reshape(n * pixels, C), err.reshape(n * pixels, C))
 
 
+@pytest.mark.parametrize("seed", range(48))
+def test_group_norm_of_random_shapes(seed):
+    """Groups of 1 to 60 channels, samples enough for slices on one die, rows apart by any number of
+    elements and from any element on, each result type, in place."""
+    rng = np.random.default_rng(1000 + seed)
+    type_ = int(rng.integers(0, 3))
+    size = 4 if type_ == ref.F32 else 2
+    per, groups = int(rng.integers(1, 61)), int(rng.integers(1, 40))
+    C = per * groups
+    n = int(np.exp(rng.uniform(0, np.log(40))))
+    pixels = int(np.exp(rng.uniform(0, np.log(max(2, 1_500_000 // (C * n))))))
+    act, gap, start = int(rng.choice([0, 1, 6])), int(rng.integers(0, 4)), int(rng.integers(0, 5))
+    x = image(rng, n, pixels, C, type_)
+    gamma, beta = (1 + 0.3 * rng.normal(0, 1, C)).astype(np.float32), rng.normal(0, 1, C).astype(np.float32)
+    want, err = ref.group_norm(ref.to_f64(x, type_), groups, gamma, beta, 1e-5, act)
+    wide = np.zeros((n * pixels, C + gap), x.dtype)
+    wide[:, :C] = x.reshape(-1, C)
+    flat = np.concatenate([np.zeros(start, x.dtype), wide.reshape(-1)])
+    dx, dg, db = capi.to_device(flat), capi.to_device(gamma), capi.to_device(beta)
+    ws_bytes = capi.group_norm_workspace_bytes(n, pixels, C, groups)
+    ws = capi.DeviceBuffer(ws_bytes)
+    pitch = (C + gap) * size
+    row = capi.mx4_row_bytes(C)
+    rows = capi.to_device(np.full((n * pixels, row + 16), 0xA5, np.uint8))
+    args = (dg, db, n, pixels, C, groups, 1e-5, act, ws, ws_bytes)
+    capi.launch_group_norm(rows, capi.TYPE_MX4, row + 16, dx.ptr + start * size, type_, pitch, *args)
+    got = rows.numpy()
+    assert (got[:, row:] == 0xA5).all()
+    ref.check_mx4(got[:, :row], C, want.reshape(-1, C), err.reshape(-1, C))
+    out = capi.to_device(np.zeros(flat.size, x.dtype))
+    capi.launch_group_norm(out.ptr + start * size, type_, pitch, dx.ptr + start * size, type_, pitch, *args)
+    apart = out.numpy()
+    capi.launch_group_norm(dx.ptr + start * size, type_, pitch, dx.ptr + start * size, type_, pitch, *args)
+    np.testing.assert_array_equal(dx.numpy(), apart)        # (the gaps are zero on both sides)
+    vals = apart[start:].reshape(n * pixels, C + gap)
+    assert not vals[:, C:].any()
+    ref.check_float(np.ascontiguousarray(vals[:, :C]).reshape(x.shape), want, err, type_)
+
+
+@pytest.mark.parametrize("type_", [ref.F32, ref.F16])
+@pytest.mark.parametrize("n, pixels, C, groups", [(2, 3, 20000, 2), (1, 5, 9000, 1), (3, 2, 8200, 8), (2, 2, 31 * 300, 300)])
+def test_slices_wider_than_a_workgroup(type_, n, pixels, C, groups):
+    rng = np.random.default_rng(C)
+    x = image(rng, n, pixels, C, type_)
+    beta = rng.normal(0, 1, C).astype(np.float32)
+    want, err = ref.group_norm(ref.to_f64(x, type_), groups, None, beta, 1e-5, 6)
+    ref.check_float(capi.group_norm(x, groups, None, beta, 1e-5, 6, type_), want, err, type_)
+    rows = capi.group_norm(x, groups, None, beta, 1e-5, 6, type_, capi.TYPE_MX4)
+    ref.check_mx4(rows.reshape(n * pixels, -1), C, want.reshape(-1, C), err.reshape(-1, C))
+
+
 @pytest.mark.parametrize("n, pixels, C, groups", [(2, 3136, 64, 8), (1, 49, 512, 32), (1, 30000, 32, 4)])
 def test_errors_are_of_32_bits(n, pixels, C, groups):
     # the norm of the error of sums whose roundings go either way: well under a hundred of the

@@ -227,6 +227,111 @@ def test_fc_of_strided_rows_leaves_the_rest_alone(M, K, N, in_type, out_type):
     check(body, want, err, out_type, N)
 
 
+@pytest.mark.parametrize("seed", range(60))
+def test_fc_of_random_shapes(seed):
+    rng = np.random.default_rng(2000 + seed)
+    M, K, N = (int(np.exp(rng.uniform(0, np.log(top)))) for top in (3000, 3000, 3000))
+    while M * K * N > 2_000_000_000:
+        K = max(1, K // 2)
+    in_type, out_type, act = int(rng.integers(0, 4)), int(rng.integers(0, 4)), int(rng.choice([0, 1, 6]))
+    x, a, w = product(rng, M, K, N, in_type)
+    bias = rng.normal(0, 1, N).astype(np.float32) if rng.random() < 0.7 else None
+    want, err = ref.fc(a, ref.values(w, K), None if bias is None else bias.astype(np.float64), act)
+    got = capi.mx4_fc(x, in_type, w, bias, K, out_type, act)
+    check(got, want, err, out_type, N)
+    np.testing.assert_array_equal(capi.mx4_fc(x, in_type, w, bias, K, out_type, act), got)   # equal calls, equal bits
+
+
+class FarRows:
+    """Rows of device memory `pitch` bytes apart, over 4 GiB in all."""
+
+    def __init__(self, rows, pitch):
+        self.rows, self.pitch = rows, pitch
+        self.memory = capi.DeviceBuffer((rows - 1) * pitch + (1 << 20))
+
+    def put(self, a):
+        a = np.ascontiguousarray(a)
+        for r in range(self.rows):
+            capi.check(capi.lib().mi355x_memcpy_h2d(capi._vp(self.memory.ptr + r * self.pitch), capi._vp(a[r]),
+                                                    capi._sz(a[r].nbytes), None))
+        capi.sync()
+        return self
+
+    def get(self, cols, dtype):
+        out = np.empty((self.rows, cols), dtype)
+        capi.sync()
+        for r in range(self.rows):
+            capi.check(capi.lib().mi355x_memcpy_d2h(capi._vp(out[r]), capi._vp(self.memory.ptr + r * self.pitch),
+                                                    capi._sz(out[r].nbytes), None))
+        capi.sync()
+        return out
+
+
+@pytest.mark.parametrize("M, K, N", [(3, 200, 3), (290, 256, 290), (290, 700, 290)])
+def test_rows_past_4_gib(M, K, N):
+    rng = np.random.default_rng(K)
+    pitch = (5 << 30) // (min(M, N) - 1) // 16 * 16
+    x, a, w = product(rng, M, K, N, ref.F16)
+    want, err = ref.fc(a, ref.values(w, K), None, 0)
+    far_x, far_w = FarRows(M, pitch).put(x), FarRows(N, pitch).put(w)
+    far_q, far_out = FarRows(M, pitch), FarRows(M, pitch)
+    capi.launch_mx4_quantize(far_q.memory, pitch, far_x.memory, ref.F16, pitch, M, K)
+    rows = ref.rows_of(ref.to_f64(x, ref.F16))
+    np.testing.assert_array_equal(far_q.get(rows.shape[1], np.uint8), rows)
+    capi.launch_mx4_fc(far_out.memory, ref.F32, pitch, far_q.memory, ref.MX4, pitch, far_w.memory, pitch, None, M, K, N)
+    ref.check_float(far_out.get(N, np.float32), want, err, ref.F32)
+    n = capi.mx4_fc_workspace_bytes(M, K, N, ref.F16)
+    ws = capi.DeviceBuffer(max(n, 1))
+    capi.launch_mx4_fc(far_out.memory, ref.MX4, pitch, far_x.memory, ref.F16, pitch, far_w.memory, pitch, None, M, K, N, 0,
+                       ws if n else None, n)
+    ref.check_mx4(far_out.get(capi.mx4_row_bytes(N), np.uint8), N, want, err)
+    capi.launch_mx4_dequantize(far_x.memory, ref.F16, pitch, far_q.memory, pitch, M, K)
+    np.testing.assert_array_equal(far_x.get(K, np.float16), ref.to_type(ref.values(rows, K), ref.F16))
+    # and the pixels of a group norm
+    C, groups = min(K, 64), 4
+    y, yerr = ref.group_norm(a[None, :, :C], groups, None, None, 1e-5, 1)
+    wsn = capi.group_norm_workspace_bytes(1, M, C, groups)
+    ws = capi.DeviceBuffer(wsn)
+    capi.launch_group_norm(far_out.memory, ref.F16, pitch, far_x.memory, ref.F16, pitch, None, None, 1, M, C, groups, 1e-5,
+                           1, ws, wsn)
+    ref.check_float(far_out.get(C, np.float16)[None], y, yerr, ref.F16)
+
+
+@pytest.mark.parametrize("M, N", [(2, 100), (40, 2000), (2100, 2100)])
+def test_first_call_inside_a_capture(M, N):
+    """Nothing has to have run before: attributes of a kernel are no stream's work."""
+    rng = np.random.default_rng(N)
+    K = 640
+    x, a, w = product(rng, M, K, N, ref.MX4)
+    dx, dw, stream = capi.to_device(x), capi.to_device(w), capi.Stream()
+    out = capi.DeviceBuffer.empty((M, N), np.float16)
+    with capi.Graph(stream) as graph:
+        capi.launch_mx4_fc(out, ref.F16, 2 * N, dx, ref.MX4, x.shape[1], dw, w.shape[1], None, M, K, N, 0, None, 0, stream)
+    want, err = ref.fc(a, ref.values(w, K), None, 0)
+    for _ in range(3):
+        out.fill(0xEE, stream)
+        graph.launch(stream)
+        check(out.numpy(stream), want, err, ref.F16, N)
+        capi.sync()
+
+
+def test_two_streams_at_once():
+    rng = np.random.default_rng(77)
+    shapes = [(700, 600, 900), (5, 900, 3000)]
+    jobs = []
+    for M, K, N in shapes:
+        x, a, w = product(rng, M, K, N, ref.F16)
+        n = capi.mx4_fc_workspace_bytes(M, K, N, ref.F16)
+        jobs.append((M, K, N, capi.to_device(x), capi.to_device(w), w.shape[1], capi.DeviceBuffer(max(n, 1)), n,
+                     capi.DeviceBuffer.empty((M, N), np.float32), capi.Stream(), ref.fc(a, ref.values(w, K), None, 0)))
+    for _ in range(4):
+        for M, K, N, dx, dw, pitch, ws, n, out, stream, _ in jobs:
+            capi.launch_mx4_fc(out, ref.F32, 4 * N, dx, ref.F16, 2 * K, dw, pitch, None, M, K, N, 0, ws if n else None, n,
+                               stream)
+    for M, K, N, *_, out, stream, (want, err) in jobs:
+        check(out.numpy(stream), want, err, ref.F32, N)
+
+
 def test_tower_hands_rows_on_and_replays():
     """Three layers as a ranking net runs them, on a stream of their own and from a graph that
     is replayed with other inputs, the library's own work between the replays."""
