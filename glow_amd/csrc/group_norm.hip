@@ -161,10 +161,13 @@ __device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, int twic
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     const float x = E::kSize == 2 ? E::get(raw, j) : E::get(raw, j) - mean[NM == 1 ? 0 : j];
-    const float v = activate<ACT>(fmaf(x, scale[j], shift[j]));
-    y[j] = OUT::kSize || j < left ? v : 0.0f;
+    y[j] = activate<ACT>(fmaf(x, scale[j], shift[j]));
   }
   if constexpr (OUT::kSize == 0) {
+    if (__ballot(left < 8)) {        // (a branch, not a selection for every value of every pixel)
+#pragma unroll
+      for (int j = 0; j < 8; j++) y[j] = j < left ? y[j] : 0.0f;
+    }
     const uint32_t byte = mx4_scale_byte(quad_max(largest8(y)));
     if (block_inside) {
       *reinterpret_cast<uint32_t *>(row + (c >> 1)) = mx4_codes8(y, byte);

@@ -140,10 +140,11 @@ template <class F> __device__ __forceinline__ void with_activation(int act, F &&
 // as whole numbers are, infinity above every number and NaN above infinity.
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t largest8(const float (&x)[8]) {
-  uint32_t m = 0;
+  // (maximum, unlike max, gives NaN as soon as one is NaN)
+  float m = __builtin_fabsf(x[0]);
 #pragma unroll
-  for (int j = 0; j < 8; j++) m = max(m, magnitude_bits(x[j]));
-  return m;
+  for (int j = 1; j < 8; j++) m = __builtin_elementwise_maximum(m, __builtin_fabsf(x[j]));
+  return magnitude_bits(m);
 }
 // The scale byte of a block whose largest magnitude has these bits: its exponent less the 2
 // of E2M1's largest value, 0 at least; 255, NaN, for infinities and NaN.

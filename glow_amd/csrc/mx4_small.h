@@ -7,9 +7,13 @@
 // is quantised there and then: a lane has its whole block, so that no lane needs another one's
 // values, and no launch in front is needed. Partial results meet in LDS.
 //
+// Up to four rows are quantised by the workgroup as a whole, a thread a block, into LDS, while
+// the weights are on their way: left to the waves, each lane would load and convert the row that
+// its number modulo sixteen stands for, the last one again and again.
+//
 // What bounds it: the launch (3 us), one round of loads of every wave, and the rate at which a CU
 // pulls rows from L2. One row, 4096 x 4096: 4.4 us from a microscaled row (9 MB of weights, 1.7 us at
-// the rate of a large copy), 6.1 from fp16, whose conversion every workgroup repeats. 128 x 1024 x
+// the rate of a large copy), 4.8 from fp16 (6.1 converted by the waves). 128 x 1024 x
 // 1024 of bf16 4.9, 61 x 415 x 509 of fp32 3.5 (rows x K x columns). Other splits of the eight waves,
 // over input rows as well as K, are slower wherever K has a group for each.
 #ifndef GLOW_MI355X_MX4_SMALL_H
@@ -53,10 +57,16 @@ template <> struct SmallBlock<MX4> {
 
 constexpr int kSmallWaves = 8;
 
-template <class IN, class OUT, int MT, int NT>
+constexpr int kSharedRows = 4;
+// Bytes from one shared row to the next in LDS: its codes, its scales, and 16 so that rows of a power of
+// two do not lie on the same banks.
+__host__ __device__ constexpr int mx4_shared_row(int groups) { return (groups * (kMxGroupBytes + 4) + 15) / 16 * 16 + 16; }
+
+template <class IN, class OUT, int MT, int NT, bool SHARED>
 __global__ __launch_bounds__(kSmallWaves * 64, 2) void mx4_fc_small_kernel(MxFc p, int K, int tiles_n) {
   // groups in flight: as many as their registers allow
-  constexpr int kRegs = IN::kSize == 0 ? 5 : IN::kSize * 8;
+  static_assert(!SHARED || (MT == 1 && IN::kSize), "shared rows");
+  constexpr int kRegs = IN::kSize == 0 || SHARED ? 5 : IN::kSize * 8;
   constexpr int D = kRegs * MT <= 20 ? 4 : kRegs * MT <= 32 ? 2 : 1;
   constexpr int kTiles = MT * NT;
   __shared__ float s_part[kSmallWaves][kTiles * 4][64];
@@ -76,21 +86,60 @@ __global__ __launch_bounds__(kSmallWaves * 64, 2) void mx4_fc_small_kernel(MxFc 
 
   const int per = (p.groups + kSmallWaves - 1) / kSmallWaves;
   const int g_begin = wave * per, g_end = min(p.groups, g_begin + per);
-  if (g_begin < g_end) {
-    // rows past the end re-read the last one; what they give is not stored
-    const uint8_t *w[NT], *x[MT];
+  // rows past the end re-read the last one; what they give is not stored
+  const uint8_t *w[NT];
 #pragma unroll
-    for (int c = 0; c < NT; c++) w[c] = p.weights + (size_t)min(n0 + c * 16 + row, p.N - 1) * p.weights_row_bytes;
+  for (int c = 0; c < NT; c++) w[c] = p.weights + (size_t)min(n0 + c * 16 + row, p.N - 1) * p.weights_row_bytes;
+  SmallBlock<MX4> wf[D][NT];
+  auto load_weights = [&](int g0) {
 #pragma unroll
-    for (int a = 0; a < MT; a++) x[a] = p.in + (size_t)min(m0 + a * 16 + row, p.M - 1) * p.in_row_bytes;
+    for (int d = 0; d < D; d++)
+      if (g0 + d < g_end) {
+#pragma unroll
+        for (int c = 0; c < NT; c++) wf[d][c].load(w[c], p.groups, g0 + d, b, 0);
+      }
+  };
+  auto multiply = [&](int d, int a, v4i codes, int byte) {
+#pragma unroll
+    for (int c = 0; c < NT; c++)
+      acc[a][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(wf[d][c].v), fp4_operand(codes),
+                                                                   acc[a][c], 4, 4, 0, wf[d][c].s, 0, byte);
+  };
+  if constexpr (SHARED) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t s_rows[];
+    const int row_bytes = mx4_shared_row(p.groups), blocks = 4 * p.groups;
+    load_weights(g_begin);
+    for (int m = 0; m < min(kSharedRows, p.M - m0); m++)
+      for (int u = tid; u < blocks; u += kSmallWaves * 64) {
+        SmallBlock<IN> x;
+        x.load(p.in + (size_t)(m0 + m) * p.in_row_bytes, p.groups, u >> 2, u & 3, K);
+        v4i codes;
+        int byte;
+        x.codes(codes, byte);
+        *reinterpret_cast<v4i *>(s_rows + m * row_bytes + u * 16) = codes;
+        s_rows[m * row_bytes + blocks * 16 + u] = (uint8_t)byte;
+      }
+    __syncthreads();
+    const uint8_t *mine = s_rows + min(row, min(kSharedRows, p.M - m0) - 1) * row_bytes;
     for (int g0 = g_begin; g0 < g_end; g0 += D) {
-      SmallBlock<MX4> wf[D][NT];
-      SmallBlock<IN> xf[D][MT];
+      if (g0 != g_begin) load_weights(g0);
 #pragma unroll
       for (int d = 0; d < D; d++)
         if (g0 + d < g_end) {
+          const int u = (g0 + d) * 4 + b;
+          multiply(d, 0, *reinterpret_cast<const v4i *>(mine + u * 16), mine[blocks * 16 + u]);
+        }
+    }
+  } else {
+    const uint8_t *x[MT];
 #pragma unroll
-          for (int c = 0; c < NT; c++) wf[d][c].load(w[c], p.groups, g0 + d, b, 0);
+    for (int a = 0; a < MT; a++) x[a] = p.in + (size_t)min(m0 + a * 16 + row, p.M - 1) * p.in_row_bytes;
+    for (int g0 = g_begin; g0 < g_end; g0 += D) {
+      SmallBlock<IN> xf[D][MT];
+      load_weights(g0);
+#pragma unroll
+      for (int d = 0; d < D; d++)
+        if (g0 + d < g_end) {
 #pragma unroll
           for (int a = 0; a < MT; a++) xf[d][a].load(x[a], p.groups, g0 + d, b, K);
         }
@@ -102,10 +151,7 @@ __global__ __launch_bounds__(kSmallWaves * 64, 2) void mx4_fc_small_kernel(MxFc 
             v4i codes;
             int byte;
             xf[d][a].codes(codes, byte);
-#pragma unroll
-            for (int c = 0; c < NT; c++)
-              acc[a][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                  fp4_operand(wf[d][c].v), fp4_operand(codes), acc[a][c], 4, 4, 0, wf[d][c].s, 0, byte);
+            multiply(d, a, codes, byte);
           }
         }
     }
@@ -184,7 +230,15 @@ static int mx4_fc_small_launch(const MxFc &p, int K, hipStream_t st) {
   const long long tiles_n = (columns + 16 * NT - 1) / (16 * NT);
   const long long blocks = tiles_n * (((long long)p.M + 16 * MT - 1) / (16 * MT));
   if (blocks > (1 << 22)) return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_fc: %d x %d results", p.M, p.N);
-  mx4_fc_small_kernel<IN, OUT, MT, NT><<<(unsigned)blocks, kSmallWaves * 64, 0, st>>>(p, K, (int)tiles_n);
+  if constexpr (IN::kSize && MT == 1) {
+    if (p.M <= kSharedRows) {
+      // (at most 96 KB of values are quantised here: a quarter of that and the pads)
+      const size_t lds = (size_t)p.M * mx4_shared_row(p.groups);
+      mx4_fc_small_kernel<IN, OUT, MT, NT, true><<<(unsigned)blocks, kSmallWaves * 64, lds, st>>>(p, K, (int)tiles_n);
+      return check_launch("mx4_fc");
+    }
+  }
+  mx4_fc_small_kernel<IN, OUT, MT, NT, false><<<(unsigned)blocks, kSmallWaves * 64, 0, st>>>(p, K, (int)tiles_n);
   return check_launch("mx4_fc");
 }
 
