@@ -557,7 +557,8 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
   // bytes: 53 / 64 / 82 us), but the launch in front that parts need is saved (26 x 2733 x 32 of bf16:
   // 16 bytes on one die 10.7, in parts 18.1; 7 x 870 x 96 of fp16: 24 bytes 10.2, 66 bytes 15.8; 1 x
   // 3136 x 256 of fp16 over all dies: 16 bytes 12.7, in parts 9.1).
-  const int wide = k, least = by_die ? 16 : 24;
+  // A vector of eight channels is the least (16 x 3136 x 40 of fp32 in 8 groups: 20 bytes 26, in parts 18).
+  const int wide = k, least = by_die ? 8 * size : std::max(24, 8 * size);
   while (k > unit && (long long)(k / 2 / unit * unit) * p.per * size >= least &&
          ((long long)N * p.slices < 256 || !fits())) {
     k = std::max(unit, k / 2 / unit * unit);
@@ -573,7 +574,8 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
     plan.regs = 1;
     auto holds = [&] { return (long long)(plan.threads >> p.lg_vec) * plan.regs; };
     while (holds() < p.pixels) {
-      if (plan.regs < 4 || plan.threads >= kGnMost || (plan.threads >= 512 && plan.regs < 8)) plan.regs *= 2;
+      if (plan.regs < 4 || (plan.threads >= 512 && plan.regs < std::min(8, most_regs)) || plan.threads >= kGnMost)
+        plan.regs *= 2;
       else plan.threads *= 2;
     }
     p.chunks = 1;

@@ -77,6 +77,17 @@ def test_group_norm_of_random_shapes(seed):
     ref.check_float(np.ascontiguousarray(vals[:, :C]).reshape(x.shape), want, err, type_)
 
 
+@pytest.mark.parametrize("type_", [ref.F32, ref.F16, ref.BF16])
+@pytest.mark.parametrize("per", [1, 2, 3, 4, 5, 6, 7, 8, 9, 12, 16, 20, 31])
+def test_large_slices_of_every_kind_of_group(per, type_):
+    """Slices that fill a workgroup to the last pixel it can hold, one more, and far more."""
+    rng = np.random.default_rng(per)
+    for n, pixels, groups in ((16, 1024, 8), (16, 1025, 8), (16, 2047, 8), (9, 4097, 3), (130, 1500, 1)):
+        x = image(rng, n, pixels, per * groups, type_)
+        want, err = ref.group_norm(ref.to_f64(x, type_), groups, None, None, 1e-5, 1)
+        ref.check_float(capi.group_norm(x, groups, activation=1, type_=type_), want, err, type_)
+
+
 @pytest.mark.parametrize("type_", [ref.F32, ref.F16])
 @pytest.mark.parametrize("n, pixels, C, groups", [(2, 3, 20000, 2), (1, 5, 9000, 1), (3, 2, 8200, 8), (2, 2, 31 * 300, 300)])
 def test_slices_wider_than_a_workgroup(type_, n, pixels, C, groups):
