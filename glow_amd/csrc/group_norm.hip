@@ -564,9 +564,11 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
     k = std::max(unit, k / 2 / unit * unit);
     set(k);
   }
-  // Few large slices leave most of the chip idle: 1 x 3136 x 256 of fp16 resident in 16 slices 9.8
-  // us, in parts 9.4; 1 x 784 x 512 in 32 slices of 25 KB 6.7, in parts 9.6.
-  plan.resident = fits() && ((long long)N * p.slices >= 128 || (long long)p.pixels * p.width * size <= 65536);
+  // Few large slices leave most of the chip idle. us, resident / in parts: 1 x 3136 x 256 of fp16 in 16
+  // slices of 100 KB 9.8 / 9.1, 4 x 52 x 626 in 4 of 65 KB 17.0 / 10.2, 4 x 268 x 260 in 16 of 35 KB 12.6 /
+  // 10.3; 1 x 784 x 512 in 32 of 25 KB 6.7 / 9.6.
+  const long long all = (long long)N * p.slices, bytes = (long long)p.pixels * p.width * size;
+  plan.resident = fits() && (all >= 128 || bytes <= 16 * 1024 || (all >= 24 && bytes <= 32 * 1024));
   if (plan.resident) {
     // few pixels a thread as long as the workgroup is small, so that several share a CU (32 x 784 x
     // 512, microscaled, 64 bytes: 512 threads of eight pixels 16.3 us, 1024 of four 19.7)
@@ -596,7 +598,7 @@ static GnPlan gn_plan(GroupNorm &p, size_t N, int size, bool mx4) {
   const int stride = plan.threads >> p.lg_vec;
   p.chunk_pixels = (int)std::min<long long>(p.pixels, ((long long)p.pixels + (long long)chunks * stride - 1) /
                                                           ((long long)chunks * stride) * stride);
-  p.chunks = (p.pixels + p.chunk_pixels - 1) / p.chunk_pixels;
+  p.chunks = (int)(((long long)p.pixels + p.chunk_pixels - 1) / p.chunk_pixels);
   return plan;
 }
 
