@@ -912,7 +912,9 @@ enum { MI355X_F32 = 0, MI355X_F16 = 1, MI355X_BF16 = 2, MI355X_MX4 = 3 };
  * In all of these, `row_bytes` is the distance between rows in bytes: for float types a
  * multiple of the element's size, rows at any address that is one too. Tensors of no rows
  * or columns are a no-op. Results may not overlap what they are made from, except where it
- * says so. Sizes up to 2^31 - 1 each. */
+ * says so. Sizes up to 2^31 - 1 each; MI355X_ERR_NOT_SUPPORTED for tensors of over 2^42
+ * columns in all, or of products of over 2^22 tiles of 64 x 64 results (16 x 16 up to four
+ * rows). */
 size_t mi355x_mx4_row_bytes(size_t cols);
 /* Each block of 32: m = the largest magnitude, scale 2^max(floor(log2 m) - 2, -127) (byte
  * 0 for a block of zeros), codes = value / scale rounded to nearest, ties to even, and
@@ -931,7 +933,7 @@ int mi355x_mx4_dequantize(void *dst, int dst_type, size_t dst_row_bytes, const u
  * image (its pixels are the rows):
  *   out[m][n] = activation(bias[n] + sum over k of in[m][k] * weights[n][k])
  * in       [M x K] float of any type, quantized first by the rule above (in the workspace,
- *          where one is asked for), or MI355X_MX4
+ *          where one is asked for), or MI355X_MX4; the results are the same
  * weights  MI355X_MX4 [N x K]
  * bias     float [N], or NULL
  * out      [M x N] of any type; MI355X_MX4: quantized by the rule above from the 32-bit
@@ -956,8 +958,8 @@ int mi355x_mx4_fc(void *out, int out_type, size_t out_row_bytes, const void *in,
  * 32 bits. out: of the input's type, also in place (same address and distance between rows),
  * or MI355X_MX4, quantized from the 32-bit results: the input of mi355x_mx4_fc. gamma, beta:
  * float [C], or NULL (1 and 0). activation as above. row_bytes: the distance between pixels;
- * samples follow each other. A NaN or an infinity makes NaN of its group. workspace as
- * above, of mi355x_group_norm_workspace_bytes. */
+ * samples follow each other, up to 2^31 - 1 pixels in all. A NaN or an infinity makes NaN of
+ * its group. workspace as above, of mi355x_group_norm_workspace_bytes. */
 int mi355x_group_norm_workspace_bytes(size_t N, size_t pixels, size_t C, size_t groups,
                                       size_t *bytes);
 int mi355x_group_norm(void *out, int out_type, size_t out_row_bytes, const void *in, int in_type,
