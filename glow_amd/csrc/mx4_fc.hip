@@ -1,7 +1,7 @@
 // The product of microscaled 4-bit rows: out[m][n] = act(bias[n] + sum_k in[m][k] w[n][k]).
 //
-// The matrix cores' scaled instruction takes 64 columns of 32 rows of both operands: a lane
-// feeds one block (16 bytes of codes of row lane % 32, block lane / 32) and its scale byte,
+// The matrix cores' scaled instruction takes 128 columns of 16 rows of both operands: a lane
+// feeds one block (16 bytes of codes of row lane % 16, block lane / 16) and its scale byte,
 // and products are summed in 32 bits. The weights are the first operand, so that a lane's
 // results belong to one row of the output and lie in fours of neighbouring columns: what a
 // microscaled result's blocks and wide stores want.
@@ -52,10 +52,13 @@ static FcTile fc_tile(long long M, long long K, long long N, bool mx4_out) {
 // (128 KB), 64 x 4096 x 4096 15.3 / 12.3 (256 KB), 61 x 415 x 509 of fp32 3.5 / 5.0; 64x64 tiles
 // without a ring: 4096 x 13 x 512 of fp32 4.7 / 5.8 (3 KB, 8 tiles to a row), 25088 x 512 x 128 of
 // fp16 11.1 / 13.8 (64 KB, 2), 2000 x 400 x 500 of fp32 8.2 / 6.9 (100 KB, 8), 8192 x 256 x 1024 of
-// fp16 10.8 / 10.0 (32 KB, 16).
-static bool fc_quantizes(FcTile tile, long long M, long long K, long long N, size_t size) {
+// fp16 10.8 / 10.0 (32 KB, 16). Rows that do not all start on a word (`words`) take three times as
+// long to load: 186 x 895 x 792 of fp16 9.2 / 6.4 (57 KB; 186 x 894 x 792 5.6 / 6.4), 40 x 895 x 400 5.5 /
+// 5.8 (29 KB); up to four rows, which are loaded once, 1 x 4095 x 4096 4.9 / 6.7.
+static bool fc_quantizes(FcTile tile, long long M, long long K, long long N, size_t size, bool words) {
   if (tile == kFcShort64) return 64 * K * (long long)size <= 64 * 1024 && N <= 8 * 64;
-  return tile <= kFc32 && std::min(M, tile == kFc16 ? 16LL : 32LL) * K * (long long)size <= 96 * 1024;
+  const long long most = words || M <= kSharedRows ? 96 * 1024 : 32 * 1024;
+  return tile <= kFc32 && std::min(M, tile == kFc16 ? 16LL : 32LL) * K * (long long)size <= most;
 }
 
 template <class IN, class OUT> static int fc_small(const MxFc &p, int K, FcTile tile, hipStream_t st) {
@@ -98,10 +101,10 @@ int mi355x_mx4_fc_workspace_bytes(size_t M, size_t K, size_t N, int in_type, siz
                  "mx4_fc_workspace_bytes: %zu x %zu x %zu, up to 2^31 - 1 each are supported", M, K, N);
   *bytes = 0;
   if (in_type == MI355X_MX4 || !M || !N) return MI355X_OK;
-  // (whatever the result's type)
+  // (whatever the result's type, and wherever the rows lie)
   for (bool mx4_out : {false, true})
     if (!fc_quantizes(fc_tile((long long)M, (long long)K, (long long)N, mx4_out), (long long)M, (long long)K, (long long)N,
-                      float_size(in_type)))
+                      float_size(in_type), in_type == MI355X_F32))
       *bytes = M * mx4_row_bytes_of(K);
   return MI355X_OK;
 }
@@ -137,7 +140,9 @@ int mi355x_mx4_fc(void *out, int out_type, size_t out_row_bytes, const void *in,
                    "mx4_fc: the workspace overlaps a tensor");
   }
   const FcTile tile = fc_tile((long long)M, (long long)K, (long long)N, out_type == MI355X_MX4);
-  if (in_type != MI355X_MX4 && !fc_quantizes(tile, (long long)M, (long long)K, (long long)N, float_size(in_type))) {
+  const bool words = ((uintptr_t)in | in_row_bytes) % 4 == 0;
+  if (in_type != MI355X_MX4 &&
+      !fc_quantizes(tile, (long long)M, (long long)K, (long long)N, float_size(in_type), words)) {
     p.in = static_cast<const uint8_t *>(workspace);
     p.in_row_bytes = mx4_row_bytes_of(K);
     if (K)

@@ -154,7 +154,7 @@ def test_fc_of_large_results(M, K, N, out_type):
 
 
 @pytest.mark.parametrize("in_type", [ref.F32, ref.F16, ref.BF16])
-@pytest.mark.parametrize("M, K, N", [(1, 4096, 70), (4, 515, 3000), (3, 5000, 40), (2, 130, 33), (1, 49152, 20), (4, 6100, 18), (1, 24576, 50), (31, 96, 700), (90, 1050, 290), (1990, 13, 300),
+@pytest.mark.parametrize("M, K, N", [(1, 4096, 70), (4, 515, 3000), (186, 895, 792), (186, 894, 792), (40, 895, 400), (3, 5000, 40), (2, 130, 33), (1, 49152, 20), (4, 6100, 18), (1, 24576, 50), (31, 96, 700), (90, 1050, 290), (1990, 13, 300),
                                      (2000, 511, 190), (700, 300, 2000)])
 def test_float_inputs_give_what_their_rows_give(M, K, N, in_type):
     """Quantised by the product or in front of it: the same bits."""
