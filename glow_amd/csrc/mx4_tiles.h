@@ -8,7 +8,7 @@
 // first operand and their rows are permuted on the way into LDS: a lane ends with sixteen
 // neighbouring columns of one output row (eight, where a wave has 32).
 //
-// 8192 x 4096 x 4096 of random codes to bf16: 75 us, 3.7 PFLOP/s (4096 x 8192 x 4096 68 us, 4.0). The
+// 8192 x 4096 x 4096 of random codes to bf16: 75 to 80 us from card to card, 3.5 PFLOP/s. The
 // matrix cores are busy for two fifths of that. Random codes draw so much power that the
 // instructions alone, from registers, reach 6.5 PFLOP/s in their 32x32 form and 7.5 in this one
 // (zeros: 9.5); a step of a 256x256 tile takes 0.95 us where they need 0.46, and 0.8 without
