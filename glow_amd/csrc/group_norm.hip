@@ -15,7 +15,8 @@
 //             workspace, a second joins them and writes
 // Sums are exact in kind: a thread's own mean first and the squares of what is left of it,
 // then the threads' (or parts') means and what they are off the whole's; no difference of
-// large sums is ever formed, whatever the mean is.
+// large sums is ever formed, whatever the mean is. (Slices of over 8192 channels, a third way: sums in
+// 64 bits.)
 //
 // us: 64 x 3136 x 256 of fp16 53 (206 MB, 3.9 TB/s: 40 at the rate of a large copy; a workgroup fills a
 // CU and reads, computes and writes in turn), 32 x 784 x 512 of bf16 with SiLU to microscaled rows 16.5
@@ -29,6 +30,7 @@ namespace mi355x {
 
 struct GroupStats {
   float mean, square;     // of a part: sum of the squares of what is left of the mean
+  float low;              // what the mean's rounding left out, where it is kept
 };
 struct GroupNorm {
   uint8_t *out;
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
     for (int g = tid; g < groups; g += (int)blockDim.x) {
       const float m = s_group[g] * over;
       if constexpr (MODE == kGnStats)
-        p.stats[((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks + chunk] = GroupStats{m, s_second[g]};
+        p.stats[((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks + chunk] = GroupStats{m, s_second[g], 0};
       else {
         s_group[g] = m;
         s_second[g] = 1.0f / sqrtf(s_second[g] / total + p.epsilon);
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
 #pragma unroll
       for (int i = 0; i < kGnMostChunks / 64; i++) {
         const int k = lane + 64 * i;
-        own[i] = k < p.chunks ? s[k] : GroupStats{0, 0};
+        own[i] = k < p.chunks ? s[k] : GroupStats{0, 0, 0};
         if (k < p.chunks) m = fmaf(own[i].mean, values(k), m);
       }
       m = wave_sum(m) / total;
@@ -440,41 +442,50 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
 }
 
 // Slices too wide for a workgroup's lanes, over 8192 channels (a group of that many, or 32 of an odd
-// number each to microscaled rows): a workgroup finds a group's mean and squares in two passes
-// over it, then sixteen lanes take 128 channels of a pixel.
+// number each to microscaled rows): a workgroup reads a group once, then sixteen lanes take 128
+// channels of a pixel.
+//
+// A thread's sums run over up to every 256th value of a group, too many for 32 bits: they are held in
+// 64, of the values' distances from the group's first one and of the squares of these. That one
+// is sqrt(values of the group) deviations from the mean at most, so that the difference of the
+// two sums loses log2(values) of their 53 bits at worst. One workgroup a group, one value a load:
+// 1 x 784 x 16384 of fp16 in one group 13.4 ms, bound by the time that loads take to arrive.
 constexpr int kGnWideThreads = 256;
-
-__device__ __forceinline__ float block_sum(float v, float *s_part) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float t = 0;
-#pragma unroll
-  for (int w = 0; w < kGnWideThreads / 64; w++) t += s_part[w];
-  return t;
-}
 
 template <class E>
 __global__ __launch_bounds__(kGnWideThreads) void group_norm_wide_stats_kernel(GroupNorm p) {
-  __shared__ float s_part[kGnWideThreads / 64];
+  __shared__ double s_sum[kGnWideThreads], s_square[kGnWideThreads];
+  const int tid = threadIdx.x;
   const int group = (int)(blockIdx.x % (unsigned)p.groups);
   const size_t sample = blockIdx.x / (unsigned)p.groups;
   const uint8_t *base = p.in + sample * p.pixels * p.in_row_bytes + (size_t)group * p.per * E::kSize;
-  const float n = (float)p.pixels * (float)p.per;
-  auto each = [&](auto &&f) {
-    for (int px = 0; px < p.pixels; px++) {
-      const typename E::T *row = reinterpret_cast<const typename E::T *>(base + (size_t)px * p.in_row_bytes);
-      for (int i = threadIdx.x; i < p.per; i += kGnWideThreads) f(E::to(row[i]));
+  const double pivot = E::to(*reinterpret_cast<const typename E::T *>(base));
+  double sum = 0, square = 0;
+  for (int px = 0; px < p.pixels; px++) {
+    const typename E::T *row = reinterpret_cast<const typename E::T *>(base + (size_t)px * p.in_row_bytes);
+    for (int i = tid; i < p.per; i += kGnWideThreads) {
+      const double d = (double)E::to(row[i]) - pivot;
+      sum += d;
+      square = fma(d, d, square);
     }
-  };
-  float sum = 0;
-  each([&](float x) { sum += x; });
-  const float mean = block_sum(sum, s_part) / n;
-  float square = 0;
-  each([&](float x) { square = fmaf(x - mean, x - mean, square); });
-  square = block_sum(square, s_part);
-  if (threadIdx.x == 0) p.stats[blockIdx.x] = GroupStats{mean, 1.0f / sqrtf(square / n + p.epsilon)};
+  }
+  s_sum[tid] = sum;
+  s_square[tid] = square;
+  for (int half = kGnWideThreads / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (tid < half) {
+      s_sum[tid] += s_sum[tid + half];
+      s_square[tid] += s_square[tid + half];
+    }
+  }
+  if (tid == 0) {
+    const double n = (double)p.pixels * p.per, rest = s_sum[0] / n, mean = pivot + rest;
+    double variance = s_square[0] / n - rest * rest;
+    variance = variance < 0 ? 0 : variance;          // (NaN stays)
+    const float high = (float)mean;
+    // (what is left of the mean is taken from its parts: their sum is rounded too)
+    p.stats[blockIdx.x] = GroupStats{high, (float)(1.0 / sqrt(variance + p.epsilon)), (float)(rest - (high - pivot))};
+  }
 }
 
 template <class E, class OUT>
@@ -494,8 +505,9 @@ __global__ __launch_bounds__(kGnWideThreads) void group_norm_wide_apply_kernel(G
       for (int j = 0; j < 8; j++) {
         if (j < left) {
           const GroupStats s = stats[(c + j) / p.per];
-          x[j] = activate<decltype(act)::value>(fmaf(x[j] - s.mean, s.square * (p.gamma ? p.gamma[c + j] : 1.0f),
-                                                     p.beta ? p.beta[c + j] : 0.0f));
+          const float scale = s.square * (p.gamma ? p.gamma[c + j] : 1.0f);
+          const float shift = fmaf(-s.low, scale, p.beta ? p.beta[c + j] : 0.0f);
+          x[j] = activate<decltype(act)::value>(fmaf(x[j] - s.mean, scale, shift));
         }
       }
     });
