@@ -13,10 +13,11 @@
 //   in parts  slices that do not fit, or too few of them to fill the chip: one launch
 //             leaves mean and sum of squares of every part of a slice's pixels in the
 //             workspace, a second joins them and writes
-// Sums are exact in kind: a thread's own mean first and the squares of what is left of it,
-// then the threads' (or parts') means and what they are off the whole's; no difference of
-// large sums is ever formed, whatever the mean is. (Slices of over 8192 channels, a third way: sums in
-// 64 bits.)
+// All sums are of distances: from the group's first value, the pivot, and with that a thread's mean;
+// then the squares of what the thread's values are off its mean, and what that is off the whole's.
+// So the error goes by how far a group's values lie from each other, whatever the mean is. That is
+// kept as its rounding and the rest of it, and a value loses the first before it is scaled. (Slices of
+// over 8192 channels, a third way: sums in 64 bits.)
 //
 // us: 64 x 3136 x 256 of fp16 53 (206 MB, 3.9 TB/s: 40 at the rate of a large copy; a workgroup fills a
 // CU and reads, computes and writes in turn), 32 x 784 x 512 of bf16 with SiLU to microscaled rows 16.5
@@ -28,9 +29,10 @@
 
 namespace mi355x {
 
-struct GroupStats {
+struct alignas(16) GroupStats {
   float mean, square;     // of a part: sum of the squares of what is left of the mean
-  float low;              // what the mean's rounding left out, where it is kept
+  float low;              // what the mean's rounding left out
+  float unused;           // (one load of sixteen bytes)
 };
 struct GroupNorm {
   uint8_t *out;
@@ -65,15 +67,41 @@ struct GnGroup {
   }
 };
 
-// Sums over a slice's pixels and a group's channels, to s_group[0 .. in_slice). A thread's eight
-// channels are NP parts that each lie in one group: one where groups are whole vectors, two (the
-// first channels and the rest) where a vector meets two groups at most, else one for each
-// channel. x[i] is the sum over part i, its place in a row of s_part `at` + i; parts before `from`
-// are another thread's. Lanes of a wave that hold the same channels are summed first, then a
-// wave takes a group.
-template <int NP>
-__device__ __forceinline__ void gn_reduce(float (&x)[NP], float *s_part, float *s_group, int at, int from,
-                                          const GroupNorm &p) {
+// Sums over a wave in 64 bits.
+template <int N> __device__ __forceinline__ double add_rotated(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, 0x120 + N, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), 0x120 + N, 0xf, 0xf, true);
+  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double add_across16(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+__device__ __forceinline__ double add_across32(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+  const auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  x = add_rotated<1>(add_rotated<2>(add_rotated<4>(add_rotated<8>(x))));
+  return add_across32(add_across16(x));
+}
+
+// Sums over a slice's pixels and a group's channels: done(g, sum) of each of the slice's groups, in one
+// thread. A thread's eight channels are NP parts that each lie in one group: one where groups are
+// whole vectors, two (the first channels and the rest) where a vector meets two groups at most,
+// else one for each channel. x[i] is the sum over part i, its place in a row of s_part `at` + i;
+// parts before `from` are another thread's. Lanes of a wave that hold the same channels are summed
+// first, then a wave takes a group, always in 64 bits. X: double where roundings of the lanes' sums
+// would be seen, in those that give means of one or two parts (as floats, a mean of 600 values is off
+// by 6 * 10^-8 of their spread, else by 10^-8; 1% of the time of small calls).
+template <int NP, class X, class Done>
+__device__ __forceinline__ void gn_reduce(X (&x)[NP], X *s_part, int at, int from, int groups,
+                                          const GroupNorm &p, Done &&done) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
   const int V = 1 << p.lg_vec;
 #pragma unroll
@@ -86,7 +114,6 @@ __device__ __forceinline__ void gn_reduce(float (&x)[NP], float *s_part, float *
     if (V <= 32) x[j] = add_across32(x[j]);
   }
   const int rows = V < 64 ? waves : (int)blockDim.x >> p.lg_vec;
-  __syncthreads();
   if (V >= 64 || lane < V) {
     const int row = V < 64 ? wave : tid >> p.lg_vec;
 #pragma unroll
@@ -96,22 +123,21 @@ __device__ __forceinline__ void gn_reduce(float (&x)[NP], float *s_part, float *
   __syncthreads();
   // many small groups: a thread each, instead of wave after wave
   const int most = NP == 8 ? p.per : (p.per + 6) / 8 + 1;
-  const bool thread_each = p.in_slice > waves && most * rows <= 32;
-  for (int g = thread_each ? tid : wave; g < p.in_slice; g += thread_each ? (int)blockDim.x : waves) {
+  const bool thread_each = groups > waves && most * rows <= 32;
+  for (int g = thread_each ? tid : wave; g < groups; g += thread_each ? (int)blockDim.x : waves) {
     // a group's parts in a row: `len` of them from `begin` on, `apart` places from each other; where
     // it begins within a vector, the first is that vector's second part
     const int channel = g * p.per;
     const int begin = NP == 8 ? channel : (channel >> 3) * NP, apart = NP == 2 ? 2 : 1;
     const int inner = NP == 2 && (channel & 7) ? 1 : 0;
     const int len = NP == 8 ? p.per : ((channel + p.per - 1) >> 3) - (channel >> 3) + 1;
+    double t = 0;
     if (thread_each) {
-      float t = 0;
       for (int row = 0; row < rows; row++)
         for (int k = 0; k < len; k++) t += s_part[(row << p.lg_vec) * NP + begin + k * apart + (k == 0 ? inner : 0)];
-      s_group[g] = t;
+      done(g, t);
       continue;
     }
-    float t = 0;
     if (len < 64) {
       for (int e = lane; e < len * rows; e += 64) {
         const int row = (int)((unsigned)e / (unsigned)len), k = e - row * len;
@@ -123,27 +149,59 @@ __device__ __forceinline__ void gn_reduce(float (&x)[NP], float *s_part, float *
           t += s_part[(row << p.lg_vec) * NP + begin + k * apart + (k == 0 ? inner : 0)];
     }
     t = wave_sum(t);
-    if (lane == 0) s_group[g] = t;
+    if (lane == 0) done(g, t);
   }
   __syncthreads();
 }
 
-// The sum of eight values: of 16-bit types two to an instruction.
-template <class E> __device__ __forceinline__ float gn_sum8(const typename E::Eight &e, float sum) {
+// 1 / (pixels * per) to 40 bits and more.
+__device__ __forceinline__ double gn_over(int pixels, int per) {
+  const double n = (double)pixels * per, r = __builtin_amdgcn_rcpf((float)n);
+  return fma(fma(-n, r, 1.0), r, r);
+}
+
+// base + rest, rounded, and what the rounding left out: exact where the base is no smaller than the
+// rest, else off by a rounding of the rest.
+struct GnMean {
+  float high, low;
+  __device__ __forceinline__ GnMean(float base, float rest) : high(base + rest), low(rest - (high - base)) {}
+  __device__ __forceinline__ GnMean(float base, double rest)
+      : high((float)(base + rest)), low((float)(rest - ((double)high - base))) {}
+};
+
+// A thread's sums, of up to 128 values at a time, of what they are from the pivot. 32-bit values lose
+// that one by one. 16-bit ones are summed as they are, kGnShare of each, so that no sum is
+// past 32 bits: where they are so near to each other that the pivot matters, they are multiples of one
+// step whose sum has 11 + 7 bits and few more, and the pivot is taken off it without a rounding (gn_rest).
+constexpr float kGnShare = 1.0f / 128;
+template <class E> __device__ __forceinline__ float gn_add(float sum, const typename E::Eight &e, int j, float pivot) {
+  if constexpr (E::kSize == 4) return sum + (e[j] - pivot);
+  else return fmaf(E::get(e, j), kGnShare, sum);
+}
+// The same of eight values: of 16-bit types two to an instruction, of others in pairs.
+template <class E> __device__ __forceinline__ float gn_sum8(float sum, const typename E::Eight &e, float pivot) {
   if constexpr (std::is_same_v<E, F16>) {
     typedef _Float16 Two __attribute__((ext_vector_type(2)));
-#pragma unroll
-    for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2(Two{e[2 * i], e[2 * i + 1]}, Two{1, 1}, sum, false);
-  } else if constexpr (std::is_same_v<E, BF16>) {
-    typedef __bf16 Two __attribute__((ext_vector_type(2)));
+    const _Float16 share = (_Float16)kGnShare;
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(Two, (uint32_t)e[i]), Two{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
-  } else {
+      sum = __builtin_amdgcn_fdot2(Two{e[2 * i], e[2 * i + 1]}, Two{share, share}, sum, false);
+  } else if constexpr (std::is_same_v<E, BF16>) {
+    typedef __bf16 Two __attribute__((ext_vector_type(2)));
+    const __bf16 share = (__bf16)kGnShare;
 #pragma unroll
-    for (int j = 0; j < 8; j++) sum += E::get(e, j);
+    for (int i = 0; i < 4; i++)
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(Two, (uint32_t)e[i]), Two{share, share}, sum, false);
+  } else {
+    const auto two = [&](int j) { return (e[j] - pivot) + (e[j + 1] - pivot); };
+    sum += (two(0) + two(2)) + (two(4) + two(6));
   }
   return sum;
+}
+// What `count` values of such a sum are from the pivot in all.
+template <class E> __device__ __forceinline__ float gn_rest(float sum, float count, float pivot) {
+  if constexpr (E::kSize == 4) return sum;
+  else return fmaf(-count * kGnShare, pivot, sum) * (1.0f / kGnShare);
 }
 // x - mean of a value; of fp16 one instruction with the widening (`one` hides a factor of 1 that
 // would be taken out of it).
@@ -152,19 +210,16 @@ template <class E> __device__ __forceinline__ float gn_less(const typename E::Ei
   else return E::get(e, j) - mean;
 }
 
-// Writes one pixel's eight channels. 32-bit values lose the mean first; of 16-bit ones it is
-// in the shift, which is off by half a step of mean * scale then, less than the values'
-// own rounding.
+// Writes one pixel's eight channels.
 template <class E, class OUT, int ACT, int NM>
 __device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, int twice, bool block_inside,
                                          const typename E::Eight &raw, const float (&mean)[NM],
-                                         const float (&scale)[8], const float (&shift)[8], const GroupNorm &p) {
+                                         const float (&scale)[8], const float (&shift)[8], float one,
+                                         const GroupNorm &p) {
   float y[8];
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const float x = E::kSize == 2 ? E::get(raw, j) : E::get(raw, j) - mean[NM == 1 ? 0 : j];
-    y[j] = activate<ACT>(fmaf(x, scale[j], shift[j]));
-  }
+  for (int j = 0; j < 8; j++)
+    y[j] = activate<ACT>(fmaf(gn_less<E>(raw, j, mean[NM == 1 ? 0 : j], one), scale[j], shift[j]));
   if constexpr (OUT::kSize == 0) {
     if (__ballot(left < 8)) {        // (a branch, not a selection for every value of every pixel)
 #pragma unroll
@@ -187,10 +242,16 @@ __device__ __forceinline__ void gn_write(uint8_t *row, int c, int left, int twic
   }
 }
 
+// what the sums that give means are held in, between lanes
+template <int NP> using GnWide = std::conditional_t<NP <= 2, double, float>;
+
 template <class E, class OUT, int R, int MODE, int NP>
 __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
+  typedef GnWide<NP> Wide;
   extern __shared__ __attribute__((aligned(16))) float s_mem[];
-  float *s_group = s_mem, *s_second = s_mem + p.in_slice, *s_part = s_mem + 2 * p.in_slice;
+  // of each group: its mean's rounding and the rest, 1 / sqrt(variance + epsilon), and a mean on the way
+  float *s_group = s_mem, *s_low = s_mem + p.in_slice, *s_second = s_mem + 2 * p.in_slice;
+  float *s_rest = s_mem + 3 * p.in_slice, *s_part = s_mem + 4 * ((p.in_slice + 1) & ~1);
   const int tid = threadIdx.x, V = 1 << p.lg_vec;
   const int v = tid & (V - 1), first = tid >> p.lg_vec, stride = (int)blockDim.x >> p.lg_vec;
 
@@ -237,6 +298,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
   };
   const int block = R * stride;
   const float of_group = (float)p.per;
+  const int groups = (c_end - c0) / p.per;
 
   load(px0);
   float scale[8], shift[8];
@@ -248,40 +310,64 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
     }
   };
   // asked for with the values, ahead of the statistics, where registers are left for it
-  if constexpr (MODE != kGnStats && R < 16) load_affine();
+  constexpr bool kAffineAhead = R < 16 && (R * E::kSize < 32 || NP == 1);
+  if constexpr (MODE != kGnStats && kAffineAhead) load_affine();
+  float one = 1.0f;
+  asm("" : "+s"(one));
   if constexpr (MODE != kGnApply) {
+    // The groups of a thread's parts: f(part, its group, the part's place in it). (Their division is made
+    // here, while the values are on their way.)
+    GnGroup own(NP == 8 ? c - c0 : v * 8, p.per);
+    asm volatile("" : "+v"(own.group), "+v"(own.in));
+    auto parts = [&](auto &&f) {
+      GnGroup of = own;
+#pragma unroll
+      for (int j = 0; j < NP; j++) {
+        f(j, min(of.group, groups - 1), of.in);
+        if (NP == 8) of.next(p.per);
+        else of.group++, of.in = 0;
+      }
+    };
+    // a group's pivot is its first channel of the sample's first pixel, whichever part of a slice this is
+    const typename E::T *pixel = reinterpret_cast<const typename E::T *>(
+        p.in + (size_t)sample * p.pixels * p.in_row_bytes) + c0;
+    float pivot[NP];
+    parts([&](int j, int g, int) { pivot[j] = E::to(pixel[g * p.per]); });
     // a thread's own counts (exact: a part of a slice has 2^24 pixels at most), means and squares.
     // Channel j belongs to part `j >= border` of two, to its own of eight.
-    int border = 8;
-    if (NP == 2 && left > 0) {
-      const GnGroup own(v * 8, p.per);
-      border = min(8, twice + p.per - own.in);
-    }
+    const int border = NP == 2 && left > 0 ? min(8, twice + p.per - own.in) : 8;
     const int channels_lo = border - twice, channels_hi = 8 - border;
-    float count[NP], mean[NP], square[NP], one = 1.0f;
-    asm("" : "+s"(one));
+    // (sum and mean are of distances from the pivot; eight parts have one count, and no registers for
+    // sums as well)
+    constexpr int NC = NP == 8 ? 1 : NP;
+    float count[NC], sum[NC], mean[NP], square[NP];
 #pragma unroll
-    for (int j = 0; j < NP; j++) count[j] = mean[j] = square[j] = 0;
+    for (int j = 0; j < NP; j++) count[j % NC] = sum[j % NC] = mean[j] = square[j] = 0;
+    // (the end of the sums finds them in s_low)
+    if (first == 0 && left > 0)
+      parts([&](int j, int g, int in) {
+        if (in == 0 && (NP == 2 ? j == 0 || border < min(8, left) : NP == 1 || (j >= twice && j < left))) s_low[g] = pivot[j];
+      });
     for (int from = px0;;) {
       const int n = mine(from);
       if (n > 0) {
         constexpr int NA = NP == 1 ? 1 : 8;       // sums in the loop over pixels
-        float m[NA], q[NA], here[NP], own[NP], rest[NP];
+        float m[NA], q[NA], here[NC], all[NP], own[NP], rest[NP];
 #pragma unroll
         for (int j = 0; j < NA; j++) m[j] = q[j] = 0;
 #pragma unroll
         for (int i = 0; i < R; i++)
           if (i < n) {
-            if constexpr (NP == 1) m[0] = gn_sum8<E>(raw[i], m[0]);
+            if constexpr (NP == 1) m[0] = gn_sum8<E>(m[0], raw[i], pivot[0]);
             else {
 #pragma unroll
-              for (int j = 0; j < 8; j++) m[j] += E::get(raw[i], j);
+              for (int j = 0; j < 8; j++)
+                m[j] = gn_add<E>(m[j], raw[i], j, NP == 8 ? pivot[j] : j < border ? pivot[0] : pivot[1]);
             }
           }
         if constexpr (NP == 1) {
           here[0] = (float)n * 8;
-          m[0] *= 1.0f / here[0];
-          own[0] = m[0];
+          all[0] = gn_rest<E>(m[0], here[0], pivot[0]);
         } else if constexpr (NP == 2) {
           here[0] = (float)(n * channels_lo);
           here[1] = (float)(n * channels_hi);
@@ -291,14 +377,26 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
             lo += j >= twice && j < border ? m[j] : 0.0f;
             hi += j >= border ? m[j] : 0.0f;
           }
-          own[0] = lo * (1.0f / here[0]);
-          own[1] = channels_hi ? hi * (1.0f / here[1]) : 0.0f;
-#pragma unroll
-          for (int j = 0; j < 8; j++) m[j] = j < border ? own[0] : own[1];
+          all[0] = gn_rest<E>(lo, here[0], pivot[0]);
+          all[1] = gn_rest<E>(hi, here[1], pivot[1]);
         } else {
-          const float over = 1.0f / (float)n;
+          here[0] = (float)n;
 #pragma unroll
-          for (int j = 0; j < 8; j++) here[j] = (float)n, m[j] *= over, own[j] = m[j];
+          for (int j = 0; j < 8; j++) all[j] = gn_rest<E>(m[j], here[0], pivot[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NP; j++) own[j] = j == 1 && NP == 2 && !channels_hi ? 0.0f : all[j] * (1.0f / here[j % NC]);
+        // the squares are of the distances from the mean's rounding, and less of what that is off
+        float low[NP];
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+          const GnMean center(pivot[j], own[j]);
+          low[j] = center.low;
+          if constexpr (NP == 2) {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+              if (j == 0 || k >= border) m[k] = center.high;
+          } else m[j] = center.high;
         }
 #pragma unroll
         for (int i = 0; i < R; i++)
@@ -321,83 +419,91 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
         }
 #pragma unroll
         for (int j = 0; j < NP; j++) {
-          if (MODE == kGnResident || count[j] == 0) {
-            count[j] = here[j], mean[j] = own[j], square[j] = rest[j];
+          rest[j] = fmaf(-low[j] * low[j], here[j % NC], rest[j]);
+          rest[j] = rest[j] < 0 ? 0.0f : rest[j];    // (NaN stays)
+          if (MODE == kGnResident || count[j % NC] == 0) {
+            mean[j] = own[j], square[j] = rest[j];
           } else {           // joins two sets: the squares of each, and of what their means are apart
-            const float all = count[j] + here[j], part = here[j] / all, d = own[j] - mean[j];
+            const float part = here[j % NC] / (count[j % NC] + here[j % NC]), d = own[j] - mean[j];
             mean[j] = fmaf(d, part, mean[j]);
-            square[j] += fmaf(d * d, count[j] * part, rest[j]);
-            count[j] = all;
+            square[j] += fmaf(d * d, count[j % NC] * part, rest[j]);
           }
         }
+#pragma unroll
+        for (int j = 0; j < NC; j++) count[j] += here[j], sum[j] += all[j];
       }
       if (MODE == kGnResident || px_end - from <= block) break;
       from += block;
       load(from);
     }
-    const float total = (float)(px_end - px0) * of_group, over = 1.0f / total;
     const int at = NP == 8 ? c - c0 : v * NP;
+    Wide wide[NP];
+#pragma unroll
+    for (int j = 0; j < NP; j++) wide[j] = NP == 8 ? mean[j] * count[0] : sum[j % NC];
+    gn_reduce<NP>(wide, reinterpret_cast<Wide *>(s_part), at, twice, groups, p, [&](int g, double all) {
+      const double rest = all * gn_over(px_end - px0, p.per);
+      const GnMean m(s_low[g], rest);
+      s_rest[g] = (float)rest;
+      s_group[g] = m.high;
+      s_low[g] = m.low;
+    });
     float x[NP];
-#pragma unroll
-    for (int j = 0; j < NP; j++) x[j] = mean[j] * count[j];
-    gn_reduce<NP>(x, s_part, s_group, at, twice, p);
-    {
-      GnGroup of(NP == 8 ? c - c0 : v * 8, p.per);
-#pragma unroll
-      for (int j = 0; j < NP; j++) {
-        const float d = mean[j] - s_group[left > 0 ? min(of.group, p.in_slice - 1) : 0] * over;
-        x[j] = left > 0 ? fmaf(d * d, count[j], square[j]) : 0.0f;
-        if (NP == 8) of.next(p.per);
-        else of.group++;
-      }
-    }
-    gn_reduce<NP>(x, s_part, s_second, at, twice, p);
-    const int groups = (c_end - c0) / p.per;
-    for (int g = tid; g < groups; g += (int)blockDim.x) {
-      const float m = s_group[g] * over;
+    parts([&](int j, int g, int) {
+      const float d = mean[j] - s_rest[g];
+      x[j] = count[j % NC] > 0 ? fmaf(d * d, count[j % NC], square[j]) : 0.0f;
+    });
+    gn_reduce<NP>(x, s_part, at, twice, groups, p, [&](int g, double all) {
       if constexpr (MODE == kGnStats)
-        p.stats[((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks + chunk] = GroupStats{m, s_second[g], 0};
-      else {
-        s_group[g] = m;
-        s_second[g] = 1.0f / sqrtf(s_second[g] / total + p.epsilon);
-      }
-    }
+        p.stats[((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks + chunk] =
+            GroupStats{s_group[g], (float)all, s_low[g], 0};
+      else s_second[g] = 1.0f / sqrtf((float)(all * gn_over(px_end - px0, p.per)) + p.epsilon);
+    });
     if (MODE == kGnStats) return;
   } else {
-    // joins the parts: their means, then their squares and what their means are off the whole's
+    // joins the parts: what their means are from the first one's, then their squares and what their
+    // means are off the whole's
     const int lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
-    const int groups = (c_end - c0) / p.per;
-    const float total = (float)p.pixels * of_group;
+    const double over = gn_over(p.pixels, p.per);
     for (int g = wave; g < groups; g += waves) {
       const GroupStats *s = p.stats + ((size_t)sample * p.groups + slice * p.in_slice + g) * p.chunks;
       GroupStats own[kGnMostChunks / 64];
-      float m = 0, q = 0;
+#pragma unroll
+      for (int i = 0; i < kGnMostChunks / 64; i++) {
+        const int k = lane + 64 * i;
+        if (k < p.chunks) own[i] = s[k];
+      }
+      const float pivot = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(own[0].mean)));
+      float mean[kGnMostChunks / 64], square[kGnMostChunks / 64];
+      double m = 0, q = 0;
       auto values = [&](int k) {     // of part k
         return (float)min(p.chunk_pixels, p.pixels - min(k, p.chunks - 1) * p.chunk_pixels) * of_group;
       };
 #pragma unroll
       for (int i = 0; i < kGnMostChunks / 64; i++) {
         const int k = lane + 64 * i;
-        own[i] = k < p.chunks ? s[k] : GroupStats{0, 0, 0};
-        if (k < p.chunks) m = fmaf(own[i].mean, values(k), m);
+        mean[i] = (own[i].mean - pivot) + own[i].low;
+        square[i] = own[i].square;
+        if (k < p.chunks) m = fma((double)mean[i], (double)values(k), m);
       }
-      m = wave_sum(m) / total;
+      m = wave_sum(m) * over;
 #pragma unroll
       for (int i = 0; i < kGnMostChunks / 64; i++) {
         const int k = lane + 64 * i;
-        const float d = own[i].mean - m;
-        if (k < p.chunks) q += fmaf(d * d, values(k), own[i].square);
+        const float d = mean[i] - (float)m;
+        if (k < p.chunks) q += fmaf(d * d, values(k), square[i]);
       }
       q = wave_sum(q);
       if (lane == 0) {
-        s_group[g] = m;
-        s_second[g] = 1.0f / sqrtf(q / total + p.epsilon);
+        const GnMean all(pivot, m);
+        s_group[g] = all.high;
+        s_low[g] = all.low;
+        s_second[g] = 1.0f / sqrtf((float)(q * over) + p.epsilon);
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
 
-  if constexpr (R >= 16) load_affine();
+  if constexpr (!kAffineAhead) load_affine();
   constexpr int NM = NP == 1 ? 1 : 8;
   float mean[NM];
   GnGroup of(c - c0, p.per);
@@ -406,7 +512,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
     const int g = j < left ? of.group : 0;
     if (NM == 8 || j == 0) mean[NM == 1 ? 0 : j] = s_group[g];
     scale[j] *= s_second[g];
-    if (E::kSize == 2) shift[j] = fmaf(-mean[NM == 1 ? 0 : j], scale[j], shift[j]);
+    shift[j] = fmaf(-s_low[g], scale[j], shift[j]);
     if (NM == 8) of.next(p.per);
   }
   uint8_t *out = p.out + (size_t)sample * p.pixels * p.out_row_bytes;
@@ -418,7 +524,7 @@ __global__ __launch_bounds__(kGnMost) void group_norm_kernel(GroupNorm p) {
       const int px = from + first + i * stride;
       if (first + i * stride < px_end - from && (OUT::kSize == 0 || inside))
         gn_write<E, OUT, decltype(act)::value, NM>(out + (size_t)px * p.out_row_bytes, c, left, twice, inside, raw[i], mean,
-                                                   scale, shift, p);
+                                                   scale, shift, one, p);
     }
   };
   for (int from = px0;;) {
@@ -484,7 +590,7 @@ __global__ __launch_bounds__(kGnWideThreads) void group_norm_wide_stats_kernel(G
     variance = variance < 0 ? 0 : variance;          // (NaN stays)
     const float high = (float)mean;
     // (what is left of the mean is taken from its parts: their sum is rounded too)
-    p.stats[blockIdx.x] = GroupStats{high, (float)(1.0 / sqrt(variance + p.epsilon)), (float)(rest - (high - pivot))};
+    p.stats[blockIdx.x] = GroupStats{high, (float)(1.0 / sqrt(variance + p.epsilon)), (float)(rest - (high - pivot)), 0};
   }
 }
 
@@ -618,7 +724,8 @@ template <class E, class OUT, int R, int MODE, int NP>
 static int gn_launch_one(const GroupNorm &p, const GnPlan &plan, hipStream_t st) {
   const int V = 1 << p.lg_vec;
   const int rows = V < 64 ? plan.threads / 64 : plan.threads >> p.lg_vec;
-  const size_t lds = (2 * (size_t)p.in_slice + (MODE == kGnApply ? 0 : (size_t)rows * V * NP)) * 4;
+  const size_t lds = 16 * ((size_t)p.in_slice + 1) +
+                     (MODE == kGnApply ? 0 : (size_t)rows * V * NP * sizeof(GnWide<NP>));
   const size_t sets = (size_t)(p.by_die ? (p.samples + 7) / 8 * 8 : p.samples) * p.slices * p.chunks;
   group_norm_kernel<E, OUT, R, MODE, NP><<<(unsigned)sets, plan.threads, lds, st>>>(p);
   return check_launch("group_norm");

@@ -954,8 +954,10 @@ int mi355x_mx4_fc(void *out, int out_type, size_t out_row_bytes, const void *in,
 /* Group norm over channels-last tensors in [N x pixels x C] of a float type, C / groups
  * neighbouring channels of all pixels of a sample to a group:
  *   out = activation((in - mean) / sqrt(variance + epsilon) * gamma[c] + beta[c])
- * with the mean and the variance (over all values, not one less) of the group, both held in
- * 32 bits. out: of the input's type, also in place (same address and distance between rows),
+ * with the mean and the variance (over all values, not one less) of the group, held in 32 bits
+ * or more, of distances within the group: their error goes by how far its values lie from each
+ * other, not from zero. (Variances past the range of 32 bits: the group becomes beta, or NaN.)
+ * out: of the input's type, also in place (same address and distance between rows),
  * or MI355X_MX4, quantized from the 32-bit results: the input of mi355x_mx4_fc. gamma, beta:
  * float [C], or NULL (1 and 0). activation as above. row_bytes: the distance between pixels;
  * samples follow each other, up to 2^31 - 1 pixels in all. A NaN or an infinity makes NaN of
