@@ -1562,6 +1562,22 @@ def _float_rows(x, type_):
     return x
 
 
+def _mx4_rows(q):
+    q = np.ascontiguousarray(q)
+    assert q.dtype == np.uint8, q.dtype
+    return q
+
+
+def _columns(what, v, n):
+    """A vector of a value for each of n columns, or None."""
+    if v is None:
+        return None
+    v = np.ascontiguousarray(v, np.float32)
+    if v.shape != (n,):
+        raise MI355XError(-1, f"{what} of shape {v.shape}, {n} columns")
+    return v
+
+
 def mx4_quantize(x, type_=TYPE_F32):
     x = _float_rows(x, type_)
     rows, cols = x.shape
@@ -1571,7 +1587,7 @@ def mx4_quantize(x, type_=TYPE_F32):
 
 
 def mx4_dequantize(q, cols, type_=TYPE_F32):
-    q = np.ascontiguousarray(q, np.uint8)
+    q = _mx4_rows(q)
     dq, out = to_device(q), DeviceBuffer.empty((q.shape[0], cols), _FLOAT_DTYPES[type_])
     launch_mx4_dequantize(out, type_, cols * out.dtype.itemsize, dq, q.shape[1], q.shape[0], cols)
     return out.numpy()
@@ -1579,13 +1595,14 @@ def mx4_dequantize(q, cols, type_=TYPE_F32):
 
 def mx4_fc(x, in_type, weights, bias, K, out_type=TYPE_F32, activation=ACT_NONE):
     """x [M, K] of a float type, or rows of TYPE_MX4; weights: rows of TYPE_MX4."""
-    x = np.ascontiguousarray(x, np.uint8) if in_type == TYPE_MX4 else _float_rows(x, in_type)
-    weights = np.ascontiguousarray(weights, np.uint8)
+    x = _mx4_rows(x) if in_type == TYPE_MX4 else _float_rows(x, in_type)
+    weights = _mx4_rows(weights)
     M, N = x.shape[0], weights.shape[0]
+    bias = _columns("mx4_fc: bias", bias, N)
     shape = (M, mx4_row_bytes(N) if out_type == TYPE_MX4 else N)
     out = DeviceBuffer.empty(shape, np.uint8 if out_type == TYPE_MX4 else _FLOAT_DTYPES[out_type])
     dx, dw = to_device(x), to_device(weights)
-    db = to_device(np.ascontiguousarray(bias, np.float32)) if bias is not None else None
+    db = to_device(bias) if bias is not None else None
     n = mx4_fc_workspace_bytes(M, K, N, in_type)
     ws = DeviceBuffer(n) if n else None
     launch_mx4_fc(out, out_type, shape[1] * out.dtype.itemsize, dx, in_type, x.shape[1] * x.dtype.itemsize, dw,
@@ -1598,10 +1615,11 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-5, activation=ACT_NO
     x = _float_rows(x, type_)
     out_type = type_ if out_type is None else out_type
     N, pixels, C_ = x.shape
+    gamma, beta = _columns("group_norm: gamma", gamma, C_), _columns("group_norm: beta", beta, C_)
     shape = (N, pixels, mx4_row_bytes(C_) if out_type == TYPE_MX4 else C_)
     out = DeviceBuffer.empty(shape, np.uint8 if out_type == TYPE_MX4 else x.dtype)
     dx = to_device(x)
-    dg, db = (to_device(np.ascontiguousarray(v, np.float32)) if v is not None else None for v in (gamma, beta))
+    dg, db = (to_device(v) if v is not None else None for v in (gamma, beta))
     n = group_norm_workspace_bytes(N, pixels, C_, groups)
     ws = DeviceBuffer(n) if n else None
     launch_group_norm(out, out_type, shape[2] * out.dtype.itemsize, dx, type_, C_ * x.itemsize, dg, db, N, pixels,
