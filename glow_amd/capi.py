@@ -1582,7 +1582,7 @@ def mx4_quantize(x, type_=TYPE_F32):
     x = _float_rows(x, type_)
     rows, cols = x.shape
     dx, out = to_device(x), DeviceBuffer.empty((rows, mx4_row_bytes(cols)), np.uint8)
-    launch_mx4_quantize(out, out.shape[1], dx, type_, x.strides[0], rows, cols)
+    launch_mx4_quantize(out, out.shape[1], dx, type_, cols * x.itemsize, rows, cols)
     return out.numpy()
 
 

@@ -55,3 +55,24 @@ def test_what_fits_goes_on():
                  lambda: capi.group_norm(IMAGE, 3, np.ones(12), None), lambda: capi.mx4_dequantize(ROWS, 100)):
         with pytest.raises(Reached):
             call()
+
+
+class Device:
+    def __init__(self, shape, dtype=np.uint8):
+        self.shape, self.dtype = shape, np.dtype(dtype)
+
+    def numpy(self):
+        return None
+
+
+@pytest.mark.parametrize("rows", [lambda x: x[::3][:1], lambda x: x[::-1][:1], lambda x: x[:1], lambda x: x[:0], lambda x: x])
+def test_rows_are_as_far_apart_as_they_are_long(monkeypatch, rows):
+    """numpy leaves the stride of an axis of one or no rows as it was, whatever it calls contiguous."""
+    seen = []
+    monkeypatch.setattr(capi, "to_device", lambda a: Device(a.shape, a.dtype))
+    monkeypatch.setattr(capi.DeviceBuffer, "empty", classmethod(lambda cls, shape, dtype: Device(shape, dtype)))
+    monkeypatch.setattr(capi, "launch_mx4_quantize", lambda *a: seen.append(a))
+    x = rows(np.ones((9, 40), np.float32))
+    capi.mx4_quantize(x)
+    (_, _, _, type_, src_row_bytes, n, cols), = seen
+    assert (type_, src_row_bytes, n, cols) == (capi.TYPE_F32, 160, x.shape[0], 40)
