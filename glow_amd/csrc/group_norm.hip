@@ -800,7 +800,11 @@ int mi355x_group_norm_workspace_bytes(size_t N, size_t pixels, size_t C, size_t 
     *bytes = 0;
     return MI355X_OK;
   }
-  *bytes = N * groups * gn_most_chunks(N, pixels) * sizeof(GroupStats);
+  size_t slots;
+  MI355X_REQUIRE(!__builtin_mul_overflow(N * groups, gn_most_chunks(N, pixels) * sizeof(GroupStats), &slots) &&
+                     slots <= PTRDIFF_MAX,
+                 "group_norm: %zu x %zu groups", N, groups);
+  *bytes = slots;
   return MI355X_OK;
 }
 

@@ -191,3 +191,25 @@ def test_empty_tensors_are_a_no_op():
     assert lib.mi355x_group_norm(*norm_args(N=0)) == 0
     assert lib.mi355x_group_norm(*norm_args(pixels=0)) == 0
     assert lib.mi355x_group_norm(*norm_args(C_=0, groups=1)) == 0
+
+
+def test_group_norm_workspace_of_more_groups_than_memory_is_refused():
+    most = 0x7fffffff
+    for N, pixels, groups in ((most, 1, most), (most, 1, 1 << 30), (1 << 30, most, 1 << 30)):
+        with pytest.raises(capi.MI355XError, match="groups"):
+            capi.group_norm_workspace_bytes(N, pixels, groups, groups)
+    assert capi.group_norm_workspace_bytes(1 << 20, 1, 1 << 20, 1 << 20) >= 1 << 40
+    # a slot is the more for every part that a slice may be cut into: never less for more pixels
+    sizes = [capi.group_norm_workspace_bytes(3, pixels, 64, 8) for pixels in (1, 7, 100, 10 ** 6)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+
+
+def test_group_norm_refuses_workspaces_of_any_size_that_do_not_fit():
+    for N, pixels, C_, groups in ((2, 5000, 100, 4), (2, 9, 100, 4), (1, 1, 9000, 1)):
+        need = capi.group_norm_workspace_bytes(N, pixels, C_, groups)
+        assert need > 0
+        a = dict(N=N, pixels=pixels, C_=C_, groups=groups, in_row=4 * C_, out_row=4 * C_)
+        for change in (dict(ws=0), dict(ws_bytes=need - 1), dict(ws_bytes=0), dict(ws=S + 4)):
+            refused("mi355x_group_norm", norm_args(**a, **change), "workspace")
+        refused("mi355x_group_norm", norm_args(**a, ws=Q + 160), "overlaps")
+        refused("mi355x_group_norm", norm_args(**a, ws=P + 160), "overlaps")
