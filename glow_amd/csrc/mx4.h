@@ -115,9 +115,12 @@ __device__ __forceinline__ void store8_end(typename E::T *p, const float (&x)[8]
     if (j < left) p[j] = E::from(x[j]);
 }
 
-// v / (1 + exp(-v)) with the hardware's exp2 and reciprocal: off by |v| + 4 steps of 2^-24 at
-// most, next to nothing beside a 16- or 4-bit result's own rounding, and two instructions
-// for the twenty of a correctly rounded quotient. exp2's infinity for v below -88 gives -0.
+// v / (1 + exp(-v)) with the hardware's exp2 and reciprocal, two instructions for the twenty of a
+// correctly rounded quotient. In steps of 2^-24: 1.23 |v| from the exponent (its product's
+// rounding and the constant's), 2 each from exp2 and the reciprocal, 1 each from the sum and the
+// last product, so 1.23 |v| + 6 at most; next to nothing beside a 16- or 4-bit result's own rounding,
+// and what a 32-bit result is off by. Below -87 the reciprocal is no normal number, or exp2 an
+// infinity: -0 for magnitudes under 2^-119.
 __device__ __forceinline__ float silu(float v) {
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
 }

@@ -34,7 +34,7 @@ __device__ __forceinline__ MxPlace mx_place(const MxRows &r, unsigned tile) {
   p.inside = p.row < r.rows && p.group < r.groups;
   return p;
 }
-// A launch has 2^24 workgroups at most (2^32 threads are the limit); they take turns then.
+// A launch has 2^23 workgroups at most, 2^31 threads (under 2^32 are the limit); they take turns then.
 constexpr unsigned kMxMostBlocks = 1u << 23;
 static int mx_rows(const char *what, size_t rows, size_t cols, MxRows *r, unsigned *blocks) {
   r->rows = (long long)rows;

@@ -773,7 +773,8 @@ typedef struct {
  * (LLVMIRGen.cpp:618-662): CLIP {min, max}; LEAKY_RELU {pre, post, scale}. */
 enum { MI355X_ACT_NONE = 0, MI355X_ACT_RELU = 1, MI355X_ACT_CLIP = 2,
        MI355X_ACT_TANH = 3, MI355X_ACT_SIGMOID = 4, MI355X_ACT_LEAKY_RELU = 5,
-       /* v / (1 + exp(-v)): of mi355x_mx4_fc and mi355x_group_norm only */
+       /* v / (1 + exp(-v)), within (1.3 |v| + 6) 2^-24 of its value before the result's own
+        * rounding, or 0 for values under 2^-119: of mi355x_mx4_fc and mi355x_group_norm only */
        MI355X_ACT_SILU = 6 };
 
 /* libjit_channelwise_quantized_conv2d_i8_i32 / _i8_i8 (reference
