@@ -124,14 +124,14 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
 template <class IN, class OUT, int BN, int BM, int WN, int WM, int BLOCKS>
 static int mx4_fc_short_launch(const MxFc &p, int K, hipStream_t st) {
   auto kern = mx4_fc_short_kernel<IN, OUT, BN, BM, WN, WM, BLOCKS>;
-  static std::atomic<uint64_t> attr_set{0};
   const auto lds = [](int groups) { return (size_t)mx4_short_bias<OUT, BN, BM, WN, WM>(groups) + BN * 4; };
-  if (int rc = set_lds_attr(kern, lds(kShortGroups), attr_set)) return rc;
   const long long columns = OUT::kSize ? p.N : (long long)p.out_groups * kMxGroup;
   const long long tiles_n = (columns + BN - 1) / BN, tiles_m = ((long long)p.M + BM - 1) / BM;
   constexpr int THREADS = MxTile<OUT, BN, BM, WN, WM>::kThreads;
   if (tiles_n * tiles_m > (1 << 22))
     return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_fc: %d x %d results", p.M, p.N);
+  static std::atomic<uint64_t> attr_set{0};
+  if (int rc = set_lds_attr(kern, lds(kShortGroups), attr_set)) return rc;
   kern<<<(unsigned)(tiles_n * tiles_m), THREADS, lds(p.groups), st>>>(p, K, (int)tiles_n, (int)tiles_m);
   return check_launch("mx4_fc");
 }

@@ -338,13 +338,13 @@ template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS>
 static int mx4_fc_tile_launch(const MxFc &p, hipStream_t st) {
   typedef MxRing<OUT, BN, BM, WN, WM, STAGES> T;
   auto kern = mx4_fc_tile_kernel<OUT, BN, BM, WN, WM, STAGES, BLOCKS>;
-  static std::atomic<uint64_t> attr_set{0};
-  if (int rc = set_lds_attr(kern, T::kLds, attr_set)) return rc;
   // a microscaled result has whole groups of columns, the ones past N zeros
   const long long columns = OUT::kSize ? p.N : (long long)p.out_groups * kMxGroup;
   const long long tiles_n = (columns + BN - 1) / BN, tiles_m = ((long long)p.M + BM - 1) / BM;
   if (tiles_n * tiles_m > (1 << 22))
     return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_fc: %d x %d results", p.M, p.N);
+  static std::atomic<uint64_t> attr_set{0};
+  if (int rc = set_lds_attr(kern, T::kLds, attr_set)) return rc;
   kern<<<(unsigned)(tiles_n * tiles_m), T::kThreads, T::kLds, st>>>(p, (int)tiles_n, (int)tiles_m);
   return check_launch("mx4_fc");
 }

@@ -914,8 +914,9 @@ enum { MI355X_F32 = 0, MI355X_F16 = 1, MI355X_BF16 = 2, MI355X_MX4 = 3 };
  * multiple of the element's size, rows at any address that is one too. Tensors of no rows
  * or columns are a no-op. Results may not overlap what they are made from, except where it
  * says so. Sizes up to 2^31 - 1 each; MI355X_ERR_NOT_SUPPORTED for tensors of over 2^42
- * columns in all, or of products of over 2^22 tiles of 64 x 64 results (16 x 16 up to four
- * rows). */
+ * columns in all, of products of over 2^22 tiles of 64 x 64 results (16 x 16 up to four
+ * rows), or of group norms of which one sample's slices take more threads than a launch
+ * has room for (none of up to 2^21 channels). */
 size_t mi355x_mx4_row_bytes(size_t cols);
 /* Each block of 32: m = the largest magnitude, scale 2^max(floor(log2 m) - 2, -127) (byte
  * 0 for a block of zeros), codes = value / scale rounded to nearest, ties to even, and

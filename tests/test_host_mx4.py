@@ -213,3 +213,17 @@ def test_group_norm_refuses_workspaces_of_any_size_that_do_not_fit():
             refused("mi355x_group_norm", norm_args(**a, **change), "workspace")
         refused("mi355x_group_norm", norm_args(**a, ws=Q + 160), "overlaps")
         refused("mi355x_group_norm", norm_args(**a, ws=P + 160), "overlaps")
+
+
+def test_sizes_past_a_launch_are_not_supported():
+    # 2^31 - 8 channels, each a group: 2^26 slices and more, of 64 threads; refused before any launch
+    C_ = (1 << 31) - 8
+    for pixels, channels in ((1, C_), (2000, 1 << 25)):
+        need = capi.group_norm_workspace_bytes(8, pixels, channels, channels)
+        far = dict(out=1 << 45, x=1 << 50, ws=1 << 55, ws_bytes=need, in_type=1, out_type=1, in_row=2 * channels, out_row=2 * channels)
+        refused("mi355x_group_norm", norm_args(N=8, pixels=pixels, C_=channels, groups=channels, **far), "channels", -4)
+    # 2^34 tiles of 128 x 128 results; 2^23 of 16 x 16
+    refused("mi355x_mx4_fc", fc_args(out=1 << 55, x=1 << 45, w=1 << 50, M=1 << 24, N=1 << 24, out_row=1 << 26), "results", -4)
+    refused("mi355x_mx4_fc", fc_args(out=1 << 55, x=1 << 45, w=1 << 50, M=3, N=1 << 27, out_row=1 << 29), "results", -4)
+    refused("mi355x_mx4_quantize", quantize_args(dst=1 << 61, src=1 << 62, rows=1 << 22, cols=(1 << 31) - 8, src_row=1 << 33,
+                                                 dst_row=1 << 31), "values", -4)
