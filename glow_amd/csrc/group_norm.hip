@@ -19,10 +19,12 @@
 // kept as its rounding and the rest of it, and a value loses the first before it is scaled. (Slices of
 // over 8192 channels, a third way: sums in 64 bits.)
 //
-// us: 64 x 3136 x 256 of fp16 53 (206 MB, 3.9 TB/s: 40 at the rate of a large copy; a workgroup fills a
-// CU and reads, computes and writes in turn), 32 x 784 x 512 of bf16 with SiLU to microscaled rows 16.5
-// (32 MB; 14.1 without SiLU: all CUs read, then compute, then write), 1 x 49 x 512 4.5 (the launch and
-// two rounds of sums), 4 x 16384 x 128 in parts 18, 3 x 1225 x 100 of fp32 in parts 8.9 (two launches).
+// us: 64 x 3136 x 256 of fp16 55 (206 MB, 3.8 TB/s: 40 at the rate of a large copy; a workgroup fills a
+// CU and reads, computes and writes in turn), 32 x 784 x 512 of bf16 with SiLU to microscaled rows 16.6
+// (32 MB; 14.4 without SiLU: all CUs read, then compute, then write), 1 x 49 x 512 4.5 (the launch and
+// two rounds of sums), 4 x 16384 x 128 in parts 18, 3 x 1225 x 100 of fp32 in parts 9.6 (two launches).
+// Distances instead of values cost 0 to 6 % of these; the times beside gn_plan's rules are of
+// before, on both sides.
 #include "mx4.h"
 
 #include <algorithm>

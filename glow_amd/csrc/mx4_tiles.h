@@ -8,14 +8,13 @@
 // first operand and their rows are permuted on the way into LDS: a lane ends with sixteen
 // neighbouring columns of one output row (eight, where a wave has 32).
 //
-// 8192 x 4096 x 4096 of random codes to bf16: 75 to 80 us from card to card, 3.5 PFLOP/s. The
-// matrix cores are busy for two fifths of that. Random codes draw so much power that the
+// 8192 x 4096 x 4096 of random codes to bf16: 80 us, 75 to 87 by card and load, 3.4 PFLOP/s. The
+// matrix cores are busy for 47 % of the cycles. Random codes draw so much power that the
 // instructions alone, from registers, reach 6.5 PFLOP/s in their 32x32 form and 7.5 in this one
 // (zeros: 9.5); a step of a 256x256 tile takes 0.95 us where they need 0.46, and 0.8 without
 // its loads; and the ends of a tile cost 8 us, where all CUs write (67 MB in all) or wait together.
-// What gave most on the way: the activation chosen once (a tile's end 17 -> 12 us), 16x16
-// instructions (92 -> 88 us), chunks placed so that reads meet no bank twice (88 -> 84 us; the
-// scales' single bytes still meet one another).
+// What gave most on the way, about 5 % each: the activation chosen once, 16x16 instructions, chunks
+// placed so that reads meet no bank twice (the scales' single bytes still meet one another).
 #ifndef GLOW_MI355X_MX4_TILES_H
 #define GLOW_MI355X_MX4_TILES_H
 
