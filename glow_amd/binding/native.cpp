@@ -238,6 +238,8 @@ PyMethodDef g_methods[] = {
     ENTRY(mx4_dequantize),
     ENTRY(mx4_fc),
     ENTRY(group_norm),
+    ENTRY(mx4_cache_write),
+    ENTRY(mx4_attention),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods,

@@ -57,6 +57,7 @@ EXPORTS = [
     "mi355x_copy_segments", "mi355x_set_device", "mi355x_stream_query", "mi355x_host_is_pinned",
     "mi355x_mx4_row_bytes", "mi355x_mx4_quantize_host", "mi355x_mx4_quantize", "mi355x_mx4_dequantize",
     "mi355x_mx4_fc_workspace_bytes", "mi355x_mx4_fc", "mi355x_group_norm_workspace_bytes", "mi355x_group_norm",
+    "mi355x_mx4_cache_write", "mi355x_mx4_attention_workspace_bytes", "mi355x_mx4_attention",
 ]
 
 
@@ -83,6 +84,13 @@ class Conv3dGeom(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "N", "IT", "IH", "IW", "IC", "OT", "OH", "OW", "OC", "KT", "KH", "KW",
         "strideT", "strideH", "strideW", "padN", "padT", "padL", "group")]
+
+
+class Mx4Cache(C.Structure):
+    """mi355x_mx4_cache; the addresses are of device memory."""
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("row_bytes", C.c_uint64), ("pages", C.c_void_p),
+                ("n_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("pages_per_sequence", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
 
 
 def conv3d_geom(N, IT, IH, IW, IC, OC, kernel, stride, pads, group=1):
@@ -1625,3 +1633,99 @@ def group_norm(x, groups, gamma=None, beta=None, epsilon=1e-5, activation=ACT_NO
     launch_group_norm(out, out_type, shape[2] * out.dtype.itemsize, dx, type_, C_ * x.itemsize, dg, db, N, pixels,
                       C_, groups, epsilon, activation, ws, n)
     return out.numpy()
+
+
+# ---- a cache of microscaled rows, attention over it ------------------------------
+
+def launch_mx4_cache_write(cache, keys, values, type_, keys_row_bytes, starts, lengths, sequences, rows, stream=None,
+                           values_row_bytes=None):
+    (_native or native()).mx4_cache_write(cache, keys, values, type_, keys_row_bytes,
+                                          keys_row_bytes if values_row_bytes is None else values_row_bytes, starts,
+                                          lengths, sequences, rows, stream)
+
+
+def mx4_attention_workspace_bytes(cache, heads, sequences, rows, max_length):
+    n = C.c_size_t(0)
+    check(lib().mi355x_mx4_attention_workspace_bytes(C.byref(cache), _sz(heads), _sz(sequences), _sz(rows),
+                                                     _sz(max_length), C.byref(n)))
+    return n.value
+
+
+def launch_mx4_attention(out, out_type, out_row_bytes, q, type_, q_row_bytes, heads, cache, starts, lengths, sequences,
+                         rows, max_length, scale, window=0, sinks=0, workspace=None, workspace_bytes=0, stream=None):
+    (_native or native()).mx4_attention(out, out_type, out_row_bytes, q, type_, q_row_bytes, heads, cache, starts,
+                                        lengths, sequences, rows, max_length, scale, window, sinks, workspace,
+                                        workspace_bytes, stream)
+
+
+def _cache_on_device(keys, values, pages, page_tokens, sequences, kv_heads, head_dim):
+    """(cache, its buffers) of host arrays: keys and values rows of TYPE_MX4, pages int32 [sequences, pages of each]
+    or None."""
+    keys, values = _mx4_rows(keys), _mx4_rows(values)
+    if keys.shape != values.shape or page_tokens <= 0 or keys.shape[0] % page_tokens:
+        raise MI355XError(-1, f"keys of shape {keys.shape}, values of {values.shape}, pages of {page_tokens} tokens")
+    n_pages = keys.shape[0] // page_tokens
+    if pages is None:
+        if not sequences or n_pages % sequences:
+            raise MI355XError(-1, f"{n_pages} pages for {sequences} sequences")
+        per = n_pages // sequences
+    else:
+        pages = np.ascontiguousarray(pages, np.int32)
+        if pages.ndim != 2 or pages.shape[0] != sequences:
+            raise MI355XError(-1, f"pages of shape {pages.shape} for {sequences} sequences")
+        per = pages.shape[1]
+    held = [to_device(keys), to_device(values), to_device(pages) if pages is not None else None]
+    cache = Mx4Cache(held[0].ptr, held[1].ptr, keys.shape[1], held[2].ptr if held[2] else None, n_pages, page_tokens, per,
+                     kv_heads, head_dim)
+    return cache, held
+
+
+def _batch_on_device(starts, lengths):
+    starts, lengths = (np.ascontiguousarray(v, np.int32) for v in (starts, lengths))
+    if starts.shape != (lengths.size + 1,):
+        raise MI355XError(-1, f"starts of shape {starts.shape} for {lengths.size} sequences")
+    return to_device(starts), to_device(lengths), lengths.size
+
+
+def mx4_cache_write(keys, values, new_keys, new_values, starts, lengths, kv_heads, head_dim, page_tokens, pages=None,
+                    type_=TYPE_F32):
+    """The cache's (keys, values), rows of TYPE_MX4, with the batch's new ones written into them."""
+    ds, dl, n = _batch_on_device(starts, lengths)
+    take = _mx4_rows if type_ == TYPE_MX4 else lambda x: _float_rows(x, type_)
+    new_keys, new_values = take(new_keys), take(new_values)
+    cols = kv_heads * head_dim
+    want = mx4_row_bytes(cols) if type_ == TYPE_MX4 else cols
+    if new_keys.shape != new_values.shape or new_keys.ndim != 2 or new_keys.shape[1] != want:
+        raise MI355XError(-1, f"new keys of shape {new_keys.shape}, values of {new_values.shape}, {cols} columns")
+    cache, held = _cache_on_device(keys, values, pages, page_tokens, n, kv_heads, head_dim)
+    dk, dv = to_device(new_keys), to_device(new_values)
+    launch_mx4_cache_write(cache, dk, dv, type_, want * new_keys.itemsize, ds, dl, n, new_keys.shape[0])
+    return held[0].numpy(), held[1].numpy()
+
+
+def mx4_attention(q, heads, keys, values, starts, lengths, kv_heads, head_dim, page_tokens, pages=None, scale=None,
+                  window=0, sinks=0, max_length=None, type_=TYPE_F32, out_type=None, out=None):
+    """q [rows, heads * head_dim] of a float type over a cache of rows of TYPE_MX4; rows of no sequence are those of `out`
+    (zeros where it is None)."""
+    q = _float_rows(q, type_)
+    out_type = type_ if out_type is None else out_type
+    ds, dl, n = _batch_on_device(starts, lengths)
+    cols = heads * head_dim
+    if q.ndim != 2 or q.shape[1] != cols:
+        raise MI355XError(-1, f"queries of shape {q.shape}, {heads} heads of {head_dim} columns")
+    shape = (q.shape[0], mx4_row_bytes(cols) if out_type == TYPE_MX4 else cols)
+    dtype = np.dtype(np.uint8 if out_type == TYPE_MX4 else q.dtype)
+    out = np.zeros(shape, dtype) if out is None else np.ascontiguousarray(out)
+    if out.shape != shape or out.dtype != dtype:
+        raise MI355XError(-1, f"a result of shape {out.shape} and {out.dtype}, {shape} and {dtype} are needed")
+    cache, held = _cache_on_device(keys, values, pages, page_tokens, n, kv_heads, head_dim)
+    if max_length is None:
+        max_length = cache.pages_per_sequence * page_tokens
+    dq, do = to_device(q), to_device(out)
+    size = mx4_attention_workspace_bytes(cache, heads, n, q.shape[0], max_length)
+    ws = DeviceBuffer(size) if size else None
+    launch_mx4_attention(do, out_type, shape[1] * dtype.itemsize, dq, type_, cols * q.itemsize, heads, cache, ds, dl, n,
+                         q.shape[0], max_length, head_dim ** -0.5 if scale is None else scale, window, sinks, ws, size)
+    got = do.numpy()
+    del held
+    return got

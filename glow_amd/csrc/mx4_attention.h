@@ -1,0 +1,318 @@
+// Attention over a cache of microscaled rows: what a wave does with sixteen rows of queries.
+//
+// For a head of the cache, "rows" are (row of the batch, query head of the group) pairs, the group's
+// heads of a row next to each other. With S = Q K^T, a softmax over tokens and O = P V, everything is
+// kept transposed, tokens and columns of values being the matrix instructions' rows, the sixteen
+// queries their columns, lane % 16 in what follows; q is lane / 16:
+//
+//   S   16 tokens x 16 queries by the scaled instruction over 128 columns: codes and scale bytes of
+//       the keys as they lie in memory (a lane has one block of a token), queries as sums of 6-bit
+//       floats (E2M3, four bits each) with a power of two for each block of 32: 3 terms for bf16, 4 for
+//       fp16, 6 for fp32. Nothing of a key is ever converted. A lane gets tokens 4 q .. 4 q + 3. 8-bit terms
+//       would be fewer (2, 3, 6) of twice the time each, and the instruction cuts small products off
+//       where exponents lie far apart (2^-17 of the sum; 6-bit products come out exact).
+//   P   is what the lane then holds of two tiles of tokens: eight weights of its query, which is what the
+//       16x16x32 instruction wants of its second operand, tokens in the order 4 q + i of the first
+//       tile, then of the second. No lane needs another's weights.
+//   O   values [32 tokens x D] are that instruction's first operand. A lane needs, of its eight tokens, D /
+//       16 columns: those next to each other, a word of codes for D = 128; the instruction of
+//       number m then has column m of each lane's.  Codes are converted to pairs of neighbouring columns and
+//       transposed to pairs of tokens by byte permutes. Results: lane q has columns 32 q .. 32 q + 31 for
+//       D = 128, a block of a microscaled result.
+//
+// The running maximum moves only when a score passes it by more than 2^8: weights stay below 2^8 then
+// (2^15 in fp16, which are shifted up so that small ones stay normal numbers), and most steps
+// have no rescaling.
+#ifndef GLOW_MI355X_MX4_ATTENTION_H
+#define GLOW_MI355X_MX4_ATTENTION_H
+
+#include "mx4_cache.h"
+
+namespace mi355x {
+
+typedef int at_v4i __attribute__((ext_vector_type(4)));
+typedef int at_v8i __attribute__((ext_vector_type(8)));
+typedef uint32_t at_v6u __attribute__((ext_vector_type(6)));
+typedef float at_v4f __attribute__((ext_vector_type(4)));
+typedef float at_v16f __attribute__((ext_vector_type(16)));
+typedef float at_v32f __attribute__((ext_vector_type(32)));
+typedef _Float16 at_v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 at_v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 at_v2b __attribute__((ext_vector_type(2)));
+typedef __bf16 at_v8b __attribute__((ext_vector_type(8)));
+
+struct Attention {
+  MxCache c;
+  const uint8_t *q;
+  uint8_t *out;
+  float *part;                    // what splits leave for the joining launch
+  size_t q_row_bytes, out_row_bytes;
+  int kv_heads, group;            // heads of queries to one of the cache
+  int most;                       // tokens of a sequence
+  int window, sinks;
+  int slots, splits;
+  int out_groups;                 // of a microscaled result's row
+  float scale;                    // |scale| * log2(e)
+  int negative;                   // of the scale
+};
+
+constexpr float kAtSlack = 8.0f;
+constexpr float kAtNone = -__builtin_inff();
+
+// Terms of a query, terms of a weight, what weights are shifted up by, and the least scale byte of values that count
+// as NaN: 2^14 times 4 is past fp16's range.
+template <class E> struct AtKind { static constexpr int kQ = 6, kP = 3, kNan = 255; static constexpr float kUp = 0; };
+template <> struct AtKind<F16> { static constexpr int kQ = 4, kP = 1, kNan = 141; static constexpr float kUp = 7; };
+template <> struct AtKind<BF16> { static constexpr int kQ = 3, kP = 1, kNan = 255; static constexpr float kUp = 0; };
+
+// Which rows a slot of sixteen has. Slots of a sequence begin at floor(start * group / 16) + its number, which leaves
+// each as many as it needs.
+struct AtRows {
+  int sequence, begin, count;     // of the sequence's rows in the batch
+  int first, last;                // its rows (row, head) of this slot: [first, last)
+  int length;
+};
+template <int ROWS> __device__ __forceinline__ long long at_first_slot(const Attention &p, int s) {
+  return (long long)batch_start(p.c, s) * p.group / ROWS + s;
+}
+template <int ROWS> __device__ __forceinline__ bool at_rows(const Attention &p, int slot, AtRows &r) {
+  r.sequence = __builtin_amdgcn_readfirstlane(
+      find_sequence<64>(p.c.sequences, slot, [&](int s) { return at_first_slot<ROWS>(p, s); }));
+  r.begin = batch_start(p.c, r.sequence);
+  r.count = max(batch_start(p.c, r.sequence + 1) - r.begin, 0);
+  const long long at = (slot - at_first_slot<ROWS>(p, r.sequence)) * ROWS;
+  const int all = r.count * p.group;
+  if (at < 0 || at >= all) return false;
+  r.first = (int)at;
+  r.last = min(all, r.first + ROWS);
+  r.length = min(max(p.c.lengths[r.sequence], 0), p.most);
+  return true;
+}
+// The tiles of tokens that rows at `low` to `high` see some of: those of the first `sinks`, then [from, ..).
+struct AtTiles {
+  int sinks, from, all;
+  __device__ __forceinline__ int at(int u) const { return u < sinks ? u : u - sinks + from; }
+};
+__device__ __forceinline__ AtTiles at_tiles(const Attention &p, int low, int high) {
+  AtTiles t;
+  t.from = max(0, low - p.window + 1) / kCacheTile;     // (low >= -1, window <= 2^31 - 1)
+  t.sinks = min((int)(((unsigned)p.sinks + kCacheTile - 1) / kCacheTile), t.from);
+  t.all = t.sinks + high / kCacheTile + 1 - t.from;
+  if (high < 0) t.all = 0;
+  return t;
+}
+
+// ---- queries -----------------------------------------------------------------------
+
+// Sixteen rows of queries of D columns as sums of 6-bit floats: 32 q to 32 q + 31 of 128 columns are lane q's, a block
+// with a power of two of its own. The largest is scaled to [4, 8); a term rounds to half (values past 7.5 become 7.5),
+// and the next has a sixteenth of its scale: after T terms what is left is 2^-4T of the largest at most.
+template <class E, int D> struct AtQueries {
+  static constexpr int kTerms = AtKind<E>::kQ, kChunks = (D + 127) / 128;
+  at_v6u codes[kChunks][kTerms];
+  int scale[kChunks][kTerms];
+
+  __device__ __forceinline__ void load(const typename E::T *row, bool negative) {
+    const int q = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      at_v16f even, odd;               // the conversion takes every second column in either
+      uint32_t most = 0;
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        float y[8];
+        load8<E>(y, row + c * 128 + 32 * (D == 64 ? q & 1 : q) + e);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          if (D == 64) y[j] = q < 2 ? y[j] : 0.0f;
+          most = max(most, magnitude_bits(y[j]));
+          y[j] = negative ? -y[j] : y[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) even[e / 2 + j] = y[2 * j], odd[e / 2 + j] = y[2 * j + 1];
+      }
+      const int exponent = (int)(most >> 23);
+#pragma unroll
+      for (int t = 0; t < kTerms; t++) {
+        const int byte = max(exponent - 2 - 4 * t, 1);
+        const float s = __uint_as_float((uint32_t)byte << 23);
+        const at_v6u six = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s);
+        // (the conversion writes words of its result before it has read all operands: they have to live on)
+        asm volatile("" ::"v"(even), "v"(odd), "v"(s), "v"(six));
+        if (t + 1 < kTerms) {
+          const at_v32f back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(six, s);
+#pragma unroll
+          for (int j = 0; j < 16; j++) even[j] -= back[2 * j], odd[j] -= back[2 * j + 1];    // (exact)
+        }
+        codes[c][t] = six;
+        scale[c][t] = exponent == 255 ? 255 : byte;
+      }
+    }
+  }
+};
+
+// Scores of sixteen tokens, 4 bits by 6.
+__device__ __forceinline__ at_v4f at_scores(at_v4i keys, int key_scale, at_v6u q, int q_scale, at_v4f acc) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      at_v8i{keys[0], keys[1], keys[2], keys[3], 0, 0, 0, 0},
+      at_v8i{(int)q[0], (int)q[1], (int)q[2], (int)q[3], (int)q[4], (int)q[5], 0, 0}, acc, 4, 2, 0, key_scale, 0, q_scale);
+}
+
+// ---- weights and values --------------------------------------------------------------
+
+// Pairs of values, and the product with weights, in the type that weights are rounded to.
+template <class E> struct AtValues {
+  typedef at_v2b Two;
+  static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 0>) {
+    return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 0);
+  }
+  static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 1>) {
+    return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 1);
+  }
+  static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 2>) {
+    return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 2);
+  }
+  static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 3>) {
+    return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 3);
+  }
+  static __device__ __forceinline__ Two pack(float a, float b) { return Two{(__bf16)a, (__bf16)b}; }
+  static __device__ __forceinline__ at_v4f multiply(at_v4i values, at_v4i weights, at_v4f acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(at_v8b, values), __builtin_bit_cast(at_v8b, weights),
+                                                   acc, 0, 0, 0);
+  }
+};
+template <> struct AtValues<F16> {
+  typedef at_v2h Two;
+  static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 0>) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 0);
+  }
+  static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 1>) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 1);
+  }
+  static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 2>) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 2);
+  }
+  static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 3>) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 3);
+  }
+  static __device__ __forceinline__ Two pack(float a, float b) { return Two{(_Float16)a, (_Float16)b}; }
+  static __device__ __forceinline__ at_v4f multiply(at_v4i values, at_v4i weights, at_v4f acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(at_v8h, values), __builtin_bit_cast(at_v8h, weights),
+                                                  acc, 0, 0, 0);
+  }
+};
+
+// Eight weights of a lane as sums of kP terms.
+template <class E> __device__ __forceinline__ void at_pack(at_v4i (&w)[AtKind<E>::kP], float (&p)[8]) {
+  typedef AtValues<E> V;
+#pragma unroll
+  for (int t = 0; t < AtKind<E>::kP; t++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const typename V::Two two = V::pack(p[2 * j], p[2 * j + 1]);
+      w[t][j] = __builtin_bit_cast(int, two);
+      if (t + 1 < AtKind<E>::kP) p[2 * j] -= (float)two[0], p[2 * j + 1] -= (float)two[1];
+    }
+}
+
+// Eight tokens' words of codes (eight neighbouring columns each; COLS = 4: the low half) -> for each column the
+// eight tokens' values, in the matrix instruction's order.
+template <class E, int COLS>
+__device__ __forceinline__ void at_transpose(at_v4i (&out)[COLS], const uint32_t (&codes)[8], const float (&scale)[8]) {
+  typedef AtValues<E> V;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    auto columns = [&](auto pair) {
+      constexpr int P = decltype(pair)::value;
+      const uint32_t a = __builtin_bit_cast(uint32_t, V::two(codes[2 * j], scale[2 * j], pair));
+      const uint32_t b = __builtin_bit_cast(uint32_t, V::two(codes[2 * j + 1], scale[2 * j + 1], pair));
+      out[2 * P][j] = (int)__builtin_amdgcn_perm(b, a, 0x05040100);
+      out[2 * P + 1][j] = (int)__builtin_amdgcn_perm(b, a, 0x07060302);
+    };
+    columns(std::integral_constant<int, 0>());
+    columns(std::integral_constant<int, 1>());
+    if constexpr (COLS == 8) {
+      columns(std::integral_constant<int, 2>());
+      columns(std::integral_constant<int, 3>());
+    }
+  }
+}
+
+// 2^x, 0 of minus infinity.
+__device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The largest of a query's scores over the four lanes that hold it.
+__device__ __forceinline__ float at_max(float x) {
+  auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+// ---- results -------------------------------------------------------------------------
+
+// Stores the results of quarter `i` of a slot's columns: those that component i of the results has, lane q's
+// 4 q + i. D = 128 and 256: columns 128 c + 8 (4 q + i) + 0 .. 7; D = 64: 4 (4 q + i) + 0 .. 3. Four waves with i of
+// their own call this together where the result is microscaled (`most`: words of LDS for [4][64]).
+template <class E, class OUT, int D>
+__device__ __forceinline__ void at_store(const Attention &p, const AtRows &r, int h, int i, float (&x)[D / 16],
+                                         uint32_t (*most)[64]) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+  const int at = r.first + l16, token = at / p.group, head = h * p.group + (at - token * p.group);
+  uint8_t *row = p.out + (size_t)(r.begin + token) * p.out_row_bytes;
+  constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
+  if constexpr (OUT::kSize != 0) {
+    if (at < r.last) {
+      typename OUT::T *o = reinterpret_cast<typename OUT::T *>(row) + (size_t)head * D;
+#pragma unroll
+      for (int c = 0; c < kChunks; c++) {
+        if constexpr (COLS == 8) {
+          float y[8];
+#pragma unroll
+          for (int m = 0; m < 8; m++) y[m] = x[c * 8 + m];
+          store8<OUT>(o + c * 128 + 8 * (4 * q + i), y);
+        } else {
+#pragma unroll
+          for (int m = 0; m < 4; m++) o[4 * (4 * q + i) + m] = OUT::from(x[m]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < COLS; j++) m = max(m, magnitude_bits(x[c * 8 + j]));
+      if (COLS == 4) m = max_across16(m);           // (a block is two lanes')
+      __syncthreads();
+      most[i][lane] = m;
+      __syncthreads();
+      m = max(max(most[0][lane], most[1][lane]), max(most[2][lane], most[3][lane]));
+      const uint32_t byte = mx4_scale_byte(m);
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) y[j] = j < COLS ? x[c * 8 + (j < COLS ? j : 0)] : 0.0f;
+      const uint32_t codes = mx4_codes8(y, byte);
+      if (at < r.last) {
+        const size_t column = (size_t)head * D + c * 128 + COLS * (4 * q + i);
+        uint8_t *scales = row + (size_t)p.out_groups * kMxGroupBytes;
+        if constexpr (COLS == 8) *reinterpret_cast<uint32_t *>(row + column / 2) = codes;
+        else *reinterpret_cast<uint16_t *>(row + column / 2) = (uint16_t)codes;
+        if (column % 32 == 0) scales[column / 32] = (uint8_t)byte;
+        // the last head fills its group and the row up with zeros
+        if (c == kChunks - 1 && head == p.kv_heads * p.group - 1) {
+          const int heads = p.kv_heads * p.group;
+          if (D == 64 && (heads & 1)) {
+            reinterpret_cast<uint16_t *>(row + (size_t)heads * 32)[4 * q + i] = 0;
+            if (i == 0 && q < 2) scales[heads * 2 + q] = 0;
+          }
+          if (i == 1 && q < ((-p.out_groups) & 3)) reinterpret_cast<uint32_t *>(scales)[p.out_groups + q] = 0;
+        }
+      }
+    }
+  }
+}
+
+} // namespace mi355x
+
+#endif

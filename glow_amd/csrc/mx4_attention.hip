@@ -1,0 +1,423 @@
+// Attention over a cache of microscaled rows: few rows of queries a sequence.
+#include "mx4_attention.h"
+
+#include "gemm_i8.h"
+
+namespace mi355x {
+
+// A workgroup has sixteen rows of queries and a share of the tokens that they see, its eight waves every
+// eighth step of 32 tokens each; their results meet in LDS, those of several shares in a second launch.
+template <int D> constexpr int kAtWaves = D == 256 ? 4 : 8;
+
+// What a wave has asked for of 32 tokens: for each of two tiles a block of a token's keys and its scale byte, and of
+// the values eight tokens' words.
+template <int D> struct AtStep {
+  static constexpr int kChunks = (D + 127) / 128;
+  at_v4i keys[2][kChunks];
+  int key_scale[2][kChunks];
+  uint32_t values[kChunks][8];
+  uint32_t value_scale[kChunks][8];
+  int first[2];                        // token of each tile; -1: none
+};
+
+template <class E, int D> struct AtWave {
+  static constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
+  const Attention &p;
+  int sequence;
+  int l16, q;
+  uint32_t key_at, key_scale_at, value_at[4], value_scale_at[4];
+
+  __device__ __forceinline__ AtWave(const Attention &p, int sequence, int h) : p(p), sequence(sequence) {
+    const int lane = threadIdx.x & 63;
+    l16 = lane & 15, q = lane >> 4;
+    const uint32_t row = (uint32_t)p.c.row_bytes, codes = (uint32_t)h * (D / 2), scales = p.c.scales_at + (uint32_t)h * (D / 32);
+    const int block = D == 64 ? q & 1 : q;          // (lanes q = 2 and 3 have no columns then)
+    key_at = l16 * row + codes + block * 16;
+    key_scale_at = l16 * row + scales + block;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      value_at[i] = (4 * q + i) * row + codes + l16 * (COLS / 2);
+      value_scale_at[i] = (4 * q + i) * row + scales + l16 * COLS / 32;
+    }
+  }
+  // Rows of the cache where tiles u and u + 1 begin.
+  __device__ __forceinline__ void locate(long long (&row)[2], const AtTiles &t, int u) const {
+#pragma unroll
+    for (int k = 0; k < 2; k++) row[k] = u + k < t.all ? cache_tile_row(p.c, sequence, (unsigned)t.at(u + k)) : -1;
+  }
+  __device__ __forceinline__ void load(AtStep<D> &s, const long long (&row)[2], const AtTiles &t, int u) const {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      s.first[k] = row[k] < 0 ? -1 : t.at(u + k) * kCacheTile;
+      // (a tile that is not there reads the cache's first rows; there is a page)
+      const size_t base = (size_t)max(row[k], 0ll) * p.c.row_bytes;
+      const uint8_t *keys = p.c.keys + base, *values = p.c.values + base;
+#pragma unroll
+      for (int c = 0; c < kChunks; c++) {
+        s.keys[k][c] = *reinterpret_cast<const at_v4i *>(keys + (key_at + c * 64));
+        s.key_scale[k][c] = keys[key_scale_at + c * 4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if constexpr (COLS == 8) s.values[c][k * 4 + i] = *reinterpret_cast<const uint32_t *>(values + (value_at[i] + c * 64));
+          else s.values[c][k * 4 + i] = *reinterpret_cast<const uint16_t *>(values + value_at[i]);
+          s.value_scale[c][k * 4 + i] = values[value_scale_at[i] + c * 4];
+        }
+      }
+    }
+  }
+};
+
+template <class E, int D> struct AtState {
+  at_v4f acc[D / 16];
+  float most, sum;                     // of this lane's query, and its part of the sum
+};
+
+template <class E, int D>
+__device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> &queries, AtStep<D> &s, const Attention &p,
+                                        int low, int high, int position) {
+  constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
+  const int lane = threadIdx.x & 63, q = lane >> 4;
+  float score[8];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    at_v4f r = {0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      at_v4i codes = s.keys[k][c];
+      int byte = s.key_scale[k][c];
+      if (D == 64 && q >= 2) codes = at_v4i{0, 0, 0, 0}, byte = 127;
+#pragma unroll
+      for (int t = 0; t < AtKind<E>::kQ; t++)
+        r = at_scores(codes, byte, queries.codes[c][t], queries.scale[c][t], r);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) score[k * 4 + i] = r[i];
+  }
+  auto sees = [&](int token) {
+    return token <= position && (token > position - p.window || token < p.sinks);
+  };
+  // whether every row sees all of these tokens
+  bool whole = true;
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+    whole = whole && s.first[k] >= 0 && s.first[k] + kCacheTile - 1 <= low && s.first[k] > high - p.window;
+  unsigned seen = 0xff;
+  if (!whole) {
+    seen = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int first = s.first[j >> 2];
+      const bool yes = first >= 0 && sees(first + 4 * q + (j & 3));
+      seen |= yes ? 1u << j : 0;
+      score[j] = yes ? score[j] : kAtNone;
+    }
+  }
+  float top = score[0];
+#pragma unroll
+  for (int j = 1; j < 8; j++) top = fmaxf(top, score[j]);
+  top = at_max(top) * p.scale;
+  const bool up = top > a.most + kAtSlack;
+  if (__ballot(up)) {
+    const float factor = up ? at_exp2(a.most - top) : 1.0f;
+    a.most = up ? top : a.most;
+    a.sum *= factor;
+#pragma unroll
+    for (int m = 0; m < D / 16; m++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) a.acc[m][i] *= factor;
+  }
+  const float off = AtKind<E>::kUp - a.most;
+  float weight[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) weight[j] = at_exp2(fmaf(score[j], p.scale, off));
+  if (!whole) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) weight[j] = seen >> j & 1 ? weight[j] : 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++) a.sum += weight[j];
+  at_v4i packed[AtKind<E>::kP];
+  at_pack<E>(packed, weight);
+
+#pragma unroll
+  for (int c = 0; c < kChunks; c++) {
+    uint32_t high_byte = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) high_byte = max(high_byte, s.value_scale[c][j]);
+    if (__ballot(high_byte >= (uint32_t)AtKind<E>::kNan)) {
+      // Blocks that are NaN count as zeros in the product; who sees them becomes NaN.
+      const float nan = __builtin_nanf("");
+      for (int j = 0; j < 8; j++) {
+        const unsigned long long bad = __ballot(s.value_scale[c][j] >= (uint32_t)AtKind<E>::kNan);
+        for (int team = 0; team < 4; team++) {
+          // lanes of the block that this lane's columns are in: 4 of a team's 16, or 8 where it has two blocks
+          const unsigned mine = D == 64 ? (unsigned)(bad >> (16 * team + 8 * (q >> 1))) & 0xff
+                                        : (unsigned)(bad >> (16 * team + 4 * q)) & 0xf;
+          const int first = s.first[j >> 2];
+          if (mine && first >= 0 && sees(first + 4 * team + (j & 3))) {
+#pragma unroll
+            for (int m = 0; m < COLS; m++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) a.acc[c * 8 + m][i] = nan;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const bool is_bad = s.value_scale[c][j] >= (uint32_t)AtKind<E>::kNan;
+        s.values[c][j] = is_bad ? 0 : s.values[c][j];
+        s.value_scale[c][j] = is_bad ? 127 : s.value_scale[c][j];
+      }
+    }
+    float scale[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) scale[j] = __uint_as_float(max(s.value_scale[c][j] << 23, 0x00400000u));
+    at_v4i columns[COLS];
+    at_transpose<E, COLS>(columns, s.values[c], scale);
+#pragma unroll
+    for (int m = 0; m < COLS; m++)
+#pragma unroll
+      for (int t = 0; t < AtKind<E>::kP; t++) a.acc[c * 8 + m] = AtValues<E>::multiply(columns[m], packed[t], a.acc[c * 8 + m]);
+  }
+}
+
+// What a share of a slot leaves: results of component i, then the largest score and the sum of each query.
+template <int D> constexpr size_t at_part_floats() { return 16 * D + 32; }
+
+// The shares of sixteen rows joined, and what is done with the whole: wave i < 4 has component i.
+template <class E, class OUT, int D>
+__global__ __launch_bounds__(256) void mx4_attention_join_kernel(Attention p) {
+  __shared__ uint32_t s_most[4][64];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, i = threadIdx.x >> 6;
+  const int h = (int)(blockIdx.x % (unsigned)p.kv_heads), slot = (int)(blockIdx.x / (unsigned)p.kv_heads);
+  AtRows r;
+  if (!at_rows<16>(p, slot, r)) return;
+  const float *part = p.part + ((size_t)slot * p.splits * p.kv_heads + h) * at_part_floats<D>();
+  const size_t next = (size_t)p.kv_heads * at_part_floats<D>();
+  float most = kAtNone;
+  for (int k = 0; k < p.splits; k++) most = fmaxf(most, part[k * next + 16 * D + l16]);
+  float sum = 0, x[D / 16];
+#pragma unroll
+  for (int m = 0; m < D / 16; m++) x[m] = 0;
+  for (int k = 0; k < p.splits; k++) {
+    const float *from = part + k * next;
+    const float of = from[16 * D + l16];
+    const float factor = of == kAtNone ? (from[16 * D + 16 + l16] == 0 ? 0.0f : __builtin_nanf("")) : at_exp2(of - most);
+    sum += from[16 * D + 16 + l16] * factor;
+#pragma unroll
+    for (int m = 0; m < D / 16; m++) x[m] += from[(i * (D / 16) + m) * 64 + lane] * factor;
+  }
+#pragma unroll
+  for (int m = 0; m < D / 16; m++) x[m] = sum == 0 ? 0.0f : x[m] / sum;
+  at_store<E, OUT, D>(p, r, h, i, x, s_most);
+}
+
+template <class E, class OUT, int D>
+__global__ __launch_bounds__(kAtWaves<D> * 64, D == 256 ? 1 : 2) void mx4_attention_rows_kernel(Attention p, unsigned blocks) {
+  constexpr int WAVES = kAtWaves<D>;
+  extern __shared__ __attribute__((aligned(16))) float s_acc[];      // [waves][4][D / 16][64]
+  __shared__ float s_top[WAVES][16], s_sum[WAVES][16];
+  __shared__ uint32_t s_most[4][64];
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // heads of the cache whose rows share lines run on one die, one behind the other
+  const unsigned per_die = gridDim.x / 8, id = (blockIdx.x & 7) * per_die + (blockIdx.x >> 3);
+  if (id >= blocks) return;
+  const int h = (int)(id % (unsigned)p.kv_heads), share = (int)(id / (unsigned)p.kv_heads % (unsigned)p.splits),
+            slot = (int)(id / (unsigned)p.kv_heads / (unsigned)p.splits);
+  AtRows r;
+  if (!at_rows<16>(p, slot, r)) return;
+
+  const int at = min(r.first + l16, r.last - 1), token = at / p.group, head = h * p.group + (at - token * p.group);
+  auto position_of = [&](int row) { return max(r.length - r.count + row / p.group, -1); };
+  const int position = position_of(at), low = position_of(r.first), high = position_of(r.last - 1);
+  AtQueries<E, D> queries;
+  queries.load(reinterpret_cast<const typename E::T *>(p.q + (size_t)(r.begin + token) * p.q_row_bytes) + (size_t)head * D,
+               p.negative);
+
+  const AtTiles tiles = at_tiles(p, low, high);
+  const long long steps = (tiles.all + 1) / 2;
+  const int begin = (int)(steps * share / p.splits), end = (int)(steps * (share + 1) / p.splits);
+  AtState<E, D> a;
+  a.most = kAtNone, a.sum = 0;
+#pragma unroll
+  for (int m = 0; m < D / 16; m++) a.acc[m] = at_v4f{0, 0, 0, 0};
+  const AtWave<E, D> w(p, r.sequence, h);
+  long long row[2];
+  AtStep<D> next;
+  int step = begin + wave;
+  if (step < end) {
+    w.locate(row, tiles, 2 * step);
+    w.load(next, row, tiles, 2 * step);
+    if (step + WAVES < end) w.locate(row, tiles, 2 * (step + WAVES));
+  }
+  for (; step < end; step += WAVES) {
+    AtStep<D> now = next;
+    if (step + WAVES < end) {
+      w.load(next, row, tiles, 2 * (step + WAVES));
+      if (step + 2 * WAVES < end) w.locate(row, tiles, 2 * (step + 2 * WAVES));
+    }
+    at_step<E, D>(a, queries, now, p, low, high, position);
+  }
+
+  const float sum = add_across32(add_across16(a.sum));
+  if (lane < 16) s_top[wave][l16] = a.most, s_sum[wave][l16] = sum;
+  __syncthreads();
+  float most = kAtNone, whole = 0;
+#pragma unroll
+  for (int k = 0; k < WAVES; k++) most = fmaxf(most, s_top[k][l16]);
+  // a wave that saw nothing has no part in it; sums of NaN come without a largest score
+  auto factor_of = [&](float top, float of) {
+    return top == kAtNone ? (of == 0 ? 0.0f : __builtin_nanf("")) : at_exp2(top - most);
+  };
+#pragma unroll
+  for (int k = 0; k < WAVES; k++) whole += s_sum[k][l16] * factor_of(s_top[k][l16], s_sum[k][l16]);
+  const float factor = factor_of(a.most, sum);
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int m = 0; m < D / 16; m++)
+      s_acc[((wave * 4 + i) * (D / 16) + m) * 64 + lane] = a.acc[m][i] * factor;     // (NaN stays)
+  __syncthreads();
+  // (where blocks of results are formed, waves 4 to 7 do what 0 to 3 do: all meet at the barriers)
+  if (wave >= 4 && (OUT::kSize != 0 || p.splits > 1)) return;
+  float x[D / 16];
+  const int i = wave & 3;
+#pragma unroll
+  for (int m = 0; m < D / 16; m++) x[m] = 0;
+#pragma unroll
+  for (int k = 0; k < WAVES; k++)
+#pragma unroll
+    for (int m = 0; m < D / 16; m++) x[m] += s_acc[((k * 4 + i) * (D / 16) + m) * 64 + lane];
+  if (p.splits > 1) {
+    float *part = p.part + (size_t)id * at_part_floats<D>();
+#pragma unroll
+    for (int m = 0; m < D / 16; m++) part[(i * (D / 16) + m) * 64 + lane] = x[m];
+    if (wave == 0 && lane < 16) part[16 * D + l16] = most, part[16 * D + 16 + l16] = whole;
+    return;
+  }
+#pragma unroll
+  for (int m = 0; m < D / 16; m++) x[m] = whole == 0 ? 0.0f : x[m] / whole;
+  at_store<E, OUT, D>(p, r, h, i, x, s_most);
+}
+
+// Shares of a slot's tokens: as many as give each CU two workgroups, of a round of the eight waves at least.
+static int at_splits(long long units, long long tokens) {
+  const long long fill = (512 + units - 1) / units, most = (tokens + 255) / 256;
+  return (int)std::max(1ll, std::min({fill, most, 256ll}));
+}
+static long long at_slots(size_t rows, size_t group, size_t sequences, int per_slot) {
+  return (long long)(rows * group / per_slot + sequences);
+}
+
+template <class E, class OUT, int D> static int at_launch(const Attention &p, hipStream_t st) {
+  const unsigned blocks = (unsigned)((long long)p.slots * p.splits * p.kv_heads);
+  constexpr size_t kLds = (size_t)kAtWaves<D> * 16 * D * 4;
+  static std::atomic<uint64_t> attr_set{0};
+  auto kernel = mx4_attention_rows_kernel<E, OUT, D>;
+  if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;
+  kernel<<<(blocks + 7) / 8 * 8, kAtWaves<D> * 64, kLds, st>>>(p, blocks);
+  if (int rc = check_launch("mx4_attention")) return rc;
+  if (p.splits == 1) return MI355X_OK;
+  mx4_attention_join_kernel<E, OUT, D><<<(unsigned)((long long)p.slots * p.kv_heads), 256, 0, st>>>(p);
+  return check_launch("mx4_attention");
+}
+template <class E, class OUT> static int at_launch_dim(const Attention &p, int dim, hipStream_t st) {
+  return dim == 64 ? at_launch<E, OUT, 64>(p, st) : dim == 128 ? at_launch<E, OUT, 128>(p, st) : at_launch<E, OUT, 256>(p, st);
+}
+static size_t at_part_bytes(size_t dim) { return (16 * dim + 32) * sizeof(float); }
+
+// What of a call does not depend on where its tensors lie.
+static int at_plan(const mi355x_mx4_cache *cache, size_t heads, size_t sequences, size_t rows, size_t max_length,
+                   size_t window, size_t sinks, Attention *p, size_t *bytes) {
+  MI355X_REQUIRE(heads > 0 && heads <= 0x7fffffff / cache->head_dim && heads % cache->kv_heads == 0,
+                 "mx4_attention: %zu heads over the cache's %u", heads, cache->kv_heads);
+  p->kv_heads = (int)cache->kv_heads;
+  p->group = (int)(heads / cache->kv_heads);
+  p->most = cache->n_pages ? (int)std::min<size_t>(max_length, (size_t)p->c.capacity) : 0;
+  p->window = window == 0 || window > 0x7fffffff ? 0x7fffffff : (int)window;
+  p->sinks = window == 0 || sinks == 0 ? 0 : (int)std::min<size_t>(sinks, 0x7fffffff);
+  *bytes = 0;
+  p->slots = 0, p->splits = 1;
+  if (!rows || !sequences) return MI355X_OK;
+  if (rows > (size_t)0x7fff0000 / p->group)
+    return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_attention: %zu rows of %d heads to one of the cache", rows, p->group);
+  const long long slots = at_slots(rows, p->group, sequences, 16), units = slots * p->kv_heads;
+  if (units > 1 << 22)
+    return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_attention: %zu rows of %zu heads, %zu sequences", rows, heads, sequences);
+  const long long tokens = std::min<long long>(p->most, (long long)p->window + p->sinks + 48);
+  p->slots = (int)slots;
+  p->splits = at_splits(units, tokens);
+  if (p->splits > 1) *bytes = (size_t)units * p->splits * at_part_bytes(cache->head_dim);
+  return MI355X_OK;
+}
+
+} // namespace mi355x
+
+using namespace mi355x;
+
+extern "C" {
+
+int mi355x_mx4_attention_workspace_bytes(const mi355x_mx4_cache *cache, size_t heads, size_t sequences, size_t rows,
+                                         size_t max_length, size_t *bytes) {
+  MI355X_REQUIRE(bytes, "mx4_attention_workspace_bytes: NULL");
+  Attention p{};
+  if (int rc = check_cache("mx4_attention", cache, &p.c)) return rc;
+  MI355X_REQUIRE(sequences <= 0x3fffffff && rows <= 0x3fffffff,
+                 "mx4_attention: %zu sequences, %zu rows: up to 2^30 - 1 are supported", sequences, rows);
+  // (a window takes no more shares)
+  return at_plan(cache, heads, sequences, rows, max_length, 0, 0, &p, bytes);
+}
+
+int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const void *q, int type, size_t q_row_bytes,
+                         size_t heads, const mi355x_mx4_cache *cache, const int32_t *starts, const int32_t *lengths,
+                         size_t sequences, size_t rows, size_t max_length, float scale, size_t window, size_t sinks,
+                         void *workspace, size_t workspace_bytes, void *stream) {
+  Attention p{};
+  if (int rc = check_cache("mx4_attention", cache, &p.c)) return rc;
+  if (int rc = check_batch("mx4_attention", starts, lengths, sequences, rows, &p.c)) return rc;
+  MI355X_REQUIRE(float_type(type), "mx4_attention: query type %d is none of the float types", type);
+  MI355X_REQUIRE(out_type == type || out_type == MI355X_MX4,
+                 "mx4_attention: result type %d: the queries' (%d) or microscaled rows are supported", out_type, type);
+  MI355X_REQUIRE(scale - scale == 0, "mx4_attention: scale %g", (double)scale);
+  size_t need;
+  if (int rc = at_plan(cache, heads, sequences, rows, max_length, window, sinks, &p, &need)) return rc;
+  const size_t cols = heads * cache->head_dim;
+  if (int rc = check_rows("mx4_attention: queries", q, type, q_row_bytes, rows, cols)) return rc;
+  if (int rc = check_rows("mx4_attention: result", out, out_type, out_row_bytes, rows, cols)) return rc;
+  if (!rows || !sequences) return MI355X_OK;
+  const size_t out_span = rows_span(out_type, out_row_bytes, rows, cols), q_span = rows_span(type, q_row_bytes, rows, cols);
+  MI355X_REQUIRE((out == q && out_type == type && out_row_bytes == q_row_bytes) || !overlaps(out, out_span, q, q_span),
+                 "mx4_attention: the result overlaps the queries without being their place");
+  const size_t span = cache_span(cache), table = cache->pages ? sequences * cache->pages_per_sequence * 4 : 0;
+  auto meets = [&](const void *a, size_t bytes) {
+    return overlaps(a, bytes, cache->keys, span) || overlaps(a, bytes, cache->values, span) ||
+           overlaps(a, bytes, cache->pages, table) || overlaps(a, bytes, starts, 4 * (sequences + 1)) ||
+           overlaps(a, bytes, lengths, 4 * sequences);
+  };
+  MI355X_REQUIRE(!meets(out, out_span), "mx4_attention: the result overlaps the cache or the batch's starts or lengths");
+  if (need) {
+    MI355X_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0,
+                   "mx4_attention: a workspace of %zu bytes on a multiple of 16 is needed "
+                   "(mi355x_mx4_attention_workspace_bytes)", need);
+    MI355X_REQUIRE(!meets(workspace, need) && !overlaps(workspace, need, out, out_span) &&
+                       !overlaps(workspace, need, q, q_span),
+                   "mx4_attention: the workspace overlaps a tensor");
+  }
+  p.q = static_cast<const uint8_t *>(q);
+  p.out = static_cast<uint8_t *>(out);
+  p.part = static_cast<float *>(workspace);
+  p.q_row_bytes = q_row_bytes;
+  p.out_row_bytes = out_row_bytes;
+  p.out_groups = (int)mx4_groups(cols);
+  p.scale = __builtin_fabsf(scale) * 1.4426950408889634f;
+  p.negative = scale < 0;
+  const int dim = (int)cache->head_dim;
+  hipStream_t st = as_stream(stream);
+  const bool mx4 = out_type == MI355X_MX4;
+  if (type == MI355X_F32) return mx4 ? at_launch_dim<F32, MX4>(p, dim, st) : at_launch_dim<F32, F32>(p, dim, st);
+  if (type == MI355X_F16) return mx4 ? at_launch_dim<F16, MX4>(p, dim, st) : at_launch_dim<F16, F16>(p, dim, st);
+  return mx4 ? at_launch_dim<BF16, MX4>(p, dim, st) : at_launch_dim<BF16, BF16>(p, dim, st);
+}
+
+} // extern "C"

@@ -971,6 +971,71 @@ int mi355x_group_norm(void *out, int out_type, size_t out_row_bytes, const void 
                       size_t pixels, size_t C, size_t groups, float epsilon, int activation,
                       void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- a transformer's layer over microscaled rows: cache, attention, adapters ------ */
+/* No counterpart in the reference. What stands between the products (mi355x_mx4_fc) of a
+ * transformer that answers requests; its norm is mi355x_group_norm over one pixel in one
+ * group. Inference only, like the products.
+ *
+ * A cache holds the keys and values of `sequences` sequences as MI355X_MX4 rows of kv_heads *
+ * head_dim columns, head after head: 17/32 byte a value. Token t of sequence s lies in row
+ *   pages[s * pages_per_sequence + t / page_tokens] * page_tokens + t % page_tokens
+ * of both; without a table (pages NULL) page k of sequence s is s * pages_per_sequence + k. A
+ * page number outside [0, n_pages) stands for no page: what lies there is neither read nor
+ * written. Rows are on multiples of 16 bytes, row_bytes (up to 2^26) apart. */
+typedef struct {
+  uint8_t *keys, *values;       /* DEVICE, n_pages * page_tokens rows each */
+  uint64_t row_bytes;
+  const int32_t *pages;         /* DEVICE [sequences x pages_per_sequence], or NULL */
+  uint32_t n_pages;
+  uint32_t page_tokens;         /* a multiple of 16 */
+  uint32_t pages_per_sequence;  /* up to 2^31 - 1 tokens of a sequence */
+  uint32_t kv_heads, head_dim;  /* head_dim 64, 128 or 256 */
+} mi355x_mx4_cache;
+
+/* The tokens of a batch: its rows are the newest tokens of each sequence, one sequence's behind
+ * the other's, rows starts[s] to starts[s + 1] - 1 those of sequence s; lengths[s] is its tokens
+ * with the new ones, so that row i of n is token lengths[s] - n + i. Both are DEVICE arrays, starts
+ * of sequences + 1 entries that do not decrease; entries outside [0, rows] and lengths outside
+ * [0, what the pages hold] count as the nearest of these. Rows of no sequence are
+ * neither read nor written. Nothing of this is read by the host: a captured launch may be
+ * replayed with other contents. */
+
+/* Writes the batch's keys and values [rows x kv_heads * head_dim], of any type, into the cache:
+ * quantised by the rule of mi355x_mx4_quantize, or as they are where they are MI355X_MX4 (results
+ * of mi355x_mx4_fc). Tokens without a place (before the first, behind the last, on no page) are left
+ * out. Two tokens on one place leave either. */
+int mi355x_mx4_cache_write(const mi355x_mx4_cache *cache, const void *keys, const void *values,
+                           int type, size_t keys_row_bytes, size_t values_row_bytes,
+                           const int32_t *starts, const int32_t *lengths, size_t sequences,
+                           size_t rows, void *stream);
+
+/* Attention of the batch's rows over the cache, which holds their own keys and values too:
+ *   out[r][h] = sum over t of p[t] values[t][h / (heads / kv_heads)] / sum over t of p[t],
+ *   p[t] = exp(scale * q[r][h] . keys[t][h / (heads / kv_heads)])
+ * over the tokens t of r's sequence that r sees: none behind its own; where window is not 0, of
+ * those only the last `window` (its own among them) and the first `sinks`. A row that sees none
+ * is 0. What a row does not see has no part in it, whatever is there.
+ *   q    [rows x heads * head_dim], a float type; heads is a multiple of kv_heads
+ *   out  the same, of q's type or MI355X_MX4, quantised from the 32-bit results; may be q's place
+ * max_length: sequences are no longer than this (a longer one counts as this long). Keys and values
+ * are what their rows stand for; with fp16 queries a block of values whose scale is above 2^13
+ * (values of 65536 on) counts as NaN. A query is taken with what is above 2^-12 (bf16), 2^-16 (fp16) or
+ * 2^-24 (fp32) of its block of 32's largest. Sums are of 32 bits; weights are rounded to the type of q before they
+ * meet values (fp32: to 24 bits). An infinity or a NaN in a query makes
+ * NaN of its head's result, one that a row sees in a key or a value of the row's heads or columns.
+ * Equal calls give equal bits. Scores past the range of 32 bits: NaN.
+ * workspace: device memory of mi355x_mx4_attention_workspace_bytes, on a multiple of 16 and
+ * overlapping no tensor; NULL where that is 0. A call leaves nothing in it for the next, and calls
+ * that may run at the same time need one each. */
+int mi355x_mx4_attention_workspace_bytes(const mi355x_mx4_cache *cache, size_t heads,
+                                         size_t sequences, size_t rows, size_t max_length,
+                                         size_t *bytes);
+int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const void *q, int type,
+                         size_t q_row_bytes, size_t heads, const mi355x_mx4_cache *cache,
+                         const int32_t *starts, const int32_t *lengths, size_t sequences,
+                         size_t rows, size_t max_length, float scale, size_t window, size_t sinks,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- fused-rowwise SparseLengths(Weighted)Sum ----------------------------------- */
 
 /* libjit_fused_rowwise_quantized_sparse_lengths_weighted_sum_f_u / _f_i32
