@@ -240,6 +240,7 @@ PyMethodDef g_methods[] = {
     ENTRY(group_norm),
     ENTRY(mx4_cache_write),
     ENTRY(mx4_attention),
+    ENTRY(mx4_fc_adapters),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods,

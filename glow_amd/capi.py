@@ -58,6 +58,7 @@ EXPORTS = [
     "mi355x_mx4_row_bytes", "mi355x_mx4_quantize_host", "mi355x_mx4_quantize", "mi355x_mx4_dequantize",
     "mi355x_mx4_fc_workspace_bytes", "mi355x_mx4_fc", "mi355x_group_norm_workspace_bytes", "mi355x_group_norm",
     "mi355x_mx4_cache_write", "mi355x_mx4_attention_workspace_bytes", "mi355x_mx4_attention",
+    "mi355x_mx4_fc_adapters_workspace_bytes", "mi355x_mx4_fc_adapters",
 ]
 
 
@@ -91,6 +92,12 @@ class Mx4Cache(C.Structure):
     _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("row_bytes", C.c_uint64), ("pages", C.c_void_p),
                 ("n_pages", C.c_uint32), ("page_tokens", C.c_uint32), ("pages_per_sequence", C.c_uint32),
                 ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class Mx4Adapters(C.Structure):
+    """mi355x_mx4_adapters; the addresses are of device memory."""
+    _fields_ = [("down", C.c_void_p), ("up", C.c_void_p), ("scales", C.c_void_p), ("count", C.c_uint32),
+                ("rank", C.c_uint32), ("type", C.c_int32)]
 
 
 def conv3d_geom(N, IT, IH, IW, IC, OC, kernel, stride, pads, group=1):
@@ -1729,3 +1736,43 @@ def mx4_attention(q, heads, keys, values, starts, lengths, kv_heads, head_dim, p
     got = do.numpy()
     del held
     return got
+
+
+# ---- low-rank adapters beside a product ------------------------------------------
+
+def mx4_fc_adapters_workspace_bytes(M, K, N, in_type, rank):
+    n = C.c_size_t(0)
+    check(lib().mi355x_mx4_fc_adapters_workspace_bytes(_sz(M), _sz(K), _sz(N), C.c_int(in_type), _sz(rank), C.byref(n)))
+    return n.value
+
+
+def launch_mx4_fc_adapters(out, out_type, out_row_bytes, in_, in_type, in_row_bytes, weights, weights_row_bytes, bias,
+                           adapters, row_adapters, M, K, N, activation=ACT_NONE, workspace=None, workspace_bytes=0,
+                           stream=None):
+    (_native or native()).mx4_fc_adapters(out, out_type, out_row_bytes, in_, in_type, in_row_bytes, weights,
+                                          weights_row_bytes, bias, adapters, row_adapters, M, K, N, activation, workspace,
+                                          workspace_bytes, stream)
+
+
+def mx4_fc_adapters(x, in_type, weights, bias, K, down, up, row_adapters, scales=None, type_=TYPE_F32, out_type=TYPE_F32,
+                    activation=ACT_NONE):
+    """mx4_fc with adapters down [count, rank, K] and up [count, N, rank] of type_; row_adapters: int32 [M]."""
+    x = _mx4_rows(x) if in_type == TYPE_MX4 else _float_rows(x, in_type)
+    weights, down, up = _mx4_rows(weights), _float_rows(down, type_), _float_rows(up, type_)
+    M, N = x.shape[0], weights.shape[0]
+    bias = _columns("mx4_fc_adapters: bias", bias, N)
+    row_adapters = np.ascontiguousarray(row_adapters, np.int32)
+    count, rank = down.shape[0], down.shape[1]
+    if down.shape != (count, rank, K) or up.shape != (count, N, rank) or row_adapters.shape != (M,):
+        raise MI355XError(-1, f"down of shape {down.shape}, up of {up.shape}, {row_adapters.shape} rows: {M} x {K} x {N}")
+    scales = _columns("mx4_fc_adapters: scales", scales, count)
+    shape = (M, mx4_row_bytes(N) if out_type == TYPE_MX4 else N)
+    out = DeviceBuffer.empty(shape, np.uint8 if out_type == TYPE_MX4 else _FLOAT_DTYPES[out_type])
+    dx, dw, dd, du, dr = to_device(x), to_device(weights), to_device(down), to_device(up), to_device(row_adapters)
+    db, ds = (to_device(v) if v is not None else None for v in (bias, scales))
+    n = mx4_fc_adapters_workspace_bytes(M, K, N, in_type, rank)
+    ws = DeviceBuffer(n) if n else None
+    adapters = Mx4Adapters(dd.ptr, du.ptr, ds.ptr if ds else None, count, rank, type_)
+    launch_mx4_fc_adapters(out, out_type, shape[1] * out.dtype.itemsize, dx, in_type, x.shape[1] * x.dtype.itemsize, dw,
+                           weights.shape[1], db, adapters, dr, M, K, N, activation, ws, n)
+    return out.numpy()

@@ -18,9 +18,9 @@ constexpr int mx4_short_bias(int groups) {
   return groups * T::kStep + T::kScales > T::kStaging ? groups * T::kStep + T::kScales : T::kStaging;
 }
 
-template <class IN, class OUT, int BN, int BM, int WN, int WM, int BLOCKS>
+template <class IN, class OUT, int BN, int BM, int WN, int WM, int BLOCKS, class P>
 __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM / WM) / 4) void mx4_fc_short_kernel(
-    MxFc p, int K, int tiles_n, int tiles_m) {
+    P p, int K, int tiles_n, int tiles_m) {
   typedef MxTile<OUT, BN, BM, WN, WM> T;
   constexpr int WAVES = T::kWaves, TN = T::TN, TM = T::TM, THREADS = T::kThreads, kStep = T::kStep;
   constexpr int A_LOADS = BN / 16 / WAVES, B_LOADS = IN::kSize ? 0 : BM / 16 / WAVES;
@@ -116,14 +116,18 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
                                                                      acc[i][j], 4, 4, 0, scale[i], 0, scale[TN + j]);
   }
   __syncthreads();
+  if constexpr (P::kAdapters)
+    p.ad.template add<TN, TM>([&](int i, int j) -> mx_v4f & { return acc[i][j]; },
+                              [&](int i) { return n0 + mx4_weight_column<T::S>(wn * WN + i * 16 + l16); },
+                              m0 + wm * WM, p.M, p.N);
   mx4_tile_results<OUT, BN, BM, WN, WM>(acc, p, lds,
                                         reinterpret_cast<float *>(lds + mx4_short_bias<OUT, BN, BM, WN, WM>(KT)), bias,
                                         m0, n0);
 }
 
-template <class IN, class OUT, int BN, int BM, int WN, int WM, int BLOCKS>
-static int mx4_fc_short_launch(const MxFc &p, int K, hipStream_t st) {
-  auto kern = mx4_fc_short_kernel<IN, OUT, BN, BM, WN, WM, BLOCKS>;
+template <class IN, class OUT, int BN, int BM, int WN, int WM, int BLOCKS, class P>
+static int mx4_fc_short_launch(const P &p, int K, hipStream_t st) {
+  auto kern = mx4_fc_short_kernel<IN, OUT, BN, BM, WN, WM, BLOCKS, P>;
   const auto lds = [](int groups) { return (size_t)mx4_short_bias<OUT, BN, BM, WN, WM>(groups) + BN * 4; };
   const long long columns = OUT::kSize ? p.N : (long long)p.out_groups * kMxGroup;
   const long long tiles_n = (columns + BN - 1) / BN, tiles_m = ((long long)p.M + BM - 1) / BM;

@@ -62,8 +62,8 @@ constexpr int kSharedRows = 4;
 // two do not lie on the same banks.
 __host__ __device__ constexpr int mx4_shared_row(int groups) { return (groups * (kMxGroupBytes + 4) + 15) / 16 * 16 + 16; }
 
-template <class IN, class OUT, int MT, int NT, bool SHARED>
-__global__ __launch_bounds__(kSmallWaves * 64, 2) void mx4_fc_small_kernel(MxFc p, int K, int tiles_n) {
+template <class IN, class OUT, int MT, int NT, bool SHARED, class P>
+__global__ __launch_bounds__(kSmallWaves * 64, 2) void mx4_fc_small_kernel(P p, int K, int tiles_n) {
   // groups in flight: as many as their registers allow
   static_assert(!SHARED || (MT == 1 && IN::kSize), "shared rows");
   constexpr int kRegs = IN::kSize == 0 || SHARED ? 5 : IN::kSize * 8;
@@ -156,6 +156,9 @@ __global__ __launch_bounds__(kSmallWaves * 64, 2) void mx4_fc_small_kernel(MxFc 
         }
     }
   }
+  if constexpr (P::kAdapters)      // (the rows' adapters are shared out among the waves)
+    p.ad.template add<NT, MT>([&](int c, int a) -> mx_v4f & { return acc[a][c]; }, [&](int c) { return n0 + c * 16 + row; },
+                              m0, p.M, p.N, wave, kSmallWaves);
   // register i of a lane: column 4 * (lane / 16) + i, row lane % 16
 #pragma unroll
   for (int a = 0; a < MT; a++)
@@ -224,8 +227,8 @@ __global__ __launch_bounds__(kSmallWaves * 64, 2) void mx4_fc_small_kernel(MxFc 
   }
 }
 
-template <class IN, class OUT, int MT, int NT>
-static int mx4_fc_small_launch(const MxFc &p, int K, hipStream_t st) {
+template <class IN, class OUT, int MT, int NT, class P>
+static int mx4_fc_small_launch(const P &p, int K, hipStream_t st) {
   const long long columns = OUT::kSize ? p.N : (long long)p.out_groups * kMxGroup;
   const long long tiles_n = (columns + 16 * NT - 1) / (16 * NT);
   const long long blocks = tiles_n * (((long long)p.M + 16 * MT - 1) / (16 * MT));
@@ -234,11 +237,11 @@ static int mx4_fc_small_launch(const MxFc &p, int K, hipStream_t st) {
     if (p.M <= kSharedRows) {
       // (at most 96 KB of values are quantised here: a quarter of that and the pads)
       const size_t lds = (size_t)p.M * mx4_shared_row(p.groups);
-      mx4_fc_small_kernel<IN, OUT, MT, NT, true><<<(unsigned)blocks, kSmallWaves * 64, lds, st>>>(p, K, (int)tiles_n);
+      mx4_fc_small_kernel<IN, OUT, MT, NT, true, P><<<(unsigned)blocks, kSmallWaves * 64, lds, st>>>(p, K, (int)tiles_n);
       return check_launch("mx4_fc");
     }
   }
-  mx4_fc_small_kernel<IN, OUT, MT, NT, false><<<(unsigned)blocks, kSmallWaves * 64, 0, st>>>(p, K, (int)tiles_n);
+  mx4_fc_small_kernel<IN, OUT, MT, NT, false, P><<<(unsigned)blocks, kSmallWaves * 64, 0, st>>>(p, K, (int)tiles_n);
   return check_launch("mx4_fc");
 }
 

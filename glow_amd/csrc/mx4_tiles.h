@@ -29,6 +29,7 @@ typedef float mx_v4f __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ mx_v8i fp4_operand(v4i v) { return mx_v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
 
 struct MxFc {
+  static constexpr bool kAdapters = false;     // (mx4_adapters.h has the ones that have)
   uint8_t *out;
   size_t out_row_bytes;
   const uint8_t *in, *weights;
@@ -168,9 +169,9 @@ struct MxRing : MxTile<OUT, BN, BM, WN, WM> {
   static constexpr size_t kLds = (size_t)kBias + BN * 4;
 };
 
-template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS>
+template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS, class P>
 __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM / WM) / 4) void mx4_fc_tile_kernel(
-    MxFc p, int tiles_n, int tiles_m) {
+    P p, int tiles_n, int tiles_m) {
   typedef MxRing<OUT, BN, BM, WN, WM, STAGES> T;
   constexpr int WAVES = T::kWaves, TN = T::TN, TM = T::TM;
   constexpr int A_LOADS = BN / 16 / WAVES, B_LOADS = BM / 16 / WAVES;  // 16 rows an instruction
@@ -330,13 +331,17 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
   }
   dma_wait<0>();                                   // the re-reads, before LDS is used again
   __syncthreads();
+  if constexpr (P::kAdapters)
+    p.ad.template add<TN, TM>([&](int i, int j) -> mx_v4f & { return acc[i][j]; },
+                              [&](int i) { return n0 + mx4_weight_column<T::S>(wn * WN + i * 16 + l16); },
+                              m0 + wm * WM, p.M, p.N);
   mx4_tile_results<OUT, BN, BM, WN, WM>(acc, p, lds, reinterpret_cast<float *>(lds + T::kBias), bias, m0, n0);
 }
 
-template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS>
-static int mx4_fc_tile_launch(const MxFc &p, hipStream_t st) {
+template <class OUT, int BN, int BM, int WN, int WM, int STAGES, int BLOCKS, class P>
+static int mx4_fc_tile_launch(const P &p, hipStream_t st) {
   typedef MxRing<OUT, BN, BM, WN, WM, STAGES> T;
-  auto kern = mx4_fc_tile_kernel<OUT, BN, BM, WN, WM, STAGES, BLOCKS>;
+  auto kern = mx4_fc_tile_kernel<OUT, BN, BM, WN, WM, STAGES, BLOCKS, P>;
   // a microscaled result has whole groups of columns, the ones past N zeros
   const long long columns = OUT::kSize ? p.N : (long long)p.out_groups * kMxGroup;
   const long long tiles_n = (columns + BN - 1) / BN, tiles_m = ((long long)p.M + BM - 1) / BM;

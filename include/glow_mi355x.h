@@ -1036,6 +1036,34 @@ int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const vo
                          size_t rows, size_t max_length, float scale, size_t window, size_t sinks,
                          void *workspace, size_t workspace_bytes, void *stream);
 
+/* mi355x_mx4_fc with low-rank adapters of its rows' own beside the weights that all share:
+ *   out[m] = activation(bias + weights in[m] + scales[a] * up[a] (down[a] in[m])),  a = row_adapters[m]
+ * where the shared product takes in[m] quantised, as mi355x_mx4_fc does, and down[a] as it is
+ * (MI355X_MX4: what the rows stand for). A row whose number is outside [0, count) has the shared
+ * product alone. What is in an adapter has no part in rows of others.
+ *   down   [count x rank x K] of `type`, a float type; up [count x N x rank]; dense. An adapter of
+ *          a lower rank has zeros in its other rows of down or columns of up.
+ *   scales float [count], or NULL: 1
+ *   rank   up to 1024
+ *   row_adapters  DEVICE int32 [M]; rows of the same adapter are fastest next to each other
+ * All sums are of 32 bits, in no particular order (equal calls give equal bits), and down[a] in[m] goes
+ * on in 24; an infinity in an adapter may come out as NaN. With K, rank or count of 0 this is mi355x_mx4_fc.
+ * workspace as there, of mi355x_mx4_fc_adapters_workspace_bytes (as much as mi355x_mx4_fc asks for). */
+typedef struct {
+  const void *down, *up;        /* DEVICE */
+  const float *scales;          /* DEVICE */
+  uint32_t count, rank;
+  int32_t type;
+} mi355x_mx4_adapters;
+int mi355x_mx4_fc_adapters_workspace_bytes(size_t M, size_t K, size_t N, int in_type, size_t rank,
+                                           size_t *bytes);
+int mi355x_mx4_fc_adapters(void *out, int out_type, size_t out_row_bytes, const void *in,
+                           int in_type, size_t in_row_bytes, const uint8_t *weights,
+                           size_t weights_row_bytes, const float *bias,
+                           const mi355x_mx4_adapters *adapters, const int32_t *row_adapters,
+                           size_t M, size_t K, size_t N, int activation, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
 /* ---- fused-rowwise SparseLengths(Weighted)Sum ----------------------------------- */
 
 /* libjit_fused_rowwise_quantized_sparse_lengths_weighted_sum_f_u / _f_i32
