@@ -238,6 +238,28 @@ __device__ __forceinline__ void at_transpose(at_v4i (&out)[COLS], const uint32_t
   }
 }
 
+// The same of four tokens, half of an operand.
+template <class E, int COLS, class HALF>
+__device__ __forceinline__ void at_transpose4(HALF (&out)[COLS], const uint32_t (&codes)[4], const float (&scale)[4]) {
+  typedef AtValues<E> V;
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    auto columns = [&](auto pair) {
+      constexpr int P = decltype(pair)::value;
+      const uint32_t a = __builtin_bit_cast(uint32_t, V::two(codes[2 * j], scale[2 * j], pair));
+      const uint32_t b = __builtin_bit_cast(uint32_t, V::two(codes[2 * j + 1], scale[2 * j + 1], pair));
+      out[2 * P][j] = (int)__builtin_amdgcn_perm(b, a, 0x05040100);
+      out[2 * P + 1][j] = (int)__builtin_amdgcn_perm(b, a, 0x07060302);
+    };
+    columns(std::integral_constant<int, 0>());
+    columns(std::integral_constant<int, 1>());
+    if constexpr (COLS == 8) {
+      columns(std::integral_constant<int, 2>());
+      columns(std::integral_constant<int, 3>());
+    }
+  }
+}
+
 // 2^x, 0 of minus infinity.
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -247,6 +269,48 @@ __device__ __forceinline__ float at_max(float x) {
   x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
   s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+// A row at `position` sees the token.
+__device__ __forceinline__ bool at_sees(const Attention &p, int position, int token) {
+  return token <= position && (token > position - p.window || token < p.sinks);
+}
+// Whether rows at `low` to `high` see all of a tile's tokens, and whether they see none.
+__device__ __forceinline__ bool at_sees_all(const Attention &p, int low, int high, int first) {
+  return first >= 0 && first + kCacheTile - 1 <= low && first > high - p.window;
+}
+__device__ __forceinline__ bool at_sees_none(const Attention &p, int low, int high, int first) {
+  return first < 0 || first > high || (first + kCacheTile - 1 <= low - p.window && first >= p.sinks);
+}
+
+// Scores of a lane's query (tokens that it does not see: minus infinity, and not in `seen`, which counts unless `whole`)
+// become weights; the results so far are rescaled where the largest score moves.
+template <class E, int N, int M>
+__device__ __forceinline__ void at_weigh(float (&score)[N], float &most, float &sum, at_v4f (&acc)[M], float scale, bool whole,
+                                         unsigned seen) {
+  float top = score[0];
+#pragma unroll
+  for (int j = 1; j < N; j++) top = fmaxf(top, score[j]);
+  top = at_max(top) * scale;
+  const bool up = top > most + kAtSlack;
+  if (__ballot(up)) {
+    const float factor = up ? at_exp2(most - top) : 1.0f;
+    most = up ? top : most;
+    sum *= factor;
+#pragma unroll
+    for (int m = 0; m < M; m++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[m][i] *= factor;
+  }
+  const float off = AtKind<E>::kUp - most;
+#pragma unroll
+  for (int j = 0; j < N; j++) score[j] = at_exp2(fmaf(score[j], scale, off));
+  if (!whole) {
+#pragma unroll
+    for (int j = 0; j < N; j++) score[j] = seen >> j & 1 ? score[j] : 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < N; j++) sum += score[j];
 }
 
 // ---- results -------------------------------------------------------------------------
@@ -312,6 +376,78 @@ __device__ __forceinline__ void at_store(const Attention &p, const AtRows &r, in
     }
   }
 }
+
+// What a share of a slot of sixteen rows leaves: its results, component by component, then the largest score and the sum
+// of each query.
+template <int D> __device__ __forceinline__ constexpr size_t at_part_floats() { return 16 * D + 32; }
+
+// The whole of a slot's results by one wave: a lane has the components of its query side by side.
+template <class OUT, int D>
+__device__ __forceinline__ void at_store_whole(const Attention &p, const AtRows &r, int h, const at_v4f (&acc)[D / 16],
+                                               float sum) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+  const int at = r.first + l16, token = at / p.group, head = h * p.group + (at - token * p.group);
+  const bool there = at < r.last;
+  uint8_t *row = p.out + (size_t)(r.begin + token) * p.out_row_bytes;
+  constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
+  const float by = sum == 0 ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int c = 0; c < kChunks; c++) {
+    float x[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int m = 0; m < 8; m++) x[i][m] = m < COLS ? acc[c * 8 + (m < COLS ? m : 0)][i] * by : 0.0f;
+    const size_t column = (size_t)head * D + c * 128 + 4 * COLS * q;
+    if constexpr (OUT::kSize != 0) {
+      typename OUT::T *o = reinterpret_cast<typename OUT::T *>(row) + column;
+      if (there) {
+        if constexpr (COLS == 8) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) store8<OUT>(o + 8 * i, x[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float y[8] = {x[i][0], x[i][1], x[i][2], x[i][3], x[i + 1][0], x[i + 1][1], x[i + 1][2], x[i + 1][3]};
+            store8<OUT>(o + 4 * i, y);
+          }
+        }
+      }
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < COLS; j++) m = max(m, magnitude_bits(x[i][j]));
+      if (COLS == 4) m = max_across16(m);           // (a block is two lanes')
+      const uint32_t byte = mx4_scale_byte(m);
+      uint32_t codes[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) codes[i] = mx4_codes8(x[i], byte);
+      if (there) {
+        uint8_t *scales = row + (size_t)p.out_groups * kMxGroupBytes;
+        if constexpr (COLS == 8) *reinterpret_cast<uint4 *>(row + column / 2) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+        else *reinterpret_cast<uint2 *>(row + column / 2) = make_uint2((codes[0] & 0xffff) | codes[1] << 16, (codes[2] & 0xffff) | codes[3] << 16);
+        if (column % 32 == 0) scales[column / 32] = (uint8_t)byte;
+        // the last head fills its group and the row up with zeros
+        const int heads = p.kv_heads * p.group;
+        if (c == kChunks - 1 && head == heads - 1) {
+          if (D == 64 && (heads & 1)) {
+            *reinterpret_cast<uint2 *>(row + (size_t)heads * 32 + 8 * q) = make_uint2(0, 0);
+            if (q < 2) scales[heads * 2 + q] = 0;
+          }
+          if (q < ((-p.out_groups) & 3)) reinterpret_cast<uint32_t *>(scales)[p.out_groups + q] = 0;
+        }
+      }
+    }
+  }
+}
+
+// Launches the kernel for many rows of queries (mx4_attention_prompt.hip).
+int at_prompt_launch(const Attention &p, int type, bool mx4, int dim, hipStream_t st);
+constexpr int kPromptWaves = 4;
+// Sixteens of rows that a wave of that kernel has: as many as its registers hold.
+constexpr int at_prompt_sixteens(int type, int dim) { return type == MI355X_F32 || dim == 256 ? 1 : 2; }
 
 } // namespace mi355x
 

@@ -93,51 +93,22 @@ __device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> 
 #pragma unroll
     for (int i = 0; i < 4; i++) score[k * 4 + i] = r[i];
   }
-  auto sees = [&](int token) {
-    return token <= position && (token > position - p.window || token < p.sinks);
-  };
   // whether every row sees all of these tokens
-  bool whole = true;
-#pragma unroll
-  for (int k = 0; k < 2; k++)
-    whole = whole && s.first[k] >= 0 && s.first[k] + kCacheTile - 1 <= low && s.first[k] > high - p.window;
+  const bool whole = at_sees_all(p, low, high, s.first[0]) && at_sees_all(p, low, high, s.first[1]);
   unsigned seen = 0xff;
   if (!whole) {
     seen = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const int first = s.first[j >> 2];
-      const bool yes = first >= 0 && sees(first + 4 * q + (j & 3));
+      const bool yes = first >= 0 && at_sees(p, position, first + 4 * q + (j & 3));
       seen |= yes ? 1u << j : 0;
       score[j] = yes ? score[j] : kAtNone;
     }
   }
-  float top = score[0];
-#pragma unroll
-  for (int j = 1; j < 8; j++) top = fmaxf(top, score[j]);
-  top = at_max(top) * p.scale;
-  const bool up = top > a.most + kAtSlack;
-  if (__ballot(up)) {
-    const float factor = up ? at_exp2(a.most - top) : 1.0f;
-    a.most = up ? top : a.most;
-    a.sum *= factor;
-#pragma unroll
-    for (int m = 0; m < D / 16; m++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) a.acc[m][i] *= factor;
-  }
-  const float off = AtKind<E>::kUp - a.most;
-  float weight[8];
-#pragma unroll
-  for (int j = 0; j < 8; j++) weight[j] = at_exp2(fmaf(score[j], p.scale, off));
-  if (!whole) {
-#pragma unroll
-    for (int j = 0; j < 8; j++) weight[j] = seen >> j & 1 ? weight[j] : 0.0f;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; j++) a.sum += weight[j];
+  at_weigh<E>(score, a.most, a.sum, a.acc, p.scale, whole, seen);
   at_v4i packed[AtKind<E>::kP];
-  at_pack<E>(packed, weight);
+  at_pack<E>(packed, score);
 
 #pragma unroll
   for (int c = 0; c < kChunks; c++) {
@@ -154,7 +125,7 @@ __device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> 
           const unsigned mine = D == 64 ? (unsigned)(bad >> (16 * team + 8 * (q >> 1))) & 0xff
                                         : (unsigned)(bad >> (16 * team + 4 * q)) & 0xf;
           const int first = s.first[j >> 2];
-          if (mine && first >= 0 && sees(first + 4 * team + (j & 3))) {
+          if (mine && first >= 0 && at_sees(p, position, first + 4 * team + (j & 3))) {
 #pragma unroll
             for (int m = 0; m < COLS; m++)
 #pragma unroll
@@ -180,9 +151,6 @@ __device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> 
       for (int t = 0; t < AtKind<E>::kP; t++) a.acc[c * 8 + m] = AtValues<E>::multiply(columns[m], packed[t], a.acc[c * 8 + m]);
   }
 }
-
-// What a share of a slot leaves: results of component i, then the largest score and the sum of each query.
-template <int D> constexpr size_t at_part_floats() { return 16 * D + 32; }
 
 // The shares of sixteen rows joined, and what is done with the whole: wave i < 4 has component i.
 template <class E, class OUT, int D>
@@ -301,35 +269,42 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, D == 256 ? 1 : 2) void mx4_attent
   at_store<E, OUT, D>(p, r, h, i, x, s_most);
 }
 
-// Shares of a slot's tokens: as many as give each CU two workgroups, of a round of the eight waves at least.
-static int at_splits(long long units, long long tokens) {
-  const long long fill = (512 + units - 1) / units, most = (tokens + 255) / 256;
+// Shares of a slot's tokens: as many as give each CU two workgroups, of `least` tokens at least.
+static int at_splits(long long units, long long tokens, long long least) {
+  const long long fill = (512 + units - 1) / units, most = (tokens + least - 1) / least;
   return (int)std::max(1ll, std::min({fill, most, 256ll}));
 }
 static long long at_slots(size_t rows, size_t group, size_t sequences, int per_slot) {
   return (long long)(rows * group / per_slot + sequences);
 }
 
-template <class E, class OUT, int D> static int at_launch(const Attention &p, hipStream_t st) {
-  const unsigned blocks = (unsigned)((long long)p.slots * p.splits * p.kv_heads);
-  constexpr size_t kLds = (size_t)kAtWaves<D> * 16 * D * 4;
-  static std::atomic<uint64_t> attr_set{0};
-  auto kernel = mx4_attention_rows_kernel<E, OUT, D>;
-  if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;
-  kernel<<<(blocks + 7) / 8 * 8, kAtWaves<D> * 64, kLds, st>>>(p, blocks);
-  if (int rc = check_launch("mx4_attention")) return rc;
+template <class E, class OUT, int D> static int at_launch(Attention p, int type, bool prompt, int sixteens, hipStream_t st) {
+  if (prompt) {
+    if (int rc = at_prompt_launch(p, type, OUT::kSize == 0, D, st)) return rc;
+  } else {
+    const unsigned blocks = (unsigned)((long long)p.slots * p.splits * p.kv_heads);
+    constexpr size_t kLds = (size_t)kAtWaves<D> * 16 * D * 4;
+    static std::atomic<uint64_t> attr_set{0};
+    auto kernel = mx4_attention_rows_kernel<E, OUT, D>;
+    if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;
+    kernel<<<(blocks + 7) / 8 * 8, kAtWaves<D> * 64, kLds, st>>>(p, blocks);
+    if (int rc = check_launch("mx4_attention")) return rc;
+  }
   if (p.splits == 1) return MI355X_OK;
+  p.slots = sixteens;
   mx4_attention_join_kernel<E, OUT, D><<<(unsigned)((long long)p.slots * p.kv_heads), 256, 0, st>>>(p);
   return check_launch("mx4_attention");
 }
-template <class E, class OUT> static int at_launch_dim(const Attention &p, int dim, hipStream_t st) {
-  return dim == 64 ? at_launch<E, OUT, 64>(p, st) : dim == 128 ? at_launch<E, OUT, 128>(p, st) : at_launch<E, OUT, 256>(p, st);
-}
 static size_t at_part_bytes(size_t dim) { return (16 * dim + 32) * sizeof(float); }
 
-// What of a call does not depend on where its tensors lie.
-static int at_plan(const mi355x_mx4_cache *cache, size_t heads, size_t sequences, size_t rows, size_t max_length,
-                   size_t window, size_t sinks, Attention *p, size_t *bytes) {
+// How a call is cut, which does not depend on where its tensors lie.
+struct AtPlan {
+  bool prompt;
+  int sixteens;                   // slots of sixteen rows
+  size_t bytes;                   // of workspace
+};
+static int at_plan(const mi355x_mx4_cache *cache, size_t heads, int type, size_t sequences, size_t rows, size_t max_length,
+                   size_t window, size_t sinks, Attention *p, AtPlan *plan) {
   MI355X_REQUIRE(heads > 0 && heads <= 0x7fffffff / cache->head_dim && heads % cache->kv_heads == 0,
                  "mx4_attention: %zu heads over the cache's %u", heads, cache->kv_heads);
   p->kv_heads = (int)cache->kv_heads;
@@ -337,18 +312,22 @@ static int at_plan(const mi355x_mx4_cache *cache, size_t heads, size_t sequences
   p->most = cache->n_pages ? (int)std::min<size_t>(max_length, (size_t)p->c.capacity) : 0;
   p->window = window == 0 || window > 0x7fffffff ? 0x7fffffff : (int)window;
   p->sinks = window == 0 || sinks == 0 ? 0 : (int)std::min<size_t>(sinks, 0x7fffffff);
-  *bytes = 0;
-  p->slots = 0, p->splits = 1;
+  *plan = AtPlan{};
+  p->splits = 1;
   if (!rows || !sequences) return MI355X_OK;
   if (rows > (size_t)0x7fff0000 / p->group)
     return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_attention: %zu rows of %d heads to one of the cache", rows, p->group);
-  const long long slots = at_slots(rows, p->group, sequences, 16), units = slots * p->kv_heads;
-  if (units > 1 << 22)
+  const long long sixteens = at_slots(rows, p->group, sequences, 16);
+  if (sixteens * p->kv_heads > 1 << 22)
     return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_attention: %zu rows of %zu heads, %zu sequences", rows, heads, sequences);
-  const long long tokens = std::min<long long>(p->most, (long long)p->window + p->sinks + 48);
-  p->slots = (int)slots;
-  p->splits = at_splits(units, tokens);
-  if (p->splits > 1) *bytes = (size_t)units * p->splits * at_part_bytes(cache->head_dim);
+  // Many rows of a sequence share what is read and converted.
+  plan->prompt = rows * p->group > 64 * sequences;
+  plan->sixteens = (int)sixteens;
+  const int per_slot = plan->prompt ? kPromptWaves * 16 * at_prompt_sixteens(type, (int)cache->head_dim) : 16;
+  p->slots = (int)at_slots(rows, p->group, sequences, per_slot);
+  const long long tokens = std::min<long long>(p->most, (long long)p->window + p->sinks + per_slot + 48);
+  p->splits = at_splits((long long)p->slots * p->kv_heads, tokens, plan->prompt ? 512 : 256);
+  if (p->splits > 1) plan->bytes = (size_t)sixteens * p->kv_heads * p->splits * at_part_bytes(cache->head_dim);
   return MI355X_OK;
 }
 
@@ -365,8 +344,14 @@ int mi355x_mx4_attention_workspace_bytes(const mi355x_mx4_cache *cache, size_t h
   if (int rc = check_cache("mx4_attention", cache, &p.c)) return rc;
   MI355X_REQUIRE(sequences <= 0x3fffffff && rows <= 0x3fffffff,
                  "mx4_attention: %zu sequences, %zu rows: up to 2^30 - 1 are supported", sequences, rows);
-  // (a window takes no more shares)
-  return at_plan(cache, heads, sequences, rows, max_length, 0, 0, &p, bytes);
+  // (whatever the type; a window takes no more shares)
+  *bytes = 0;
+  for (int type : {MI355X_F32, MI355X_BF16}) {
+    AtPlan plan;
+    if (int rc = at_plan(cache, heads, type, sequences, rows, max_length, 0, 0, &p, &plan)) return rc;
+    *bytes = std::max(*bytes, plan.bytes);
+  }
+  return MI355X_OK;
 }
 
 int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const void *q, int type, size_t q_row_bytes,
@@ -380,8 +365,9 @@ int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const vo
   MI355X_REQUIRE(out_type == type || out_type == MI355X_MX4,
                  "mx4_attention: result type %d: the queries' (%d) or microscaled rows are supported", out_type, type);
   MI355X_REQUIRE(scale - scale == 0, "mx4_attention: scale %g", (double)scale);
-  size_t need;
-  if (int rc = at_plan(cache, heads, sequences, rows, max_length, window, sinks, &p, &need)) return rc;
+  AtPlan plan;
+  if (int rc = at_plan(cache, heads, type, sequences, rows, max_length, window, sinks, &p, &plan)) return rc;
+  const size_t need = plan.bytes;
   const size_t cols = heads * cache->head_dim;
   if (int rc = check_rows("mx4_attention: queries", q, type, q_row_bytes, rows, cols)) return rc;
   if (int rc = check_rows("mx4_attention: result", out, out_type, out_row_bytes, rows, cols)) return rc;
@@ -415,9 +401,16 @@ int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const vo
   const int dim = (int)cache->head_dim;
   hipStream_t st = as_stream(stream);
   const bool mx4 = out_type == MI355X_MX4;
-  if (type == MI355X_F32) return mx4 ? at_launch_dim<F32, MX4>(p, dim, st) : at_launch_dim<F32, F32>(p, dim, st);
-  if (type == MI355X_F16) return mx4 ? at_launch_dim<F16, MX4>(p, dim, st) : at_launch_dim<F16, F16>(p, dim, st);
-  return mx4 ? at_launch_dim<BF16, MX4>(p, dim, st) : at_launch_dim<BF16, BF16>(p, dim, st);
+  auto launch = [&](auto e, auto result) {
+    typedef decltype(e) E;
+    typedef decltype(result) OUT;
+    return dim == 64    ? at_launch<E, OUT, 64>(p, type, plan.prompt, plan.sixteens, st)
+           : dim == 128 ? at_launch<E, OUT, 128>(p, type, plan.prompt, plan.sixteens, st)
+                        : at_launch<E, OUT, 256>(p, type, plan.prompt, plan.sixteens, st);
+  };
+  if (type == MI355X_F32) return mx4 ? launch(F32(), MX4()) : launch(F32(), F32());
+  if (type == MI355X_F16) return mx4 ? launch(F16(), MX4()) : launch(F16(), F16());
+  return mx4 ? launch(BF16(), MX4()) : launch(BF16(), BF16());
 }
 
 } // extern "C"

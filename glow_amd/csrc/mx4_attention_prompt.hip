@@ -1,0 +1,307 @@
+// Attention over a cache of microscaled rows: many rows of queries a sequence.
+#include "mx4_attention.h"
+
+#include "gemm_i8.h"
+
+namespace mi355x {
+
+// A workgroup has 128 rows of queries (64 in fp32 or of 256 columns), 32 a wave, and takes the tokens that they see
+// 64 at a time: each wave brings one tile of sixteen into LDS, keys as they are, values converted and transposed to
+// what the matrix instructions want, once for all waves. Two buffers: a step is prepared while the one in front is
+// multiplied, and its successor's rows are on their way from memory into registers.
+constexpr int kPromptTiles = kPromptWaves;
+
+template <class E, int D> struct PromptLds {
+  static constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
+  at_v4i values[2][kChunks * COLS][64];             // [32 tokens][column][lane]
+  at_v4i keys[kPromptTiles][kChunks][64];
+  uint8_t key_scale[kPromptTiles][kChunks][64];
+  unsigned long long bad[kPromptTiles][kChunks][4];     // lanes whose values are NaN, for each of a lane's tokens
+  int first[kPromptTiles], any_bad[kPromptTiles];
+};
+
+// What a wave has asked for of a tile.
+template <int D> struct PromptTile {
+  static constexpr int kChunks = (D + 127) / 128;
+  at_v4i keys[kChunks];
+  int key_scale[kChunks];
+  uint32_t values[kChunks][4], value_scale[kChunks][4];
+  int first;
+};
+
+template <class E, class OUT, int D, int QT>
+__global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_kernel(Attention p, unsigned blocks) {
+  constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8, ROWS = kPromptWaves * QT * 16, P = AtKind<E>::kP;
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_all[];
+  PromptLds<E, D> *const lds = reinterpret_cast<PromptLds<E, D> *>(s_all);
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the last rows, which see most, begin
+  const unsigned id = blockIdx.x;
+  if (id >= blocks) return;
+  const int h = (int)(id % (unsigned)p.kv_heads), share = (int)(id / (unsigned)p.kv_heads % (unsigned)p.splits),
+            slot = p.slots - 1 - (int)(id / (unsigned)p.kv_heads / (unsigned)p.splits);
+  AtRows r;
+  if (!at_rows<ROWS>(p, slot, r)) return;
+  auto position_of = [&](int row) { return max(r.length - r.count + row / p.group, -1); };
+  const int low = position_of(r.first), high = position_of(r.last - 1);
+
+  // this wave's rows
+  AtQueries<E, D> queries[QT];
+  int position[QT], my_low[QT], my_high[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const int first = r.first + (wave * QT + t) * 16, at = min(first + l16, r.last - 1);
+    const int token = at / p.group, head = h * p.group + (at - token * p.group);
+    position[t] = position_of(at);
+    // (none: rows that see nothing)
+    my_low[t] = first < r.last ? position_of(first) : -1;
+    my_high[t] = first < r.last ? position_of(min(first + 15, r.last - 1)) : -1;
+    queries[t].load(reinterpret_cast<const typename E::T *>(p.q + (size_t)(r.begin + token) * p.q_row_bytes) + (size_t)head * D,
+                    p.negative);
+  }
+  at_v4f acc[QT][D / 16];
+  float most[QT], sum[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    most[t] = kAtNone, sum[t] = 0;
+#pragma unroll
+    for (int m = 0; m < D / 16; m++) acc[t][m] = at_v4f{0, 0, 0, 0};
+  }
+
+  const AtTiles tiles = at_tiles(p, low, high);
+  const long long steps = (tiles.all + kPromptTiles - 1) / kPromptTiles;
+  const int begin = (int)(steps * share / p.splits), end = (int)(steps * (share + 1) / p.splits);
+
+  // ---- a tile from memory to LDS
+  const uint32_t row_bytes = (uint32_t)p.c.row_bytes, codes_at = (uint32_t)h * (D / 2), scales_at = p.c.scales_at + (uint32_t)h * (D / 32);
+  const int block = D == 64 ? q & 1 : q;
+  const uint32_t key_at = l16 * row_bytes + codes_at + block * 16, key_scale_at = l16 * row_bytes + scales_at + block;
+  uint32_t value_at[4], value_scale_at[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    value_at[i] = (4 * q + i) * row_bytes + codes_at + l16 * (COLS / 2);
+    value_scale_at[i] = (4 * q + i) * row_bytes + scales_at + l16 * COLS / 32;
+  }
+  auto locate = [&](int step) {
+    const int u = step * kPromptTiles + wave;
+    return u < tiles.all ? cache_tile_row(p.c, r.sequence, (unsigned)tiles.at(u)) : -1ll;
+  };
+  auto load = [&](PromptTile<D> &t, long long row, int step) {
+    t.first = row < 0 ? -1 : tiles.at(step * kPromptTiles + wave) * kCacheTile;
+    // (a tile that is not there reads the cache's first rows; there is a page)
+    const size_t base = (size_t)max(row, 0ll) * p.c.row_bytes;
+    const uint8_t *keys = p.c.keys + base, *values = p.c.values + base;
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      t.keys[c] = *reinterpret_cast<const at_v4i *>(keys + (key_at + c * 64));
+      t.key_scale[c] = keys[key_scale_at + c * 4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (COLS == 8) t.values[c][i] = *reinterpret_cast<const uint32_t *>(values + (value_at[i] + c * 64));
+        else t.values[c][i] = *reinterpret_cast<const uint16_t *>(values + value_at[i]);
+        t.value_scale[c][i] = values[value_scale_at[i] + c * 4];
+      }
+    }
+  };
+  auto store = [&](PromptTile<D> &t, PromptLds<E, D> &to) {
+    bool any = false;
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      const bool none = D == 64 && q >= 2;           // (these lanes have no columns)
+      to.keys[wave][c][lane] = none ? at_v4i{0, 0, 0, 0} : t.keys[c];
+      to.key_scale[wave][c][lane] = none ? 127 : (uint8_t)t.key_scale[c];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) top = max(top, t.value_scale[c][i]);
+      if (__ballot(top >= (uint32_t)AtKind<E>::kNan)) {
+        // blocks that are NaN count as zeros in the product; who sees them becomes NaN
+        any = true;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const bool is_bad = t.value_scale[c][i] >= (uint32_t)AtKind<E>::kNan;
+          const unsigned long long mask = __ballot(is_bad);
+          if (lane == 0) to.bad[wave][c][i] = mask;
+          t.values[c][i] = is_bad ? 0 : t.values[c][i];
+          t.value_scale[c][i] = is_bad ? 127 : t.value_scale[c][i];
+        }
+      } else if (kChunks > 1 && lane == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) to.bad[wave][c][i] = 0;
+      }
+      float scale[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) scale[i] = __uint_as_float(max(t.value_scale[c][i] << 23, 0x00400000u));
+      typedef int Half __attribute__((ext_vector_type(2)));
+      Half columns[COLS];
+      at_transpose4<E, COLS>(columns, t.values[c], scale);
+#pragma unroll
+      for (int m = 0; m < COLS; m++) reinterpret_cast<Half *>(&to.values[wave >> 1][c * COLS + m][lane])[wave & 1] = columns[m];
+    }
+    if (lane == 0) to.first[wave] = t.first, to.any_bad[wave] = any;
+  };
+
+  PromptTile<D> next;
+  long long row = -1;
+  if (begin < end) {
+    load(next, locate(begin), begin);
+    store(next, lds[0]);
+    if (begin + 1 < end) {
+      load(next, locate(begin + 1), begin + 1);
+      if (begin + 2 < end) row = locate(begin + 2);
+    }
+  }
+  __syncthreads();
+  for (int step = begin; step < end; step++) {
+    const PromptLds<E, D> &now = lds[(step - begin) & 1];
+    if (step + 1 < end) {
+      store(next, lds[(step - begin + 1) & 1]);
+      if (step + 2 < end) {
+        load(next, row, step + 2);
+        if (step + 3 < end) row = locate(step + 3);
+      }
+    }
+    int first[kPromptTiles];
+    bool any_bad = false;
+#pragma unroll
+    for (int k = 0; k < kPromptTiles; k++) {
+      first[k] = __builtin_amdgcn_readfirstlane(now.first[k]);
+      any_bad = any_bad || __builtin_amdgcn_readfirstlane(now.any_bad[k]);
+    }
+    at_v4i packed[QT][2][P];
+    bool none = true;
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      bool nothing = true, whole = true;
+#pragma unroll
+      for (int k = 0; k < kPromptTiles; k++) {
+        nothing = nothing && at_sees_none(p, my_low[t], my_high[t], first[k]);
+        whole = whole && at_sees_all(p, my_low[t], my_high[t], first[k]);
+      }
+      if (nothing) {
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int s = 0; s < P; s++) packed[t][k][s] = at_v4i{0, 0, 0, 0};
+        continue;
+      }
+      none = false;
+      float score[16];
+#pragma unroll
+      for (int k = 0; k < kPromptTiles; k++) {
+        at_v4f s = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+          const at_v4i codes = now.keys[k][c][lane];
+          const int byte = now.key_scale[k][c][lane];
+#pragma unroll
+          for (int term = 0; term < AtKind<E>::kQ; term++)
+            s = at_scores(codes, byte, queries[t].codes[c][term], queries[t].scale[c][term], s);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) score[k * 4 + i] = s[i];
+      }
+      unsigned seen = 0xffff;
+      if (!whole) {
+        seen = 0;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const bool yes = first[j >> 2] >= 0 && at_sees(p, position[t], first[j >> 2] + 4 * q + (j & 3));
+          seen |= yes ? 1u << j : 0;
+          score[j] = yes ? score[j] : kAtNone;
+        }
+      }
+      at_weigh<E>(score, most[t], sum[t], acc[t], p.scale, whole, seen);
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        float part[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) part[j] = score[k * 8 + j];
+        at_pack<E>(packed[t][k], part);
+      }
+    }
+    if (!none) {
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int m = 0; m < kChunks * COLS; m++) {
+          const at_v4i values = now.values[k][m][lane];
+#pragma unroll
+          for (int t = 0; t < QT; t++)
+#pragma unroll
+            for (int s = 0; s < P; s++) acc[t][m] = AtValues<E>::multiply(values, packed[t][k][s], acc[t][m]);
+        }
+      if (any_bad) {
+        const float nan = __builtin_nanf("");
+        for (int k = 0; k < kPromptTiles; k++) {
+          if (!now.any_bad[k]) continue;
+          const int from = now.first[k];
+#pragma unroll
+          for (int c = 0; c < kChunks; c++)
+            for (int i = 0; i < 4; i++) {
+              const unsigned long long bad = now.bad[k][c][i];
+              for (int team = 0; team < 4; team++) {
+                // lanes of the block that this lane's columns are in: 4 of a team's 16, or 8 where it has two blocks
+                const unsigned mine = D == 64 ? (unsigned)(bad >> (16 * team + 8 * (q >> 1))) & 0xff
+                                              : (unsigned)(bad >> (16 * team + 4 * q)) & 0xf;
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+                  if (mine && from >= 0 && at_sees(p, position[t], from + 4 * team + i)) {
+#pragma unroll
+                    for (int m = 0; m < COLS; m++)
+#pragma unroll
+                      for (int e = 0; e < 4; e++) acc[t][c * COLS + m][e] = nan;
+                  }
+              }
+            }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    AtRows mine = r;
+    mine.first = r.first + (wave * QT + t) * 16;
+    mine.last = min(r.last, mine.first + 16);
+    if (mine.first >= mine.last) continue;
+    const float whole = add_across32(add_across16(sum[t]));
+    if (p.splits == 1) {
+      at_store_whole<OUT, D>(p, mine, h, acc[t], whole);
+    } else {
+      const long long sixteen = at_first_slot<16>(p, r.sequence) + mine.first / 16;
+      float *part = p.part + ((size_t)(sixteen * p.splits + share) * p.kv_heads + h) * at_part_floats<D>();
+#pragma unroll
+      for (int m = 0; m < D / 16; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) part[(i * (D / 16) + m) * 64 + lane] = acc[t][m][i];
+      if (lane < 16) part[16 * D + l16] = most[t], part[16 * D + 16 + l16] = whole;
+    }
+  }
+}
+
+template <class E, class OUT, int D, int TYPE> static int prompt_launch(const Attention &p, hipStream_t st) {
+  constexpr int QT = at_prompt_sixteens(TYPE, D);
+  constexpr size_t kLds = 2 * sizeof(PromptLds<E, D>);
+  static std::atomic<uint64_t> attr_set{0};
+  auto kernel = mx4_attention_prompt_kernel<E, OUT, D, QT>;
+  if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;
+  const unsigned blocks = (unsigned)((long long)p.slots * p.splits * p.kv_heads);
+  kernel<<<blocks, kPromptWaves * 64, kLds, st>>>(p, blocks);
+  return check_launch("mx4_attention");
+}
+template <class E, class OUT, int TYPE> static int prompt_launch_dim(const Attention &p, int dim, hipStream_t st) {
+  return dim == 64    ? prompt_launch<E, OUT, 64, TYPE>(p, st)
+         : dim == 128 ? prompt_launch<E, OUT, 128, TYPE>(p, st)
+                      : prompt_launch<E, OUT, 256, TYPE>(p, st);
+}
+int at_prompt_launch(const Attention &p, int type, bool mx4, int dim, hipStream_t st) {
+  if (type == MI355X_F32)
+    return mx4 ? prompt_launch_dim<F32, MX4, MI355X_F32>(p, dim, st) : prompt_launch_dim<F32, F32, MI355X_F32>(p, dim, st);
+  if (type == MI355X_F16)
+    return mx4 ? prompt_launch_dim<F16, MX4, MI355X_F16>(p, dim, st) : prompt_launch_dim<F16, F16, MI355X_F16>(p, dim, st);
+  return mx4 ? prompt_launch_dim<BF16, MX4, MI355X_BF16>(p, dim, st) : prompt_launch_dim<BF16, BF16, MI355X_BF16>(p, dim, st);
+}
+
+} // namespace mi355x
