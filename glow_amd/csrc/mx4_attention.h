@@ -216,25 +216,27 @@ template <class E> __device__ __forceinline__ void at_pack(at_v4i (&w)[AtKind<E>
 }
 
 // Eight tokens' words of codes (eight neighbouring columns each; COLS = 4: the low half) -> for each column the
-// eight tokens' values, in the matrix instruction's order.
-template <class E, int COLS>
-__device__ __forceinline__ void at_transpose(at_v4i (&out)[COLS], const uint32_t (&codes)[8], const float (&scale)[8]) {
+// eight tokens' values, in the matrix instruction's order: use(column, values).
+template <class E, int COLS, class USE>
+__device__ __forceinline__ void at_transpose(const uint32_t (&codes)[8], const float (&scale)[8], USE &&use) {
   typedef AtValues<E> V;
+  auto columns = [&](auto pair) {
+    at_v4i even, odd;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    auto columns = [&](auto pair) {
-      constexpr int P = decltype(pair)::value;
+    for (int j = 0; j < 4; j++) {
       const uint32_t a = __builtin_bit_cast(uint32_t, V::two(codes[2 * j], scale[2 * j], pair));
       const uint32_t b = __builtin_bit_cast(uint32_t, V::two(codes[2 * j + 1], scale[2 * j + 1], pair));
-      out[2 * P][j] = (int)__builtin_amdgcn_perm(b, a, 0x05040100);
-      out[2 * P + 1][j] = (int)__builtin_amdgcn_perm(b, a, 0x07060302);
-    };
-    columns(std::integral_constant<int, 0>());
-    columns(std::integral_constant<int, 1>());
-    if constexpr (COLS == 8) {
-      columns(std::integral_constant<int, 2>());
-      columns(std::integral_constant<int, 3>());
+      even[j] = (int)__builtin_amdgcn_perm(b, a, 0x05040100);
+      odd[j] = (int)__builtin_amdgcn_perm(b, a, 0x07060302);
     }
+    use(2 * decltype(pair)::value, even);
+    use(2 * decltype(pair)::value + 1, odd);
+  };
+  columns(std::integral_constant<int, 0>());
+  columns(std::integral_constant<int, 1>());
+  if constexpr (COLS == 8) {
+    columns(std::integral_constant<int, 2>());
+    columns(std::integral_constant<int, 3>());
   }
 }
 
@@ -281,6 +283,12 @@ __device__ __forceinline__ bool at_sees_all(const Attention &p, int low, int hig
 }
 __device__ __forceinline__ bool at_sees_none(const Attention &p, int low, int high, int first) {
   return first < 0 || first > high || (first + kCacheTile - 1 <= low - p.window && first >= p.sinks);
+}
+
+// Whether lanes of `bad`, values of a team's token, hold a bad block of which this lane has columns: 4 of the team's 16
+// lanes, or 8 where it has two blocks.
+template <int D> __device__ __forceinline__ bool at_bad_block(unsigned long long bad, int team, int q) {
+  return D == 64 ? (bad >> (16 * team + 8 * (q >> 1)) & 0xff) != 0 : (bad >> (16 * team + 4 * q) & 0xf) != 0;
 }
 
 // Scores of a lane's query (tokens that it does not see: minus infinity, and not in `seen`, which counts unless `whole`)

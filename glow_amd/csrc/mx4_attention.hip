@@ -1,16 +1,34 @@
 // Attention over a cache of microscaled rows: few rows of queries a sequence.
 #include "mx4_attention.h"
-
-#include "gemm_i8.h"
+#include "mx4_tiles.h"
 
 namespace mi355x {
 
 // A workgroup has sixteen rows of queries and a share of the tokens that they see, its eight waves every
 // eighth step of 32 tokens each; their results meet in LDS, those of several shares in a second launch.
+//
+// Rows go from memory to LDS without registers between, a step ahead, each wave into a ring of its own that no other
+// reads: there is no barrier in the loop. A load moves 16 bytes a lane, 1 KB at once, and a lane picks the piece that
+// makes the reads free of bank conflicts: keys' blocks in the order of the products' tiles (mx4_swizzle), token 4 q + i of
+// the values in row q + 4 i, so that word i of a lane lies at 64 i + lane.
 template <int D> constexpr int kAtWaves = D == 256 ? 4 : 8;
+constexpr int kAtStages = 2;
 
-// What a wave has asked for of 32 tokens: for each of two tiles a block of a token's keys and its scale byte, and of
-// the values eight tokens' words.
+template <int D> struct AtRing {
+  static constexpr int kTile = 8 * D;                    // bytes of sixteen tokens' codes
+  static constexpr int kKeys = 0, kValues = 2 * kTile, kScales = 4 * kTile;
+  static constexpr int kWords = D <= 128 ? 1 : 2;        // of a token's scales
+  static constexpr int kStage = kScales + 256 * kWords;
+  static constexpr int kLoads = 4 * kTile / 1024 + kWords;
+};
+
+// Four bytes a lane from global memory straight into LDS at lds_addr + 4 * lane.
+__device__ __forceinline__ void dma4(const void *gptr, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_addr), "v"(gptr) : "memory");
+}
+
+// 32 tokens as a wave has them in registers: for each of two tiles a block of a token's keys and its scale byte, and of
+// the values eight tokens' words and the words of their scales.
 template <int D> struct AtStep {
   static constexpr int kChunks = (D + 127) / 128;
   at_v4i keys[2][kChunks];
@@ -20,50 +38,101 @@ template <int D> struct AtStep {
   int first[2];                        // token of each tile; -1: none
 };
 
-template <class E, int D> struct AtWave {
+template <int D> struct AtLoader {
+  typedef AtRing<D> R;
   static constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
   const Attention &p;
-  int sequence;
-  int l16, q;
-  uint32_t key_at, key_scale_at, value_at[4], value_scale_at[4];
+  const AtTiles tiles;
+  const int sequence, begin, stride, end;     // this wave's steps: begin, begin + stride, ..
+  const int lane, l16, q;
+  uint32_t key_at, value_at[D == 256 ? 2 : 1], scale_at, lds;
+  long long row_of;                    // the row where the tile of this lane begins, of 32 steps' 64
 
-  __device__ __forceinline__ AtWave(const Attention &p, int sequence, int h) : p(p), sequence(sequence) {
-    const int lane = threadIdx.x & 63;
-    l16 = lane & 15, q = lane >> 4;
-    const uint32_t row = (uint32_t)p.c.row_bytes, codes = (uint32_t)h * (D / 2), scales = p.c.scales_at + (uint32_t)h * (D / 32);
-    const int block = D == 64 ? q & 1 : q;          // (lanes q = 2 and 3 have no columns then)
-    key_at = l16 * row + codes + block * 16;
-    key_scale_at = l16 * row + scales + block;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      value_at[i] = (4 * q + i) * row + codes + l16 * (COLS / 2);
-      value_scale_at[i] = (4 * q + i) * row + scales + l16 * COLS / 32;
+  __device__ __forceinline__ AtLoader(const Attention &p, const AtTiles &tiles, int sequence, int h, int begin, int stride, int end,
+                                      uint32_t lds)
+      : p(p), tiles(tiles), sequence(sequence), begin(begin), stride(stride), end(end), lane(threadIdx.x & 63), l16(lane & 15),
+        q(lane >> 4), lds(lds) {
+    const uint32_t row = (uint32_t)p.c.row_bytes, codes = (uint32_t)h * (D / 2);
+    if constexpr (D == 64) {
+      // a load has both tiles, rows of two pieces
+      key_at = (lane >> 1 & 15) * row + codes + (lane & 1) * 16;
+      const int r = lane >> 1 & 15;
+      value_at[0] = (4 * (r & 3) + (r >> 2)) * row + codes + (lane & 1) * 16;
+      scale_at = l16 * row + ((p.c.scales_at + (uint32_t)h * 2) & ~3u);
+    } else {
+      // (D = 256: two loads a tile, 128 columns each)
+      key_at = (lane >> 2) * row + codes + ((lane & 3) ^ mx4_swizzle(lane >> 2)) * 16;
+      const int r = lane >> 2;
+      value_at[0] = (4 * (r & 3) + (r >> 2)) * row + codes + (lane & 3) * 16;
+      scale_at = l16 * row + p.c.scales_at + (uint32_t)h * (D / 32);
     }
   }
-  // Rows of the cache where tiles u and u + 1 begin.
-  __device__ __forceinline__ void locate(long long (&row)[2], const AtTiles &t, int u) const {
-#pragma unroll
-    for (int k = 0; k < 2; k++) row[k] = u + k < t.all ? cache_tile_row(p.c, sequence, (unsigned)t.at(u + k)) : -1;
+  __device__ __forceinline__ int step_of(int n) const { return min(begin + n * stride, end - 1); }
+  // Finds the rows of steps n to n + 31.
+  __device__ __forceinline__ void locate(int n) {
+    const long long step = begin + (long long)(n + (lane >> 1)) * stride;
+    const int u = (int)min(2 * step + (lane & 1), (long long)tiles.all);
+    row_of = step < end && u < tiles.all ? cache_tile_row(p.c, sequence, (unsigned)tiles.at(u)) : -1;
   }
-  __device__ __forceinline__ void load(AtStep<D> &s, const long long (&row)[2], const AtTiles &t, int u) const {
+  // Asks for step n (the last one again where there is none), says which tokens come.
+  __device__ __forceinline__ void issue(int n, int (&first)[2]) {
+    if ((n & 31) == 0) locate(n);
+    const uint8_t *keys[2], *values[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-      s.first[k] = row[k] < 0 ? -1 : t.at(u + k) * kCacheTile;
+      const int at = 2 * (n & 31) + k;
+      const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)row_of, at), high = __builtin_amdgcn_readlane((int)(row_of >> 32), at);
+      const long long row = (long long)((uint64_t)high << 32 | low);
+      first[k] = row < 0 ? -1 : tiles.at(2 * step_of(n) + k) * kCacheTile;
       // (a tile that is not there reads the cache's first rows; there is a page)
-      const size_t base = (size_t)max(row[k], 0ll) * p.c.row_bytes;
-      const uint8_t *keys = p.c.keys + base, *values = p.c.values + base;
+      const size_t base = (size_t)max(row, 0ll) * p.c.row_bytes;
+      keys[k] = p.c.keys + base, values[k] = p.c.values + base;
+    }
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds + (n % kAtStages) * R::kStage));
+    if constexpr (D == 64) {
+      const bool second = lane >= 32;
+      dma16((second ? keys[1] : keys[0]) + key_at, to + R::kKeys);
+      dma16((second ? values[1] : values[0]) + value_at[0], to + R::kValues);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+          dma16(keys[k] + key_at + c * 64, to + R::kKeys + k * R::kTile + c * 1024);
+          dma16(values[k] + value_at[0] + c * 64, to + R::kValues + k * R::kTile + c * 1024);
+        }
+    }
+    const uint8_t *scales = q == 0 ? keys[0] : q == 1 ? keys[1] : q == 2 ? values[0] : values[1];
+#pragma unroll
+    for (int w = 0; w < R::kWords; w++) dma4(scales + scale_at + w * 4, to + R::kScales + w * 256);
+  }
+  // A step that has landed, from LDS.
+  __device__ __forceinline__ void read(AtStep<D> &s, const uint8_t *ring, int n, int h) const {
+    const uint8_t *at = ring + (n % kAtStages) * R::kStage;
+#pragma unroll
+    for (int k = 0; k < 2; k++)
 #pragma unroll
       for (int c = 0; c < kChunks; c++) {
-        s.keys[k][c] = *reinterpret_cast<const at_v4i *>(keys + (key_at + c * 64));
-        s.key_scale[k][c] = keys[key_scale_at + c * 4];
+        const uint8_t *scales = at + R::kScales + c * 256;
+        if constexpr (D == 64) {
+          const int block = q & 1;                  // (lanes q = 2 and 3 have no columns)
+          s.keys[k][c] = *reinterpret_cast<const at_v4i *>(at + R::kKeys + k * R::kTile + l16 * 32 + block * 16);
+          s.key_scale[k][c] = scales[(k * 16 + l16) * 4 + (h & 1) * 2 + block];
+        } else {
+          s.keys[k][c] = *reinterpret_cast<const at_v4i *>(at + R::kKeys + k * R::kTile + c * 1024 + l16 * 64 +
+                                                           ((q ^ mx4_swizzle(l16)) << 4));
+          s.key_scale[k][c] = scales[(k * 16 + l16) * 4 + q];
+        }
+        const at_v4i words = *reinterpret_cast<const at_v4i *>(scales + 128 + (k * 16 + 4 * q) * 4);
+        const int shift = D == 64 ? 8 * ((h & 1) * 2 + (l16 >> 3)) : 8 * (l16 >> 2);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          if constexpr (COLS == 8) s.values[c][k * 4 + i] = *reinterpret_cast<const uint32_t *>(values + (value_at[i] + c * 64));
-          else s.values[c][k * 4 + i] = *reinterpret_cast<const uint16_t *>(values + value_at[i]);
-          s.value_scale[c][k * 4 + i] = values[value_scale_at[i] + c * 4];
+          const uint8_t *v = at + R::kValues + k * R::kTile + c * 1024;
+          if constexpr (COLS == 8) s.values[c][k * 4 + i] = reinterpret_cast<const uint32_t *>(v)[i * 64 + lane];
+          else s.values[c][k * 4 + i] = reinterpret_cast<const uint16_t *>(v)[i * 64 + lane];
+          s.value_scale[c][k * 4 + i] = (uint32_t)words[i] >> shift & 255;
         }
       }
-    }
   }
 };
 
@@ -117,38 +186,31 @@ __device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> 
     for (int j = 0; j < 8; j++) high_byte = max(high_byte, s.value_scale[c][j]);
     if (__ballot(high_byte >= (uint32_t)AtKind<E>::kNan)) {
       // Blocks that are NaN count as zeros in the product; who sees them becomes NaN.
-      const float nan = __builtin_nanf("");
-      for (int j = 0; j < 8; j++) {
-        const unsigned long long bad = __ballot(s.value_scale[c][j] >= (uint32_t)AtKind<E>::kNan);
-        for (int team = 0; team < 4; team++) {
-          // lanes of the block that this lane's columns are in: 4 of a team's 16, or 8 where it has two blocks
-          const unsigned mine = D == 64 ? (unsigned)(bad >> (16 * team + 8 * (q >> 1))) & 0xff
-                                        : (unsigned)(bad >> (16 * team + 4 * q)) & 0xf;
-          const int first = s.first[j >> 2];
-          if (mine && first >= 0 && at_sees(p, position, first + 4 * team + (j & 3))) {
-#pragma unroll
-            for (int m = 0; m < COLS; m++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) a.acc[c * 8 + m][i] = nan;
-          }
-        }
-      }
+      bool hit = false;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const bool is_bad = s.value_scale[c][j] >= (uint32_t)AtKind<E>::kNan;
+        const unsigned long long bad = __ballot(is_bad);
         s.values[c][j] = is_bad ? 0 : s.values[c][j];
         s.value_scale[c][j] = is_bad ? 127 : s.value_scale[c][j];
+        const int first = s.first[j >> 2];
+        if (bad && first >= 0) {
+#pragma unroll 1
+          for (int team = 0; team < 4; team++) hit = hit || (at_bad_block<D>(bad, team, q) && at_sees(p, position, first + 4 * team + (j & 3)));
+        }
       }
+#pragma unroll
+      for (int m = 0; m < COLS; m++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) a.acc[c * 8 + m][i] = hit ? __builtin_nanf("") : a.acc[c * 8 + m][i];
     }
     float scale[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) scale[j] = __uint_as_float(max(s.value_scale[c][j] << 23, 0x00400000u));
-    at_v4i columns[COLS];
-    at_transpose<E, COLS>(columns, s.values[c], scale);
+    at_transpose<E, COLS>(s.values[c], scale, [&](int m, at_v4i values) {
 #pragma unroll
-    for (int m = 0; m < COLS; m++)
-#pragma unroll
-      for (int t = 0; t < AtKind<E>::kP; t++) a.acc[c * 8 + m] = AtValues<E>::multiply(columns[m], packed[t], a.acc[c * 8 + m]);
+      for (int t = 0; t < AtKind<E>::kP; t++) a.acc[c * 8 + m] = AtValues<E>::multiply(values, packed[t], a.acc[c * 8 + m]);
+    });
   }
 }
 
@@ -180,10 +242,14 @@ __global__ __launch_bounds__(256) void mx4_attention_join_kernel(Attention p) {
   at_store<E, OUT, D>(p, r, h, i, x, s_most);
 }
 
+// Waves that share a SIMD's registers.
+template <class E, int D> constexpr int at_rows_waves() { return D == 256 ? 1 : AtKind<E>::kQ == 6 ? 2 : 4; }
+
 template <class E, class OUT, int D>
-__global__ __launch_bounds__(kAtWaves<D> * 64, D == 256 ? 1 : 2) void mx4_attention_rows_kernel(Attention p, unsigned blocks) {
+__global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4_attention_rows_kernel(Attention p, unsigned blocks) {
   constexpr int WAVES = kAtWaves<D>;
-  extern __shared__ __attribute__((aligned(16))) float s_acc[];      // [waves][4][D / 16][64]
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_ring[];
+  float *const s_acc = reinterpret_cast<float *>(s_ring);           // [waves][4][D / 16][64]
   __shared__ float s_top[WAVES][16], s_sum[WAVES][16];
   __shared__ uint32_t s_most[4][64];
   const int lane = threadIdx.x & 63, l16 = lane & 15;
@@ -210,23 +276,27 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, D == 256 ? 1 : 2) void mx4_attent
   a.most = kAtNone, a.sum = 0;
 #pragma unroll
   for (int m = 0; m < D / 16; m++) a.acc[m] = at_v4f{0, 0, 0, 0};
-  const AtWave<E, D> w(p, r.sequence, h);
-  long long row[2];
-  AtStep<D> next;
-  int step = begin + wave;
-  if (step < end) {
-    w.locate(row, tiles, 2 * step);
-    w.load(next, row, tiles, 2 * step);
-    if (step + WAVES < end) w.locate(row, tiles, 2 * (step + WAVES));
-  }
-  for (; step < end; step += WAVES) {
-    AtStep<D> now = next;
-    if (step + WAVES < end) {
-      w.load(next, row, tiles, 2 * (step + WAVES));
-      if (step + 2 * WAVES < end) w.locate(row, tiles, 2 * (step + 2 * WAVES));
+  const uint8_t *ring = s_ring + (size_t)wave * kAtStages * AtRing<D>::kStage;
+  const int mine = end - begin - wave > 0 ? (end - begin - wave + WAVES - 1) / WAVES : 0;
+  if (mine > 0) {
+    AtLoader<D> loader(p, tiles, r.sequence, h, begin + wave, WAVES, end, lds_address(ring));
+    int first[kAtStages][2];
+#pragma unroll
+    for (int k = 0; k < kAtStages; k++) loader.issue(k, first[k]);
+    for (int n = 0; n < mine; n++) {
+      AtStep<D> s;
+      dma_wait<(kAtStages - 1) * AtRing<D>::kLoads>();
+      loader.read(s, ring, n, h);
+      s.first[0] = first[0][0], s.first[1] = first[0][1];
+      first[0][0] = first[1][0], first[0][1] = first[1][1];
+      // the slot is free when it has been read
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      loader.issue(n + kAtStages, first[1]);
+      at_step<E, D>(a, queries, s, p, low, high, position);
     }
-    at_step<E, D>(a, queries, now, p, low, high, position);
+    dma_wait<0>();
   }
+  __syncthreads();                    // the rings' memory is used again
 
   const float sum = add_across32(add_across16(a.sum));
   if (lane < 16) s_top[wave][l16] = a.most, s_sum[wave][l16] = sum;
@@ -283,7 +353,7 @@ template <class E, class OUT, int D> static int at_launch(Attention p, int type,
     if (int rc = at_prompt_launch(p, type, OUT::kSize == 0, D, st)) return rc;
   } else {
     const unsigned blocks = (unsigned)((long long)p.slots * p.splits * p.kv_heads);
-    constexpr size_t kLds = (size_t)kAtWaves<D> * 16 * D * 4;
+    constexpr size_t kLds = (size_t)kAtWaves<D> * std::max(16 * D * 4, kAtStages * AtRing<D>::kStage);
     static std::atomic<uint64_t> attr_set{0};
     auto kernel = mx4_attention_rows_kernel<E, OUT, D>;
     if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;

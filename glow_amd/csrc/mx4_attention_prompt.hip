@@ -232,29 +232,28 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
             for (int s = 0; s < P; s++) acc[t][m] = AtValues<E>::multiply(values, packed[t][k][s], acc[t][m]);
         }
       if (any_bad) {
-        const float nan = __builtin_nanf("");
+        bool hit[QT][kChunks] = {};
+#pragma unroll 1
         for (int k = 0; k < kPromptTiles; k++) {
-          if (!now.any_bad[k]) continue;
           const int from = now.first[k];
+          if (!now.any_bad[k] || from < 0) continue;
+#pragma unroll 1
+          for (int x = 0; x < 16; x++)
 #pragma unroll
-          for (int c = 0; c < kChunks; c++)
-            for (int i = 0; i < 4; i++) {
-              const unsigned long long bad = now.bad[k][c][i];
-              for (int team = 0; team < 4; team++) {
-                // lanes of the block that this lane's columns are in: 4 of a team's 16, or 8 where it has two blocks
-                const unsigned mine = D == 64 ? (unsigned)(bad >> (16 * team + 8 * (q >> 1))) & 0xff
-                                              : (unsigned)(bad >> (16 * team + 4 * q)) & 0xf;
+            for (int c = 0; c < kChunks; c++) {
+              const bool mine = at_bad_block<D>(now.bad[k][c][x & 3], x >> 2, q);
 #pragma unroll
-                for (int t = 0; t < QT; t++)
-                  if (mine && from >= 0 && at_sees(p, position[t], from + 4 * team + i)) {
-#pragma unroll
-                    for (int m = 0; m < COLS; m++)
-#pragma unroll
-                      for (int e = 0; e < 4; e++) acc[t][c * COLS + m][e] = nan;
-                  }
-              }
+              for (int t = 0; t < QT; t++) hit[t][c] = hit[t][c] || (mine && at_sees(p, position[t], from + x));
             }
         }
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int c = 0; c < kChunks; c++)
+#pragma unroll
+            for (int m = 0; m < COLS; m++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) acc[t][c * COLS + m][e] = hit[t][c] ? __builtin_nanf("") : acc[t][c * COLS + m][e];
       }
     }
     __syncthreads();
