@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void mx4_attention_join_kernel(Attention p) {
 template <class E, int D> constexpr int at_rows_waves() { return D == 256 ? 1 : AtKind<E>::kQ == 6 ? 2 : 4; }
 
 template <class E, class OUT, int D>
-__global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4_attention_rows_kernel(Attention p, unsigned blocks) {
+__global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4_attention_rows_kernel(Attention p, unsigned units) {
   constexpr int WAVES = kAtWaves<D>;
   extern __shared__ __attribute__((aligned(16))) uint8_t s_ring[];
   float *const s_acc = reinterpret_cast<float *>(s_ring);           // [waves][4][D / 16][64]
@@ -254,11 +254,10 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
   __shared__ uint32_t s_most[4][64];
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // heads of the cache whose rows share lines run on one die, one behind the other
-  const unsigned per_die = gridDim.x / 8, id = (blockIdx.x & 7) * per_die + (blockIdx.x >> 3);
-  if (id >= blocks) return;
-  const int h = (int)(id % (unsigned)p.kv_heads), share = (int)(id / (unsigned)p.kv_heads % (unsigned)p.splits),
-            slot = (int)(id / (unsigned)p.kv_heads / (unsigned)p.splits);
+  // heads of the cache whose rows share lines run on one die, one behind the other, and shares on all dies in turn
+  const unsigned place = blockIdx.x >> 3, of_all = place / (unsigned)p.kv_heads * 8 + (blockIdx.x & 7);
+  if (of_all >= units) return;
+  const int h = (int)(place % (unsigned)p.kv_heads), share = (int)(of_all % (unsigned)p.splits), slot = (int)(of_all / (unsigned)p.splits);
   AtRows r;
   if (!at_rows<16>(p, slot, r)) return;
 
@@ -328,7 +327,7 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
 #pragma unroll
     for (int m = 0; m < D / 16; m++) x[m] += s_acc[((k * 4 + i) * (D / 16) + m) * 64 + lane];
   if (p.splits > 1) {
-    float *part = p.part + (size_t)id * at_part_floats<D>();
+    float *part = p.part + ((size_t)of_all * p.kv_heads + h) * at_part_floats<D>();
 #pragma unroll
     for (int m = 0; m < D / 16; m++) part[(i * (D / 16) + m) * 64 + lane] = x[m];
     if (wave == 0 && lane < 16) part[16 * D + l16] = most, part[16 * D + 16 + l16] = whole;
@@ -352,12 +351,12 @@ template <class E, class OUT, int D> static int at_launch(Attention p, int type,
   if (prompt) {
     if (int rc = at_prompt_launch(p, type, OUT::kSize == 0, D, st)) return rc;
   } else {
-    const unsigned blocks = (unsigned)((long long)p.slots * p.splits * p.kv_heads);
+    const unsigned units = (unsigned)((long long)p.slots * p.splits);
     constexpr size_t kLds = (size_t)kAtWaves<D> * std::max(16 * D * 4, kAtStages * AtRing<D>::kStage);
     static std::atomic<uint64_t> attr_set{0};
     auto kernel = mx4_attention_rows_kernel<E, OUT, D>;
     if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;
-    kernel<<<(blocks + 7) / 8 * 8, kAtWaves<D> * 64, kLds, st>>>(p, blocks);
+    kernel<<<(units + 7) / 8 * 8 * p.kv_heads, kAtWaves<D> * 64, kLds, st>>>(p, units);
     if (int rc = check_launch("mx4_attention")) return rc;
   }
   if (p.splits == 1) return MI355X_OK;
@@ -396,7 +395,9 @@ static int at_plan(const mi355x_mx4_cache *cache, size_t heads, int type, size_t
   const int per_slot = plan->prompt ? kPromptWaves * 16 * at_prompt_sixteens(type, (int)cache->head_dim) : 16;
   p->slots = (int)at_slots(rows, p->group, sequences, per_slot);
   const long long tokens = std::min<long long>(p->most, (long long)p->window + p->sinks + per_slot + 48);
-  p->splits = at_splits((long long)p->slots * p->kv_heads, tokens, plan->prompt ? 512 : 256);
+  // (slots that have rows: not many more than this)
+  const long long filled = std::max<long long>(sequences, rows * p->group / per_slot);
+  p->splits = at_splits(filled * p->kv_heads, tokens, plan->prompt ? 512 : 256);
   if (p->splits > 1) plan->bytes = (size_t)sixteens * p->kv_heads * p->splits * at_part_bytes(cache->head_dim);
   return MI355X_OK;
 }
