@@ -324,11 +324,12 @@ __device__ __forceinline__ void at_weigh(float (&score)[N], float &most, float &
 // ---- results -------------------------------------------------------------------------
 
 // Stores the results of quarter `i` of a slot's columns: those that component i of the results has, lane q's
-// 4 q + i. D = 128 and 256: columns 128 c + 8 (4 q + i) + 0 .. 7; D = 64: 4 (4 q + i) + 0 .. 3. Four waves with i of
-// their own call this together where the result is microscaled (`most`: words of LDS for [4][64]).
+// 4 q + i. D = 128 and 256: columns 128 c + 8 (4 q + i) + 0 .. 7; D = 64: 4 (4 q + i) + 0 .. 3. Where the
+// result is microscaled, all waves of a workgroup call this together, four of them with results (`mine`) and i of their
+// own (`most`: words of LDS for [4][64]).
 template <class E, class OUT, int D>
 __device__ __forceinline__ void at_store(const Attention &p, const AtRows &r, int h, int i, float (&x)[D / 16],
-                                         uint32_t (*most)[64]) {
+                                         uint32_t (*most)[64], bool mine) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
   const int at = r.first + l16, token = at / p.group, head = h * p.group + (at - token * p.group);
   uint8_t *row = p.out + (size_t)(r.begin + token) * p.out_row_bytes;
@@ -357,7 +358,7 @@ __device__ __forceinline__ void at_store(const Attention &p, const AtRows &r, in
       for (int j = 0; j < COLS; j++) m = max(m, magnitude_bits(x[c * 8 + j]));
       if (COLS == 4) m = max_across16(m);           // (a block is two lanes')
       __syncthreads();
-      most[i][lane] = m;
+      if (mine) most[i][lane] = m;
       __syncthreads();
       m = max(max(most[0][lane], most[1][lane]), max(most[2][lane], most[3][lane]));
       const uint32_t byte = mx4_scale_byte(m);
@@ -365,7 +366,7 @@ __device__ __forceinline__ void at_store(const Attention &p, const AtRows &r, in
 #pragma unroll
       for (int j = 0; j < 8; j++) y[j] = j < COLS ? x[c * 8 + (j < COLS ? j : 0)] : 0.0f;
       const uint32_t codes = mx4_codes8(y, byte);
-      if (at < r.last) {
+      if (mine && at < r.last) {
         const size_t column = (size_t)head * D + c * 128 + COLS * (4 * q + i);
         uint8_t *scales = row + (size_t)p.out_groups * kMxGroupBytes;
         if constexpr (COLS == 8) *reinterpret_cast<uint32_t *>(row + column / 2) = codes;

@@ -27,15 +27,18 @@ __device__ __forceinline__ void dma4(const void *gptr, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_addr), "v"(gptr) : "memory");
 }
 
-// 32 tokens as a wave has them in registers: for each of two tiles a block of a token's keys and its scale byte, and of
-// the values eight tokens' words and the words of their scales.
-template <int D> struct AtStep {
+// 32 tokens as a wave has them in registers: for each of two tiles a block of a token's keys and its scale byte, and
+// then, when these have become weights, of the values eight tokens' words and their scales. (Both at once take 26
+// registers, with which four waves no longer share a SIMD: 225 us for 137 over 4 x 115 000 tokens where some went to memory.)
+template <int D> struct AtKeys {
   static constexpr int kChunks = (D + 127) / 128;
-  at_v4i keys[2][kChunks];
-  int key_scale[2][kChunks];
-  uint32_t values[kChunks][8];
-  uint32_t value_scale[kChunks][8];
+  at_v4i codes[2][kChunks];
+  int scale[2][kChunks];
   int first[2];                        // token of each tile; -1: none
+};
+template <int D> struct AtWords {
+  static constexpr int kChunks = (D + 127) / 128;
+  uint32_t codes[kChunks][8], scale[kChunks][8];
 };
 
 template <int D> struct AtLoader {
@@ -46,7 +49,7 @@ template <int D> struct AtLoader {
   const int sequence, begin, stride, end;     // this wave's steps: begin, begin + stride, ..
   const int lane, l16, q;
   uint32_t key_at, value_at[D == 256 ? 2 : 1], scale_at, lds;
-  long long row_of;                    // the row where the tile of this lane begins, of 32 steps' 64
+  int tile_of;                         // which rows the tile of this lane has, of 32 steps' 64
 
   __device__ __forceinline__ AtLoader(const Attention &p, const AtTiles &tiles, int sequence, int h, int begin, int stride, int end,
                                       uint32_t lds)
@@ -72,7 +75,7 @@ template <int D> struct AtLoader {
   __device__ __forceinline__ void locate(int n) {
     const long long step = begin + (long long)(n + (lane >> 1)) * stride;
     const int u = (int)min(2 * step + (lane & 1), (long long)tiles.all);
-    row_of = step < end && u < tiles.all ? cache_tile_row(p.c, sequence, (unsigned)tiles.at(u)) : -1;
+    tile_of = step < end && u < tiles.all ? cache_tile(p.c, sequence, (unsigned)tiles.at(u)) : -1;
   }
   // Asks for step n (the last one again where there is none), says which tokens come.
   __device__ __forceinline__ void issue(int n, int (&first)[2]) {
@@ -80,12 +83,10 @@ template <int D> struct AtLoader {
     const uint8_t *keys[2], *values[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-      const int at = 2 * (n & 31) + k;
-      const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)row_of, at), high = __builtin_amdgcn_readlane((int)(row_of >> 32), at);
-      const long long row = (long long)((uint64_t)high << 32 | low);
-      first[k] = row < 0 ? -1 : tiles.at(2 * step_of(n) + k) * kCacheTile;
+      const int tile = __builtin_amdgcn_readlane(tile_of, 2 * (n & 31) + k);
+      first[k] = tile < 0 ? -1 : tiles.at(2 * step_of(n) + k) * kCacheTile;
       // (a tile that is not there reads the cache's first rows; there is a page)
-      const size_t base = (size_t)max(row, 0ll) * p.c.row_bytes;
+      const size_t base = (size_t)max(tile, 0) * kCacheTile * p.c.row_bytes;
       keys[k] = p.c.keys + base, values[k] = p.c.values + base;
     }
     const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds + (n % kAtStages) * R::kStage));
@@ -107,7 +108,7 @@ template <int D> struct AtLoader {
     for (int w = 0; w < R::kWords; w++) dma4(scales + scale_at + w * 4, to + R::kScales + w * 256);
   }
   // A step that has landed, from LDS.
-  __device__ __forceinline__ void read(AtStep<D> &s, const uint8_t *ring, int n, int h) const {
+  __device__ __forceinline__ void read(AtKeys<D> &s, const uint8_t *ring, int n, int h) const {
     const uint8_t *at = ring + (n % kAtStages) * R::kStage;
 #pragma unroll
     for (int k = 0; k < 2; k++)
@@ -116,21 +117,29 @@ template <int D> struct AtLoader {
         const uint8_t *scales = at + R::kScales + c * 256;
         if constexpr (D == 64) {
           const int block = q & 1;                  // (lanes q = 2 and 3 have no columns)
-          s.keys[k][c] = *reinterpret_cast<const at_v4i *>(at + R::kKeys + k * R::kTile + l16 * 32 + block * 16);
-          s.key_scale[k][c] = scales[(k * 16 + l16) * 4 + (h & 1) * 2 + block];
+          s.codes[k][c] = *reinterpret_cast<const at_v4i *>(at + R::kKeys + k * R::kTile + l16 * 32 + block * 16);
+          s.scale[k][c] = scales[(k * 16 + l16) * 4 + (h & 1) * 2 + block];
         } else {
-          s.keys[k][c] = *reinterpret_cast<const at_v4i *>(at + R::kKeys + k * R::kTile + c * 1024 + l16 * 64 +
-                                                           ((q ^ mx4_swizzle(l16)) << 4));
-          s.key_scale[k][c] = scales[(k * 16 + l16) * 4 + q];
+          s.codes[k][c] = *reinterpret_cast<const at_v4i *>(at + R::kKeys + k * R::kTile + c * 1024 + l16 * 64 +
+                                                            ((q ^ mx4_swizzle(l16)) << 4));
+          s.scale[k][c] = scales[(k * 16 + l16) * 4 + q];
         }
-        const at_v4i words = *reinterpret_cast<const at_v4i *>(scales + 128 + (k * 16 + 4 * q) * 4);
+      }
+  }
+  __device__ __forceinline__ void read(AtWords<D> &s, const uint8_t *ring, int n, int h) const {
+    const uint8_t *at = ring + (n % kAtStages) * R::kStage;
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int c = 0; c < kChunks; c++) {
+        const at_v4i words = *reinterpret_cast<const at_v4i *>(at + R::kScales + c * 256 + 128 + (k * 16 + 4 * q) * 4);
         const int shift = D == 64 ? 8 * ((h & 1) * 2 + (l16 >> 3)) : 8 * (l16 >> 2);
+        const uint8_t *v = at + R::kValues + k * R::kTile + c * 1024;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const uint8_t *v = at + R::kValues + k * R::kTile + c * 1024;
-          if constexpr (COLS == 8) s.values[c][k * 4 + i] = reinterpret_cast<const uint32_t *>(v)[i * 64 + lane];
-          else s.values[c][k * 4 + i] = reinterpret_cast<const uint16_t *>(v)[i * 64 + lane];
-          s.value_scale[c][k * 4 + i] = (uint32_t)words[i] >> shift & 255;
+          if constexpr (COLS == 8) s.codes[c][k * 4 + i] = reinterpret_cast<const uint32_t *>(v)[i * 64 + lane];
+          else s.codes[c][k * 4 + i] = reinterpret_cast<const uint16_t *>(v)[i * 64 + lane];
+          s.scale[c][k * 4 + i] = (uint32_t)words[i] >> shift & 255;
         }
       }
   }
@@ -141,10 +150,11 @@ template <class E, int D> struct AtState {
   float most, sum;                     // of this lane's query, and its part of the sum
 };
 
+// Keys to weights.
 template <class E, int D>
-__device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> &queries, AtStep<D> &s, const Attention &p,
-                                        int low, int high, int position) {
-  constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
+__device__ __forceinline__ void at_keys(AtState<E, D> &a, at_v4i (&packed)[AtKind<E>::kP], const AtQueries<E, D> &queries,
+                                        const AtKeys<D> &s, const Attention &p, int low, int high, int position) {
+  constexpr int kChunks = (D + 127) / 128;
   const int lane = threadIdx.x & 63, q = lane >> 4;
   float score[8];
 #pragma unroll
@@ -152,8 +162,8 @@ __device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> 
     at_v4f r = {0, 0, 0, 0};
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
-      at_v4i codes = s.keys[k][c];
-      int byte = s.key_scale[k][c];
+      at_v4i codes = s.codes[k][c];
+      int byte = s.scale[k][c];
       if (D == 64 && q >= 2) codes = at_v4i{0, 0, 0, 0}, byte = 127;
 #pragma unroll
       for (int t = 0; t < AtKind<E>::kQ; t++)
@@ -176,24 +186,30 @@ __device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> 
     }
   }
   at_weigh<E>(score, a.most, a.sum, a.acc, p.scale, whole, seen);
-  at_v4i packed[AtKind<E>::kP];
   at_pack<E>(packed, score);
+}
 
+// Weights by values.
+template <class E, int D>
+__device__ __forceinline__ void at_values(AtState<E, D> &a, const at_v4i (&packed)[AtKind<E>::kP], AtWords<D> &s,
+                                          const int (&tile)[2], const Attention &p, int position) {
+  constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
+  const int q = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int c = 0; c < kChunks; c++) {
     uint32_t high_byte = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) high_byte = max(high_byte, s.value_scale[c][j]);
+    for (int j = 0; j < 8; j++) high_byte = max(high_byte, s.scale[c][j]);
     if (__ballot(high_byte >= (uint32_t)AtKind<E>::kNan)) {
       // Blocks that are NaN count as zeros in the product; who sees them becomes NaN.
       bool hit = false;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const bool is_bad = s.value_scale[c][j] >= (uint32_t)AtKind<E>::kNan;
+        const bool is_bad = s.scale[c][j] >= (uint32_t)AtKind<E>::kNan;
         const unsigned long long bad = __ballot(is_bad);
-        s.values[c][j] = is_bad ? 0 : s.values[c][j];
-        s.value_scale[c][j] = is_bad ? 127 : s.value_scale[c][j];
-        const int first = s.first[j >> 2];
+        s.codes[c][j] = is_bad ? 0 : s.codes[c][j];
+        s.scale[c][j] = is_bad ? 127 : s.scale[c][j];
+        const int first = tile[j >> 2];
         if (bad && first >= 0) {
 #pragma unroll 1
           for (int team = 0; team < 4; team++) hit = hit || (at_bad_block<D>(bad, team, q) && at_sees(p, position, first + 4 * team + (j & 3)));
@@ -206,40 +222,65 @@ __device__ __forceinline__ void at_step(AtState<E, D> &a, const AtQueries<E, D> 
     }
     float scale[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) scale[j] = __uint_as_float(max(s.value_scale[c][j] << 23, 0x00400000u));
-    at_transpose<E, COLS>(s.values[c], scale, [&](int m, at_v4i values) {
+    for (int j = 0; j < 8; j++) scale[j] = __uint_as_float(max(s.scale[c][j] << 23, 0x00400000u));
+    at_transpose<E, COLS>(s.codes[c], scale, [&](int m, at_v4i values) {
 #pragma unroll
       for (int t = 0; t < AtKind<E>::kP; t++) a.acc[c * 8 + m] = AtValues<E>::multiply(values, packed[t], a.acc[c * 8 + m]);
     });
   }
 }
 
-// The shares of sixteen rows joined, and what is done with the whole: wave i < 4 has component i.
+// The shares of sixteen rows joined, and what is done with the whole: wave 4 g + i has component i of every fourth share,
+// from the g-th on, and the four meet in LDS.
 template <class E, class OUT, int D>
-__global__ __launch_bounds__(256) void mx4_attention_join_kernel(Attention p) {
+__global__ __launch_bounds__(1024) void mx4_attention_join_kernel(Attention p) {
+  __shared__ float s_x[12][D / 16][64], s_sum[4][16];
   __shared__ uint32_t s_most[4][64];
-  const int lane = threadIdx.x & 63, l16 = lane & 15, i = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = wave & 3, g = wave >> 2;
   const int h = (int)(blockIdx.x % (unsigned)p.kv_heads), slot = (int)(blockIdx.x / (unsigned)p.kv_heads);
   AtRows r;
   if (!at_rows<16>(p, slot, r)) return;
   const float *part = p.part + ((size_t)slot * p.splits * p.kv_heads + h) * at_part_floats<D>();
   const size_t next = (size_t)p.kv_heads * at_part_floats<D>();
+  const bool there = r.first + l16 < r.last;
   float most = kAtNone;
-  for (int k = 0; k < p.splits; k++) most = fmaxf(most, part[k * next + 16 * D + l16]);
+  for (int k = q; k < p.splits; k += 4) most = fmaxf(most, there ? part[k * next + 16 * D + l16] : kAtNone);
+  most = at_max(most);
   float sum = 0, x[D / 16];
 #pragma unroll
   for (int m = 0; m < D / 16; m++) x[m] = 0;
-  for (int k = 0; k < p.splits; k++) {
-    const float *from = part + k * next;
-    const float of = from[16 * D + l16];
-    const float factor = of == kAtNone ? (from[16 * D + 16 + l16] == 0 ? 0.0f : __builtin_nanf("")) : at_exp2(of - most);
-    sum += from[16 * D + 16 + l16] * factor;
+  if (there) {
+#pragma unroll 2
+    for (int k = g; k < p.splits; k += 4) {
+      const float *from = part + k * next;
+      const float of = from[16 * D + l16], weight = from[16 * D + 16 + l16];
+      float y[D / 16];
 #pragma unroll
-    for (int m = 0; m < D / 16; m++) x[m] += from[(i * (D / 16) + m) * 64 + lane] * factor;
+      for (int m = 0; m < D / 16; m++) y[m] = from[(i * (D / 16) + m) * 64 + lane];
+      const float factor = of == kAtNone ? (weight == 0 ? 0.0f : __builtin_nanf("")) : at_exp2(of - most);
+      sum += weight * factor;
+#pragma unroll
+      for (int m = 0; m < D / 16; m++) x[m] += y[m] * factor;
+    }
   }
+  if (g > 0) {
 #pragma unroll
-  for (int m = 0; m < D / 16; m++) x[m] = sum == 0 ? 0.0f : x[m] / sum;
-  at_store<E, OUT, D>(p, r, h, i, x, s_most);
+    for (int m = 0; m < D / 16; m++) s_x[wave - 4][m][lane] = x[m];
+  }
+  if (i == 0 && lane < 16) s_sum[g][l16] = sum;
+  __syncthreads();
+  // (where blocks of results are formed, all waves meet at the barriers)
+  if (g > 0 && OUT::kSize != 0) return;
+  sum = s_sum[0][l16] + s_sum[1][l16] + s_sum[2][l16] + s_sum[3][l16];
+#pragma unroll
+  for (int m = 0; m < D / 16; m++) {
+    if (g == 0)
+#pragma unroll
+      for (int k = 0; k < 3; k++) x[m] += s_x[k * 4 + i][m][lane];
+    x[m] = sum == 0 ? 0.0f : x[m] / sum;
+  }
+  at_store<E, OUT, D>(p, r, h, i, x, s_most, g == 0);
 }
 
 // Waves that share a SIMD's registers.
@@ -283,15 +324,19 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
 #pragma unroll
     for (int k = 0; k < kAtStages; k++) loader.issue(k, first[k]);
     for (int n = 0; n < mine; n++) {
-      AtStep<D> s;
+      AtKeys<D> keys;
+      AtWords<D> words;
+      at_v4i packed[AtKind<E>::kP];
       dma_wait<(kAtStages - 1) * AtRing<D>::kLoads>();
-      loader.read(s, ring, n, h);
-      s.first[0] = first[0][0], s.first[1] = first[0][1];
+      loader.read(keys, ring, n, h);
+      keys.first[0] = first[0][0], keys.first[1] = first[0][1];
       first[0][0] = first[1][0], first[0][1] = first[1][1];
+      at_keys<E, D>(a, packed, queries, keys, p, low, high, position);
+      loader.read(words, ring, n, h);
       // the slot is free when it has been read
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       loader.issue(n + kAtStages, first[1]);
-      at_step<E, D>(a, queries, s, p, low, high, position);
+      at_values<E, D>(a, packed, words, keys.first, p, position);
     }
     dma_wait<0>();
   }
@@ -316,7 +361,7 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
     for (int m = 0; m < D / 16; m++)
       s_acc[((wave * 4 + i) * (D / 16) + m) * 64 + lane] = a.acc[m][i] * factor;     // (NaN stays)
   __syncthreads();
-  // (where blocks of results are formed, waves 4 to 7 do what 0 to 3 do: all meet at the barriers)
+  // (where blocks of results are formed, all waves meet at the barriers)
   if (wave >= 4 && (OUT::kSize != 0 || p.splits > 1)) return;
   float x[D / 16];
   const int i = wave & 3;
@@ -328,14 +373,230 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
     for (int m = 0; m < D / 16; m++) x[m] += s_acc[((k * 4 + i) * (D / 16) + m) * 64 + lane];
   if (p.splits > 1) {
     float *part = p.part + ((size_t)of_all * p.kv_heads + h) * at_part_floats<D>();
+    if (r.first + l16 < r.last) {
 #pragma unroll
-    for (int m = 0; m < D / 16; m++) part[(i * (D / 16) + m) * 64 + lane] = x[m];
+      for (int m = 0; m < D / 16; m++) part[(i * (D / 16) + m) * 64 + lane] = x[m];
+    }
     if (wave == 0 && lane < 16) part[16 * D + l16] = most, part[16 * D + 16 + l16] = whole;
     return;
   }
 #pragma unroll
   for (int m = 0; m < D / 16; m++) x[m] = whole == 0 ? 0.0f : x[m] / whole;
-  at_store<E, OUT, D>(p, r, h, i, x, s_most);
+  at_store<E, OUT, D>(p, r, h, i, x, s_most, wave < 4);
+}
+
+// The same for heads of 128 columns of which two, four or eight neighbours share a workgroup (HG), a wave each; where they
+// are fewer than eight, further waves have further steps. What these heads have of a token is one stretch of memory: a load
+// of 1 KB has 16 / HG tokens of all of them, lines whole, where a head's own rows come in pieces of 64 bytes and its
+// scales in pieces of four (a large copy's rate against 60 % of it, nothing but loads). Waves wait for
+// each other's loads at two barriers a step: when rows have landed, and when they are in registers.
+//
+// Piece k of a load, 16 bytes, lies at 16 k in LDS, and lanes choose theirs so that no read meets a bank twice, pieces of a
+// head's 64 bytes side by side: with k = 16 xh + 4 xl + c', t a token of the tile, c a piece of its head,
+//   keys    xl = (t ^ h) & 3, c' = c ^ t / 4    (a read has sixteen tokens, one c for each team of lanes)
+//   values  xl = (t / 4 ^ h') & 3, c' = c       (a read has four tokens 4 q + i and all c; h' = 2 h for HG = 2)
+// and xh what these leave open.
+template <int HG> struct AtHeads {
+  static constexpr int kWaves = 8, kGroups = kWaves / HG;       // groups of waves with steps of their own
+  static constexpr int kTile = HG * 1024, kScales = 4 * kTile;  // sixteen tokens' codes; keys, keys, values, values, scales
+  static constexpr int kGroup = kScales + HG * 256, kStage = kGroups * kGroup, kLoads = 5;
+  static constexpr int kTokens = 16 / HG;                       // of a load
+
+  // The token and head of piece group x (k / 4) of load j of a tile.
+  static __device__ __forceinline__ void key(int x, int j, int &t, int &h) {
+    const int xl = x & 3, xh = x >> 2;
+    if constexpr (HG == 8) t = 2 * j + (xh & 1), h = (xh >> 1) * 4 + (xl ^ (t & 3));
+    else if constexpr (HG == 4) h = xh, t = 4 * j + (xl ^ h);
+    else h = xh & 1, t = 8 * j + 4 * (xh >> 1) + (xl ^ h);
+  }
+  static __device__ __forceinline__ void value(int x, int j, int &t, int &h) {
+    const int xl = x & 3, xh = x >> 2;
+    if constexpr (HG == 8) t = 2 * j + (xh & 1), h = (xh >> 1) * 4 + (xl ^ (j >> 1));
+    else if constexpr (HG == 4) t = 4 * j + xh, h = xl ^ j;
+    else t = 8 * j + 4 * (xl & 1) + xh, h = (xl >> 1) ^ j;
+  }
+  // Where piece c of a token's head lies in a tile.
+  static __device__ __forceinline__ int key_place(int t, int h, int c) {
+    const int xl = (t ^ h) & 3, xh = HG == 8 ? (h >> 2) * 2 + (t & 1) : HG == 4 ? h : (t >> 2 & 1) * 2 + h;
+    return t / kTokens * 1024 + ((xh * 4 + xl) * 4 + (c ^ (t >> 2))) * 16;
+  }
+  static __device__ __forceinline__ int value_place(int t, int h, int c) {
+    const int xl = ((t >> 2) ^ (HG == 2 ? 2 * h : h)) & 3, xh = HG == 8 ? (h >> 2) * 2 + (t & 1) : t & 3;
+    return t / kTokens * 1024 + ((xh * 4 + xl) * 4 + c) * 16;
+  }
+  // How much further on token 4 q + i lies than token 4 q.
+  static __device__ __forceinline__ constexpr int value_next(int i) { return HG == 8 ? (i >> 1) * 1024 + (i & 1) * 256 : i * 256; }
+};
+
+template <class E, class OUT, int HG>
+__global__ __launch_bounds__(512, AtKind<E>::kQ == 6 ? 2 : 4) void mx4_attention_heads_kernel(Attention p, unsigned units) {
+  typedef AtHeads<HG> H;
+  constexpr int D = 128, TG = H::kGroups;
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_ring[];
+  __shared__ float s_top[8][16], s_sum[8][16];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), own = wave % HG, group = wave / HG;
+  const unsigned sets = (unsigned)p.kv_heads / HG;
+  const unsigned place = blockIdx.x >> 3, of_all = place / sets * 8 + (blockIdx.x & 7);
+  if (of_all >= units) return;
+  const int head0 = (int)(place % sets) * HG, h = head0 + own;
+  const int share = (int)(of_all % (unsigned)p.splits), slot = (int)(of_all / (unsigned)p.splits);
+  AtRows r;
+  if (!at_rows<16>(p, slot, r)) return;
+
+  const int at = min(r.first + l16, r.last - 1), token = at / p.group, head = h * p.group + (at - token * p.group);
+  auto position_of = [&](int row) { return max(r.length - r.count + row / p.group, -1); };
+  const int position = position_of(at), low = position_of(r.first), high = position_of(r.last - 1);
+  AtQueries<E, D> queries;
+  queries.load(reinterpret_cast<const typename E::T *>(p.q + (size_t)(r.begin + token) * p.q_row_bytes) + (size_t)head * D,
+               p.negative);
+  const AtTiles tiles = at_tiles(p, low, high);
+  const long long steps = (tiles.all + 1) / 2;
+  const int begin = (int)(steps * share / p.splits), end = (int)(steps * (share + 1) / p.splits);
+  AtState<E, D> a;
+  a.most = kAtNone, a.sum = 0;
+#pragma unroll
+  for (int m = 0; m < D / 16; m++) a.acc[m] = at_v4f{0, 0, 0, 0};
+
+  // what this lane asks for of each step, and where it finds its own
+  const uint32_t row_bytes = (uint32_t)p.c.row_bytes, ring = lds_address(s_ring) + (uint32_t)group * H::kGroup;
+  uint32_t key_at, value_at, scale_at;
+  // (scales: keys, keys, values or values of the step's two tiles)
+  const int array = HG == 2 ? own * 2 + (lane >> 5) : own * 64 / (16 * HG);
+  {
+    int t, of;
+    H::key(lane >> 2, own, t, of);
+    key_at = t * row_bytes + (uint32_t)(head0 + of) * 64 + ((lane & 3) ^ (t >> 2)) * 16;
+    H::value(lane >> 2, own, t, of);
+    value_at = t * row_bytes + (uint32_t)(head0 + of) * 64 + (lane & 3) * 16;
+    const int word = own * 64 + lane;            // of [4 arrays][16 tokens][HG heads]
+    scale_at = (word / HG % 16) * row_bytes + p.c.scales_at + (uint32_t)(head0 + word % HG) * 4;
+  }
+  const int key_place = H::key_place(l16, own, q);
+  const int value_place = H::value_place(4 * q, own, l16 >> 2) + (l16 & 3) * 4;
+  const int count = (end - begin + TG - 1) / TG;       // steps of every wave
+  int tile_of = -1;
+  auto issue = [&](int n, int (&first)[2]) {
+    if ((n & 31) == 0) {                               // the rows of 32 steps' tiles, a lane each
+      const long long step = begin + (long long)(n + (lane >> 1)) * TG + group;
+      const int u = (int)min(2 * step + (lane & 1), (long long)tiles.all);
+      tile_of = step < end && u < tiles.all ? cache_tile(p.c, r.sequence, (unsigned)tiles.at(u)) : -1;
+    }
+    const uint8_t *keys[2], *values[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int tile = __builtin_amdgcn_readlane(tile_of, 2 * (n & 31) + k);
+      first[k] = tile < 0 ? -1 : tiles.at(2 * (begin + n * TG + group) + k) * kCacheTile;
+      // (a tile that is not there reads the cache's first rows; there is a page)
+      const size_t base = (size_t)max(tile, 0) * kCacheTile * p.c.row_bytes;
+      keys[k] = p.c.keys + base, values[k] = p.c.values + base;
+    }
+    const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(ring + (n & 1) * H::kStage));
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      dma16(keys[k] + key_at, to + k * H::kTile + own * 1024);
+      dma16(values[k] + value_at, to + (2 + k) * H::kTile + own * 1024);
+    }
+    dma4((array == 0 ? keys[0] : array == 1 ? keys[1] : array == 2 ? values[0] : values[1]) + scale_at,
+         to + H::kScales + own * 256);
+  };
+  if (count > 0) {
+    int first[2][2];
+    issue(0, first[0]);
+    issue(1, first[1]);
+    for (int n = 0; n < count; n++) {
+      dma_wait<H::kLoads>();
+      __syncthreads();
+      const uint8_t *from = s_ring + (size_t)group * H::kGroup + (n & 1) * H::kStage;
+      const uint32_t *scales = reinterpret_cast<const uint32_t *>(from + H::kScales) + own;
+      AtKeys<D> keys;
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        keys.codes[k][0] = *reinterpret_cast<const at_v4i *>(from + k * H::kTile + key_place);
+        keys.scale[k][0] = reinterpret_cast<const uint8_t *>(scales + (k * 16 + l16) * HG)[q];
+        keys.first[k] = first[0][k];
+        first[0][k] = first[1][k];
+      }
+      const bool some = keys.first[0] >= 0 || keys.first[1] >= 0;
+      at_v4i packed[AtKind<E>::kP];
+      if (some) at_keys<E, D>(a, packed, queries, keys, p, low, high, position);
+      AtWords<D> words;
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          words.codes[0][k * 4 + i] = *reinterpret_cast<const uint32_t *>(from + (2 + k) * H::kTile + value_place + H::value_next(i));
+          words.scale[0][k * 4 + i] = reinterpret_cast<const uint8_t *>(scales + (32 + k * 16 + 4 * q + i) * HG)[l16 >> 2];
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __syncthreads();
+      issue(n + 2, first[1]);
+      if (some) at_values<E, D>(a, packed, words, keys.first, p, position);
+    }
+    dma_wait<0>();
+  }
+  float whole = add_across32(add_across16(a.sum));
+  if constexpr (TG > 1) {
+    // the first group's waves take what the others have; a wave that saw nothing has no part in it, and sums of NaN
+    // come without a largest score
+    float *const s_acc = reinterpret_cast<float *>(s_ring);
+    __syncthreads();
+    if (lane < 16) s_top[wave][l16] = a.most, s_sum[wave][l16] = whole;
+    __syncthreads();
+    auto factor_of = [&](float top, float of, float most) {
+      return top == kAtNone ? (of == 0 ? 0.0f : __builtin_nanf("")) : at_exp2(top - most);
+    };
+    float most = kAtNone;
+#pragma unroll
+    for (int k = 0; k < TG; k++) most = fmaxf(most, s_top[k * HG + own][l16]);
+    const float factor = factor_of(a.most, whole, most);
+#pragma unroll
+    for (int m = 0; m < D / 16; m++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) a.acc[m][i] *= factor;
+    if (group > 0) {
+#pragma unroll
+      for (int m = 0; m < D / 16; m++) *reinterpret_cast<at_v4f *>(s_acc + (((wave - HG) * (D / 16) + m) * 64 + lane) * 4) = a.acc[m];
+    }
+    __syncthreads();
+    if (group > 0) return;
+    whole = 0;
+#pragma unroll
+    for (int k = 0; k < TG; k++) whole += s_sum[k * HG + own][l16] * factor_of(s_top[k * HG + own][l16], s_sum[k * HG + own][l16], most);
+#pragma unroll
+    for (int k = 1; k < TG; k++)
+#pragma unroll
+      for (int m = 0; m < D / 16; m++)
+        a.acc[m] += *reinterpret_cast<const at_v4f *>(s_acc + ((((k - 1) * HG + own) * (D / 16) + m) * 64 + lane) * 4);
+    a.most = most;
+  }
+  if (p.splits == 1) {
+    at_store_whole<OUT, D>(p, r, h, a.acc, whole);
+    return;
+  }
+  float *part = p.part + ((size_t)of_all * p.kv_heads + h) * at_part_floats<D>();
+  if (r.first + l16 < r.last) {
+#pragma unroll
+    for (int m = 0; m < D / 16; m++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) part[(i * (D / 16) + m) * 64 + lane] = a.acc[m][i];
+  }
+  if (lane < 16) part[16 * D + l16] = a.most, part[16 * D + 16 + l16] = whole;
+}
+
+// How many heads of the cache a workgroup has.
+static int at_head_set(const Attention &p, int dim) {
+  return dim != 128 ? 1 : p.kv_heads % 8 == 0 ? 8 : p.kv_heads % 4 == 0 ? 4 : p.kv_heads % 2 == 0 ? 2 : 1;
+}
+template <class E, class OUT, int HG> static int at_heads_launch(const Attention &p, hipStream_t st) {
+  constexpr size_t kLds = 2 * AtHeads<HG>::kStage;
+  static_assert(kLds >= (8 - HG) * 16 * 128 * 4, "results of the other groups");
+  static std::atomic<uint64_t> attr_set{0};
+  auto kernel = mx4_attention_heads_kernel<E, OUT, HG>;
+  if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;
+  const unsigned units = (unsigned)((long long)p.slots * p.splits);
+  kernel<<<(units + 7) / 8 * 8 * (p.kv_heads / HG), 512, kLds, st>>>(p, units);
+  return check_launch("mx4_attention");
 }
 
 // Shares of a slot's tokens: as many as give each CU two workgroups, of `least` tokens at least.
@@ -350,6 +611,12 @@ static long long at_slots(size_t rows, size_t group, size_t sequences, int per_s
 template <class E, class OUT, int D> static int at_launch(Attention p, int type, bool prompt, int sixteens, hipStream_t st) {
   if (prompt) {
     if (int rc = at_prompt_launch(p, type, OUT::kSize == 0, D, st)) return rc;
+  } else if (D == 128 && at_head_set(p, D) > 1) {
+    const int set = at_head_set(p, D);
+    if (int rc = set == 8   ? at_heads_launch<E, OUT, 8>(p, st)
+                 : set == 4 ? at_heads_launch<E, OUT, 4>(p, st)
+                            : at_heads_launch<E, OUT, 2>(p, st))
+      return rc;
   } else {
     const unsigned units = (unsigned)((long long)p.slots * p.splits);
     constexpr size_t kLds = (size_t)kAtWaves<D> * std::max(16 * D * 4, kAtStages * AtRing<D>::kStage);
@@ -361,7 +628,7 @@ template <class E, class OUT, int D> static int at_launch(Attention p, int type,
   }
   if (p.splits == 1) return MI355X_OK;
   p.slots = sixteens;
-  mx4_attention_join_kernel<E, OUT, D><<<(unsigned)((long long)p.slots * p.kv_heads), 256, 0, st>>>(p);
+  mx4_attention_join_kernel<E, OUT, D><<<(unsigned)((long long)p.slots * p.kv_heads), 1024, 0, st>>>(p);
   return check_launch("mx4_attention");
 }
 static size_t at_part_bytes(size_t dim) { return (16 * dim + 32) * sizeof(float); }
@@ -397,7 +664,8 @@ static int at_plan(const mi355x_mx4_cache *cache, size_t heads, int type, size_t
   const long long tokens = std::min<long long>(p->most, (long long)p->window + p->sinks + per_slot + 48);
   // (slots that have rows: not many more than this)
   const long long filled = std::max<long long>(sequences, rows * p->group / per_slot);
-  p->splits = at_splits(filled * p->kv_heads, tokens, plan->prompt ? 512 : 256);
+  const int set = plan->prompt ? 1 : at_head_set(*p, (int)cache->head_dim);
+  p->splits = at_splits(filled * p->kv_heads / set, tokens, plan->prompt ? 512 : 256);
   if (p->splits > 1) plan->bytes = (size_t)sixteens * p->kv_heads * p->splits * at_part_bytes(cache->head_dim);
   return MI355X_OK;
 }

@@ -85,12 +85,12 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
   }
   auto locate = [&](int step) {
     const int u = step * kPromptTiles + wave;
-    return u < tiles.all ? cache_tile_row(p.c, r.sequence, (unsigned)tiles.at(u)) : -1ll;
+    return u < tiles.all ? cache_tile(p.c, r.sequence, (unsigned)tiles.at(u)) : -1;
   };
-  auto load = [&](PromptTile<D> &t, long long row, int step) {
-    t.first = row < 0 ? -1 : tiles.at(step * kPromptTiles + wave) * kCacheTile;
+  auto load = [&](PromptTile<D> &t, int tile, int step) {
+    t.first = tile < 0 ? -1 : tiles.at(step * kPromptTiles + wave) * kCacheTile;
     // (a tile that is not there reads the cache's first rows; there is a page)
-    const size_t base = (size_t)max(row, 0ll) * p.c.row_bytes;
+    const size_t base = (size_t)max(tile, 0) * kCacheTile * p.c.row_bytes;
     const uint8_t *keys = p.c.keys + base, *values = p.c.values + base;
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
@@ -142,13 +142,13 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
   };
 
   PromptTile<D> next;
-  long long row = -1;
+  int coming = -1;
   if (begin < end) {
     load(next, locate(begin), begin);
     store(next, lds[0]);
     if (begin + 1 < end) {
       load(next, locate(begin + 1), begin + 1);
-      if (begin + 2 < end) row = locate(begin + 2);
+      if (begin + 2 < end) coming = locate(begin + 2);
     }
   }
   __syncthreads();
@@ -157,8 +157,8 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
     if (step + 1 < end) {
       store(next, lds[(step - begin + 1) & 1]);
       if (step + 2 < end) {
-        load(next, row, step + 2);
-        if (step + 3 < end) row = locate(step + 3);
+        load(next, coming, step + 2);
+        if (step + 3 < end) coming = locate(step + 3);
       }
     }
     int first[kPromptTiles];

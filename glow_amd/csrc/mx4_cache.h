@@ -29,14 +29,14 @@ __device__ __forceinline__ unsigned divide(unsigned a, unsigned d, unsigned magi
   const unsigned e = __umulhi(a, magic);
   return e + (a - e * d >= d);
 }
-// The row of the cache where a tile of sixteen tokens of a sequence begins; -1: on no page.
-__device__ __forceinline__ long long cache_tile_row(const MxCache &c, int sequence, unsigned tile) {
+// Which sixteen rows of the cache a tile of sixteen tokens of a sequence has; -1: on no page.
+__device__ __forceinline__ int cache_tile(const MxCache &c, int sequence, unsigned tile) {
   const unsigned k = divide(tile, c.page_tiles, c.page_magic);
   if (k >= c.per_sequence) return -1;
   const size_t slot = (size_t)sequence * c.per_sequence + k;
   const size_t page = c.pages ? (size_t)(unsigned)c.pages[slot] : slot;   // (negative ones: past the last)
   if (page >= c.n_pages) return -1;
-  return ((long long)page * c.page_tiles + (tile - k * c.page_tiles)) * kCacheTile;
+  return (int)((unsigned)page * c.page_tiles + (tile - k * c.page_tiles));
 }
 
 __device__ __forceinline__ int batch_start(const MxCache &c, int s) { return min(max(c.starts[s], 0), c.rows); }
@@ -79,10 +79,9 @@ inline int check_cache(const char *what, const mi355x_mx4_cache *cache, MxCache 
                  "%s: the cache's addresses and the distance between rows have to be multiples of 16", what);
   MI355X_REQUIRE((uintptr_t)cache->pages % 4 == 0, "%s: the pages have to lie on a multiple of 4", what);
   MI355X_REQUIRE(cache->n_pages == 0 || (cache->keys && cache->values), "%s: NULL", what);
-  // (2^32 pages of 2^31 tokens of 2^26 bytes pass 64 bits)
-  const unsigned __int128 span = (unsigned __int128)cache->n_pages * cache->page_tokens * cache->row_bytes;
-  MI355X_REQUIRE(span <= PTRDIFF_MAX, "%s: %u pages of %u tokens %llu bytes apart", what, cache->n_pages,
-                 cache->page_tokens, (unsigned long long)cache->row_bytes);
+  if ((uint64_t)cache->n_pages * (cache->page_tokens / kCacheTile) > 0x7fffffff)
+    return fail(MI355X_ERR_NOT_SUPPORTED, "%s: %u pages of %u tokens, up to 2^35 - 16 rows are supported", what,
+                cache->n_pages, cache->page_tokens);
   c->keys = cache->keys;
   c->values = cache->values;
   c->row_bytes = cache->row_bytes;

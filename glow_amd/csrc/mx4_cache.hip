@@ -23,9 +23,9 @@ __global__ __launch_bounds__(kCacheThreads) void mx4_cache_write_kernel(MxCache 
     const int length = min(max(c.lengths[s], 0), c.capacity);
     const int t = length - (end - begin) + (r - begin);
     if (t < 0 || t >= length) continue;
-    const long long row = cache_tile_row(c, s, (unsigned)t / kCacheTile);
-    if (row < 0) continue;
-    uint8_t *dst = (is_value ? c.values : c.keys) + (size_t)(row + t % kCacheTile) * c.row_bytes;
+    const int tile = cache_tile(c, s, (unsigned)t / kCacheTile);
+    if (tile < 0) continue;
+    uint8_t *dst = (is_value ? c.values : c.keys) + ((size_t)tile * kCacheTile + t % kCacheTile) * c.row_bytes;
     const uint8_t *src = is_value ? values + (size_t)r * values_row_bytes : keys + (size_t)r * keys_row_bytes;
     if constexpr (E::kSize == 0) {
       reinterpret_cast<uint32_t *>(dst + (size_t)g * kMxGroupBytes)[l] =
