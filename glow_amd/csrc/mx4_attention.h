@@ -7,9 +7,9 @@
 //
 //   S   16 tokens x 16 queries by the scaled instruction over 128 columns: codes and scale bytes of
 //       the keys as they lie in memory (a lane has one block of a token), queries as sums of 6-bit
-//       floats (E2M3, four bits each) with a power of two for each block of 32: 3 terms for bf16, 4 for
-//       fp16, 6 for fp32. Nothing of a key is ever converted. A lane gets tokens 4 q .. 4 q + 3. 8-bit terms
-//       would be fewer (2, 3, 6) of twice the time each, and the instruction cuts small products off
+//       floats (E2M3, four bits each) with a power of two for each block of 32: 3 terms for 16-bit types,
+//       6 for fp32. Nothing of a key is ever converted. A lane gets tokens 4 q .. 4 q + 3. 8-bit terms
+//       would be as many (2, 3, 6) of twice the time each, and the instruction cuts small products off
 //       where exponents lie far apart (2^-17 of the sum; 6-bit products come out exact).
 //   P   is what the lane then holds of two tiles of tokens: eight weights of its query, which is what the
 //       16x16x32 instruction wants of its second operand, tokens in the order 4 q + i of the first
@@ -50,7 +50,8 @@ struct Attention {
   int kv_heads, group;            // heads of queries to one of the cache
   int most;                       // tokens of a sequence
   int window, sinks;
-  int slots, splits;
+  int slots, splits;              // splits: shares of a slot's tokens at most
+  int target;                     // shares in all that are to run at once; 0: every slot has all of its shares
   int out_groups;                 // of a microscaled result's row
   float scale;                    // |scale| * log2(e)
   int negative;                   // of the scale
@@ -62,7 +63,7 @@ constexpr float kAtNone = -__builtin_inff();
 // Terms of a query, terms of a weight, what weights are shifted up by, and the least scale byte of values that count
 // as NaN: 2^14 times 4 is past fp16's range.
 template <class E> struct AtKind { static constexpr int kQ = 6, kP = 3, kNan = 255; static constexpr float kUp = 0; };
-template <> struct AtKind<F16> { static constexpr int kQ = 4, kP = 1, kNan = 141; static constexpr float kUp = 7; };
+template <> struct AtKind<F16> { static constexpr int kQ = 3, kP = 1, kNan = 141; static constexpr float kUp = 7; };
 template <> struct AtKind<BF16> { static constexpr int kQ = 3, kP = 1, kNan = 255; static constexpr float kUp = 0; };
 
 // Which rows a slot of sixteen has. Slots of a sequence begin at floor(start * group / 16) + its number, which leaves
@@ -76,16 +77,28 @@ template <int ROWS> __device__ __forceinline__ long long at_first_slot(const Att
   return (long long)batch_start(p.c, s) * p.group / ROWS + s;
 }
 template <int ROWS> __device__ __forceinline__ bool at_rows(const Attention &p, int slot, AtRows &r) {
-  r.sequence = __builtin_amdgcn_readfirstlane(
-      find_sequence<64>(p.c.sequences, slot, [&](int s) { return at_first_slot<ROWS>(p, s); }));
-  r.begin = batch_start(p.c, r.sequence);
-  r.count = max(batch_start(p.c, r.sequence + 1) - r.begin, 0);
-  const long long at = (slot - at_first_slot<ROWS>(p, r.sequence)) * ROWS;
+  int length;
+  if (p.c.sequences < 64) {                       // one round of loads, a sequence a lane
+    const int lane = threadIdx.x & 63, s = min(lane, p.c.sequences);
+    const int start = batch_start(p.c, s), tokens = p.c.lengths[min(s, p.c.sequences - 1)];
+    const unsigned long long fits = __ballot(lane < p.c.sequences && (long long)start * p.group / ROWS + lane <= slot);
+    r.sequence = fits ? 63 - __clzll((long long)fits) : 0;
+    r.begin = __builtin_amdgcn_readlane(start, r.sequence);
+    r.count = max(__builtin_amdgcn_readlane(start, r.sequence + 1) - r.begin, 0);
+    length = __builtin_amdgcn_readlane(tokens, r.sequence);
+  } else {
+    r.sequence = __builtin_amdgcn_readfirstlane(
+        find_sequence<64>(p.c.sequences, slot, [&](int s) { return at_first_slot<ROWS>(p, s); }));
+    r.begin = batch_start(p.c, r.sequence);
+    r.count = max(batch_start(p.c, r.sequence + 1) - r.begin, 0);
+    length = p.c.lengths[r.sequence];
+  }
+  const long long at = (slot - ((long long)r.begin * p.group / ROWS + r.sequence)) * ROWS;
   const int all = r.count * p.group;
   if (at < 0 || at >= all) return false;
   r.first = (int)at;
   r.last = min(all, r.first + ROWS);
-  r.length = min(max(p.c.lengths[r.sequence], 0), p.most);
+  r.length = min(max(length, 0), p.most);
   return true;
 }
 // The tiles of tokens that rows at `low` to `high` see some of: those of the first `sinks`, then [from, ..).
@@ -102,6 +115,21 @@ __device__ __forceinline__ AtTiles at_tiles(const Attention &p, int low, int hig
   return t;
 }
 
+// Steps of 32 tokens in a share of a slot that has `steps`: what gives all sequences together `target` shares, so that long
+// and short ones have shares of a size, but `least` steps at least and no more than `splits` shares. (Lengths of over
+// 1024 sequences are not looked through.)
+__device__ __forceinline__ int at_share_steps(const Attention &p, int steps, int least) {
+  int chunk = max((int)(((long long)steps + p.splits - 1) / p.splits), least);
+  if (p.target && p.c.sequences <= 1024) {
+    float all = 0;                                  // (in steps; equal in all waves of all launches)
+    const long long most = (long long)p.window + p.sinks;
+    for (int i = threadIdx.x & 63; i < p.c.sequences; i += 64)
+      all += (float)((min((long long)min(max(p.c.lengths[i], 0), p.most), most) + 31) / 32);
+    chunk = max(chunk, (int)fminf(__builtin_ceilf(wave_sum(all) / (float)p.target), 1e9f));
+  }
+  return __builtin_amdgcn_readfirstlane(chunk);
+}
+
 // ---- queries -----------------------------------------------------------------------
 
 // Sixteen rows of queries of D columns as sums of 6-bit floats: 32 q to 32 q + 31 of 128 columns are lane q's, a block
@@ -110,7 +138,7 @@ __device__ __forceinline__ AtTiles at_tiles(const Attention &p, int low, int hig
 template <class E, int D> struct AtQueries {
   static constexpr int kTerms = AtKind<E>::kQ, kChunks = (D + 127) / 128;
   at_v6u codes[kChunks][kTerms];
-  int scale[kChunks][kTerms];
+  int scale[kChunks][(kTerms + 3) / 4];          // a byte a term
 
   __device__ __forceinline__ void load(const typename E::T *row, bool negative) {
     const int q = (threadIdx.x & 63) >> 4;
@@ -133,6 +161,8 @@ template <class E, int D> struct AtQueries {
       }
       const int exponent = (int)(most >> 23);
 #pragma unroll
+      for (int w = 0; w < (kTerms + 3) / 4; w++) scale[c][w] = 0;
+#pragma unroll
       for (int t = 0; t < kTerms; t++) {
         const int byte = max(exponent - 2 - 4 * t, 1);
         const float s = __uint_as_float((uint32_t)byte << 23);
@@ -145,17 +175,24 @@ template <class E, int D> struct AtQueries {
           for (int j = 0; j < 16; j++) even[j] -= back[2 * j], odd[j] -= back[2 * j + 1];    // (exact)
         }
         codes[c][t] = six;
-        scale[c][t] = exponent == 255 ? 255 : byte;
+        scale[c][t / 4] |= (exponent == 255 ? 255 : byte) << (8 * (t % 4));
       }
     }
   }
 };
 
-// Scores of sixteen tokens, 4 bits by 6.
-__device__ __forceinline__ at_v4f at_scores(at_v4i keys, int key_scale, at_v6u q, int q_scale, at_v4f acc) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-      at_v8i{keys[0], keys[1], keys[2], keys[3], 0, 0, 0, 0},
-      at_v8i{(int)q[0], (int)q[1], (int)q[2], (int)q[3], (int)q[4], (int)q[5], 0, 0}, acc, 4, 2, 0, key_scale, 0, q_scale);
+// Scores of sixteen tokens, 4 bits by 6, of all terms of 128 columns.
+template <int T, int TERMS>
+__device__ __forceinline__ at_v4f at_scores(at_v4i keys, int key_scale, const at_v6u (&q)[TERMS], const int (&scale)[(TERMS + 3) / 4],
+                                            at_v4f acc) {
+  if constexpr (T == TERMS) return acc;
+  else {
+    const at_v4f sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+        at_v8i{keys[0], keys[1], keys[2], keys[3], 0, 0, 0, 0},
+        at_v8i{(int)q[T][0], (int)q[T][1], (int)q[T][2], (int)q[T][3], (int)q[T][4], (int)q[T][5], 0, 0}, acc, 4, 2, 0, key_scale,
+        T % 4, scale[T / 4]);
+    return at_scores<T + 1, TERMS>(keys, key_scale, q, scale, sum);
+  }
 }
 
 // ---- weights and values --------------------------------------------------------------
@@ -387,8 +424,8 @@ __device__ __forceinline__ void at_store(const Attention &p, const AtRows &r, in
 }
 
 // What a share of a slot of sixteen rows leaves: its results, component by component, then the largest score and the sum
-// of each query.
-template <int D> __device__ __forceinline__ constexpr size_t at_part_floats() { return 16 * D + 32; }
+// of each query; the first share how many there are, too.
+template <int D> __device__ __forceinline__ constexpr size_t at_part_floats() { return 16 * D + 48; }
 
 // The whole of a slot's results by one wave: a lane has the components of its query side by side.
 template <class OUT, int D>

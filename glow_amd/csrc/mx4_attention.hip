@@ -13,6 +13,7 @@ namespace mi355x {
 // the values in row q + 4 i, so that word i of a lane lies at 64 i + lane.
 template <int D> constexpr int kAtWaves = D == 256 ? 4 : 8;
 constexpr int kAtStages = 2;
+constexpr int kAtLeast = 8;            // steps of a share at least
 
 template <int D> struct AtRing {
   static constexpr int kTile = 8 * D;                    // bytes of sixteen tokens' codes
@@ -165,9 +166,7 @@ __device__ __forceinline__ void at_keys(AtState<E, D> &a, at_v4i (&packed)[AtKin
       at_v4i codes = s.codes[k][c];
       int byte = s.scale[k][c];
       if (D == 64 && q >= 2) codes = at_v4i{0, 0, 0, 0}, byte = 127;
-#pragma unroll
-      for (int t = 0; t < AtKind<E>::kQ; t++)
-        r = at_scores(codes, byte, queries.codes[c][t], queries.scale[c][t], r);
+      r = at_scores<0>(codes, byte, queries.codes[c], queries.scale[c], r);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) score[k * 4 + i] = r[i];
@@ -230,56 +229,76 @@ __device__ __forceinline__ void at_values(AtState<E, D> &a, const at_v4i (&packe
   }
 }
 
-// The shares of sixteen rows joined, and what is done with the whole: wave 4 g + i has component i of every fourth share,
-// from the g-th on, and the four meet in LDS.
-template <class E, class OUT, int D>
-__global__ __launch_bounds__(1024) void mx4_attention_join_kernel(Attention p) {
-  __shared__ float s_x[12][D / 16][64], s_sum[4][16];
+// The shares of sixteen rows joined, and what is done with the whole: wave 4 g + i has component i of every G-th share,
+// from the g-th on, and these meet in LDS.
+template <class E, class OUT, int D, int G>
+__global__ __launch_bounds__(256 * G) void mx4_attention_join_kernel(Attention p) {
+  __shared__ float s_x[G > 1 ? 4 * G - 4 : 1][D / 16][64], s_sum[G][16];
   __shared__ uint32_t s_most[4][64];
-  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = wave & 3, g = wave >> 2;
   const int h = (int)(blockIdx.x % (unsigned)p.kv_heads), slot = (int)(blockIdx.x / (unsigned)p.kv_heads);
-  AtRows r;
-  if (!at_rows<16>(p, slot, r)) return;
   const float *part = p.part + ((size_t)slot * p.splits * p.kv_heads + h) * at_part_floats<D>();
   const size_t next = (size_t)p.kv_heads * at_part_floats<D>();
+  // the first share says how many there are; a single one has stored the whole
+  const int shares = p.target ? (int)part[16 * D + 32] : p.splits;
+  AtRows r;
+  if (!at_rows<16>(p, slot, r) || shares <= 1) return;
   const bool there = r.first + l16 < r.last;
-  float most = kAtNone;
-  for (int k = q; k < p.splits; k += 4) most = fmaxf(most, there ? part[k * next + 16 * D + l16] : kAtNone);
-  most = at_max(most);
-  float sum = 0, x[D / 16];
+  float most = kAtNone, sum = 0, x[D / 16];
 #pragma unroll
   for (int m = 0; m < D / 16; m++) x[m] = 0;
   if (there) {
-#pragma unroll 2
-    for (int k = g; k < p.splits; k += 4) {
+#pragma unroll 4
+    for (int k = g; k < shares; k += G) {
       const float *from = part + k * next;
       const float of = from[16 * D + l16], weight = from[16 * D + 16 + l16];
       float y[D / 16];
 #pragma unroll
       for (int m = 0; m < D / 16; m++) y[m] = from[(i * (D / 16) + m) * 64 + lane];
-      const float factor = of == kAtNone ? (weight == 0 ? 0.0f : __builtin_nanf("")) : at_exp2(of - most);
-      sum += weight * factor;
+      const float top = fmaxf(most, of);
+      // (sums of NaN come without a largest score)
+      const float before = most == kAtNone ? 1.0f : at_exp2(most - top);
+      const float factor = of == kAtNone ? (weight == 0 ? 0.0f : __builtin_nanf("")) : at_exp2(of - top);
+      sum = sum * before + weight * factor;
 #pragma unroll
-      for (int m = 0; m < D / 16; m++) x[m] += y[m] * factor;
+      for (int m = 0; m < D / 16; m++) x[m] = x[m] * before + y[m] * factor;
+      most = top;
     }
   }
-  if (g > 0) {
+  if (G > 1) {
+    __shared__ float s_top[G][16];
+    if (i == 0 && lane < 16) s_top[g][l16] = most;
+    __syncthreads();
+    float top = kAtNone;
 #pragma unroll
-    for (int m = 0; m < D / 16; m++) s_x[wave - 4][m][lane] = x[m];
+    for (int k = 0; k < G; k++) top = fmaxf(top, s_top[k][l16]);
+    const float factor = most == kAtNone ? 1.0f : at_exp2(most - top);
+    sum *= factor;
+#pragma unroll
+    for (int m = 0; m < D / 16; m++) x[m] *= factor;
   }
-  if (i == 0 && lane < 16) s_sum[g][l16] = sum;
-  __syncthreads();
-  // (where blocks of results are formed, all waves meet at the barriers)
-  if (g > 0 && OUT::kSize != 0) return;
-  sum = s_sum[0][l16] + s_sum[1][l16] + s_sum[2][l16] + s_sum[3][l16];
+  if (G > 1) {
+    if (g > 0) {
 #pragma unroll
-  for (int m = 0; m < D / 16; m++) {
-    if (g == 0)
+      for (int m = 0; m < D / 16; m++) s_x[wave - 4][m][lane] = x[m];
+    }
+    if (i == 0 && lane < 16) s_sum[g][l16] = sum;
+    __syncthreads();
+    // (where blocks of results are formed, all waves meet at the barriers)
+    if (g > 0 && OUT::kSize != 0) return;
+    sum = 0;
 #pragma unroll
-      for (int k = 0; k < 3; k++) x[m] += s_x[k * 4 + i][m][lane];
-    x[m] = sum == 0 ? 0.0f : x[m] / sum;
+    for (int k = 0; k < G; k++) sum += s_sum[k][l16];
+    if (g == 0) {
+#pragma unroll
+      for (int k = 1; k < G; k++)
+#pragma unroll
+        for (int m = 0; m < D / 16; m++) x[m] += s_x[(k - 1) * 4 + i][m][lane];
+    }
   }
+#pragma unroll
+  for (int m = 0; m < D / 16; m++) x[m] = sum == 0 ? 0.0f : x[m] / sum;
   at_store<E, OUT, D>(p, r, h, i, x, s_most, g == 0);
 }
 
@@ -310,8 +329,13 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
                p.negative);
 
   const AtTiles tiles = at_tiles(p, low, high);
-  const long long steps = (tiles.all + 1) / 2;
-  const int begin = (int)(steps * share / p.splits), end = (int)(steps * (share + 1) / p.splits);
+  const int steps = (int)((tiles.all + 1ll) / 2), chunk = at_share_steps(p, steps, kAtLeast);
+  const int begin = (int)min((long long)share * chunk, (long long)steps), end = (int)min((long long)begin + chunk, (long long)steps);
+  const bool alone = steps <= chunk;            // (a slot without tokens is the first share's)
+  if (share > 0 && begin >= steps) return;
+  // (the joining launch asks how many shares there are; every wave of a head's tells it the same)
+  if (share == 0 && p.splits > 1 && lane == 0)
+    p.part[((size_t)of_all * p.kv_heads + h) * at_part_floats<D>() + 16 * D + 32] = alone ? 1.0f : (float)(((long long)steps + chunk - 1) / chunk);
   AtState<E, D> a;
   a.most = kAtNone, a.sum = 0;
 #pragma unroll
@@ -332,6 +356,7 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
       keys.first[0] = first[0][0], keys.first[1] = first[0][1];
       first[0][0] = first[1][0], first[0][1] = first[1][1];
       at_keys<E, D>(a, packed, queries, keys, p, low, high, position);
+      asm volatile("" ::: "memory");                   // (not read before the keys' registers are free)
       loader.read(words, ring, n, h);
       // the slot is free when it has been read
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -362,7 +387,7 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
       s_acc[((wave * 4 + i) * (D / 16) + m) * 64 + lane] = a.acc[m][i] * factor;     // (NaN stays)
   __syncthreads();
   // (where blocks of results are formed, all waves meet at the barriers)
-  if (wave >= 4 && (OUT::kSize != 0 || p.splits > 1)) return;
+  if (wave >= 4 && (OUT::kSize != 0 || !alone)) return;
   float x[D / 16];
   const int i = wave & 3;
 #pragma unroll
@@ -371,7 +396,7 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
   for (int k = 0; k < WAVES; k++)
 #pragma unroll
     for (int m = 0; m < D / 16; m++) x[m] += s_acc[((k * 4 + i) * (D / 16) + m) * 64 + lane];
-  if (p.splits > 1) {
+  if (!alone) {
     float *part = p.part + ((size_t)of_all * p.kv_heads + h) * at_part_floats<D>();
     if (r.first + l16 < r.last) {
 #pragma unroll
@@ -451,8 +476,13 @@ __global__ __launch_bounds__(512, AtKind<E>::kQ == 6 ? 2 : 4) void mx4_attention
   queries.load(reinterpret_cast<const typename E::T *>(p.q + (size_t)(r.begin + token) * p.q_row_bytes) + (size_t)head * D,
                p.negative);
   const AtTiles tiles = at_tiles(p, low, high);
-  const long long steps = (tiles.all + 1) / 2;
-  const int begin = (int)(steps * share / p.splits), end = (int)(steps * (share + 1) / p.splits);
+  const int steps = (int)((tiles.all + 1ll) / 2), chunk = at_share_steps(p, steps, kAtLeast);
+  const int begin = (int)min((long long)share * chunk, (long long)steps), end = (int)min((long long)begin + chunk, (long long)steps);
+  const bool alone = steps <= chunk;            // (a slot without tokens is the first share's)
+  if (share > 0 && begin >= steps) return;
+  // (the joining launch asks how many shares there are; every wave of a head's tells it the same)
+  if (share == 0 && p.splits > 1 && lane == 0)
+    p.part[((size_t)of_all * p.kv_heads + h) * at_part_floats<D>() + 16 * D + 32] = alone ? 1.0f : (float)(((long long)steps + chunk - 1) / chunk);
   AtState<E, D> a;
   a.most = kAtNone, a.sum = 0;
 #pragma unroll
@@ -492,6 +522,8 @@ __global__ __launch_bounds__(512, AtKind<E>::kQ == 6 ? 2 : 4) void mx4_attention
       keys[k] = p.c.keys + base, values[k] = p.c.values + base;
     }
     const uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(ring + (n & 1) * H::kStage));
+    // (added to each step's addresses, not kept as 64-bit sums with the cache's: registers)
+    asm volatile("" : "+v"(key_at), "+v"(value_at), "+v"(scale_at));
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       dma16(keys[k] + key_at, to + k * H::kTile + own * 1024);
@@ -504,29 +536,32 @@ __global__ __launch_bounds__(512, AtKind<E>::kQ == 6 ? 2 : 4) void mx4_attention
     int first[2][2];
     issue(0, first[0]);
     issue(1, first[1]);
+    int key_from = key_place, value_from = value_place, key_scale = l16 * HG * 4 + q, value_scale = (32 + 4 * q) * HG * 4 + (l16 >> 2);
     for (int n = 0; n < count; n++) {
+      asm volatile("" : "+v"(key_from), "+v"(value_from), "+v"(key_scale), "+v"(value_scale));
       dma_wait<H::kLoads>();
       __syncthreads();
       const uint8_t *from = s_ring + (size_t)group * H::kGroup + (n & 1) * H::kStage;
-      const uint32_t *scales = reinterpret_cast<const uint32_t *>(from + H::kScales) + own;
+      const uint8_t *scales = from + H::kScales + own * 4;
       AtKeys<D> keys;
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        keys.codes[k][0] = *reinterpret_cast<const at_v4i *>(from + k * H::kTile + key_place);
-        keys.scale[k][0] = reinterpret_cast<const uint8_t *>(scales + (k * 16 + l16) * HG)[q];
+        keys.codes[k][0] = *reinterpret_cast<const at_v4i *>(from + k * H::kTile + key_from);
+        keys.scale[k][0] = scales[k * 64 * HG + key_scale];
         keys.first[k] = first[0][k];
         first[0][k] = first[1][k];
       }
       const bool some = keys.first[0] >= 0 || keys.first[1] >= 0;
       at_v4i packed[AtKind<E>::kP];
       if (some) at_keys<E, D>(a, packed, queries, keys, p, low, high, position);
+      asm volatile("" ::: "memory");                   // (not read before the keys' registers are free)
       AtWords<D> words;
 #pragma unroll
       for (int k = 0; k < 2; k++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          words.codes[0][k * 4 + i] = *reinterpret_cast<const uint32_t *>(from + (2 + k) * H::kTile + value_place + H::value_next(i));
-          words.scale[0][k * 4 + i] = reinterpret_cast<const uint8_t *>(scales + (32 + k * 16 + 4 * q + i) * HG)[l16 >> 2];
+          words.codes[0][k * 4 + i] = *reinterpret_cast<const uint32_t *>(from + (2 + k) * H::kTile + H::value_next(i) + value_from);
+          words.scale[0][k * 4 + i] = scales[(k * 16 + i) * 4 * HG + value_scale];
         }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __syncthreads();
@@ -570,7 +605,7 @@ __global__ __launch_bounds__(512, AtKind<E>::kQ == 6 ? 2 : 4) void mx4_attention
         a.acc[m] += *reinterpret_cast<const at_v4f *>(s_acc + ((((k - 1) * HG + own) * (D / 16) + m) * 64 + lane) * 4);
     a.most = most;
   }
-  if (p.splits == 1) {
+  if (alone) {
     at_store_whole<OUT, D>(p, r, h, a.acc, whole);
     return;
   }
@@ -601,7 +636,7 @@ template <class E, class OUT, int HG> static int at_heads_launch(const Attention
 
 // Shares of a slot's tokens: as many as give each CU two workgroups, of `least` tokens at least.
 static int at_splits(long long units, long long tokens, long long least) {
-  const long long fill = (512 + units - 1) / units, most = (tokens + least - 1) / least;
+  const long long fill = 512 / units, most = (tokens + least - 1) / least;
   return (int)std::max(1ll, std::min({fill, most, 256ll}));
 }
 static long long at_slots(size_t rows, size_t group, size_t sequences, int per_slot) {
@@ -628,10 +663,12 @@ template <class E, class OUT, int D> static int at_launch(Attention p, int type,
   }
   if (p.splits == 1) return MI355X_OK;
   p.slots = sixteens;
-  mx4_attention_join_kernel<E, OUT, D><<<(unsigned)((long long)p.slots * p.kv_heads), 1024, 0, st>>>(p);
+  const unsigned blocks = (unsigned)((long long)p.slots * p.kv_heads);
+  if (p.splits > 16) mx4_attention_join_kernel<E, OUT, D, 4><<<blocks, 1024, 0, st>>>(p);
+  else mx4_attention_join_kernel<E, OUT, D, 1><<<blocks, 256, 0, st>>>(p);
   return check_launch("mx4_attention");
 }
-static size_t at_part_bytes(size_t dim) { return (16 * dim + 32) * sizeof(float); }
+static size_t at_part_bytes(size_t dim) { return (16 * dim + 48) * sizeof(float); }
 
 // How a call is cut, which does not depend on where its tensors lie.
 struct AtPlan {
@@ -665,7 +702,10 @@ static int at_plan(const mi355x_mx4_cache *cache, size_t heads, int type, size_t
   // (slots that have rows: not many more than this)
   const long long filled = std::max<long long>(sequences, rows * p->group / per_slot);
   const int set = plan->prompt ? 1 : at_head_set(*p, (int)cache->head_dim);
-  p->splits = at_splits(filled * p->kv_heads / set, tokens, plan->prompt ? 512 : 256);
+  p->splits = at_splits(filled * p->kv_heads / set, tokens, plan->prompt ? 512 : 32 * kAtLeast);
+  // (no more shares than run at once: a few more would run alone, and a workgroup that finds nothing to do still takes
+  // a place for a while: twice the shares, half of them without tokens, 165 us for 134 over 4 x 115 000 tokens)
+  if (!plan->prompt && p->splits > 1) p->target = (int)std::max<long long>(filled, 512 / (p->kv_heads / set) - filled);
   if (p->splits > 1) plan->bytes = (size_t)sixteens * p->kv_heads * p->splits * at_part_bytes(cache->head_dim);
   return MI355X_OK;
 }

@@ -194,9 +194,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
         for (int c = 0; c < kChunks; c++) {
           const at_v4i codes = now.keys[k][c][lane];
           const int byte = now.key_scale[k][c][lane];
-#pragma unroll
-          for (int term = 0; term < AtKind<E>::kQ; term++)
-            s = at_scores(codes, byte, queries[t].codes[c][term], queries[t].scale[c][term], s);
+          s = at_scores<0>(codes, byte, queries[t].codes[c], queries[t].scale[c], s);
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) score[k * 4 + i] = s[i];

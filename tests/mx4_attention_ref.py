@@ -55,14 +55,14 @@ def attention(b, q, heads, type_, scale=None, window=0, sinks=0, max_length=None
     """(results [rows, heads * dim], bound of the error before the result's own rounding, rows that belong to a
     sequence) for q in 64 bits.
 
-    A query is a sum of 3 (bf16), 4 (fp16) or 6 (fp32) terms of four bits, each of which leaves a sixteenth of the block's
+    A query is a sum of 3 (16-bit types) or 6 (fp32) terms of four bits, each of which leaves a sixteenth of the block's
     largest at most. Scores are D products a term in any order and the sums of the terms, in 32 bits; a weight's exponent is
     rounded at the size of its score and of the largest, twice, and 2^x within 2^-22. Weights are rounded to the type, in fp16
     shifted so that the smallest step is 2^-32 of the largest weight; in fp32 to 24 bits."""
     d, group = b.head_dim, heads // b.kv_heads
     scale = d ** -0.5 if scale is None else scale
     half = {ref.F32: 2.0 ** -24, ref.F16: 2.0 ** -11, ref.BF16: 2.0 ** -8}[type_]
-    cut = {ref.F32: 2.0 ** -24, ref.F16: 2.0 ** -16, ref.BF16: 2.0 ** -12}[type_]
+    cut = 2.0 ** -24 if type_ == ref.F32 else 2.0 ** -12
     out, err = np.zeros((b.rows, heads, d)), np.zeros((b.rows, heads, d))
     used = np.zeros(b.rows, bool)
     q = q.reshape(b.rows, heads, d)
