@@ -38,44 +38,85 @@ struct MxAdapters {
   const int32_t *of_row;
   int type, rank, ranks, count;    // ranks: rank up to a multiple of 32, the rest zeros
 
-  // Eight ranks of a row of up, as terms.
-  template <class E, int TERMS> __device__ __forceinline__ void load_up(v4i (&u)[TERMS], size_t row, int r) const {
+  // Eight ranks of a row of up; zeros behind the last.
+  template <class E> __device__ __forceinline__ typename E::Eight load_up(size_t row, int r) const {
     const typename E::T *at = reinterpret_cast<const typename E::T *>(up) + row * rank + r;
-    float x[8];
-    if (r + 8 <= rank) load8<E>(x, at);
-    else load8_end<E>(x, at, rank - r);
-    ad_split<TERMS>(u, x);
+    return r + 8 <= rank ? load_eight<E>(at) : load_eight_end<E>(at, rank - r);
+  }
+  template <class E, int TERMS> static __device__ __forceinline__ void split(v4i (&u)[TERMS], const typename E::Eight &e) {
+    if constexpr (std::is_same<E, BF16>::value) u[0] = __builtin_bit_cast(v4i, e);
+    else {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = E::get(e, j);
+      ad_split<TERMS>(u, x);
+    }
   }
 
   // Adds to the results acc(i, j) of 16 columns by 16 rows: columns column(i) of this lane (lane % 16 of a subtile), rows from
   // m0. Of the adapters that these rows have, number k * share + mine are this wave's.
   template <int TN, int TM, class ACC, class COLUMN>
   __device__ __forceinline__ void add(ACC &&acc, COLUMN &&column, int m0, int M, int N, int mine = 0, int share = 1) const {
-    static_assert(TM <= 4, "rows are held a lane each");
-    const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63;
     const int id = lane < 16 * TM && m0 + lane < M ? of_row[m0 + lane] : -1;
-    unsigned long long left = __ballot(id >= 0 && id < count);
-    for (int k = 0; left; k++) {
-      const int a = __builtin_amdgcn_readlane(id, __ffsll(left) - 1);
-      const unsigned long long rows = __ballot(id == a);
-      left &= ~rows;
-      if (k % share != mine) continue;
-      for (int r0 = 0; r0 < ranks; r0 += 32) {
-        v4i low_terms[TM][kLowTerms];
+    const unsigned long long rows = __ballot(id >= 0 && id < count);
+    if (!rows) return;
+    if (type == MI355X_BF16) add_of<BF16, TN, TM>(acc, column, m0, M, N, mine, share, id, rows);
+    else if (type == MI355X_F16) add_of<F16, TN, TM>(acc, column, m0, M, N, mine, share, id, rows);
+    else add_of<F32, TN, TM>(acc, column, m0, M, N, mine, share, id, rows);
+  }
+  // The columns of several subtiles are asked for at once, and those of the next adapter, or of the next subtiles, while the
+  // ones in front are multiplied: a load takes as long as ten such products.
+  template <class E, int TN, int TM, class ACC, class COLUMN>
+  __device__ __forceinline__ void add_of(ACC &acc, COLUMN &column, int m0, int M, int N, int mine, int share, int id,
+                                         unsigned long long all) const {
+    static_assert(TM <= 4, "rows are held a lane each");
+    constexpr int TERMS = std::is_same<E, F32>::value ? 3 : std::is_same<E, F16>::value ? 2 : 1;
+    constexpr int AT_ONCE = TN < (E::kSize == 4 ? 2 : 4) ? TN : (E::kSize == 4 ? 2 : 4), PARTS = TN / AT_ONCE;
+    static_assert(TN % AT_ONCE == 0, "subtiles");
+    const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+    for (int r0 = 0; r0 < ranks; r0 += 32) {
+      v4i low_terms[TM][kLowTerms];
 #pragma unroll
-        for (int j = 0; j < TM; j++) {
-          const uint16_t *at = low + (size_t)min(m0 + j * 16 + l16, M - 1) * kLowTerms * ranks + r0 + 8 * q;
+      for (int j = 0; j < TM; j++) {
+        const uint16_t *at = low + (size_t)min(m0 + j * 16 + l16, M - 1) * kLowTerms * ranks + r0 + 8 * q;
 #pragma unroll
-          for (int t = 0; t < kLowTerms; t++) low_terms[j][t] = *reinterpret_cast<const v4i *>(at + t * ranks);
+        for (int t = 0; t < kLowTerms; t++) low_terms[j][t] = *reinterpret_cast<const v4i *>(at + t * ranks);
+      }
+      // this wave's adapters one after the other: `a` and its rows
+      unsigned long long left = all;
+      int k = 0;
+      auto following = [&](int &a, unsigned long long &rows) {
+        while (left) {
+          a = __builtin_amdgcn_readlane(id, __ffsll(left) - 1);
+          rows = __ballot(id == a);
+          left &= ~rows;
+          if (k++ % share == mine) return true;
         }
+        return false;
+      };
+      typename E::Eight coming[AT_ONCE];
+      auto ask = [&](int a, int part) {
 #pragma unroll
-        for (int i = 0; i < TN; i++) {
-          const size_t row = (size_t)a * N + min(column(i), N - 1);
-          auto products = [&](auto kind) {
-            typedef decltype(kind) E;
-            constexpr int TERMS = std::is_same<E, F32>::value ? 3 : std::is_same<E, F16>::value ? 2 : 1;
+        for (int i = 0; i < AT_ONCE; i++) coming[i] = load_up<E>((size_t)a * N + min(column(part * AT_ONCE + i), N - 1), r0 + 8 * q);
+      };
+      int a = 0, next_a = 0;
+      unsigned long long rows = 0, next_rows = 0;
+      bool more = following(a, rows);
+      if (more) ask(a, 0);
+      while (more) {
+        more = following(next_a, next_rows);
+#pragma unroll
+        for (int part = 0; part < PARTS; part++) {
+          typename E::Eight now[AT_ONCE];
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; i++) now[i] = coming[i];
+          if (part + 1 < PARTS) ask(a, part + 1);
+          else if (more) ask(next_a, 0);
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; i++) {
             v4i u[TERMS];
-            load_up<E, TERMS>(u, row, r0 + 8 * q);
+            split<E, TERMS>(u, now[i]);
 #pragma unroll
             for (int j = 0; j < TM; j++) {
               if (!(rows >> (16 * j) & 0xffff)) continue;
@@ -88,13 +129,11 @@ struct MxAdapters {
                   if (order - t >= 0 && order - t < kLowTerms && order <= 3) sum = ad_multiply(u[t], low_terms[j][order - t], sum);
               const bool own = rows >> (16 * j + l16) & 1;
 #pragma unroll
-              for (int e = 0; e < 4; e++) acc(i, j)[e] += own ? sum[e] : 0.0f;
+              for (int e = 0; e < 4; e++) acc(part * AT_ONCE + i, j)[e] += own ? sum[e] : 0.0f;
             }
-          };
-          if (type == MI355X_BF16) products(BF16());
-          else if (type == MI355X_F16) products(F16());
-          else products(F32());
+          }
         }
+        a = next_a, rows = next_rows;
       }
     }
   }

@@ -21,23 +21,28 @@ struct MxDown {
   int row_tiles, rank_tiles, turns;  // workgroups: row tiles x rank tiles x turns
 };
 
-// Eight neighbouring values of a row from k on, zeros behind column K.
+// Eight neighbouring values of a row from k on, zeros behind column K, as they are in memory.
 template <class E> struct DownValues {
-  static __device__ __forceinline__ void load(float (&x)[8], const uint8_t *row, int k, int K, int) {
+  typedef typename E::Eight Raw;
+  static __device__ __forceinline__ Raw load(const uint8_t *row, int k, int K, int) {
     const typename E::T *at = reinterpret_cast<const typename E::T *>(row) + k;
-    if (k + 8 <= K) load8<E>(x, at);
-    else load8_end<E>(x, at, K - k);
+    return k + 8 <= K ? load_eight<E>(at) : load_eight_end<E>(at, K - k);
+  }
+  static __device__ __forceinline__ void floats(float (&x)[8], const Raw &r) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = E::get(r, j);
   }
 };
 template <> struct DownValues<MX4> {
-  static __device__ __forceinline__ void load(float (&x)[8], const uint8_t *row, int k, int, int groups) {
+  struct Raw {
+    uint32_t codes, byte;
+  };
+  static __device__ __forceinline__ Raw load(const uint8_t *row, int k, int, int groups) {
     // (what is past K is zero up to whole groups, and nothing of a row is read past these)
-    if (k < groups * kMxGroup)
-      mx4_values8(x, *reinterpret_cast<const uint32_t *>(row + (k >> 1)), row[(size_t)groups * kMxGroupBytes + (k >> 5)]);
-    else
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = 0;
+    if (k >= groups * kMxGroup) return Raw{0, 0};
+    return Raw{*reinterpret_cast<const uint32_t *>(row + (k >> 1)), row[(size_t)groups * kMxGroupBytes + (k >> 5)]};
   }
+  static __device__ __forceinline__ void floats(float (&x)[8], const Raw &r) { mx4_values8(x, r.codes, r.byte); }
 };
 
 // 16 ranks by 16 rows over 32 columns: bf16 as it is (microscaled values are bf16 numbers), fp16 by fp16, anything
@@ -45,20 +50,24 @@ template <> struct DownValues<MX4> {
 template <class IN, class A> struct DownProduct {
   static constexpr bool kBf16 = std::is_same<A, BF16>::value && (std::is_same<IN, BF16>::value || std::is_same<IN, MX4>::value);
   static constexpr bool kF16 = std::is_same<A, F16>::value && std::is_same<IN, F16>::value;
-  static __device__ __forceinline__ mx_v4f run(const float (&a)[8], const float (&x)[8], mx_v4f acc) {
+  static __device__ __forceinline__ mx_v4f run(const typename DownValues<A>::Raw &a, const typename DownValues<IN>::Raw &x, mx_v4f acc) {
     if constexpr (kBf16) {
-      ad_v8b u, v;
-#pragma unroll
-      for (int j = 0; j < 8; j++) u[j] = (__bf16)a[j], v[j] = (__bf16)x[j];
-      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, v, acc, 0, 0, 0);
+      v4i v;
+      if constexpr (IN::kSize != 0) v = __builtin_bit_cast(v4i, x);
+      else {
+        float y[8];
+        DownValues<IN>::floats(y, x);
+        v = __builtin_bit_cast(v4i, BF16::put(y));             // (exact)
+      }
+      return ad_multiply(__builtin_bit_cast(v4i, a), v, acc);
     } else if constexpr (kF16) {
-      mx_v8h u, v;
-#pragma unroll
-      for (int j = 0; j < 8; j++) u[j] = (_Float16)a[j], v[j] = (_Float16)x[j];
-      return __builtin_amdgcn_mfma_f32_16x16x32_f16(u, v, acc, 0, 0, 0);
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, x, acc, 0, 0, 0);
     } else {
+      float u[8], v[8];
+      DownValues<A>::floats(u, a);
+      DownValues<IN>::floats(v, x);
 #pragma unroll
-      for (int j = 0; j < 8; j++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], x[j], acc, 0, 0, 0);
+      for (int j = 0; j < 8; j++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(u[j], v[j], acc, 0, 0, 0);
       return acc;
     }
   }
@@ -106,13 +115,24 @@ __global__ __launch_bounds__(kDownThreads) void mx4_adapters_down_kernel(MxDown 
       // ranks past the last re-read it; what they give is not stored
       a_row[t] = p.down + ((size_t)a * p.rank + min(rank0 + t * 16 + l16, p.rank - 1)) * p.K * A::kSize;
     }
-    for (int c = begin; c < end; c += 32) {
-      float x[8], y[RT][8];
-      DownValues<IN>::load(x, x_row, c + 8 * q, p.K, p.groups);
+    // several steps' loads at once: a step alone is bound by the time that they take
+    constexpr int AHEAD = A::kSize == 4 ? 2 : RT == 4 ? 3 : 4;
+    for (int c = begin; c < end; c += 32 * AHEAD) {
+      typename DownValues<IN>::Raw x[AHEAD];
+      typename DownValues<A>::Raw y[AHEAD][RT];
 #pragma unroll
-      for (int t = 0; t < RT; t++) DownValues<A>::load(y[t], a_row[t], c + 8 * q, p.K, 0);
+      for (int s = 0; s < AHEAD; s++)
+        if (c + 32 * s < end) {
+          x[s] = DownValues<IN>::load(x_row, c + 32 * s + 8 * q, p.K, p.groups);
 #pragma unroll
-      for (int t = 0; t < RT; t++) acc[t] = DownProduct<IN, A>::run(y[t], x, acc[t]);
+          for (int t = 0; t < RT; t++) y[s][t] = DownValues<A>::load(a_row[t], c + 32 * s + 8 * q, p.K, 0);
+        }
+#pragma unroll
+      for (int s = 0; s < AHEAD; s++)
+        if (c + 32 * s < end) {
+#pragma unroll
+          for (int t = 0; t < RT; t++) acc[t] = DownProduct<IN, A>::run(y[s][t], x[s], acc[t]);
+        }
     }
     __syncthreads();                               // (the adapter in front may still be read)
 #pragma unroll
@@ -121,14 +141,14 @@ __global__ __launch_bounds__(kDownThreads) void mx4_adapters_down_kernel(MxDown 
       for (int e = 0; e < 4; e++) s_part[wave][t * 4 + e][lane] = acc[t][e];
     __syncthreads();
     // lane (row l16, ranks 4 q + e)
-    for (int t = wave; t < RT; t += kDownWaves) {
+    for (int t = wave; t < (RT == 1 ? 2 : RT); t += kDownWaves) {      // (ranks up to a multiple of 32: zeros)
       const float scale = p.scales ? p.scales[a] : 1.0f;
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         float sum = 0;
 #pragma unroll
-        for (int w = 0; w < kDownWaves; w++) sum += s_part[w][t * 4 + e][lane];
+        for (int w = 0; w < kDownWaves; w++) sum += s_part[w][min(t, RT - 1) * 4 + e][lane];
         v[e] = rank0 + t * 16 + 4 * q + e < p.rank ? sum * scale : 0.0f;
       }
       const int r = rank0 + t * 16 + 4 * q;
@@ -147,7 +167,8 @@ __global__ __launch_bounds__(kDownThreads) void mx4_adapters_down_kernel(MxDown 
 }
 
 template <class IN, class A> static void down_launch(const MxDown &p, unsigned blocks, hipStream_t st) {
-  if (p.ranks <= 32) mx4_adapters_down_kernel<IN, A, 2><<<blocks, kDownThreads, 0, st>>>(p);
+  if (p.rank <= 16) mx4_adapters_down_kernel<IN, A, 1><<<blocks, kDownThreads, 0, st>>>(p);
+  else if (p.ranks <= 32) mx4_adapters_down_kernel<IN, A, 2><<<blocks, kDownThreads, 0, st>>>(p);
   else mx4_adapters_down_kernel<IN, A, 4><<<blocks, kDownThreads, 0, st>>>(p);
 }
 template <class IN> static void down_launch_type(const MxDown &p, int type, unsigned blocks, hipStream_t st) {

@@ -117,9 +117,11 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
   }
   __syncthreads();
   if constexpr (P::kAdapters)
-    p.ad.template add<TN, TM>([&](int i, int j) -> mx_v4f & { return acc[i][j]; },
-                              [&](int i) { return n0 + mx4_weight_column<T::S>(wn * WN + i * 16 + l16); },
-                              m0 + wm * WM, p.M, p.N);
+#pragma unroll
+    for (int j0 = 0; j0 < TM; j0 += 2)             // (as in the tiles through the ring)
+      p.ad.template add<TN, 2>([&](int i, int j) -> mx_v4f & { return acc[i][j0 + j]; },
+                               [&](int i) { return n0 + mx4_weight_column<T::S>(wn * WN + i * 16 + l16); },
+                               m0 + wm * WM + j0 * 16, p.M, p.N);
   mx4_tile_results<OUT, BN, BM, WN, WM>(acc, p, lds,
                                         reinterpret_cast<float *>(lds + mx4_short_bias<OUT, BN, BM, WN, WM>(KT)), bias,
                                         m0, n0);

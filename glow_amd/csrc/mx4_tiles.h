@@ -332,9 +332,12 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, BLOCKS *(BN / WN) * (BM
   dma_wait<0>();                                   // the re-reads, before LDS is used again
   __syncthreads();
   if constexpr (P::kAdapters)
-    p.ad.template add<TN, TM>([&](int i, int j) -> mx_v4f & { return acc[i][j]; },
-                              [&](int i) { return n0 + mx4_weight_column<T::S>(wn * WN + i * 16 + l16); },
-                              m0 + wm * WM, p.M, p.N);
+    // (32 rows at a time: what 64 rows have beside the results of 128 columns is more than there are registers)
+#pragma unroll
+    for (int j0 = 0; j0 < TM; j0 += 2)
+      p.ad.template add<TN, 2>([&](int i, int j) -> mx_v4f & { return acc[i][j0 + j]; },
+                               [&](int i) { return n0 + mx4_weight_column<T::S>(wn * WN + i * 16 + l16); },
+                               m0 + wm * WM + j0 * 16, p.M, p.N);
   mx4_tile_results<OUT, BN, BM, WN, WM>(acc, p, lds, reinterpret_cast<float *>(lds + T::kBias), bias, m0, n0);
 }
 
