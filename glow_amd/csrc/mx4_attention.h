@@ -213,6 +213,7 @@ template <class E> struct AtValues {
     return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 3);
   }
   static __device__ __forceinline__ Two pack(float a, float b) { return Two{(__bf16)a, (__bf16)b}; }
+  static constexpr int kOnes = 0x3f803f80;
   static __device__ __forceinline__ at_v4f multiply(at_v4i values, at_v4i weights, at_v4f acc) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(at_v8b, values), __builtin_bit_cast(at_v8b, weights),
                                                    acc, 0, 0, 0);
@@ -233,6 +234,7 @@ template <> struct AtValues<F16> {
     return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 3);
   }
   static __device__ __forceinline__ Two pack(float a, float b) { return Two{(_Float16)a, (_Float16)b}; }
+  static constexpr int kOnes = 0x3c003c00;
   static __device__ __forceinline__ at_v4f multiply(at_v4i values, at_v4i weights, at_v4f acc) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(at_v8h, values), __builtin_bit_cast(at_v8h, weights),
                                                   acc, 0, 0, 0);
@@ -305,9 +307,9 @@ __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2
 // The largest of a query's scores over the four lanes that hold it.
 __device__ __forceinline__ float at_max(float x) {
   auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  x = __builtin_elementwise_maximum(__uint_as_float(s[0]), __uint_as_float(s[1]));
   s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  return __builtin_elementwise_maximum(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 
 // A row at `position` sees the token.
@@ -328,15 +330,20 @@ template <int D> __device__ __forceinline__ bool at_bad_block(unsigned long long
   return D == 64 ? (bad >> (16 * team + 8 * (q >> 1)) & 0xff) != 0 : (bad >> (16 * team + 4 * q) & 0xf) != 0;
 }
 
+// The largest of a lane's query's scores, scaled. (maximum gives NaN as soon as one is NaN, which max would have to be kept
+// from by another instruction for each.)
+template <int N> __device__ __forceinline__ float at_top(const float (&score)[N], float scale) {
+  float top = score[0];
+#pragma unroll
+  for (int j = 1; j < N; j++) top = __builtin_elementwise_maximum(top, score[j]);
+  return at_max(top) * scale;
+}
 // Scores of a lane's query (tokens that it does not see: minus infinity, and not in `seen`, which counts unless `whole`)
 // become weights; the results so far are rescaled where the largest score moves.
 template <class E, int N, int M>
 __device__ __forceinline__ void at_weigh(float (&score)[N], float &most, float &sum, at_v4f (&acc)[M], float scale, bool whole,
                                          unsigned seen) {
-  float top = score[0];
-#pragma unroll
-  for (int j = 1; j < N; j++) top = fmaxf(top, score[j]);
-  top = at_max(top) * scale;
+  const float top = at_top(score, scale);
   const bool up = top > most + kAtSlack;
   if (__ballot(up)) {
     const float factor = up ? at_exp2(most - top) : 1.0f;
@@ -428,9 +435,9 @@ __device__ __forceinline__ void at_store(const Attention &p, const AtRows &r, in
 template <int D> __device__ __forceinline__ constexpr size_t at_part_floats() { return 16 * D + 48; }
 
 // The whole of a slot's results by one wave: a lane has the components of its query side by side.
-template <class OUT, int D>
-__device__ __forceinline__ void at_store_whole(const Attention &p, const AtRows &r, int h, const at_v4f (&acc)[D / 16],
-                                               float sum) {
+template <class OUT, int D, int M>
+__device__ __forceinline__ void at_store_whole(const Attention &p, const AtRows &r, int h, const at_v4f (&acc)[M], float sum) {
+  static_assert(M >= D / 16, "results");
   const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
   const int at = r.first + l16, token = at / p.group, head = h * p.group + (at - token * p.group);
   const bool there = at < r.last;

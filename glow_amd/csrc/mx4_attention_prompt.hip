@@ -11,13 +11,16 @@ namespace mi355x {
 // multiplied, and its successor's rows are on their way from memory into registers.
 constexpr int kPromptTiles = kPromptWaves;
 
+// What is said of a tile.
+constexpr int kPromptNan = 1, kPromptAbsent = 2;
+
 template <class E, int D> struct PromptLds {
   static constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
   at_v4i values[2][kChunks * COLS][64];             // [32 tokens][column][lane]
   at_v4i keys[kPromptTiles][kChunks][64];
   uint8_t key_scale[kPromptTiles][kChunks][64];
   unsigned long long bad[kPromptTiles][kChunks][4];     // lanes whose values are NaN, for each of a lane's tokens
-  int first[kPromptTiles], any_bad[kPromptTiles];
+  int flags[kPromptTiles];
 };
 
 // What a wave has asked for of a tile.
@@ -26,7 +29,7 @@ template <int D> struct PromptTile {
   at_v4i keys[kChunks];
   int key_scale[kChunks];
   uint32_t values[kChunks][4], value_scale[kChunks][4];
-  int first;
+  bool there;
 };
 
 template <class E, class OUT, int D, int QT>
@@ -60,13 +63,15 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
     queries[t].load(reinterpret_cast<const typename E::T *>(p.q + (size_t)(r.begin + token) * p.q_row_bytes) + (size_t)head * D,
                     p.negative);
   }
-  at_v4f acc[QT][D / 16];
-  float most[QT], sum[QT];
+  // Sums of weights are products with a column of ones, whose results are all the same: the vector unit has more to do than
+  // the matrix cores (16 additions of 110 instructions for sixteen rows and 64 tokens).
+  at_v4f acc[QT][D / 16 + 1];
+  float most[QT];
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    most[t] = kAtNone, sum[t] = 0;
+    most[t] = kAtNone;
 #pragma unroll
-    for (int m = 0; m < D / 16; m++) acc[t][m] = at_v4f{0, 0, 0, 0};
+    for (int m = 0; m <= D / 16; m++) acc[t][m] = at_v4f{0, 0, 0, 0};
   }
 
   const AtTiles tiles = at_tiles(p, low, high);
@@ -87,8 +92,8 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
     const int u = step * kPromptTiles + wave;
     return u < tiles.all ? cache_tile(p.c, r.sequence, (unsigned)tiles.at(u)) : -1;
   };
-  auto load = [&](PromptTile<D> &t, int tile, int step) {
-    t.first = tile < 0 ? -1 : tiles.at(step * kPromptTiles + wave) * kCacheTile;
+  auto load = [&](PromptTile<D> &t, int tile) {
+    t.there = tile >= 0;
     // (a tile that is not there reads the cache's first rows; there is a page)
     const size_t base = (size_t)max(tile, 0) * kCacheTile * p.c.row_bytes;
     const uint8_t *keys = p.c.keys + base, *values = p.c.values + base;
@@ -138,16 +143,16 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
 #pragma unroll
       for (int m = 0; m < COLS; m++) reinterpret_cast<Half *>(&to.values[wave >> 1][c * COLS + m][lane])[wave & 1] = columns[m];
     }
-    if (lane == 0) to.first[wave] = t.first, to.any_bad[wave] = any;
+    if (lane == 0) to.flags[wave] = t.there ? (any ? kPromptNan : 0) : kPromptAbsent;
   };
 
   PromptTile<D> next;
   int coming = -1;
   if (begin < end) {
-    load(next, locate(begin), begin);
+    load(next, locate(begin));
     store(next, lds[0]);
     if (begin + 1 < end) {
-      load(next, locate(begin + 1), begin + 1);
+      load(next, locate(begin + 1));
       if (begin + 2 < end) coming = locate(begin + 2);
     }
   }
@@ -157,68 +162,110 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
     if (step + 1 < end) {
       store(next, lds[(step - begin + 1) & 1]);
       if (step + 2 < end) {
-        load(next, coming, step + 2);
+        load(next, coming);
         if (step + 3 < end) coming = locate(step + 3);
       }
     }
+    // (which tokens come is known without LDS; whether they are there, and are numbers, when it is needed)
     int first[kPromptTiles];
-    bool any_bad = false;
+    bool nothing = true, whole = true;
 #pragma unroll
     for (int k = 0; k < kPromptTiles; k++) {
-      first[k] = __builtin_amdgcn_readfirstlane(now.first[k]);
-      any_bad = any_bad || __builtin_amdgcn_readfirstlane(now.any_bad[k]);
-    }
-    at_v4i packed[QT][2][P];
-    bool none = true;
+      const int u = step * kPromptTiles + k;
+      first[k] = u < tiles.all ? tiles.at(u) * kCacheTile : -1;
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-      bool nothing = true, whole = true;
-#pragma unroll
-      for (int k = 0; k < kPromptTiles; k++) {
+      for (int t = 0; t < QT; t++) {
         nothing = nothing && at_sees_none(p, my_low[t], my_high[t], first[k]);
         whole = whole && at_sees_all(p, my_low[t], my_high[t], first[k]);
       }
-      if (nothing) {
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int s = 0; s < P; s++) packed[t][k][s] = at_v4i{0, 0, 0, 0};
-        continue;
-      }
-      none = false;
-      float score[16];
+    }
+    if (!nothing) {
+      // The sixteens of rows go through each step side by side: alone, each would wait for its own results.
+      const at_v4i flag = *reinterpret_cast<const at_v4i *>(now.flags);
+      float score[QT][16];
 #pragma unroll
       for (int k = 0; k < kPromptTiles; k++) {
-        at_v4f s = {0, 0, 0, 0};
+        at_v4f s[QT];
+#pragma unroll
+        for (int t = 0; t < QT; t++) s[t] = at_v4f{0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < kChunks; c++) {
           const at_v4i codes = now.keys[k][c][lane];
           const int byte = now.key_scale[k][c][lane];
-          s = at_scores<0>(codes, byte, queries[t].codes[c], queries[t].scale[c], s);
+#pragma unroll
+          for (int t = 0; t < QT; t++) s[t] = at_scores<0>(codes, byte, queries[t].codes[c], queries[t].scale[c], s[t]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) score[k * 4 + i] = s[i];
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) score[t][k * 4 + i] = s[t][i];
       }
-      unsigned seen = 0xffff;
+      const int flags = __builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3]);
+      whole = whole && !(flags & kPromptAbsent);
+      unsigned seen[QT];
       if (!whole) {
-        seen = 0;
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-          const bool yes = first[j >> 2] >= 0 && at_sees(p, position[t], first[j >> 2] + 4 * q + (j & 3));
-          seen |= yes ? 1u << j : 0;
-          score[j] = yes ? score[j] : kAtNone;
+        for (int k = 0; k < kPromptTiles; k++)
+          if (__builtin_amdgcn_readfirstlane(flag[k]) & kPromptAbsent) first[k] = -1;
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          seen[t] = 0;
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            const bool yes = first[j >> 2] >= 0 && at_sees(p, position[t], first[j >> 2] + 4 * q + (j & 3));
+            seen[t] |= yes ? 1u << j : 0;
+            score[t][j] = yes ? score[t][j] : kAtNone;
+          }
         }
       }
-      at_weigh<E>(score, most[t], sum[t], acc[t], p.scale, whole, seen);
+      float top[QT];
+      bool up = false;
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        float part[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) part[j] = score[k * 8 + j];
-        at_pack<E>(packed[t][k], part);
+      for (int t = 0; t < QT; t++) {
+        top[t] = at_top(score[t], p.scale);
+        up = up || top[t] > most[t] + kAtSlack;
       }
-    }
-    if (!none) {
+      if (__ballot(up)) {
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          const bool mine = top[t] > most[t] + kAtSlack;
+          const float factor = mine ? at_exp2(most[t] - top[t]) : 1.0f;
+          most[t] = mine ? top[t] : most[t];
+#pragma unroll
+          for (int m = 0; m <= D / 16; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[t][m][i] *= factor;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        const float off = AtKind<E>::kUp - most[t];
+#pragma unroll
+        for (int j = 0; j < 16; j++) score[t][j] = at_exp2(fmaf(score[t][j], p.scale, off));
+      }
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int j = 0; j < 16; j++) score[t][j] = seen[t] >> j & 1 ? score[t][j] : 0.0f;
+      }
+      at_v4i packed[QT][2][P];
+#pragma unroll
+      for (int t = 0; t < QT; t++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          float part[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) part[j] = score[t][k * 8 + j];
+          at_pack<E>(packed[t][k], part);
+        }
+      const at_v4i ones = {AtValues<E>::kOnes, AtValues<E>::kOnes, AtValues<E>::kOnes, AtValues<E>::kOnes};
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int s = 0; s < P; s++) acc[t][D / 16] = AtValues<E>::multiply(ones, packed[t][k][s], acc[t][D / 16]);
 #pragma unroll
       for (int k = 0; k < 2; k++)
 #pragma unroll
@@ -229,12 +276,12 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
 #pragma unroll
             for (int s = 0; s < P; s++) acc[t][m] = AtValues<E>::multiply(values, packed[t][k][s], acc[t][m]);
         }
-      if (any_bad) {
+      if (flags & kPromptNan) {
         bool hit[QT][kChunks] = {};
 #pragma unroll 1
         for (int k = 0; k < kPromptTiles; k++) {
-          const int from = now.first[k];
-          if (!now.any_bad[k] || from < 0) continue;
+          const int u = step * kPromptTiles + k, from = u < tiles.all ? tiles.at(u) * kCacheTile : -1;
+          if (now.flags[k] != kPromptNan || from < 0) continue;        // (not there: not seen)
 #pragma unroll 1
           for (int x = 0; x < 16; x++)
 #pragma unroll
@@ -263,7 +310,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
     mine.first = r.first + (wave * QT + t) * 16;
     mine.last = min(r.last, mine.first + 16);
     if (mine.first >= mine.last) continue;
-    const float whole = add_across32(add_across16(sum[t]));
+    const float whole = acc[t][D / 16][0];
     if (p.splits == 1) {
       at_store_whole<OUT, D>(p, mine, h, acc[t], whole);
     } else {
