@@ -1,8 +1,8 @@
 // Low-rank adapters beside a product of microscaled rows: out[m] += up[a] (scale[a] down[a] x[m]), a the row's own.
 //
-// A launch in front makes low[m] = scale[a] down[a] x[m], 32-bit sums, and keeps it as three bf16 terms (24 bits): the
-// product's tiles add up[a] low[m] to their sums before bias and activation, by 16x16x32 instructions over 32 ranks. up
-// is one (bf16), two (fp16) or three terms. Rows of a subtile may have adapters of their own: one after the other is
+// A launch in front makes low[m] = scale[a] down[a] x[m], 32-bit sums, in parts of K where rows are few: the product's
+// tiles add the parts, split them into three bf16 terms (24 bits) and add up[a] low[m] to their sums before bias and
+// activation, by 16x16x32 instructions over 32 ranks. up is one (bf16), two (fp16) or three terms. Rows of a subtile may have adapters of their own: one after the other is
 // multiplied by all sixteen rows, and each row takes what its own gives, so that what is in one adapter
 // stays with its rows.
 #ifndef GLOW_MI355X_MX4_ADAPTERS_H
@@ -30,18 +30,21 @@ __device__ __forceinline__ mx_v4f ad_multiply(v4i a, v4i b, mx_v4f acc) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ad_v8b, a), __builtin_bit_cast(ad_v8b, b), acc, 0, 0, 0);
 }
 
-constexpr int kLowTerms = 3;
+constexpr int kLowTerms = 3, kMostParts = 4;
 
 struct MxAdapters {
   const uint8_t *up;
-  const uint16_t *low;             // [M][kLowTerms][ranks]
+  const float *low;                // [parts][M][ranks]
   const int32_t *of_row;
   int type, rank, ranks, count;    // ranks: rank up to a multiple of 32, the rest zeros
+  int parts;
 
   // Eight ranks of a row of up; zeros behind the last.
   template <class E> __device__ __forceinline__ typename E::Eight load_up(size_t row, int r) const {
     const typename E::T *at = reinterpret_cast<const typename E::T *>(up) + row * rank + r;
-    return r + 8 <= rank ? load_eight<E>(at) : load_eight_end<E>(at, rank - r);
+    if (r + 8 <= rank) return load_eight<E>(at);
+    if (r >= rank) return typename E::Eight{};       // (not value by value: half of the lanes where rank is 16)
+    return load_eight_end<E>(at, rank - r);
   }
   template <class E, int TERMS> static __device__ __forceinline__ void split(v4i (&u)[TERMS], const typename E::Eight &e) {
     if constexpr (std::is_same<E, BF16>::value) u[0] = __builtin_bit_cast(v4i, e);
@@ -79,9 +82,19 @@ struct MxAdapters {
       v4i low_terms[TM][kLowTerms];
 #pragma unroll
       for (int j = 0; j < TM; j++) {
-        const uint16_t *at = low + (size_t)min(m0 + j * 16 + l16, M - 1) * kLowTerms * ranks + r0 + 8 * q;
+        const float *at = low + (size_t)min(m0 + j * 16 + l16, M - 1) * ranks + r0 + 8 * q;
+        float x[8];
+        load8<F32>(x, at);
+        if (parts > 1) {                           // (all asked for before the first is added)
+          float y[kMostParts - 1][8];
 #pragma unroll
-        for (int t = 0; t < kLowTerms; t++) low_terms[j][t] = *reinterpret_cast<const v4i *>(at + t * ranks);
+          for (int k = 1; k < kMostParts; k++) load8<F32>(y[k - 1], at + (size_t)min(k, parts - 1) * M * ranks);
+#pragma unroll
+          for (int k = 1; k < kMostParts; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] += k < parts ? y[k - 1][e] : 0.0f;
+        }
+        ad_split<kLowTerms>(low_terms[j], x);
       }
       // this wave's adapters one after the other: `a` and its rows
       unsigned long long left = all;

@@ -5,7 +5,9 @@ namespace mi355x {
 
 // The launch in front of the product: low[m] for tiles of sixteen rows and up to 64 ranks, K over the eight waves of a
 // workgroup, and (behind these workgroups) float rows quantised for the product. Rows of a tile may have up to sixteen
-// adapters: workgroups take them in turns, one each while rows are few.
+// adapters: workgroups take them in turns, one each while rows are few. Where that leaves CUs idle, or a workgroup each,
+// K goes to several workgroups too: a CU alone pulls some 30 GB/s from behind its L2. What is left is the latency
+// of a few rounds of loads.
 constexpr int kDownThreads = 512, kDownWaves = kDownThreads / 64;
 
 struct MxDown {
@@ -14,11 +16,11 @@ struct MxDown {
   const uint8_t *down;
   const float *scales;
   const int32_t *of_row;
-  uint16_t *low;
+  float *low;
   uint8_t *packed;                 // float rows' microscaled form
   size_t packed_row_bytes;
   int M, K, groups, rank, ranks, count;
-  int row_tiles, rank_tiles, turns;  // workgroups: row tiles x rank tiles x turns
+  int row_tiles, rank_tiles, turns, parts;  // workgroups: row tiles x rank tiles x turns x parts of K
 };
 
 // Eight neighbouring values of a row from k on, zeros behind column K, as they are in memory.
@@ -77,7 +79,7 @@ template <class IN, class A, int RT>
 __global__ __launch_bounds__(kDownThreads) void mx4_adapters_down_kernel(MxDown p) {
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned tiles = (unsigned)p.row_tiles * p.rank_tiles * p.turns;
+  const unsigned tiles = (unsigned)p.row_tiles * p.rank_tiles * p.turns * p.parts;
   if (blockIdx.x >= tiles) {
     if constexpr (IN::kSize != 0) {
       const unsigned long long unit = (blockIdx.x - tiles) * (unsigned long long)(kDownThreads / 16) + (tid >> 4);
@@ -94,14 +96,16 @@ __global__ __launch_bounds__(kDownThreads) void mx4_adapters_down_kernel(MxDown 
     return;
   }
   __shared__ float s_part[kDownWaves][RT * 4][64];
-  const int turn = (int)(blockIdx.x % (unsigned)p.turns);
-  const int rank0 = (int)(blockIdx.x / (unsigned)p.turns % (unsigned)p.rank_tiles) * 16 * RT;
-  const int m0 = (int)(blockIdx.x / (unsigned)p.turns / (unsigned)p.rank_tiles) * 16;
+  const int part = (int)(blockIdx.x % (unsigned)p.parts);
+  unsigned block = blockIdx.x / (unsigned)p.parts;
+  const int turn = (int)(block % (unsigned)p.turns);
+  block /= (unsigned)p.turns;
+  const int rank0 = (int)(block % (unsigned)p.rank_tiles) * 16 * RT, m0 = (int)(block / (unsigned)p.rank_tiles) * 16;
   const int m = m0 + l16;
   const int id = m < p.M ? p.of_row[m] : -1;
   unsigned left = (unsigned)__ballot(id >= 0 && id < p.count) & 0xffff;
-  const int per = ((p.K + 31) / 32 + kDownWaves - 1) / kDownWaves * 32;
-  const int begin = wave * per, end = min(p.K, begin + per);
+  const int shares = kDownWaves * p.parts, per = ((p.K + 31) / 32 + shares - 1) / shares * 32;
+  const int begin = min(p.K, (part * kDownWaves + wave) * per), end = min(p.K, begin + per);
   const uint8_t *x_row = p.in + (size_t)min(m, p.M - 1) * p.in_row_bytes;
   for (int k = 0; left; k++) {
     const int a = __builtin_amdgcn_readlane(id, __ffs(left) - 1);
@@ -153,14 +157,7 @@ __global__ __launch_bounds__(kDownThreads) void mx4_adapters_down_kernel(MxDown 
       }
       const int r = rank0 + t * 16 + 4 * q;
       if (id == a && r < p.ranks) {
-        uint16_t *to = p.low + (size_t)m * kLowTerms * p.ranks + r;
-#pragma unroll
-        for (int term = 0; term < kLowTerms; term++) {
-          const ad_v2b one = {(__bf16)v[0], (__bf16)v[1]}, two = {(__bf16)v[2], (__bf16)v[3]};
-          *reinterpret_cast<uint2 *>(to + term * p.ranks) =
-              make_uint2(__builtin_bit_cast(uint32_t, one), __builtin_bit_cast(uint32_t, two));
-          v[0] -= (float)one[0], v[1] -= (float)one[1], v[2] -= (float)two[0], v[3] -= (float)two[1];
-        }
+        *reinterpret_cast<float4 *>(p.low + ((size_t)part * p.M + m) * p.ranks + r) = make_float4(v[0], v[1], v[2], v[3]);
       }
     }
   }
@@ -194,7 +191,18 @@ template <class OUT> static int adapted_launch(const MxFcAdapted &p, int K, FcTi
 
 constexpr size_t kMostRank = 1024;
 
-static size_t low_bytes(size_t M, size_t rank) { return M * kLowTerms * ((rank + 31) / 32 * 32) * sizeof(uint16_t); }
+static int down_turns(size_t M) { return M <= 256 ? (int)std::min<size_t>(16, M) : 1; }
+// Parts of K, of two steps a wave at least, for up to 256 rows. us, this launch / the product, 64 rows of 64 adapters of rank 16,
+// 4096 x 4096 weights: 1 part 11.0 / 15.8, 4 parts 5.6 / PRODUCT4. More rows have a workgroup for each CU: 4096 of six adapters of
+// rank 64, 1 part 41.0 / 71.2, 2 parts 41.4 / 83.7.
+static int down_parts(size_t M, size_t K, size_t rank) {
+  if (M > 256) return 1;
+  const size_t tiles = (M + 15) / 16 * (rank <= 32 ? 1 : (rank + 63) / 64) * down_turns(M);
+  return (int)std::max<size_t>(1, std::min<size_t>({(size_t)kMostParts, 512 / tiles, K / 512}));
+}
+static size_t low_bytes(size_t M, size_t K, size_t rank) {
+  return down_parts(M, K, rank) * M * ((rank + 31) / 32 * 32) * sizeof(float);
+}
 
 } // namespace mi355x
 
@@ -209,7 +217,7 @@ int mi355x_mx4_fc_adapters_workspace_bytes(size_t M, size_t K, size_t N, int in_
   MI355X_REQUIRE(M <= 0x7fffffff && K <= 0x7fffffff && N <= 0x7fffffff,
                  "mx4_fc_adapters_workspace_bytes: %zu x %zu x %zu, up to 2^31 - 1 each are supported", M, K, N);
   MI355X_REQUIRE(rank <= kMostRank, "mx4_fc_adapters: rank %zu, up to %zu is supported", rank, kMostRank);
-  *bytes = !M || !N ? 0 : low_bytes(M, rank) + (in_type == MI355X_MX4 ? 0 : M * mx4_row_bytes_of(K));
+  *bytes = !M || !N || !rank ? (in_type == MI355X_MX4 || !M || !N ? 0 : M * mx4_row_bytes_of(K)) : low_bytes(M, K, rank) + (in_type == MI355X_MX4 ? 0 : M * mx4_row_bytes_of(K));
   return MI355X_OK;
 }
 
@@ -263,8 +271,8 @@ int mi355x_mx4_fc_adapters(void *out, int out_type, size_t out_row_bytes, const 
   d.down = static_cast<const uint8_t *>(adapters->down);
   d.scales = adapters->scales;
   d.of_row = row_adapters;
-  d.low = static_cast<uint16_t *>(workspace);
-  d.packed = static_cast<uint8_t *>(workspace) + low_bytes(M, rank);
+  d.low = static_cast<float *>(workspace);
+  d.packed = static_cast<uint8_t *>(workspace) + low_bytes(M, K, rank);
   d.packed_row_bytes = mx4_row_bytes_of(K);
   d.M = (int)M;
   d.K = (int)K;
@@ -274,8 +282,9 @@ int mi355x_mx4_fc_adapters(void *out, int out_type, size_t out_row_bytes, const 
   d.count = (int)count;
   d.row_tiles = (int)((M + 15) / 16);
   d.rank_tiles = d.ranks <= 32 ? 1 : (d.ranks + 63) / 64;
-  d.turns = M <= 256 ? (int)std::min<size_t>(16, M) : 1;
-  unsigned long long blocks = (unsigned long long)d.row_tiles * d.rank_tiles * d.turns;
+  d.turns = down_turns(M);
+  d.parts = down_parts(M, K, rank);
+  unsigned long long blocks = (unsigned long long)d.row_tiles * d.rank_tiles * d.turns * d.parts;
   if (in_type != MI355X_MX4) blocks += ((unsigned long long)M * d.groups + kDownThreads / 16 - 1) / (kDownThreads / 16);
   if (blocks > (1u << 22)) return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_fc_adapters: %zu rows of %zu columns", M, K);
   if (in_type == MI355X_F32) down_launch_type<F32>(d, adapters->type, (unsigned)blocks, st);
@@ -304,6 +313,7 @@ int mi355x_mx4_fc_adapters(void *out, int out_type, size_t out_row_bytes, const 
   p.ad.rank = d.rank;
   p.ad.ranks = d.ranks;
   p.ad.count = d.count;
+  p.ad.parts = d.parts;
   const FcTile tile = fc_tile((long long)M, (long long)K, (long long)N, out_type == MI355X_MX4);
   const int k = (int)K;
   if (out_type == MI355X_F32) return adapted_launch<F32>(p, k, tile, st);

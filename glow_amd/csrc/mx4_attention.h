@@ -333,10 +333,14 @@ template <int D> __device__ __forceinline__ bool at_bad_block(unsigned long long
 // The largest of a lane's query's scores, scaled. (maximum gives NaN as soon as one is NaN, which max would have to be kept
 // from by another instruction for each.)
 template <int N> __device__ __forceinline__ float at_top(const float (&score)[N], float scale) {
-  float top = score[0];
+  float top[N];
 #pragma unroll
-  for (int j = 1; j < N; j++) top = __builtin_elementwise_maximum(top, score[j]);
-  return at_max(top) * scale;
+  for (int j = 0; j < N; j++) top[j] = score[j];
+#pragma unroll
+  for (int half = N / 2; half > 0; half /= 2)
+#pragma unroll
+    for (int j = 0; j < half; j++) top[j] = __builtin_elementwise_maximum(top[j], top[j + half]);
+  return at_max(top[0]) * scale;
 }
 // Scores of a lane's query (tokens that it does not see: minus infinity, and not in `seen`, which counts unless `whole`)
 // become weights; the results so far are rescaled where the largest score moves.
