@@ -193,7 +193,7 @@ constexpr size_t kMostRank = 1024;
 
 static int down_turns(size_t M) { return M <= 256 ? (int)std::min<size_t>(16, M) : 1; }
 // Parts of K, of two steps a wave at least, for up to 256 rows. us, this launch / the product, 64 rows of 64 adapters of rank 16,
-// 4096 x 4096 weights: 1 part 11.0 / 15.8, 4 parts 5.6 / PRODUCT4. More rows have a workgroup for each CU: 4096 of six adapters of
+// 4096 x 4096 weights: 1 part 11.0 / 15.8, 4 parts 5.6 / 19.3. More rows have a workgroup for each CU: 4096 of six adapters of
 // rank 64, 1 part 41.0 / 71.2, 2 parts 41.4 / 83.7.
 static int down_parts(size_t M, size_t K, size_t rank) {
   if (M > 256) return 1;
