@@ -41,10 +41,12 @@ struct MxAdapters {
 
   // Eight ranks of a row of up; zeros behind the last.
   template <class E> __device__ __forceinline__ typename E::Eight load_up(size_t row, int r) const {
-    const typename E::T *at = reinterpret_cast<const typename E::T *>(up) + row * rank + r;
-    if (r + 8 <= rank) return load_eight<E>(at);
-    if (r >= rank) return typename E::Eight{};       // (not value by value: half of the lanes where rank is 16)
-    return load_eight_end<E>(at, rank - r);
+    const typename E::T *at = reinterpret_cast<const typename E::T *>(up) + row * rank;
+    if (rank % 8 == 0) {                             // (no condition of each lane's: loads behind one are not asked for together)
+      const typename E::Eight e = load_eight<E>(at + min(r, rank - 8));
+      return r < rank ? e : typename E::Eight{};
+    }
+    return r + 8 <= rank ? load_eight<E>(at + r) : load_eight_end<E>(at + r, rank - r);
   }
   template <class E, int TERMS> static __device__ __forceinline__ void split(v4i (&u)[TERMS], const typename E::Eight &e) {
     if constexpr (std::is_same<E, BF16>::value) u[0] = __builtin_bit_cast(v4i, e);

@@ -5,9 +5,10 @@ namespace mi355x {
 
 // The launch in front of the product: low[m] for tiles of sixteen rows and up to 64 ranks, K over the eight waves of a
 // workgroup, and (behind these workgroups) float rows quantised for the product. Rows of a tile may have up to sixteen
-// adapters: workgroups take them in turns, one each while rows are few. Where that leaves CUs idle, or a workgroup each,
-// K goes to several workgroups too: a CU alone pulls some 30 GB/s from behind its L2. What is left is the latency
-// of a few rounds of loads.
+// adapters: workgroups take them in turns, one each while rows are few. Where rows are so few that CUs are idle, K goes to
+// several workgroups too. What bounds it with many rows is the rate at which a CU pulls rows from its L2, 17 bytes a cycle, however
+// many loads it has asked for: 640 KB a workgroup over 4096 columns and 64 ranks. 4096 rows of six adapters of rank 64 / 32 / 16 /
+// none 41 / 27 / 20 / 12 us, fp16; 64 rows of 64 adapters of rank 16, bf16, 5.5 us.
 constexpr int kDownThreads = 512, kDownWaves = kDownThreads / 64;
 
 struct MxDown {
@@ -23,12 +24,12 @@ struct MxDown {
   int row_tiles, rank_tiles, turns, parts;  // workgroups: row tiles x rank tiles x turns x parts of K
 };
 
-// Eight neighbouring values of a row from k on, zeros behind column K, as they are in memory.
+// Eight neighbouring values of a row from k on, as they are in memory; zeros from column `end` on unless WHOLE.
 template <class E> struct DownValues {
   typedef typename E::Eight Raw;
-  static __device__ __forceinline__ Raw load(const uint8_t *row, int k, int K, int) {
+  template <bool WHOLE> static __device__ __forceinline__ Raw load(const uint8_t *row, int k, int end, int) {
     const typename E::T *at = reinterpret_cast<const typename E::T *>(row) + k;
-    return k + 8 <= K ? load_eight<E>(at) : load_eight_end<E>(at, K - k);
+    return WHOLE || k + 8 <= end ? load_eight<E>(at) : load_eight_end<E>(at, end - k);
   }
   static __device__ __forceinline__ void floats(float (&x)[8], const Raw &r) {
 #pragma unroll
@@ -39,9 +40,9 @@ template <> struct DownValues<MX4> {
   struct Raw {
     uint32_t codes, byte;
   };
-  static __device__ __forceinline__ Raw load(const uint8_t *row, int k, int, int groups) {
-    // (what is past K is zero up to whole groups, and nothing of a row is read past these)
-    if (k >= groups * kMxGroup) return Raw{0, 0};
+  template <bool WHOLE> static __device__ __forceinline__ Raw load(const uint8_t *row, int k, int end, int groups) {
+    // (what is past K is zero up to whole groups; `end` is that of a range of eights, or K)
+    if (!WHOLE && k >= end) return Raw{0, 0};
     return Raw{*reinterpret_cast<const uint32_t *>(row + (k >> 1)), row[(size_t)groups * kMxGroupBytes + (k >> 5)]};
   }
   static __device__ __forceinline__ void floats(float (&x)[8], const Raw &r) { mx4_values8(x, r.codes, r.byte); }
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(kDownThreads) void mx4_adapters_down_kernel(MxDown 
   const int m = m0 + l16;
   const int id = m < p.M ? p.of_row[m] : -1;
   unsigned left = (unsigned)__ballot(id >= 0 && id < p.count) & 0xffff;
-  const int shares = kDownWaves * p.parts, per = ((p.K + 31) / 32 + shares - 1) / shares * 32;
+  const int shares = kDownWaves * p.parts, per = ((p.K + 63) / 64 + shares - 1) / shares * 64;
   const int begin = min(p.K, (part * kDownWaves + wave) * per), end = min(p.K, begin + per);
   const uint8_t *x_row = p.in + (size_t)min(m, p.M - 1) * p.in_row_bytes;
   for (int k = 0; left; k++) {
@@ -119,25 +120,29 @@ __global__ __launch_bounds__(kDownThreads) void mx4_adapters_down_kernel(MxDown 
       // ranks past the last re-read it; what they give is not stored
       a_row[t] = p.down + ((size_t)a * p.rank + min(rank0 + t * 16 + l16, p.rank - 1)) * p.K * A::kSize;
     }
-    // several steps' loads at once: a step alone is bound by the time that they take
-    constexpr int AHEAD = A::kSize == 4 ? 2 : RT == 4 ? 3 : 4;
-    for (int c = begin; c < end; c += 32 * AHEAD) {
+    // Several steps' loads at once, without a condition of each lane's while all columns are there. A lane takes 16 neighbouring
+    // columns of 64, eight a step, so that two loads in a row use lines of 128 bytes whole.
+    constexpr int AHEAD = A::kSize == 4 || IN::kSize == 4 || RT == 4 ? 2 : 4;
+    auto steps = [&](int c, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
       typename DownValues<IN>::Raw x[AHEAD];
       typename DownValues<A>::Raw y[AHEAD][RT];
 #pragma unroll
+      for (int s = 0; s < AHEAD; s++) {
+        const int k = c + s / 2 * 64 + 16 * q + s % 2 * 8;
+        x[s] = DownValues<IN>::template load<WHOLE>(x_row, k, end, p.groups);
+#pragma unroll
+        for (int t = 0; t < RT; t++) y[s][t] = DownValues<A>::template load<WHOLE>(a_row[t], k, end, 0);
+      }
+#pragma unroll
       for (int s = 0; s < AHEAD; s++)
-        if (c + 32 * s < end) {
-          x[s] = DownValues<IN>::load(x_row, c + 32 * s + 8 * q, p.K, p.groups);
 #pragma unroll
-          for (int t = 0; t < RT; t++) y[s][t] = DownValues<A>::load(a_row[t], c + 32 * s + 8 * q, p.K, 0);
-        }
-#pragma unroll
-      for (int s = 0; s < AHEAD; s++)
-        if (c + 32 * s < end) {
-#pragma unroll
-          for (int t = 0; t < RT; t++) acc[t] = DownProduct<IN, A>::run(y[s][t], x[s], acc[t]);
-        }
-    }
+        for (int t = 0; t < RT; t++) acc[t] = DownProduct<IN, A>::run(y[s][t], x[s], acc[t]);
+    };
+    int c = begin;
+    for (; c + 32 * AHEAD <= end; c += 32 * AHEAD) steps(c, std::true_type());
+    // (columns from `end` on are the next wave's, or not there: with the range cut at `end` they are zeros)
+    for (; c < end; c += 32 * AHEAD) steps(c, std::false_type());
     __syncthreads();                               // (the adapter in front may still be read)
 #pragma unroll
     for (int t = 0; t < RT; t++)
@@ -191,7 +196,8 @@ template <class OUT> static int adapted_launch(const MxFcAdapted &p, int K, FcTi
 
 constexpr size_t kMostRank = 1024;
 
-static int down_turns(size_t M) { return M <= 256 ? (int)std::min<size_t>(16, M) : 1; }
+// Two turns for many rows: where requests meet in a tile, its two adapters would take turns in one workgroup.
+static int down_turns(size_t M) { return M <= 256 ? (int)std::min<size_t>(16, M) : 2; }
 // Parts of K, of two steps a wave at least, for up to 256 rows. us, this launch / the product, 64 rows of 64 adapters of rank 16,
 // 4096 x 4096 weights: 1 part 11.0 / 15.8, 4 parts 5.6 / 19.3. More rows have a workgroup for each CU: 4096 of six adapters of
 // rank 64, 1 part 41.0 / 71.2, 2 parts 41.4 / 83.7.
