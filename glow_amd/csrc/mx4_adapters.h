@@ -39,10 +39,13 @@ struct MxAdapters {
   int type, rank, ranks, count;    // ranks: rank up to a multiple of 32, the rest zeros
   int parts;
 
-  // Eight ranks of a row of up; zeros behind the last.
-  template <class E> __device__ __forceinline__ typename E::Eight load_up(size_t row, int r) const {
+  // Eight ranks of a row of up, q's of those from r0 on; zeros behind the last.
+  template <class E> __device__ __forceinline__ typename E::Eight load_up(size_t row, int r0, int q) const {
     const typename E::T *at = reinterpret_cast<const typename E::T *>(up) + row * rank;
-    if (rank % 8 == 0) {                             // (no condition of each lane's: loads behind one are not asked for together)
+    const int r = r0 + 8 * q;
+    // (no condition of each lane's where it can be done without: loads behind one are not asked for together)
+    if (r0 + 32 <= rank) return load_eight<E>(at + r);
+    if (rank % 8 == 0) {
       const typename E::Eight e = load_eight<E>(at + min(r, rank - 8));
       return r < rank ? e : typename E::Eight{};
     }
@@ -113,7 +116,7 @@ struct MxAdapters {
       typename E::Eight coming[AT_ONCE];
       auto ask = [&](int a, int part) {
 #pragma unroll
-        for (int i = 0; i < AT_ONCE; i++) coming[i] = load_up<E>((size_t)a * N + min(column(part * AT_ONCE + i), N - 1), r0 + 8 * q);
+        for (int i = 0; i < AT_ONCE; i++) coming[i] = load_up<E>((size_t)a * N + min(column(part * AT_ONCE + i), N - 1), r0, q);
       };
       int a = 0, next_a = 0;
       unsigned long long rows = 0, next_rows = 0;

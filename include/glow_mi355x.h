@@ -981,7 +981,8 @@ int mi355x_group_norm(void *out, int out_type, size_t out_row_bytes, const void 
  *   pages[s * pages_per_sequence + t / page_tokens] * page_tokens + t % page_tokens
  * of both; without a table (pages NULL) page k of sequence s is s * pages_per_sequence + k. A
  * page number outside [0, n_pages) stands for no page: what lies there is neither read nor
- * written. Rows are on multiples of 16 bytes, row_bytes (up to 2^26) apart. */
+ * written. Rows are on multiples of 16 bytes, row_bytes (up to 2^26) apart. A cache of 2^35 rows or
+ * more is MI355X_ERR_NOT_SUPPORTED. */
 typedef struct {
   uint8_t *keys, *values;       /* DEVICE, n_pages * page_tokens rows each */
   uint64_t row_bytes;
@@ -1023,7 +1024,8 @@ int mi355x_mx4_cache_write(const mi355x_mx4_cache *cache, const void *keys, cons
  * block of 32's largest. Sums are of 32 bits; weights are rounded to the type of q before they
  * meet values (fp32: to 24 bits). An infinity or a NaN in a query makes
  * NaN of its head's result, one that a row sees in a key or a value of the row's heads or columns.
- * Equal calls give equal bits. Scores past the range of 32 bits: NaN.
+ * Equal calls give equal bits. Scores past the range of 32 bits: NaN. MI355X_ERR_NOT_SUPPORTED where
+ * rows * heads / 16 + sequences * kv_heads is over 2^22.
  * workspace: device memory of mi355x_mx4_attention_workspace_bytes, on a multiple of 16 and
  * overlapping no tensor; NULL where that is 0. A call leaves nothing in it for the next, and calls
  * that may run at the same time need one each. */
@@ -1047,7 +1049,8 @@ int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const vo
  *   rank   up to 1024
  *   row_adapters  DEVICE int32 [M]; rows of the same adapter are fastest next to each other
  * All sums are of 32 bits, in no particular order (equal calls give equal bits), and down[a] in[m] goes
- * on in 24; an infinity in an adapter may come out as NaN. With K, rank or count of 0 this is mi355x_mx4_fc.
+ * on in 24; an infinity in an adapter may come out as NaN. With K, rank or count of 0 this is
+ * mi355x_mx4_fc, whose limits it has, and M * (K / 4096 + ranks in 64s / 8) up to 2^22.
  * workspace as there, of mi355x_mx4_fc_adapters_workspace_bytes (as much as mi355x_mx4_fc asks for). */
 typedef struct {
   const void *down, *up;        /* DEVICE */
