@@ -9,6 +9,10 @@ namespace mi355x {
 // 64 at a time: each wave brings one tile of sixteen into LDS, keys as they are, values converted and transposed to
 // what the matrix instructions want, once for all waves. Two buffers: a step is prepared while the one in front is
 // multiplied, and its successor's rows are on their way from memory into registers.
+//
+// Two prompts of 4096, 32 heads of 128 over 8, bf16: 393 us, 700 TFLOP/s (a workgroup for sixteen rows, each converting
+// values for itself: 1884). A step takes a SIMD 3200 cycles for 960 of matrix and 1200 of vector instructions: the chain of a step, the
+// largest score above all, is waited for, and no more than two waves fit the registers.
 constexpr int kPromptTiles = kPromptWaves;
 
 // What is said of a tile.
