@@ -72,11 +72,17 @@ def attention(b, q, heads, type_, scale=None, window=0, sinks=0, max_length=None
         used[begin:begin + n] = True
         if not length or not n:
             continue
+        # tokens on no page are not seen
         at = b.places(i, length)
+        there = np.ones(length, bool)
+        if b.pages is not None:
+            page = b.pages[i, np.arange(length) // b.page_tokens]
+            there = (page >= 0) & (page < b.n_pages)
+        at = np.where(there, at, 0)
         K = ref.values(b.keys[at], b.kv_heads * d).reshape(length, b.kv_heads, d)
         V = ref.values(b.values[at], b.kv_heads * d).reshape(length, b.kv_heads, d)
         for r in range(n):
-            seen = sees(length - n + r, length, window, sinks)
+            seen = sees(length - n + r, length, window, sinks) & there
             if not seen.any():
                 continue
             for h in range(heads):

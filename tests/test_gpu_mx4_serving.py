@@ -88,6 +88,25 @@ def test_sets_of_heads(kv_heads):
         check(b, q, kv_heads * 2, type_, ref.MX4, window=700, sinks=9)
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("dim, kv_heads, new", [(64, 1, 1), (128, 2, 1), (256, 1, 2), (64, 2, 70), (128, 2, 70), (256, 1, 70)])
+def test_shared_pages_and_pages_that_are_none(dim, kv_heads, new, type_):
+    """Sequences with the same first pages, and sequences with holes: what is on no page is not seen."""
+    rng = np.random.default_rng(15)
+    b = aref.Batch(rng, [200, 150, 700], [new] * 3, kv_heads, dim, 32)
+    b.pages[1, :2] = b.pages[0, :2]
+    b.pages[2, [0, 5, 6, 21]] = -1, b.n_pages, 2 ** 31 - 1, -2 ** 31
+    q = queries(rng, b, kv_heads * 4, type_)
+    check(b, q, kv_heads * 4, type_)
+    check(b, q, kv_heads * 4, type_, ref.MX4, window=90, sinks=40)
+    b.pages[:] = -1
+    assert not run(b, q, kv_heads * 4, type_).view(np.uint8).any()
+    x = ref.to_type(rng.normal(0, 1, (b.rows, kv_heads * dim)), type_)
+    for g, w in zip(capi.mx4_cache_write(b.keys, b.values, x, x, b.starts, b.lengths, kv_heads, dim, 32, b.pages, type_),
+                    (b.keys, b.values)):
+        np.testing.assert_array_equal(g, w)
+
+
 def test_starts_and_lengths_out_of_range():
     """Entries outside of the batch, and lengths past the pages, count as the nearest."""
     rng = np.random.default_rng(8)
