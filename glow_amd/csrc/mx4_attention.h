@@ -116,11 +116,11 @@ __device__ __forceinline__ AtTiles at_tiles(const Attention &p, int low, int hig
 }
 
 // Steps of 32 tokens in a share of a slot that has `steps`: what gives all sequences together `target` shares, so that long
-// and short ones have shares of a size, but `least` steps at least and no more than `splits` shares. (Lengths of over
-// 1024 sequences are not looked through.)
+// and short ones have shares of a size, but `least` steps at least and no more than `splits` shares. (There is a target
+// for a few hundred sequences at most: more need no shares.)
 __device__ __forceinline__ int at_share_steps(const Attention &p, int steps, int least) {
   int chunk = max((int)(((long long)steps + p.splits - 1) / p.splits), least);
-  if (p.target && p.c.sequences <= 1024) {
+  if (p.target) {
     float all = 0;                                  // (in steps; equal in all waves of all launches)
     const long long most = (long long)p.window + p.sinks;
     for (int i = threadIdx.x & 63; i < p.c.sequences; i += 64)
