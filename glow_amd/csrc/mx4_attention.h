@@ -60,11 +60,12 @@ struct Attention {
 constexpr float kAtSlack = 8.0f;
 constexpr float kAtNone = -__builtin_inff();
 
-// Terms of a query, terms of a weight, what weights are shifted up by, and the least scale byte of values that count
-// as NaN: 2^14 times 4 is past fp16's range.
-template <class E> struct AtKind { static constexpr int kQ = 6, kP = 3, kNan = 255; static constexpr float kUp = 0; };
-template <> struct AtKind<F16> { static constexpr int kQ = 3, kP = 1, kNan = 141; static constexpr float kUp = 7; };
-template <> struct AtKind<BF16> { static constexpr int kQ = 3, kP = 1, kNan = 255; static constexpr float kUp = 0; };
+// Terms of a query, terms of a weight, what weights are shifted up by, the least scale byte of values that count as NaN
+// (2^14 times 4 is past fp16's range), and what values are shifted down by until they are divided by the sum of the
+// weights: 6 times 2^127 is past bf16's range, and an infinity would make NaN of the rows that do not see it, whose weight is 0.
+template <class E> struct AtKind { static constexpr int kQ = 6, kP = 3, kNan = 255, kDown = 3; static constexpr float kUp = 0; };
+template <> struct AtKind<F16> { static constexpr int kQ = 3, kP = 1, kNan = 141, kDown = 0; static constexpr float kUp = 7; };
+template <> struct AtKind<BF16> { static constexpr int kQ = 3, kP = 1, kNan = 255, kDown = 3; static constexpr float kUp = 0; };
 
 // Which rows a slot of sixteen has. Slots of a sequence begin at floor(start * group / 16) + its number, which leaves
 // each as many as it needs.
@@ -196,6 +197,15 @@ __device__ __forceinline__ at_v4f at_scores(at_v4i keys, int key_scale, const at
 }
 
 // ---- weights and values --------------------------------------------------------------
+
+// The power of two that a block of values is multiplied by, 2^-127 at least: what that makes too large is below 2^-121.
+template <class E> __device__ __forceinline__ float at_value_scale(uint32_t byte) {
+  return __uint_as_float((uint32_t)max((int)(byte << 23) - (AtKind<E>::kDown << 23), 0x00400000));
+}
+// What results are divided by.
+template <class E> __device__ __forceinline__ float at_divisor(float sum) {
+  return AtKind<E>::kDown ? sum * (1.0f / (1 << AtKind<E>::kDown)) : sum;
+}
 
 // Pairs of values, and the product with weights, in the type that weights are rounded to.
 template <class E> struct AtValues {
@@ -439,7 +449,7 @@ __device__ __forceinline__ void at_store(const Attention &p, const AtRows &r, in
 template <int D> __device__ __forceinline__ constexpr size_t at_part_floats() { return 16 * D + 48; }
 
 // The whole of a slot's results by one wave: a lane has the components of its query side by side.
-template <class OUT, int D, int M>
+template <class E, class OUT, int D, int M>
 __device__ __forceinline__ void at_store_whole(const Attention &p, const AtRows &r, int h, const at_v4f (&acc)[M], float sum) {
   static_assert(M >= D / 16, "results");
   const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
@@ -447,7 +457,7 @@ __device__ __forceinline__ void at_store_whole(const Attention &p, const AtRows 
   const bool there = at < r.last;
   uint8_t *row = p.out + (size_t)(r.begin + token) * p.out_row_bytes;
   constexpr int kChunks = (D + 127) / 128, COLS = D == 64 ? 4 : 8;
-  const float by = sum == 0 ? 0.0f : 1.0f / sum;
+  const float by = sum == 0 ? 0.0f : 1.0f / at_divisor<E>(sum);
 #pragma unroll
   for (int c = 0; c < kChunks; c++) {
     float x[4][8];

@@ -222,7 +222,7 @@ __device__ __forceinline__ void at_values(AtState<E, D> &a, const at_v4i (&packe
     }
     float scale[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) scale[j] = __uint_as_float(max(s.scale[c][j] << 23, 0x00400000u));
+    for (int j = 0; j < 8; j++) scale[j] = at_value_scale<E>(s.scale[c][j]);
     at_transpose<E, COLS>(s.codes[c], scale, [&](int m, at_v4i values) {
 #pragma unroll
       for (int t = 0; t < AtKind<E>::kP; t++) a.acc[c * 8 + m] = AtValues<E>::multiply(values, packed[t], a.acc[c * 8 + m]);
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256 * G) void mx4_attention_join_kernel(Attention p
     }
   }
 #pragma unroll
-  for (int m = 0; m < D / 16; m++) x[m] = sum == 0 ? 0.0f : x[m] / sum;
+  for (int m = 0; m < D / 16; m++) x[m] = sum == 0 ? 0.0f : x[m] / at_divisor<E>(sum);
   at_store<E, OUT, D>(p, r, h, i, x, s_most, g == 0);
 }
 
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
     return;
   }
 #pragma unroll
-  for (int m = 0; m < D / 16; m++) x[m] = whole == 0 ? 0.0f : x[m] / whole;
+  for (int m = 0; m < D / 16; m++) x[m] = whole == 0 ? 0.0f : x[m] / at_divisor<E>(whole);
   at_store<E, OUT, D>(p, r, h, i, x, s_most, wave < 4);
 }
 
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(512, AtKind<E>::kQ == 6 ? 2 : 4) void mx4_attention
     a.most = most;
   }
   if (alone) {
-    at_store_whole<OUT, D>(p, r, h, a.acc, whole);
+    at_store_whole<E, OUT, D>(p, r, h, a.acc, whole);
     return;
   }
   float *part = p.part + ((size_t)of_all * p.kv_heads + h) * at_part_floats<D>();

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
       }
       float scale[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) scale[i] = __uint_as_float(max(t.value_scale[c][i] << 23, 0x00400000u));
+      for (int i = 0; i < 4; i++) scale[i] = at_value_scale<E>(t.value_scale[c][i]);
       typedef int Half __attribute__((ext_vector_type(2)));
       Half columns[COLS];
       at_transpose4<E, COLS>(columns, t.values[c], scale);
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
     if (mine.first >= mine.last) continue;
     const float whole = acc[t][D / 16][0];
     if (p.splits == 1) {
-      at_store_whole<OUT, D>(p, mine, h, acc[t], whole);
+      at_store_whole<E, OUT, D>(p, mine, h, acc[t], whole);
     } else {
       const long long sixteen = at_first_slot<16>(p, r.sequence) + mine.first / 16;
       float *part = p.part + ((size_t)(sixteen * p.splits + share) * p.kv_heads + h) * at_part_floats<D>();
