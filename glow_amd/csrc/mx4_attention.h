@@ -20,9 +20,10 @@
 //       transposed to pairs of tokens by byte permutes. Results: lane q has columns 32 q .. 32 q + 31 for
 //       D = 128, a block of a microscaled result.
 //
-// The running maximum moves only when a score passes it by more than 2^8: weights stay below 2^8 then
-// (2^15 in fp16, which are shifted up so that small ones stay normal numbers), and most steps
-// have no rescaling.
+// The running maximum moves only when a score passes it by more than 2^8: weights stay below 2^8 times what they are
+// shifted by then, and most steps have no rescaling. fp16's are shifted up by 2^7, so that small ones stay normal
+// numbers; the others' down by 2^39: 2^31 of them are no more than 1, and their sum with values of any size stays in
+// the range of 32 bits, as the mean does.
 #ifndef GLOW_MI355X_MX4_ATTENTION_H
 #define GLOW_MI355X_MX4_ATTENTION_H
 
@@ -63,9 +64,9 @@ constexpr float kAtNone = -__builtin_inff();
 // Terms of a query, terms of a weight, what weights are shifted up by, the least scale byte of values that count as NaN
 // (2^14 times 4 is past fp16's range), and what values are shifted down by until they are divided by the sum of the
 // weights: 6 times 2^127 is past bf16's range, and an infinity would make NaN of the rows that do not see it, whose weight is 0.
-template <class E> struct AtKind { static constexpr int kQ = 6, kP = 3, kNan = 255, kDown = 3; static constexpr float kUp = 0; };
+template <class E> struct AtKind { static constexpr int kQ = 6, kP = 3, kNan = 255, kDown = 3; static constexpr float kUp = -39; };
 template <> struct AtKind<F16> { static constexpr int kQ = 3, kP = 1, kNan = 141, kDown = 0; static constexpr float kUp = 7; };
-template <> struct AtKind<BF16> { static constexpr int kQ = 3, kP = 1, kNan = 255, kDown = 3; static constexpr float kUp = 0; };
+template <> struct AtKind<BF16> { static constexpr int kQ = 3, kP = 1, kNan = 255, kDown = 3; static constexpr float kUp = -39; };
 
 // Which rows a slot of sixteen has. Slots of a sequence begin at floor(start * group / 16) + its number, which leaves
 // each as many as it needs.
@@ -198,7 +199,8 @@ __device__ __forceinline__ at_v4f at_scores(at_v4i keys, int key_scale, const at
 
 // ---- weights and values --------------------------------------------------------------
 
-// The power of two that a block of values is multiplied by, 2^-127 at least: what that makes too large is below 2^-121.
+// The power of two that a block of values is multiplied by, 2^-127 at least: what that makes too large is below 2^-124, nothing
+// once it is multiplied by a weight of up to 2^-31.
 template <class E> __device__ __forceinline__ float at_value_scale(uint32_t byte) {
   return __uint_as_float((uint32_t)max((int)(byte << 23) - (AtKind<E>::kDown << 23), 0x00400000));
 }

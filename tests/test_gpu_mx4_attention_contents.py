@@ -121,3 +121,28 @@ def test_large_values_that_are_seen(dim, kv_heads, group, new, byte, type_):
     assert np.isnan(got[sees, :group, 32:64]).all()
     got[sees, :group, 32:64] = 0
     assert not np.isnan(got).any()
+
+
+@pytest.mark.parametrize("type_", [ref.F32, ref.BF16])
+@pytest.mark.parametrize("size", [250, 252, 70])
+@pytest.mark.parametrize("dim, kv_heads, group, new, longest", SHAPES)
+def test_values_at_the_ends_of_the_range(dim, kv_heads, group, new, longest, size, type_):
+    """Sums over many tokens of values up to 2^127, whose mean is within the range, and of values down to 2^-60. Scores rise
+    from token to token, so that weights are as large as they get before the running maximum moves."""
+    rng = np.random.default_rng(size + dim)
+    b = aref.Batch(rng, [longest], [new], kv_heads, dim, 32)
+    heads, cols = kv_heads * group, kv_heads * dim
+    groups = ref.groups(cols)
+    at = b.places(0, longest)
+    b.values[np.ix_(at, 64 * groups + np.arange(cols // 32))] = size
+    b.values[at, :64 * groups] |= 0x44                   # (magnitudes 2 to 6: sums without much cancelling)
+    b.values[at, :64 * groups] &= 0x77
+    rising = rng.normal(0, 0.2, (longest, cols))
+    rising[:, ::32] = np.linspace(-4, 4, longest)[:, None]
+    b.keys[at] = ref.rows_of(rising)
+    q = rng.normal(0, 0.3, (b.rows, heads * dim))
+    q[:, ::32] = 1.5
+    q = ref.to_type(q, type_)
+    scale = 8 / dim
+    check(b, q, heads, type_, scale=scale)
+    check(b, q, heads, type_, ref.MX4, scale=scale, window=90, sinks=7)
