@@ -7,9 +7,9 @@
 //
 //   S   16 tokens x 16 queries by the scaled instruction over 128 columns: codes and scale bytes of
 //       the keys as they lie in memory (a lane has one block of a token), queries as sums of 6-bit
-//       floats (E2M3, four bits each) with a power of two for each block of 32: 3 terms for 16-bit types,
+//       floats (E2M3) with a power of two for each block of 32: 3 terms and a 4-bit one (E2M1) for 16-bit types,
 //       6 for fp32. Nothing of a key is ever converted. A lane gets tokens 4 q .. 4 q + 3. 8-bit terms
-//       would be as many (2, 3, 6) of twice the time each, and the instruction cuts small products off
+//       would be 3, 3 and 6 of twice the time each, and the instruction cuts small products off
 //       where exponents lie far apart (2^-17 of the sum; 6-bit products come out exact).
 //   P   is what the lane then holds of two tiles of tokens: eight weights of its query, which is what the
 //       16x16x32 instruction wants of its second operand, tokens in the order 4 q + i of the first
@@ -61,12 +61,24 @@ struct Attention {
 constexpr float kAtSlack = 8.0f;
 constexpr float kAtNone = -__builtin_inff();
 
-// Terms of a query, terms of a weight, what weights are shifted up by, the least scale byte of values that count as NaN
+// 6-bit terms of a query, whether a 4-bit one follows, terms of a weight, what weights are shifted up by, the least scale byte of values that count as NaN
 // (2^14 times 4 is past fp16's range), and what values are shifted down by until they are divided by the sum of the
 // weights: 6 times 2^127 is past bf16's range, and an infinity would make NaN of the rows that do not see it, whose weight is 0.
-template <class E> struct AtKind { static constexpr int kQ = 6, kP = 3, kNan = 255, kDown = 3; static constexpr float kUp = -39; };
-template <> struct AtKind<F16> { static constexpr int kQ = 3, kP = 1, kNan = 141, kDown = 0; static constexpr float kUp = 7; };
-template <> struct AtKind<BF16> { static constexpr int kQ = 3, kP = 1, kNan = 255, kDown = 3; static constexpr float kUp = -39; };
+template <class E> struct AtKind {
+  static constexpr int kQ = 6, kP = 3, kNan = 255, kDown = 3;
+  static constexpr bool kLast = false;
+  static constexpr float kUp = -39;
+};
+template <> struct AtKind<F16> {
+  static constexpr int kQ = 3, kP = 1, kNan = 141, kDown = 0;
+  static constexpr bool kLast = true;
+  static constexpr float kUp = 7;
+};
+template <> struct AtKind<BF16> {
+  static constexpr int kQ = 3, kP = 1, kNan = 255, kDown = 3;
+  static constexpr bool kLast = true;
+  static constexpr float kUp = -39;
+};
 
 // Which rows a slot of sixteen has. Slots of a sequence begin at floor(start * group / 16) + its number, which leaves
 // each as many as it needs.
@@ -134,16 +146,24 @@ __device__ __forceinline__ int at_share_steps(const Attention &p, int steps, int
 
 // ---- queries -----------------------------------------------------------------------
 
-// Sixteen rows of queries of D columns as sums of 6-bit floats: 32 q to 32 q + 31 of 128 columns are lane q's, a block
-// with a power of two of its own. The largest is scaled to [4, 8); a term rounds to half (values past 7.5 become 7.5),
-// and the next has a sixteenth of its scale: after T terms what is left is 2^-4T of the largest at most.
+// Sixteen rows of queries of D columns as sums of small floats: 32 q to 32 q + 31 of 128 columns are lane q's, a block
+// with a power of two of its own. The largest is scaled to [2, 4); a 6-bit term rounds to an eighth at most, and the next has
+// a thirty-second of its scale, in which that is 4 at most: after T terms what is left is 2^(1 - 5T) of the largest at most,
+// 2^-29 after six. Behind three terms (2^-14) a 4-bit one rounds to a half what is up to 4, which leaves 2^-17: rotary
+// queries have columns that stand out, next to which the others' bits would be lost. It lies in LDS: where four waves share a SIMD's
+// registers, or two with 32 rows each, a term more in registers had 7 to 49 of them in memory, in LDS 3 to 9, as with three
+// terms. With / without it, us: four long sequences 134 / 130, two prompts of 4096 411 / 393.
 template <class E, int D> struct AtQueries {
-  static constexpr int kTerms = AtKind<E>::kQ, kChunks = (D + 127) / 128;
+  static constexpr int kTerms = AtKind<E>::kQ, kAll = kTerms + AtKind<E>::kLast, kChunks = (D + 127) / 128, kWords = (kAll + 3) / 4;
+  static constexpr int kLds = AtKind<E>::kLast ? kChunks * 1024 : 0;      // bytes of a wave
   at_v6u codes[kChunks][kTerms];
-  int scale[kChunks][(kTerms + 3) / 4];          // a byte a term
+  int scale[kChunks][kWords];                    // a byte a term
+  const at_v4i *last;                            // of this lane, 64 apart
 
-  __device__ __forceinline__ void load(const typename E::T *row, bool negative) {
+  // `lds`: this wave's.
+  __device__ __forceinline__ void load(const typename E::T *row, bool negative, uint8_t *lds) {
     const int q = (threadIdx.x & 63) >> 4;
+    last = reinterpret_cast<const at_v4i *>(lds) + (threadIdx.x & 63);
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
       at_v16f even, odd;               // the conversion takes every second column in either
@@ -162,39 +182,62 @@ template <class E, int D> struct AtQueries {
         for (int j = 0; j < 4; j++) even[e / 2 + j] = y[2 * j], odd[e / 2 + j] = y[2 * j + 1];
       }
       const int exponent = (int)(most >> 23);
+      auto byte_of = [&](int t) { return max(exponent - 1 - 5 * t, 1); };
 #pragma unroll
-      for (int w = 0; w < (kTerms + 3) / 4; w++) scale[c][w] = 0;
+      for (int w = 0; w < kWords; w++) scale[c][w] = 0;
+#pragma unroll
+      for (int t = 0; t < kAll; t++) scale[c][t / 4] |= (exponent == 255 ? 255 : byte_of(t)) << (8 * (t % 4));
 #pragma unroll
       for (int t = 0; t < kTerms; t++) {
-        const int byte = max(exponent - 2 - 4 * t, 1);
-        const float s = __uint_as_float((uint32_t)byte << 23);
+        const float s = __uint_as_float((uint32_t)byte_of(t) << 23);
         const at_v6u six = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s);
         // (the conversion writes words of its result before it has read all operands: they have to live on)
         asm volatile("" ::"v"(even), "v"(odd), "v"(s), "v"(six));
-        if (t + 1 < kTerms) {
+        if (t + 1 < kAll) {
           const at_v32f back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(six, s);
 #pragma unroll
           for (int j = 0; j < 16; j++) even[j] -= back[2 * j], odd[j] -= back[2 * j + 1];    // (exact)
         }
         codes[c][t] = six;
-        scale[c][t / 4] |= (exponent == 255 ? 255 : byte) << (8 * (t % 4));
+      }
+      if constexpr (AtKind<E>::kLast) {
+        at_v4i four;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          float y[8];
+#pragma unroll
+          for (int j = 0; j < 4; j++) y[2 * j] = even[4 * w + j], y[2 * j + 1] = odd[4 * w + j];
+          four[w] = (int)mx4_codes8(y, (uint32_t)byte_of(kTerms));
+        }
+        reinterpret_cast<at_v4i *>(lds)[c * 64 + (threadIdx.x & 63)] = four;
       }
     }
   }
 };
 
-// Scores of sixteen tokens, 4 bits by 6, of all terms of 128 columns.
-template <int T, int TERMS>
-__device__ __forceinline__ at_v4f at_scores(at_v4i keys, int key_scale, const at_v6u (&q)[TERMS], const int (&scale)[(TERMS + 3) / 4],
-                                            at_v4f acc) {
+// Scores of sixteen tokens of all terms of 128 columns, 4 bits by 6 and by 4.
+template <int T, int TERMS, int WORDS>
+__device__ __forceinline__ at_v4f at_terms(at_v4i keys, int key_scale, const at_v6u (&q)[TERMS], const int (&scale)[WORDS], at_v4f acc) {
   if constexpr (T == TERMS) return acc;
   else {
     const at_v4f sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
         at_v8i{keys[0], keys[1], keys[2], keys[3], 0, 0, 0, 0},
         at_v8i{(int)q[T][0], (int)q[T][1], (int)q[T][2], (int)q[T][3], (int)q[T][4], (int)q[T][5], 0, 0}, acc, 4, 2, 0, key_scale,
         T % 4, scale[T / 4]);
-    return at_scores<T + 1, TERMS>(keys, key_scale, q, scale, sum);
+    return at_terms<T + 1>(keys, key_scale, q, scale, sum);
   }
+}
+template <class E, int D>
+__device__ __forceinline__ at_v4f at_scores(at_v4i keys, int key_scale, const AtQueries<E, D> &q, int c, at_v4f acc) {
+  const at_v4f sum = at_terms<0>(keys, key_scale, q.codes[c], q.scale[c], acc);
+  if constexpr (AtKind<E>::kLast) {
+    constexpr int T = AtKind<E>::kQ;
+    const at_v4i four = q.last[c * 64];
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(at_v8i{keys[0], keys[1], keys[2], keys[3], 0, 0, 0, 0},
+                                                            at_v8i{four[0], four[1], four[2], four[3], 0, 0, 0, 0}, sum, 4, 4, 0,
+                                                            key_scale, T % 4, q.scale[c][T / 4]);
+  }
+  return sum;
 }
 
 // ---- weights and values --------------------------------------------------------------

@@ -167,7 +167,7 @@ __device__ __forceinline__ void at_keys(AtState<E, D> &a, at_v4i (&packed)[AtKin
       at_v4i codes = s.codes[k][c];
       int byte = s.scale[k][c];
       if (D == 64 && q >= 2) codes = at_v4i{0, 0, 0, 0}, byte = 127;
-      r = at_scores<0>(codes, byte, queries.codes[c], queries.scale[c], r);
+      r = at_scores<E, D>(codes, byte, queries, c, r);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) score[k * 4 + i] = r[i];
@@ -304,6 +304,9 @@ __global__ __launch_bounds__(256 * G) void mx4_attention_join_kernel(Attention p
   at_store<E, OUT, D>(p, r, h, i, x, s_most, g == 0);
 }
 
+// Bytes of the rings, in which results meet afterwards; queries' last terms lie behind them.
+template <int D> constexpr int at_rows_rings() { return kAtWaves<D> * std::max(16 * D * 4, kAtStages * AtRing<D>::kStage); }
+template <class E, int D> constexpr int at_rows_lds() { return at_rows_rings<D>() + kAtWaves<D> * AtQueries<E, D>::kLds; }
 // Waves that share a SIMD's registers.
 template <class E, int D> constexpr int at_rows_waves() { return D == 256 ? 1 : AtKind<E>::kQ == 6 ? 2 : 4; }
 
@@ -328,7 +331,7 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
   const int position = position_of(at), low = position_of(r.first), high = position_of(r.last - 1);
   AtQueries<E, D> queries;
   queries.load(reinterpret_cast<const typename E::T *>(p.q + (size_t)(r.begin + token) * p.q_row_bytes) + (size_t)head * D,
-               p.negative);
+               p.negative, s_ring + at_rows_rings<D>() + wave * AtQueries<E, D>::kLds);
 
   const AtTiles tiles = at_tiles(p, low, high);
   const int steps = (int)((tiles.all + 1ll) / 2), chunk = at_share_steps(p, steps, kAtLeast);
@@ -429,6 +432,7 @@ template <int HG> struct AtHeads {
   static constexpr int kWaves = 8, kGroups = kWaves / HG;       // groups of waves with steps of their own
   static constexpr int kTile = HG * 1024, kScales = 4 * kTile;  // sixteen tokens' codes; keys, keys, values, values, scales
   static constexpr int kGroup = kScales + HG * 256, kStage = kGroups * kGroup, kLoads = 5;
+  static constexpr int kRings = 2 * kStage;
   static constexpr int kTokens = 16 / HG;                       // of a load
 
   // The token and head of piece group x (k / 4) of load j of a tile.
@@ -478,7 +482,7 @@ __global__ __launch_bounds__(512, AtKind<E>::kQ == 6 ? 2 : 4) void mx4_attention
   const int position = position_of(at), low = position_of(r.first), high = position_of(r.last - 1);
   AtQueries<E, D> queries;
   queries.load(reinterpret_cast<const typename E::T *>(p.q + (size_t)(r.begin + token) * p.q_row_bytes) + (size_t)head * D,
-               p.negative);
+               p.negative, s_ring + H::kRings + wave * AtQueries<E, D>::kLds);
   const AtTiles tiles = at_tiles(p, low, high);
   const int steps = (int)((tiles.all + 1ll) / 2), chunk = at_share_steps(p, steps, kAtLeast);
   const int begin = (int)min((long long)share * chunk, (long long)steps), end = (int)min((long long)begin + chunk, (long long)steps);
@@ -628,8 +632,8 @@ static int at_head_set(const Attention &p, int dim) {
   return dim != 128 ? 1 : p.kv_heads % 8 == 0 ? 8 : p.kv_heads % 4 == 0 ? 4 : p.kv_heads % 2 == 0 ? 2 : 1;
 }
 template <class E, class OUT, int HG> static int at_heads_launch(const Attention &p, hipStream_t st) {
-  constexpr size_t kLds = 2 * AtHeads<HG>::kStage;
-  static_assert(kLds >= (8 - HG) * 16 * 128 * 4, "results of the other groups");
+  constexpr size_t kLds = AtHeads<HG>::kRings + 8 * AtQueries<E, 128>::kLds;
+  static_assert(AtHeads<HG>::kRings >= (8 - HG) * 16 * 128 * 4, "results of the other groups");
   static std::atomic<uint64_t> attr_set{0};
   auto kernel = mx4_attention_heads_kernel<E, OUT, HG>;
   if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;
@@ -658,7 +662,7 @@ template <class E, class OUT, int D> static int at_launch(Attention p, int type,
       return rc;
   } else {
     const unsigned units = (unsigned)((long long)p.slots * p.splits);
-    constexpr size_t kLds = (size_t)kAtWaves<D> * std::max(16 * D * 4, kAtStages * AtRing<D>::kStage);
+    constexpr size_t kLds = at_rows_lds<E, D>();
     static std::atomic<uint64_t> attr_set{0};
     auto kernel = mx4_attention_rows_kernel<E, OUT, D>;
     if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
     my_low[t] = first < r.last ? position_of(first) : -1;
     my_high[t] = first < r.last ? position_of(min(first + 15, r.last - 1)) : -1;
     queries[t].load(reinterpret_cast<const typename E::T *>(p.q + (size_t)(r.begin + token) * p.q_row_bytes) + (size_t)head * D,
-                    p.negative);
+                    p.negative, s_all + 2 * sizeof(PromptLds<E, D>) + (wave * QT + t) * AtQueries<E, D>::kLds);
   }
   // Sums of weights are products with a column of ones, whose results are all the same: the vector unit has more to do than
   // the matrix cores (16 additions of 110 instructions for sixteen rows and 64 tokens).
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
           const at_v4i codes = now.keys[k][c][lane];
           const int byte = now.key_scale[k][c][lane];
 #pragma unroll
-          for (int t = 0; t < QT; t++) s[t] = at_scores<0>(codes, byte, queries[t].codes[c], queries[t].scale[c], s[t]);
+          for (int t = 0; t < QT; t++) s[t] = at_scores<E, D>(codes, byte, queries[t], c, s[t]);
         }
 #pragma unroll
         for (int t = 0; t < QT; t++)
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
 
 template <class E, class OUT, int D, int TYPE> static int prompt_launch(const Attention &p, hipStream_t st) {
   constexpr int QT = at_prompt_sixteens(TYPE, D);
-  constexpr size_t kLds = 2 * sizeof(PromptLds<E, D>);
+  constexpr size_t kLds = 2 * sizeof(PromptLds<E, D>) + kPromptWaves * QT * AtQueries<E, D>::kLds;
   static std::atomic<uint64_t> attr_set{0};
   auto kernel = mx4_attention_prompt_kernel<E, OUT, D, QT>;
   if (int rc = set_lds_attr(kernel, kLds, attr_set)) return rc;
