@@ -79,6 +79,10 @@ template <> struct AtKind<BF16> {
   static constexpr bool kLast = true;
   static constexpr float kUp = -39;
 };
+// Queries in fp16 whose result is microscaled: that holds numbers fp16 does not, as the values may be, and so these are bf16
+// and weights two terms.
+struct AtWide : F16 {};
+template <> struct AtKind<AtWide> : AtKind<BF16> { static constexpr int kP = 2; };
 
 // Which rows a slot of sixteen has. Slots of a sequence begin at floor(start * group / 16) + its number, which leaves
 // each as many as it needs.
@@ -252,7 +256,7 @@ template <class E> __device__ __forceinline__ float at_divisor(float sum) {
   return AtKind<E>::kDown ? sum * (1.0f / (1 << AtKind<E>::kDown)) : sum;
 }
 
-// Pairs of values, and the product with weights, in the type that weights are rounded to.
+// Pairs of values, and the product with weights, in the type that weights are rounded to: bf16 but for fp16's.
 template <class E> struct AtValues {
   typedef at_v2b Two;
   static __device__ __forceinline__ Two two(uint32_t codes, float s, std::integral_constant<int, 0>) {

@@ -798,7 +798,7 @@ int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const vo
                         : at_launch<E, OUT, 256>(p, type, plan.prompt, plan.sixteens, st);
   };
   if (type == MI355X_F32) return mx4 ? launch(F32(), MX4()) : launch(F32(), F32());
-  if (type == MI355X_F16) return mx4 ? launch(F16(), MX4()) : launch(F16(), F16());
+  if (type == MI355X_F16) return mx4 ? launch(AtWide(), MX4()) : launch(F16(), F16());
   return mx4 ? launch(BF16(), MX4()) : launch(BF16(), BF16());
 }
 

@@ -352,7 +352,7 @@ int at_prompt_launch(const Attention &p, int type, bool mx4, int dim, hipStream_
   if (type == MI355X_F32)
     return mx4 ? prompt_launch_dim<F32, MX4, MI355X_F32>(p, dim, st) : prompt_launch_dim<F32, F32, MI355X_F32>(p, dim, st);
   if (type == MI355X_F16)
-    return mx4 ? prompt_launch_dim<F16, MX4, MI355X_F16>(p, dim, st) : prompt_launch_dim<F16, F16, MI355X_F16>(p, dim, st);
+    return mx4 ? prompt_launch_dim<AtWide, MX4, MI355X_F16>(p, dim, st) : prompt_launch_dim<F16, F16, MI355X_F16>(p, dim, st);
   return mx4 ? prompt_launch_dim<BF16, MX4, MI355X_BF16>(p, dim, st) : prompt_launch_dim<BF16, BF16, MI355X_BF16>(p, dim, st);
 }
 

@@ -1019,11 +1019,11 @@ int mi355x_mx4_cache_write(const mi355x_mx4_cache *cache, const void *keys, cons
  *   q    [rows x heads * head_dim], a float type; heads is a multiple of kv_heads
  *   out  the same, of q's type or MI355X_MX4, quantised from the 32-bit results; may be q's place
  * max_length: sequences are no longer than this (a longer one counts as this long). Keys and values
- * are what their rows stand for; with fp16 queries a block of values whose scale is above 2^13
- * (values of 65536 on) counts as NaN. A query is taken with what is above 2^-17 (fp32: 2^-29) of its
+ * are what their rows stand for; where the result is fp16, a block of values whose scale is above 2^13
+ * (values of 65536 on) counts as NaN, and values are rounded to multiples of 2^-24. A query is taken with what is above 2^-17 (fp32: 2^-29) of its
  * block of 32's largest, and above 2^-130. Sums are of 32 bits; weights are rounded to the type of q
  * before they meet values (fp32: to 24 bits). What adds less than 2^-84 to a sum whose largest weight is 1
- * may be left out (bf16 and fp32 queries); no sum passes the range that its result has. An infinity or a NaN in a query makes
+ * may be left out; no sum passes the range that its result has. An infinity or a NaN in a query makes
  * NaN of its head's result, one that a row sees in a key or a value of the row's heads or columns.
  * Equal calls give equal bits. Scores past the range of 32 bits: NaN. MI355X_ERR_NOT_SUPPORTED where
  * rows * heads / 16 + sequences * kv_heads is over 2^22.

@@ -146,3 +146,32 @@ def test_values_at_the_ends_of_the_range(dim, kv_heads, group, new, longest, siz
     scale = 8 / dim
     check(b, q, heads, type_, scale=scale)
     check(b, q, heads, type_, ref.MX4, scale=scale, window=90, sinks=7)
+
+
+@pytest.mark.parametrize("sizes", [(75, 78), (85, 110), (120, 150), (140, 142), (240, 252)])
+@pytest.mark.parametrize("dim, kv_heads, group, new, longest", SHAPES)
+def test_values_that_fp16_does_not_hold_in_a_microscaled_result(dim, kv_heads, group, new, longest, sizes):
+    """Blocks with scales from 2^-52 to 2^125 under fp16 queries: a microscaled result is quantised from what they stand for."""
+    rng = np.random.default_rng(sizes[0] + dim)
+    b = aref.Batch(rng, [longest, 40], [new, min(new, 40)], kv_heads, dim, 32)
+    heads, cols = kv_heads * group, kv_heads * dim
+    groups = ref.groups(cols)
+    for i, length in enumerate(b.lengths):
+        at = b.places(i, int(length))
+        b.values[np.ix_(at, 64 * groups + np.arange(cols // 32))] = rng.integers(*sizes, (at.size, cols // 32))
+    q = queries(rng, b, heads, ref.F16)
+    check(b, q, heads, ref.F16, ref.MX4)
+    check(b, q, heads, ref.F16, ref.MX4, window=50, sinks=4)
+
+
+@pytest.mark.parametrize("dim, kv_heads, group, new, longest", SHAPES)
+def test_small_values_under_fp16(dim, kv_heads, group, new, longest):
+    """An fp16 result of values with scales from 2^-40 on: each is rounded to a multiple of 2^-24, by half of one at most."""
+    rng = np.random.default_rng(dim)
+    b = aref.Batch(rng, [longest], [new], kv_heads, dim, 32)
+    heads, cols = kv_heads * group, kv_heads * dim
+    groups, at = ref.groups(cols), b.places(0, longest)
+    b.values[np.ix_(at, 64 * groups + np.arange(cols // 32))] = rng.integers(87, 112, (at.size, cols // 32))
+    q = queries(rng, b, heads, ref.F16)
+    want, err, used = aref.attention(b, ref.to_f64(q, ref.F16), heads, ref.F16)
+    ref.check_float(run(b, q, heads, ref.F16)[used], want[used], err[used] + 2.0 ** -25, ref.F16)
