@@ -195,6 +195,8 @@ template <class OUT> static int adapted_launch(const MxFcAdapted &p, int K, FcTi
 }
 
 constexpr size_t kMostRank = 1024;
+// Columns are counted in 32 bits, by waves that have up to 2048 of them behind the last and look two steps ahead.
+constexpr size_t kMostColumns = 0x7fffffff - 4096;
 
 // Two turns for many rows: where requests meet in a tile, its two adapters would take turns in one workgroup.
 static int down_turns(size_t M) { return M <= 256 ? (int)std::min<size_t>(16, M) : 2; }
@@ -246,6 +248,7 @@ int mi355x_mx4_fc_adapters(void *out, int out_type, size_t out_row_bytes, const 
   if (!rank || !count || !K)                       // nothing beside the product
     return mi355x_mx4_fc(out, out_type, out_row_bytes, in, in_type, in_row_bytes, weights, weights_row_bytes, bias, M, K, N,
                          activation, workspace, workspace_bytes, stream);
+  if (K > kMostColumns) return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_fc_adapters: %zu columns, up to %zu are supported", K, kMostColumns);
   const size_t size = float_size(adapters->type);
   MI355X_REQUIRE(count <= 0x7fffffff, "mx4_fc_adapters: %zu adapters", count);
   MI355X_REQUIRE(adapters->down && adapters->up && row_adapters, "mx4_fc_adapters: NULL");

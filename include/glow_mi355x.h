@@ -1051,7 +1051,8 @@ int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const vo
  *   row_adapters  DEVICE int32 [M]; rows of the same adapter are fastest next to each other
  * All sums are of 32 bits, in no particular order (equal calls give equal bits), and down[a] in[m] goes
  * on in 24; an infinity in an adapter may come out as NaN. With K, rank or count of 0 this is
- * mi355x_mx4_fc, whose limits it has, and M * (K / 4096 + ranks in 64s / 8) up to 2^22.
+ * mi355x_mx4_fc, whose limits it has, and M * (K / 4096 + ranks in 64s / 8) up to 2^22 and K up to
+ * 2^31 - 4097.
  * workspace as there, of mi355x_mx4_fc_adapters_workspace_bytes (as much as mi355x_mx4_fc asks for). */
 typedef struct {
   const void *down, *up;        /* DEVICE */
