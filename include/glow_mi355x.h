@@ -1053,7 +1053,8 @@ int mi355x_mx4_attention(void *out, int out_type, size_t out_row_bytes, const vo
  * on in 24; an infinity in an adapter may come out as NaN. With K, rank or count of 0 this is
  * mi355x_mx4_fc, whose limits it has, and M * (K / 4096 + ranks in 64s / 8) up to 2^22 and K up to
  * 2^31 - 4097.
- * workspace as there, of mi355x_mx4_fc_adapters_workspace_bytes (as much as mi355x_mx4_fc asks for). */
+ * workspace as there, but of mi355x_mx4_fc_adapters_workspace_bytes: what `down` gives lies there beside a
+ * float input's quantised rows, so that one is needed, whatever the input's type, unless M, N or rank is 0. */
 typedef struct {
   const void *down, *up;        /* DEVICE */
   const float *scales;          /* DEVICE */
