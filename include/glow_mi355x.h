@@ -1004,7 +1004,7 @@ typedef struct {
 /* Writes the batch's keys and values [rows x kv_heads * head_dim], of any type, into the cache:
  * quantised by the rule of mi355x_mx4_quantize, or as they are where they are MI355X_MX4 (results
  * of mi355x_mx4_fc). Tokens without a place (before the first, behind the last, on no page) are left
- * out. Two tokens on one place leave either. */
+ * out. Two tokens of a call on one place leave what may be a mixture of both, even in one block. */
 int mi355x_mx4_cache_write(const mi355x_mx4_cache *cache, const void *keys, const void *values,
                            int type, size_t keys_row_bytes, size_t values_row_bytes,
                            const int32_t *starts, const int32_t *lengths, size_t sequences,
