@@ -1028,7 +1028,9 @@ int mi355x_mx4_cache_write(const mi355x_mx4_cache *cache, const void *keys, cons
  * Equal calls give equal bits. Scores past the range of 32 bits: NaN. MI355X_ERR_NOT_SUPPORTED where
  * rows * heads / 16 + sequences * kv_heads is over 2^22.
  * workspace: device memory of mi355x_mx4_attention_workspace_bytes, on a multiple of 16 and
- * overlapping no tensor; NULL where that is 0. A call leaves nothing in it for the next, and calls
+ * overlapping no tensor; NULL where that is 0. Few rows over long sequences need one, more rows less or
+ * none: a program asks for each of its batches, or has 66 MiB, which hold for any. It holds for
+ * every type, window and first tokens. A call leaves nothing in it for the next, and calls
  * that may run at the same time need one each. */
 int mi355x_mx4_attention_workspace_bytes(const mi355x_mx4_cache *cache, size_t heads,
                                          size_t sequences, size_t rows, size_t max_length,
