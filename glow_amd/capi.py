@@ -1669,7 +1669,7 @@ def _cache_on_device(keys, values, pages, page_tokens, sequences, kv_heads, head
     """(cache, its buffers) of host arrays: keys and values rows of TYPE_MX4, pages int32 [sequences, pages of each]
     or None."""
     keys, values = _mx4_rows(keys), _mx4_rows(values)
-    if keys.shape != values.shape or page_tokens <= 0 or keys.shape[0] % page_tokens:
+    if keys.ndim != 2 or keys.shape != values.shape or page_tokens <= 0 or keys.shape[0] % page_tokens:
         raise MI355XError(-1, f"keys of shape {keys.shape}, values of {values.shape}, pages of {page_tokens} tokens")
     n_pages = keys.shape[0] // page_tokens
     if pages is None:
@@ -1759,9 +1759,11 @@ def mx4_fc_adapters(x, in_type, weights, bias, K, down, up, row_adapters, scales
     """mx4_fc with adapters down [count, rank, K] and up [count, N, rank] of type_; row_adapters: int32 [M]."""
     x = _mx4_rows(x) if in_type == TYPE_MX4 else _float_rows(x, in_type)
     weights, down, up = _mx4_rows(weights), _float_rows(down, type_), _float_rows(up, type_)
+    row_adapters = np.ascontiguousarray(row_adapters, np.int32)
+    if down.ndim != 3 or up.ndim != 3 or x.ndim != 2 or weights.ndim != 2:
+        raise MI355XError(-1, f"x of shape {x.shape}, weights of {weights.shape}, down of {down.shape}, up of {up.shape}")
     M, N = x.shape[0], weights.shape[0]
     bias = _columns("mx4_fc_adapters: bias", bias, N)
-    row_adapters = np.ascontiguousarray(row_adapters, np.int32)
     count, rank = down.shape[0], down.shape[1]
     if down.shape != (count, rank, K) or up.shape != (count, N, rank) or row_adapters.shape != (M,):
         raise MI355XError(-1, f"down of shape {down.shape}, up of {up.shape}, {row_adapters.shape} rows: {M} x {K} x {N}")

@@ -1,4 +1,5 @@
 """What products with low-rank adapters refuse for their sizes, as far as no GPU is involved."""
+import numpy as np
 import pytest
 
 from glow_amd import capi
@@ -31,3 +32,15 @@ def test_workspaces_hold_both_launches(M, K, N, rank, in_type):
     shape = dict(M=M, K=K, N=N, in_type=in_type, in_row=max(4 * K, row_bytes(K)), w_row=row_bytes(K), out_row=2 * N)
     for change in (dict(ws=0), dict(ws_bytes=n - 1)):
         refused("mi355x_mx4_fc_adapters", fc_args(adapters(rank=rank), **shape, **change), "workspace")
+
+
+@pytest.mark.parametrize("change", [dict(x=(100,)), dict(weights=(80,)), dict(down=(100,)), dict(down=(4, 100)), dict(up=(5,)), dict(up=(5, 4))])
+def test_conveniences_refuse_arrays_of_other_ranks(change):
+    shapes = dict(x=(2, 100), weights=(5, 80), down=(1, 4, 100), up=(1, 5, 4))
+    shapes.update(change)
+    x, weights, down, up = (np.zeros(shapes[k], np.uint8 if k == "weights" else np.float32) for k in ("x", "weights", "down", "up"))
+    with pytest.raises(capi.MI355XError, match="of shape"):
+        capi.mx4_fc_adapters(x, 0, weights, None, 100, down, up, np.zeros(2, np.int32))
+    rows = np.zeros(160, np.uint8)
+    with pytest.raises(capi.MI355XError, match="of shape"):
+        capi.mx4_attention(np.zeros((1, 128), np.float32), 1, rows, rows, [0, 1], [1], 1, 128, 16, [[0]])
