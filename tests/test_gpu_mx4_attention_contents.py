@@ -175,3 +175,11 @@ def test_small_values_under_fp16(dim, kv_heads, group, new, longest):
     q = queries(rng, b, heads, ref.F16)
     want, err, used = aref.attention(b, ref.to_f64(q, ref.F16), heads, ref.F16)
     ref.check_float(run(b, q, heads, ref.F16)[used], want[used], err[used] + 2.0 ** -25, ref.F16)
+
+
+def test_a_vector_is_no_cache():
+    rows, one = np.zeros(160, np.uint8), np.zeros((1, 128), np.float32)
+    with pytest.raises(capi.MI355XError, match="keys of shape"):
+        capi.mx4_attention(one, 1, rows, rows, [0, 1], [1], 1, 128, 16, [[0]])
+    with pytest.raises(capi.MI355XError, match="keys of shape"):
+        capi.mx4_cache_write(rows, rows, one, one, [0, 1], [1], 1, 128, 16, [[0]])

@@ -35,12 +35,9 @@ def test_workspaces_hold_both_launches(M, K, N, rank, in_type):
 
 
 @pytest.mark.parametrize("change", [dict(x=(100,)), dict(weights=(80,)), dict(down=(100,)), dict(down=(4, 100)), dict(up=(5,)), dict(up=(5, 4))])
-def test_conveniences_refuse_arrays_of_other_ranks(change):
+def test_the_convenience_refuses_arrays_of_other_ranks(change):
     shapes = dict(x=(2, 100), weights=(5, 80), down=(1, 4, 100), up=(1, 5, 4))
     shapes.update(change)
     x, weights, down, up = (np.zeros(shapes[k], np.uint8 if k == "weights" else np.float32) for k in ("x", "weights", "down", "up"))
     with pytest.raises(capi.MI355XError, match="of shape"):
         capi.mx4_fc_adapters(x, 0, weights, None, 100, down, up, np.zeros(2, np.int32))
-    rows = np.zeros(160, np.uint8)
-    with pytest.raises(capi.MI355XError, match="of shape"):
-        capi.mx4_attention(np.zeros((1, 128), np.float32), 1, rows, rows, [0, 1], [1], 1, 128, 16, [[0]])
