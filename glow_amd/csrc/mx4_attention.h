@@ -80,7 +80,7 @@ template <> struct AtKind<BF16> {
   static constexpr float kUp = -39;
 };
 // Queries in fp16 whose result is microscaled: that holds numbers fp16 does not, as the values may be, and so these are bf16
-// and weights two terms.
+// and weights two terms. us, with them / with fp16: four long sequences 150 / 132, a prompt of 16384 through a window of 1024 528 / 441.
 struct AtWide : F16 {};
 template <> struct AtKind<AtWide> : AtKind<BF16> { static constexpr int kP = 2; };
 

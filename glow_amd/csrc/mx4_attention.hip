@@ -11,7 +11,7 @@ namespace mi355x {
 // reads: there is no barrier in the loop. A load moves 16 bytes a lane, 1 KB at once, and a lane picks the piece that
 // makes the reads free of bank conflicts: keys' blocks in the order of the products' tiles (mx4_swizzle), token 4 q + i of
 // the values in row q + 4 i, so that word i of a lane lies at 64 i + lane. What bounds it: the launch and four rounds of
-// dependent loads (one token over 200, 8 heads of 64: 6.5 us), then memory.
+// dependent loads (one token over 200, 8 heads of 64: 6.8 us), then memory.
 template <int D> constexpr int kAtWaves = D == 256 ? 4 : 8;
 constexpr int kAtStages = 2;
 constexpr int kAtLeast = 8;            // steps of a share at least
@@ -420,8 +420,8 @@ __global__ __launch_bounds__(kAtWaves<D> * 64, (at_rows_waves<E, D>())) void mx4
 // of 1 KB has 16 / HG tokens of all of them, lines whole, where a head's own rows come in pieces of 64 bytes and its
 // scales in pieces of four (a large copy's rate against 60 % of it, nothing but loads). Waves wait for
 // each other's loads at two barriers a step: when rows have landed, and when they are in registers. Bound by memory:
-// four sequences of 100 000 to 131 072 tokens, 8 heads, fp16 queries 112 us (513 MB, 4.6 TB/s; 105 with nothing but the loads, 66 with
-// nothing but the rest), and 21 to join them; 171 in all with a head a workgroup.
+// four sequences of 100 000 to 131 072 tokens, 8 heads, fp16 queries 113 us (513 MB, 4.5 TB/s; 105 with nothing but the loads), and 21 to
+// join them. A head a workgroup, before queries had a fourth term: 171 in all for 130.
 //
 // Piece k of a load, 16 bytes, lies at 16 k in LDS, and lanes choose theirs so that no read meets a bank twice, pieces of a
 // head's 64 bytes side by side: with k = 16 xh + 4 xl + c', t a token of the tile, c a piece of its head,
@@ -702,8 +702,8 @@ static int at_plan(const mi355x_mx4_cache *cache, size_t heads, int type, size_t
   if (sixteens * p->kv_heads > 1 << 22)
     return fail(MI355X_ERR_NOT_SUPPORTED, "mx4_attention: %zu rows of %zu heads, %zu sequences", rows, heads, sequences);
   // Many rows of a sequence share what is read and converted. us, sixteens of rows / prompts' kernel, 32 heads of 128 over 8, bf16, 16
-  // sequences of 4096 tokens: 32 pairs of a row and a head a sequence 38 / 56, 64 55 / 65, 96 82 / 69, 256 152 / 117; of 500 tokens: 96
-  // 24.5 / 26.5, 128 32.6 / 27.7.
+  // sequences of 4096 tokens: 32 pairs of a row and a head a sequence 41 / 58, 64 58 / 66, 96 83 / 71, 256 161 / 123; of 500 tokens: 96
+  // 26 / 27.5, 128 34 / 28. (The average decides for the whole batch: single tokens beside a long prompt go with it.)
   plan->prompt = rows * p->group > 64 * sequences;
   plan->sixteens = (int)sixteens;
   const int per_slot = plan->prompt ? kPromptWaves * 16 * at_prompt_sixteens(type, (int)cache->head_dim) : 16;

@@ -10,9 +10,10 @@ namespace mi355x {
 // what the matrix instructions want, once for all waves. Two buffers: a step is prepared while the one in front is
 // multiplied, and its successor's rows are on their way from memory into registers.
 //
-// Two prompts of 4096, 32 heads of 128 over 8, bf16: 393 us, 700 TFLOP/s (a workgroup for sixteen rows, each converting
-// values for itself: 1884). A step takes a SIMD 3200 cycles for 960 of matrix and 1200 of vector instructions: the chain of a step, the
-// largest score above all, is waited for, and no more than two waves fit the registers.
+// Two prompts of 4096, 32 heads of 128 over 8, bf16: 411 us, 669 TFLOP/s (a workgroup for sixteen rows, each converting
+// values for itself: 1884). A wave's step is 68 matrix instructions of 16 cycles and 365 others. Matrix cores are busy for 26 % of the
+// cycles, vector instructions for 48 %: the chain of a step, the largest score above all, is waited for, and no more than two waves
+// fit the registers.
 constexpr int kPromptTiles = kPromptWaves;
 
 // What is said of a tile.
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, 2) void mx4_attention_prompt_ker
     value_scale_at[i] = (4 * q + i) * row_bytes + scales_at + l16 * COLS / 32;
   }
   // Where this wave's tiles lie, a lane each of 64 steps, which are asked for in order: an entry of the page table asked for
-  // at each step would be waited for together with all that was asked for in front of it (411 us for 394 over 2 x 4096).
+  // at each step would be waited for together with all that was asked for in front of it (4 % over 2 x 4096).
   int tile_of = -1;
   auto locate = [&](int step) {
     const int n = step - begin;
