@@ -9,7 +9,7 @@
 //       the keys as they lie in memory (a lane has one block of a token), queries as sums of 6-bit
 //       floats (E2M3) with a power of two for each block of 32: 3 terms and a 4-bit one (E2M1) for 16-bit types,
 //       6 for fp32. Nothing of a key is ever converted. A lane gets tokens 4 q .. 4 q + 3. 8-bit terms
-//       would be 3, 3 and 6 of twice the time each, and the instruction cuts small products off
+//       (E4M3) have as many bits and take twice the time each, and the instruction cuts small products off
 //       where exponents lie far apart (2^-17 of the sum; 6-bit products come out exact).
 //   P   is what the lane then holds of two tiles of tokens: eight weights of its query, which is what the
 //       16x16x32 instruction wants of its second operand, tokens in the order 4 q + i of the first
